@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define SC_ABI_VERSION 13
+#define SC_ABI_VERSION 14
 
 /* Kernel selection for sc_qmm_bf16_path. */
 #define SC_QMM_PATH_AUTO 0 /* M <= 16: GEMV or band kernel (8-16 rows, by shape);
@@ -304,6 +304,87 @@ int sc_rope_append_kv_bf16(uint16_t *qkv, int64_t qkv_stride, int64_t B, int64_t
                            int64_t D, const float *cos_t, const float *sin_t, int64_t table_len, uint16_t *k_cache,
                            uint16_t *v_cache_t, int64_t T_cap, const int32_t *cache_len, int64_t pos_offset,
                            void *hip_stream);
+
+/* ------------------------------------------------------------------------------
+ * A key/value cache in blocks, for a ragged batch of sequences that share a prefix
+ * (no reference counterpart: the reference holds one dense cache of equal lengths,
+ * src/shardcompute/parallel/attention.py:429-433).
+ *
+ * Pool per layer, block_size (bs) one of 16, 32, 64, 128, 256 positions:
+ *   k_blocks  [n_blocks, Hkv, bs, D] bf16
+ *   vt_blocks [n_blocks, Hkv, D, bs] bf16 (values transposed)
+ * Position p of sequence r's own keys lies in block tables[r, p / bs] at offset p % bs,
+ * its slot is tables[r, p / bs] * bs + p % bs; position p of the shared prefix likewise in
+ * prefix_table[p / bs].  Sequence r's own positions follow the prefix: its position p is
+ * rotated for prefix length + p.  Lengths, tables, row starts, slots and positions are
+ * int32 in device memory, so a captured step replays at any length.
+ * ---------------------------------------------------------------------------- */
+
+/* Bits of block_tables' status word. */
+#define SC_BLOCKS_NO_BLOCKS 1 /* more new blocks than the stack holds             */
+#define SC_BLOCKS_NO_TABLE 2  /* a sequence outgrows its table                    */
+#define SC_BLOCKS_NO_ROWS 4   /* more new positions than rows                     */
+#define SC_BLOCKS_NO_STACK 8  /* more blocks given back than the stack has room for */
+
+/*
+ * The tables and rows of one model step.  Sequence r holds lengths[r] positions and gets
+ * new_positions[r] more (negative: none); where release_or_null[r] is nonzero its blocks
+ * go back to the stack first and it starts from 0.  free_blocks [cap] is a stack of the
+ * blocks nobody holds, n_free[0] of them: blocks given back are pushed in the order
+ * (sequence, place), then new blocks are popped in that order and written to
+ * tables [R, width].  Writes
+ *   lengths_out[R]     the new lengths          n_free_out[1]  the stack's new height
+ *   row_starts[R + 1]  exclusive sum of the new positions
+ *   slots[rows], positions[rows]   of row row_starts[r] + i: the slot of position
+ *       old length + i and its rotary position prefix_len_or_null[0] + that; rows behind
+ *       the last get -1.
+ * lengths_out and n_free_out may be lengths and n_free.  A step that does not fit is
+ * refused as a whole: tables, stack, lengths stay as they are, row_starts is all 0, every
+ * row -1, and the reasons are or-ed into status[0] (the caller's to clear).  R <= 65536.
+ */
+int sc_block_tables_i32(const int32_t *lengths, const int32_t *new_positions, const uint8_t *release_or_null,
+                        int32_t *tables, int32_t *free_blocks, const int32_t *n_free,
+                        const int32_t *prefix_len_or_null, int64_t R, int64_t width, int64_t block_size, int64_t cap,
+                        int64_t rows, int32_t *lengths_out, int32_t *n_free_out, int32_t *row_starts, int32_t *slots,
+                        int32_t *positions, int32_t *status, void *hip_stream);
+
+/*
+ * RoPE and cache append of N rows of the fused projection qkv [N, qkv_stride] (q heads,
+ * then k heads, then v heads, each D wide; 64 or 128): row t is rotated for positions[t]
+ * (rotate-half, fp32 tables [table_len, D/2]), its q written to q_out row t (stride
+ * q_stride; q_out may be the q part of qkv), its k and v to slot slots[t].  A row whose
+ * slot lies outside the pool or whose position outside the tables is left alone.  Slots of
+ * different rows differ.  The rotation's arithmetic is sc_rope_append_kv_bf16's, bit for bit.
+ */
+int sc_rope_append_blocks_bf16(const uint16_t *qkv, int64_t qkv_stride, uint16_t *q_out, int64_t q_stride, int64_t N,
+                               int64_t H, int64_t Hkv, int64_t D, const float *cos_t, const float *sin_t,
+                               int64_t table_len, uint16_t *k_blocks, uint16_t *vt_blocks, int64_t n_blocks,
+                               int64_t block_size, const int32_t *slots, const int32_t *positions, void *hip_stream);
+
+/* Bytes of workspace sc_attention_shared_bf16 needs: own_cap = width * block_size,
+ * prefix_cap = prefix_width * block_size. */
+int64_t sc_attention_shared_workspace_bytes(int64_t N, int64_t R, int64_t H, int64_t Hkv, int64_t D, int64_t own_cap,
+                                            int64_t prefix_cap, int64_t max_new);
+
+/*
+ * Attention of a step's rows: row row_starts[r] + i, the i-th of sequence r's n_r new
+ * positions, attends the prefix_len[0] positions of the shared prefix and its sequence's
+ * own positions 0 .. lengths[r] - n_r + i (lengths: with the new positions, which have been
+ * appended): out = softmax(q k^T * scale) v, q head h reading KV head h / (H / Hkv).  The
+ * prefix is read once for the whole batch.  q rows at q + row*q_stride + h*D, output rows
+ * likewise with out_stride; rows at or past row_starts[R] are left as they were; a row with
+ * no key is 0.  prefix_width 0: no prefix (null pointers).  max_new: at least the most new
+ * positions of one sequence (N does; a smaller bound saves launches; below the truth the
+ * rows of sequences above it are unspecified).  Slots that no row attends may hold anything.
+ * Block numbers, lengths and row starts out of range are clamped: the result is then
+ * unspecified, the access in bounds.  scale must be positive; D 64 or 128; R <= 2048.
+ */
+int sc_attention_shared_bf16(const uint16_t *q, int64_t q_stride, const uint16_t *k_blocks, const uint16_t *vt_blocks,
+                             int64_t n_blocks, int64_t block_size, const int32_t *row_starts, const int32_t *lengths,
+                             const int32_t *tables, int64_t width, const int32_t *prefix_table, int64_t prefix_width,
+                             const int32_t *prefix_len, uint16_t *out, int64_t out_stride, int64_t N, int64_t R,
+                             int64_t H, int64_t Hkv, int64_t D, float scale, int64_t max_new, void *workspace,
+                             int64_t workspace_bytes, void *hip_stream);
 
 /* Bytes of workspace sc_attention_bf16 needs for these sizes (0: none). */
 int64_t sc_attention_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t T_cap);

@@ -9,12 +9,13 @@ built, or a tensor is not on a GPU, the call raises.
 import ctypes
 import os
 import threading
+from typing import NamedTuple
 
 import torch
 
 from .build import LIB_PATH
 
-ABI_VERSION = 13
+ABI_VERSION = 14
 PATH_AUTO, PATH_GEMV, PATH_GEMM, PATH_BAND = 0, 1, 2, 3
 
 # Exported symbols (must match include/shardcompute_hip.h).
@@ -40,6 +41,10 @@ EXPORTS = (
     "sc_qmm_swiglu_bf16",
     "sc_rms_norm_bf16",
     "sc_rope_append_kv_bf16",
+    "sc_block_tables_i32",
+    "sc_rope_append_blocks_bf16",
+    "sc_attention_shared_workspace_bytes",
+    "sc_attention_shared_bf16",
     "sc_attention_workspace_bytes",
     "sc_attention_bf16",
     "sc_attention_masked_bf16",
@@ -126,6 +131,16 @@ def load():
         lib.sc_rms_norm_bf16.restype = i32
         lib.sc_rope_append_kv_bf16.argtypes = [p, i64, i64, i64, i64, i64, i64, p, p, i64, p, p, i64, p, i64, p]
         lib.sc_rope_append_kv_bf16.restype = i32
+        lib.sc_block_tables_i32.argtypes = [p, p, p, p, p, p, p, i64, i64, i64, i64, i64, p, p, p, p, p, p, p]
+        lib.sc_block_tables_i32.restype = i32
+        lib.sc_rope_append_blocks_bf16.argtypes = [p, i64, p, i64, i64, i64, i64, i64, p, p, i64, p, p, i64, i64, p, p,
+                                                   p]
+        lib.sc_rope_append_blocks_bf16.restype = i32
+        lib.sc_attention_shared_workspace_bytes.argtypes = [i64] * 8
+        lib.sc_attention_shared_workspace_bytes.restype = i64
+        lib.sc_attention_shared_bf16.argtypes = [p, i64, p, p, i64, i64, p, p, p, i64, p, i64, p, p, i64, i64, i64, i64,
+                                                 i64, i64, f32, i64, p, i64, p]
+        lib.sc_attention_shared_bf16.restype = i32
         lib.sc_attention_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i64]
         lib.sc_attention_workspace_bytes.restype = i64
         lib.sc_attention_bf16.argtypes = [p, i64, p, p, i64, p, p, i64, i64, i64, i64, i64, i64, f32, p, i64, p]
@@ -810,3 +825,212 @@ def add_i32(counters, delta, n=None):
     n = counters.numel() if n is None else n
     rc = lib.sc_add_i32(_ptr(counters), n, int(delta), _stream(counters))
     _check(rc, "sc_add_i32")
+
+
+# ---------------------------------------------------------------- key/value cache in blocks
+
+BLOCK_SIZES = (16, 32, 64, 128, 256)
+# bits of the status word of block_tables
+BLOCKS_NO_BLOCKS, BLOCKS_NO_TABLE, BLOCKS_NO_ROWS, BLOCKS_NO_STACK = 1, 2, 4, 8
+
+
+class BlockStep(NamedTuple):
+    """What ``block_tables`` writes for one model step (int32 device tensors)."""
+    lengths: torch.Tensor       # [R] positions each sequence holds, the new ones included
+    n_free: torch.Tensor        # [1] blocks left on the stack
+    row_starts: torch.Tensor    # [R + 1] first row of each sequence, and the number of rows
+    slots: torch.Tensor         # [rows] where each row's key and value go (-1: no such row)
+    positions: torch.Tensor     # [rows] rotary position of each row (-1: no such row)
+    status: torch.Tensor        # [1] BLOCKS_* bits of every refused step so far
+
+
+def block_step_buffers(R, rows, device):
+    """A :class:`BlockStep` for ``R`` sequences and steps of up to ``rows`` rows, status 0."""
+    def i32(n):
+        return torch.empty(n, dtype=torch.int32, device=device)
+    return BlockStep(i32(R), i32(1), i32(R + 1), i32(rows), i32(rows), torch.zeros(1, dtype=torch.int32, device=device))
+
+
+def _i32_flat(t, n, name):
+    if t.dtype != torch.int32 or t.numel() < n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of at least {n} entries")
+    return t
+
+
+def _same_device(t, *others):
+    dev = t.get_device()
+    for x in others:
+        if x is not None and x.get_device() != dev:
+            raise RuntimeError("all tensors of a call must be on one GPU")
+
+
+class _on_device:
+    """Makes a tensor's GPU the current one for a launch, when it is not already."""
+
+    def __init__(self, t):
+        self.dev = t.get_device()
+        self.back = None
+
+    def __enter__(self):
+        cur = torch.cuda.current_device()
+        if cur != self.dev:
+            torch.cuda.set_device(self.dev)
+            self.back = cur
+
+    def __exit__(self, *exc):
+        if self.back is not None:
+            torch.cuda.set_device(self.back)
+
+
+def block_tables(lengths, new, tables, free_blocks, n_free, block_size, rows, prefix_len=None, release=None, out=None):
+    """The block tables, row starts, slots and positions of one model step, on the device.
+
+    ``lengths`` [R] (positions each sequence holds), ``new`` [R] (positions it gets),
+    ``tables`` [R, width] (updated in place), ``free_blocks`` (a stack of unused blocks,
+    ``n_free`` [1] of them) are int32; ``release`` [R] bool gives a sequence's blocks back
+    before the step, ``prefix_len`` [1] is added to the rotary positions.  ``rows``: room for
+    the step's rows.  ``out``: a :class:`BlockStep` to fill (its ``lengths`` and ``n_free``
+    may be the ones passed in); without it a new one is allocated.  A step that does not fit
+    changes nothing, has no rows and sets ``status`` (see ``sc_block_tables_i32``)."""
+    lib = load()
+    _require_gpu(lengths, new, tables, free_blocks, n_free, prefix_len, release)
+    R = lengths.numel()
+    _i32_flat(lengths, 1, "lengths"), _i32_flat(new, R, "new"), _i32_flat(n_free, 1, "n_free")
+    _i32_flat(free_blocks, 1, "free_blocks")
+    if tables.dtype != torch.int32 or tables.dim() != 2 or tables.shape[0] != R or not tables.is_contiguous():
+        raise ValueError(f"tables must be a contiguous int32 [{R}, width] tensor")
+    if block_size not in BLOCK_SIZES:
+        raise ValueError(f"block_size must be one of {BLOCK_SIZES}, got {block_size}")
+    if new.numel() != R:
+        raise ValueError(f"new must hold {R} entries")
+    if prefix_len is not None:
+        _i32_flat(prefix_len, 1, "prefix_len")
+    if release is not None and (release.dtype not in (torch.bool, torch.uint8) or release.numel() != R
+                                or not release.is_contiguous()):
+        raise ValueError(f"release must be a contiguous bool tensor of {R} entries")
+    if out is None:
+        out = block_step_buffers(R, rows, lengths.device)
+    else:
+        _require_gpu(*out)
+        _i32_flat(out.lengths, R, "out.lengths"), _i32_flat(out.n_free, 1, "out.n_free")
+        _i32_flat(out.row_starts, R + 1, "out.row_starts"), _i32_flat(out.slots, rows, "out.slots")
+        _i32_flat(out.positions, rows, "out.positions"), _i32_flat(out.status, 1, "out.status")
+    _same_device(lengths, new, tables, free_blocks, n_free, prefix_len, release, *out)
+    with _on_device(lengths):
+        rc = lib.sc_block_tables_i32(_ptr(lengths), _ptr(new), _ptr(release), _ptr(tables), _ptr(free_blocks),
+                                     _ptr(n_free), _ptr(prefix_len), R, tables.shape[1], block_size,
+                                     free_blocks.numel(), rows, _ptr(out.lengths), _ptr(out.n_free),
+                                     _ptr(out.row_starts), _ptr(out.slots), _ptr(out.positions), _ptr(out.status),
+                                     _stream(lengths))
+    if rc:
+        _check(rc, "sc_block_tables_i32")
+    return out
+
+
+def _pool(k_blocks, vt_blocks, Hkv, D):
+    """(blocks, block size) of a pool's layer."""
+    _bf16(k_blocks, "k_blocks"), _bf16(vt_blocks, "vt_blocks")
+    if k_blocks.dim() != 4 or k_blocks.shape[1] != Hkv or k_blocks.shape[3] != D:
+        raise ValueError(f"k_blocks must be [blocks, {Hkv}, block_size, {D}], got {tuple(k_blocks.shape)}")
+    nb, _, bs, _ = k_blocks.shape
+    if tuple(vt_blocks.shape) != (nb, Hkv, D, bs):
+        raise ValueError(f"vt_blocks must be [{nb}, {Hkv}, {D}, {bs}], got {tuple(vt_blocks.shape)}")
+    if not (k_blocks.is_contiguous() and vt_blocks.is_contiguous()):
+        raise ValueError("the pool's tensors must be contiguous")
+    if bs not in BLOCK_SIZES:
+        raise ValueError(f"block_size must be one of {BLOCK_SIZES}, got {bs}")
+    return nb, bs
+
+
+def rope_append_blocks(qkv, H, Hkv, D, cos_t, sin_t, k_blocks, vt_blocks, slots, positions, out=None):
+    """RoPE of the rows qkv [N, >= (H+2Hkv)*D] for ``positions`` and append of their k and v
+    at ``slots`` of the pool k_blocks [blocks, Hkv, block_size, D], vt_blocks
+    [blocks, Hkv, D, block_size].  Returns the rotated q [N, H*D] (``out`` when given; it may
+    be the q part of qkv).  Rows whose slot is outside the pool (-1) or whose position is
+    outside the tables are left alone.  The slots of different rows must differ."""
+    lib = load()
+    _require_gpu(qkv, cos_t, sin_t, k_blocks, vt_blocks, slots, positions, out)
+    _bf16(qkv, "qkv")
+    if qkv.dim() != 2 or qkv.shape[1] < (H + 2 * Hkv) * D or qkv.stride(1) != 1:
+        raise ValueError(f"qkv must be a row-major [N, >= {(H + 2 * Hkv) * D}] matrix")
+    N = qkv.shape[0]
+    nb, bs = _pool(k_blocks, vt_blocks, Hkv, D)
+    _i32_flat(slots, N, "slots"), _i32_flat(positions, N, "positions")
+    if (cos_t.dtype != torch.float32 or sin_t.dtype != torch.float32 or cos_t.shape != sin_t.shape
+            or cos_t.dim() != 2 or cos_t.shape[1] != D // 2 or not cos_t.is_contiguous() or not sin_t.is_contiguous()):
+        raise ValueError("cos/sin tables must be contiguous fp32 [L, D/2]")
+    if out is None:
+        out = torch.empty((N, H * D), dtype=torch.bfloat16, device=qkv.device)
+    elif out.dtype != torch.bfloat16 or out.dim() != 2 or tuple(out.shape) != (N, H * D) or out.stride(1) != 1:
+        raise ValueError(f"out must be a row-major bf16 [{N}, {H * D}] matrix")
+    _same_device(qkv, cos_t, sin_t, k_blocks, vt_blocks, slots, positions, out)
+    if N == 0:
+        return out
+    with _on_device(qkv):
+        rc = lib.sc_rope_append_blocks_bf16(_ptr(qkv), qkv.stride(0) if N > 1 else qkv.shape[1], _ptr(out),
+                                            out.stride(0) if N > 1 else H * D, N, H, Hkv, D, _ptr(cos_t), _ptr(sin_t),
+                                            cos_t.shape[0], _ptr(k_blocks), _ptr(vt_blocks), nb, bs, _ptr(slots),
+                                            _ptr(positions), _stream(qkv))
+    if rc:
+        _check(rc, "sc_rope_append_blocks_bf16")
+    return out
+
+
+def attention_shared_workspace_bytes(N, R, H, Hkv, D, own_cap, prefix_cap, max_new):
+    """Workspace of ``attention_shared`` for N rows of R sequences; ``own_cap`` and
+    ``prefix_cap``: positions the tables have room for."""
+    return int(load().sc_attention_shared_workspace_bytes(N, R, H, Hkv, D, own_cap, prefix_cap, max_new))
+
+
+def attention_shared(q, H, Hkv, D, k_blocks, vt_blocks, row_starts, lengths, tables, scale, prefix_table=None,
+                     prefix_len=None, max_new=None, out=None, workspace=None):
+    """Attention of a step's rows over a shared prefix and each sequence's own positions.
+
+    Rows ``row_starts[r] .. row_starts[r + 1] - 1`` of q [N, >= H*D] are sequence r's new
+    positions, the last of its ``lengths[r]`` own ones (``tables`` [R, width] says in which
+    blocks).  Each attends the ``prefix_len[0]`` positions of ``prefix_table`` [width'], read
+    once for the batch, and its own sequence up to itself.  ``max_new``: an upper bound of
+    the rows of one sequence (default N).  Returns out [N, H*D] bf16; rows past the last
+    sequence's are left as they were."""
+    lib = load()
+    _require_gpu(q, k_blocks, vt_blocks, row_starts, lengths, tables, prefix_table, prefix_len, out, workspace)
+    _bf16(q, "q")
+    if q.dim() != 2 or q.shape[1] < H * D or q.stride(1) != 1:
+        raise ValueError(f"q must be a row-major [N, >= {H * D}] matrix")
+    N = q.shape[0]
+    nb, bs = _pool(k_blocks, vt_blocks, Hkv, D)
+    if tables.dtype != torch.int32 or tables.dim() != 2 or not tables.is_contiguous():
+        raise ValueError("tables must be a contiguous int32 [R, width] tensor")
+    R, width = tables.shape
+    _i32_flat(lengths, R, "lengths"), _i32_flat(row_starts, R + 1, "row_starts")
+    pw = 0
+    if prefix_table is not None:
+        if prefix_len is None:
+            raise ValueError("a prefix table needs prefix_len")
+        _i32_flat(prefix_len, 1, "prefix_len")
+        pw = _i32_flat(prefix_table, 0, "prefix_table").numel()
+    if out is None:
+        out = torch.empty((N, H * D), dtype=torch.bfloat16, device=q.device)
+    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (N, H * D) or out.stride(1) != 1:
+        raise ValueError(f"out must be a row-major bf16 [{N}, {H * D}] matrix")
+    if max_new is None:
+        max_new = N
+    elif max_new < 0:
+        raise ValueError("max_new must not be negative")
+    _same_device(q, k_blocks, vt_blocks, row_starts, lengths, tables, prefix_table, prefix_len, out, workspace)
+    if N == 0:
+        return out
+    with _on_device(q):
+        need = lib.sc_attention_shared_workspace_bytes(N, R, H, Hkv, D, width * bs, pw * bs, max_new)
+        ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        if ws_bytes < need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+            ws_bytes = need
+        rc = lib.sc_attention_shared_bf16(_ptr(q), q.stride(0) if N > 1 else H * D, _ptr(k_blocks), _ptr(vt_blocks), nb,
+                                          bs, _ptr(row_starts), _ptr(lengths), _ptr(tables), width,
+                                          _ptr(prefix_table) if pw else None, pw, _ptr(prefix_len) if pw else None,
+                                          _ptr(out), out.stride(0) if N > 1 else H * D, N, R, H, Hkv, D, float(scale),
+                                          int(max_new), _ptr(workspace), ws_bytes, _stream(q))
+    if rc:
+        _check(rc, "sc_attention_shared_bf16")
+    return out

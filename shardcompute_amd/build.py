@@ -19,7 +19,8 @@ BUILD_DIR = os.path.join(PKG, "_build")
 LIB_PATH = os.path.join(PKG, "libshardcompute_hip.so")
 ARCH = os.environ.get("SC_OFFLOAD_ARCH", "gfx950")
 
-SOURCES = ["abi.hip", "qgemv_dma.hip", "qgemv_m1.hip", "qgemv16.hip", "qgemv.hip", "qgemm.hip", "qgemm_dense.hip", "qgemm_mid.hip", "qgemm_band.hip", "gather.hip", "quant.hip", "decode.hip", "attn_prefill.hip", "decode_step.hip", "act.hip"]
+SOURCES = ["abi.hip", "qgemv_dma.hip", "qgemv_m1.hip", "qgemv16.hip", "qgemv.hip", "qgemm.hip", "qgemm_dense.hip", "qgemm_mid.hip", "qgemm_band.hip", "gather.hip", "quant.hip", "decode.hip", "attn_prefill.hip", "decode_step.hip", "act.hip", "blocks.hip",
+           "attn_shared.hip"]
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",
@@ -33,11 +34,12 @@ HIPCC_FLAGS = [
     "-I", os.path.join(ROOT, "include"),
 ]
 
-# per-source additions: the prefill attention kernel keeps its MFMA accumulators in
-# VGPRs (it rescales them in place every few blocks; in AGPRs each block would copy
+# per-source additions: the prefill attention kernels keep their MFMA accumulators in
+# VGPRs (they rescale them in place every few blocks; in AGPRs each block would copy
 # them to VGPRs and back)
 EXTRA_FLAGS = {
     "attn_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "attn_shared.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -64,6 +64,21 @@ int launch_attention(const uint16_t *q, long q_stride, const uint16_t *kc, const
                      const int32_t *cache_len, uint16_t *out, long out_stride, long B, long S, long H, long Hkv,
                      long D, float scale, void *workspace, long workspace_bytes, hipStream_t stream,
                      const float *mask, const long *mask_strides);
+int launch_block_tables(const int32_t *lengths, const int32_t *fresh, const uint8_t *release, int32_t *tables,
+                        int32_t *free_blocks, const int32_t *n_free, const int32_t *prefix_len, long R, long width,
+                        long bs, long cap, long rows, int32_t *lengths_out, int32_t *n_free_out, int32_t *row_starts,
+                        int32_t *slots, int32_t *positions, int32_t *status, hipStream_t stream);
+int launch_rope_append_blocks(const uint16_t *qkv, long qkv_stride, uint16_t *q, long q_stride, long N, long H,
+                              long Hkv, long D, const float *cos_t, const float *sin_t, long table_len, uint16_t *kc,
+                              uint16_t *vt, long n_blocks, long bs, const int32_t *slots, const int32_t *positions,
+                              hipStream_t stream);
+long attention_shared_workspace_bytes(long N, long R, long H, long Hkv, long D, long own_cap, long prefix_cap,
+                                      long max_new);
+int launch_attention_shared(const uint16_t *q, long q_stride, const uint16_t *kc, const uint16_t *vt, long n_blocks,
+                            long bs, const int32_t *row_starts, const int32_t *lengths, const int32_t *tables,
+                            long width, const int32_t *prefix_table, long prefix_width, const int32_t *prefix_len,
+                            uint16_t *out, long out_stride, long N, long R, long H, long Hkv, long D, float scale,
+                            long max_new, void *workspace, long workspace_bytes, hipStream_t stream);
 int launch_argmax(const uint16_t *logits, long rows, long V, int32_t *ids, int32_t *tokens, long tok_stride,
                   long tok_cols, const int32_t *step, hipStream_t stream);
 int launch_add_bf16(const uint16_t *a, const uint16_t *b, uint16_t *out, long n, hipStream_t stream);
@@ -455,6 +470,42 @@ int sc_rope_append_kv_bf16(uint16_t *qkv, int64_t qkv_stride, int64_t B, int64_t
                            void *hip_stream) {
     return launch_rope_append(qkv, qkv_stride, B, S, H, Hkv, D, cos_t, sin_t, table_len, k_cache, v_cache_t, T_cap,
                               cache_len, pos_offset, reinterpret_cast<hipStream_t>(hip_stream));
+}
+
+int sc_block_tables_i32(const int32_t *lengths, const int32_t *new_positions, const uint8_t *release_or_null,
+                        int32_t *tables, int32_t *free_blocks, const int32_t *n_free,
+                        const int32_t *prefix_len_or_null, int64_t R, int64_t width, int64_t block_size, int64_t cap,
+                        int64_t rows, int32_t *lengths_out, int32_t *n_free_out, int32_t *row_starts, int32_t *slots,
+                        int32_t *positions, int32_t *status, void *hip_stream) {
+    return launch_block_tables(lengths, new_positions, release_or_null, tables, free_blocks, n_free,
+                               prefix_len_or_null, R, width, block_size, cap, rows, lengths_out, n_free_out, row_starts,
+                               slots, positions, status, reinterpret_cast<hipStream_t>(hip_stream));
+}
+
+int sc_rope_append_blocks_bf16(const uint16_t *qkv, int64_t qkv_stride, uint16_t *q_out, int64_t q_stride, int64_t N,
+                               int64_t H, int64_t Hkv, int64_t D, const float *cos_t, const float *sin_t,
+                               int64_t table_len, uint16_t *k_blocks, uint16_t *vt_blocks, int64_t n_blocks,
+                               int64_t block_size, const int32_t *slots, const int32_t *positions, void *hip_stream) {
+    return launch_rope_append_blocks(qkv, qkv_stride, q_out, q_stride, N, H, Hkv, D, cos_t, sin_t, table_len, k_blocks,
+                                     vt_blocks, n_blocks, block_size, slots, positions,
+                                     reinterpret_cast<hipStream_t>(hip_stream));
+}
+
+int64_t sc_attention_shared_workspace_bytes(int64_t N, int64_t R, int64_t H, int64_t Hkv, int64_t D, int64_t own_cap,
+                                            int64_t prefix_cap, int64_t max_new) {
+    return attention_shared_workspace_bytes(N, R, H, Hkv, D, own_cap, prefix_cap, max_new);
+}
+
+int sc_attention_shared_bf16(const uint16_t *q, int64_t q_stride, const uint16_t *k_blocks, const uint16_t *vt_blocks,
+                             int64_t n_blocks, int64_t block_size, const int32_t *row_starts, const int32_t *lengths,
+                             const int32_t *tables, int64_t width, const int32_t *prefix_table, int64_t prefix_width,
+                             const int32_t *prefix_len, uint16_t *out, int64_t out_stride, int64_t N, int64_t R,
+                             int64_t H, int64_t Hkv, int64_t D, float scale, int64_t max_new, void *workspace,
+                             int64_t workspace_bytes, void *hip_stream) {
+    return launch_attention_shared(q, q_stride, k_blocks, vt_blocks, n_blocks, block_size, row_starts, lengths, tables,
+                                   width, prefix_table, prefix_width, prefix_len, out, out_stride, N, R, H, Hkv, D,
+                                   scale, max_new, workspace, workspace_bytes,
+                                   reinterpret_cast<hipStream_t>(hip_stream));
 }
 
 int64_t sc_attention_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t T_cap) {

@@ -1,0 +1,840 @@
+// Attention over a key/value cache in blocks, for a ragged batch whose sequences share
+// one prefix: row i of sequence r attends the prefix's P positions and its sequence's own
+// positions up to its own,
+//   out = softmax(scale q k^T) v   over prefix[0, P) + own_r[0, lengths[r] - new_r + i].
+//
+// The prefix is one set of keys for every row, so its part is a product of all the
+// batch's rows at once (128 "columns" = (row, q head of the kv head) a workgroup, matrix
+// instructions, keys through LDS); read once for all instead of once per sequence.  A
+// sequence's own keys serve its rows alone: few rows (a decoded token, a few guessed ones)
+// make it a stream of memory, many rows (a prompt) a product again.  So:
+//   attn_tile_kernel   128 columns: the prefix, then the own keys of sequences with many
+//                      rows; over several workgroups where there are few
+//   attn_own_kernel    16 columns: the own keys of sequences with few rows (and the prefix
+//                      where all the rows are few), the work cut evenly over the
+//                      workgroups whatever the lengths are
+//   attn_merge_kernel  joins the parts of a row by their softmax maxima and sums
+// Parts are fp32 (O unnormalised, maximum in log2 units, sum).
+//
+// Pool layout as in blocks.hip: K [n_blocks, Hkv, bs, D], Vt [n_blocks, Hkv, D, bs].
+// Block numbers outside the pool are clamped into it; lengths to the tables' width and
+// row starts to the rows, so nothing outside the buffers is touched whatever they hold.
+#include "sc_common.h"
+#include "dma_util.h"
+
+#include <math.h>
+#include <type_traits>
+
+namespace sc {
+
+int block_shift(long bs);       // blocks.hip
+
+namespace {
+
+using f4 = dma::f4;
+
+constexpr int SA_COLS = 128, SA_KB = 64, SA_THREADS = 256;
+constexpr int SO_WAVES = 4, SO_KB = 32, SO_TILE = SO_WAVES * SO_KB;      // keys a workgroup takes at a time
+constexpr int SA_MAX_SEQ = 2048;         // attn_own_kernel keeps two numbers of each in LDS
+
+struct SaArgs {
+    const uint16_t *q;
+    long q_stride;
+    const uint16_t *kc, *vt;
+    uint16_t *out;
+    long out_stride;
+    const int32_t *row_starts, *lengths, *tables, *prefix_table, *prefix_len;
+    int N, R, H, Hkv, G, width, shift, n_blocks, prefix_width;
+    int small_rows;          // a sequence of at most this many rows is attn_own_kernel's
+    int any_big;             // some sequence may have more
+    int nsplit;              // workgroups a column tile's keys are cut into
+    int own_prefix;          // the prefix is attn_own_kernel's
+    int own_wgs;             // attn_own_kernel's workgroups
+    float scale_log2;
+    // parts: of attn_tile_kernel [nsplit][N * H] rows, of attn_own_kernel [own_parts][16] columns
+    float *tile_o;
+    float2 *tile_ml;
+    float *own_o;
+    float2 *own_ml;
+    int own_parts;
+    int32_t *own_off, *own_unit;         // [R + 2]: first key tile and first unit of a sequence
+};
+
+__device__ __forceinline__ int clampi(int v, int lo, int hi) { return min(max(v, lo), hi); }
+
+// rows of the batch that are there
+__device__ __forceinline__ int live_rows(const SaArgs &a) { return clampi(a.row_starts[a.R], 0, a.N); }
+
+struct Seq {
+    int first, n, len;       // first row, rows, keys (its rows' own included)
+};
+__device__ __forceinline__ Seq seq_of(const SaArgs &a, int r, int rows) {
+    Seq s;
+    s.first = clampi(a.row_starts[r], 0, rows);
+    s.n = max(clampi(a.row_starts[r + 1], 0, rows) - s.first, 0);
+    s.len = clampi(a.lengths[r], 0, a.width << a.shift);
+    return s;
+}
+__device__ __forceinline__ int prefix_keys(const SaArgs &a) {
+    return a.prefix_width ? clampi(a.prefix_len[0], 0, a.prefix_width << a.shift) : 0;
+}
+
+// the sequence a row belongs to: the last r with row_starts[r] <= row, the 64 lanes
+// looking at 64 candidates a step
+__device__ __forceinline__ int find_seq(const SaArgs &a, int row) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = a.R;
+    while (n > 1) {
+        const int step = (n + 63) >> 6, i = lo + lane * step;
+        const bool le = lane * step < n && a.row_starts[i] <= row;
+        const int c = max(__popcll(__ballot(le)), 1);
+        const int cut = (c - 1) * step;
+        lo += cut;
+        n = min(step, n - cut);
+    }
+    return lo;
+}
+
+// ---------------------------------------------------------------- 128 columns
+//
+// As the dense prefill attention: 4 waves, wave w the columns [32 w, 32 w + 32), S^T[64 keys
+// x 32] = K Q^T and O^T[D x 32] += Vt P^T on v_mfma_f32_32x32x16_bf16, keys swapped on their
+// way into S^T (bits 2 and 3) so that the probabilities are operand B in registers, K and
+// Vt by LDS-DMA one block of 64 keys ahead into a 2-stage ring, chunks XOR-swizzled by row.
+// A key block takes its four 16-key groups from up to four cache blocks (block sizes below
+// 64) or one.
+template <int D>
+struct SaGeo {
+    static constexpr int KROW = D * 2;
+    static constexpr int KTILE = SA_KB * KROW, VTILE = D * SA_KB * 2;
+    static constexpr int STAGE = KTILE + VTILE;
+    static constexpr int LDS = 2 * STAGE;
+    static constexpr int KSTEPS = D / 16;
+    static constexpr int DB = D / 32;
+    static constexpr int DMA = KTILE / 1024 / 4;
+};
+
+__device__ __forceinline__ int sa_swap23(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }
+template <int D>
+__device__ __forceinline__ uint32_t sa_kswz(int r, int c) {
+    const int p = D == 128 ? c ^ (sa_swap23(r) & 15) : c ^ ((r >> 1) & 7);
+    return (uint32_t)(r * (D * 2) + (p << 4));
+}
+__device__ __forceinline__ uint32_t sa_vswz(int d, int c) { return (uint32_t)(d * 128 + ((c ^ ((d >> 1) & 7)) << 4)); }
+
+// any bf16 of 8 is inf or NaN
+__device__ __forceinline__ bool nonfinite8(uint4 v) {
+    auto bad = [](uint32_t x) { return (x & 0x7F80u) == 0x7F80u || (x & 0x7F800000u) == 0x7F800000u; };
+    return bad(v.x) || bad(v.y) || bad(v.z) || bad(v.w);
+}
+
+// word masks of 8 consecutive keys k0 .. k0 + 7, of which those below end are kept
+__device__ __forceinline__ uint4 keep_below(int k0, int end) {
+    uint4 m;
+    m.x = (k0 + 0 < end ? 0xFFFFu : 0u) | (k0 + 1 < end ? 0xFFFF0000u : 0u);
+    m.y = (k0 + 2 < end ? 0xFFFFu : 0u) | (k0 + 3 < end ? 0xFFFF0000u : 0u);
+    m.z = (k0 + 4 < end ? 0xFFFFu : 0u) | (k0 + 5 < end ? 0xFFFF0000u : 0u);
+    m.w = (k0 + 6 < end ? 0xFFFFu : 0u) | (k0 + 7 < end ? 0xFFFF0000u : 0u);
+    return m;
+}
+// key e of 8 alone
+__device__ __forceinline__ uint4 keep_one(int e, bool on) {
+    const uint32_t h = on ? ((e & 1) ? 0xFFFF0000u : 0xFFFFu) : 0u;
+    const int w = e >> 1;
+    return make_uint4(w == 0 ? h : 0u, w == 1 ? h : 0u, w == 2 ? h : 0u, w == 3 ? h : 0u);
+}
+__device__ __forceinline__ uint4 and4(uint4 v, uint4 m) { return make_uint4(v.x & m.x, v.y & m.y, v.z & m.z, v.w & m.w); }
+
+template <int D>
+__global__ void __launch_bounds__(SA_THREADS) attn_tile_kernel(SaArgs a) {
+    using Gm = SaGeo<D>;
+    extern __shared__ __align__(16) uint8_t smem[];
+    static_assert(Gm::LDS <= 65536, "no larger dynamic LDS is asked for at the launch");
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int li = lane & 31, lh = lane >> 5;
+    int id = (int)blockIdx.x;
+    const int hk = id % a.Hkv;
+    id /= a.Hkv;
+    const int split = id % a.nsplit, tile = id / a.nsplit;
+    const int rows = live_rows(a);
+    const int col = tile * SA_COLS + 32 * w + li;
+    const int row = col / a.G, h = hk * a.G + col - row * a.G;
+    const int row0 = tile * SA_COLS / a.G, row1 = min((tile * SA_COLS + SA_COLS - 1) / a.G, rows - 1);
+    if (row0 >= rows) return;
+    const bool col_ok = row < rows;
+    const int P = a.own_prefix ? 0 : prefix_keys(a);
+    const int sh = a.shift, bs = 1 << sh;
+
+    // the column tile's keys: the prefix, then the own keys of its sequences with many
+    // rows; this workgroup takes key blocks [t0, t1) of them
+    auto own_blocks = [&](const Seq &s) {
+        if (s.n <= a.small_rows) return 0;
+        return (clampi(s.len - s.n + row1 - s.first + 1, 0, s.len) + SA_KB - 1) / SA_KB;
+    };
+    const int r0 = a.any_big ? find_seq(a, row0) : 0;
+    int total = (P + SA_KB - 1) / SA_KB;
+    bool big = false;                                   // this column's own keys are taken here
+    if (a.any_big)
+        for (int r = r0; r < a.R; ++r) {
+            const Seq s = seq_of(a, r, rows);
+            if (s.first > row1) break;
+            if (s.n > a.small_rows && row >= s.first && row < s.first + s.n) big = true;
+            total += own_blocks(s);
+        }
+    const int t0 = (int)((long)total * split / a.nsplit), t1 = (int)((long)total * (split + 1) / a.nsplit);
+
+    bf16x8_t qv[Gm::KSTEPS];
+#pragma unroll
+    for (int ks = 0; ks < Gm::KSTEPS; ++ks) {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (col_ok) v = *reinterpret_cast<const uint4 *>(a.q + (size_t)row * a.q_stride + (size_t)h * D + 16 * ks + 8 * lh);
+        qv[ks] = as_bf16x8(v);
+    }
+    f32x16_t o[Gm::DB];
+#pragma unroll
+    for (int db = 0; db < Gm::DB; ++db) o[db] = f32x16_t{};
+    float m = -INFINITY, lsum = 0.f;
+    const float sc = a.scale_log2;
+    const int arow = sa_swap23(li);
+    const size_t blk_elems = (size_t)a.Hkv * D << sh;
+    const uint16_t *kbase = a.kc + ((size_t)hk * D << sh), *vbase = a.vt + ((size_t)hk * D << sh);
+
+    // key blocks [b0, b1) of one table with `end` keys; the column sees keys <= limit
+    auto segment = [&](const int32_t *table, int width, int end, int b0, int b1, int limit) {
+        if (b0 >= b1) return;
+        // the cache blocks of a key block's four 16-key groups: lane l loads group l % 4's
+        // number, one key block before its copies are issued
+        auto load_ids = [&](int kb) { return table[min((kb + 16 * (lane & 3)) >> sh, width - 1)]; };
+        auto stage_blk = [&](int kb, int st, int ids) {
+            ids = clampi(ids, 0, a.n_blocks - 1);
+            const int i0 = __builtin_amdgcn_readlane(ids, 0), i1 = __builtin_amdgcn_readlane(ids, 1);
+            const int i2 = __builtin_amdgcn_readlane(ids, 2), i3 = __builtin_amdgcn_readlane(ids, 3);
+            auto pick = [&](int g) { return g < 2 ? (g == 0 ? i0 : i1) : (g == 2 ? i2 : i3); };
+            const uint32_t kl = (uint32_t)(uintptr_t)(smem + st * Gm::STAGE);
+            const uint32_t vl = kl + Gm::KTILE;
+#pragma unroll
+            for (int qq = 0; qq < Gm::DMA; ++qq) {
+                const int qi = Gm::DMA * w + qq;
+                const int r = D == 128 ? 4 * qi + (lane >> 4) : 8 * qi + (lane >> 3);
+                const int c = D == 128 ? (lane & 15) ^ (sa_swap23(r) & 15) : (lane & 7) ^ ((r >> 1) & 7);
+                dma::dma16(kbase + (size_t)pick(r >> 4) * blk_elems + (size_t)((kb + r) & (bs - 1)) * D + 8 * c,
+                           kl + 1024 * qi);
+            }
+#pragma unroll
+            for (int qq = 0; qq < Gm::DMA; ++qq) {
+                const int qi = Gm::DMA * w + qq;
+                const int d = 8 * qi + (lane >> 3);
+                const int c = (lane & 7) ^ ((d >> 1) & 7);
+                dma::dma16(vbase + (size_t)pick(c >> 1) * blk_elems + ((size_t)d << sh) + ((kb + 8 * c) & (bs - 1)),
+                           vl + 1024 * qi);
+            }
+        };
+        // of the wave's columns: the fewest and the most keys one of them sees
+        int lo = limit, hi = limit;
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) {
+            lo = min(lo, __shfl_xor(lo, x));
+            hi = max(hi, __shfl_xor(hi, x));
+        }
+        auto block = [&](int blk, int ids_next, auto mask_tag) {
+            constexpr bool MASK = decltype(mask_tag)::value;
+            const int kb = blk * SA_KB, st = (blk - b0) & 1;
+            const uint8_t *K = smem + st * Gm::STAGE;
+            const uint8_t *V = K + Gm::KTILE;
+            if (blk + 1 < b1) stage_blk(kb + SA_KB, st ^ 1, ids_next);
+            if (MASK && kb > hi) return;                 // nothing of it is seen by the wave
+            f32x16_t sacc[2] = {f32x16_t{}, f32x16_t{}};
+#pragma unroll
+            for (int ks = 0; ks < Gm::KSTEPS; ++ks)
+#pragma unroll
+                for (int kh = 0; kh < 2; ++kh) {
+                    const bf16x8_t ka = as_bf16x8(*reinterpret_cast<const uint4 *>(K + sa_kswz<D>(32 * kh + arow, 2 * ks + lh)));
+                    sacc[kh] = mfma32x32x16(ka, qv[ks], sacc[kh]);
+                }
+            if (MASK) {
+                const int rel = limit - kb - 8 * lh;
+#pragma unroll
+                for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (32 * kh + 16 * (r >> 3) + (r & 7) > rel) sacc[kh][r] = -INFINITY;
+            }
+            float bm = -INFINITY;
+#pragma unroll
+            for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) bm = fmaxf(bm, sacc[kh][r]);
+            bm = fmaxf(bm, __shfl_xor(bm, 32));
+            float alpha = 1.f;
+            if (bm > m) {
+                alpha = __builtin_amdgcn_exp2f((m - bm) * sc);
+                m = bm;
+            }
+            const float nms = -m * sc;
+            float ps = 0.f;
+#pragma unroll
+            for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float p = __builtin_amdgcn_exp2f(fmaf(sacc[kh][r], sc, nms));
+                    // a column that has seen no key yet has m = -inf: 0, not NaN
+                    if (MASK && sacc[kh][r] == -INFINITY) p = 0.f;
+                    sacc[kh][r] = p;
+                    ps += p;
+                }
+            lsum = lsum * alpha + ps;
+            if (__ballot(alpha != 1.f) != 0ull) {
+#pragma unroll
+                for (int db = 0; db < Gm::DB; ++db)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
+            }
+            // keys at or past `end` may hold anything: their V is dropped.  Keys of the
+            // sequence that only some of the columns see (a later row's, or another
+            // sequence's keys) meet zero probabilities, which an inf or NaN would turn into
+            // NaN: where there is one, key by key, each column taking the keys it sees
+            bool bad = false;
+            if (MASK) {
+#pragma unroll
+                for (int s4 = 0; s4 < 4; ++s4) {
+                    const int c = 2 * s4 + lh;
+                    const uint4 mk = keep_below(kb + 8 * c, end);
+#pragma unroll
+                    for (int db = 0; db < Gm::DB; ++db)
+                        bad = bad || nonfinite8(and4(*reinterpret_cast<const uint4 *>(V + sa_vswz(32 * db + li, c)), mk));
+                }
+                bad = __ballot(bad) != 0ull;
+            }
+#pragma unroll
+            for (int s4 = 0; s4 < 4; ++s4) {
+                const int kh = s4 >> 1, q0 = 8 * (s4 & 1), c = 2 * s4 + lh;
+                const uint4 pw = make_uint4(cvt_pk_bf16(sacc[kh][q0], sacc[kh][q0 + 1]),
+                                            cvt_pk_bf16(sacc[kh][q0 + 2], sacc[kh][q0 + 3]),
+                                            cvt_pk_bf16(sacc[kh][q0 + 4], sacc[kh][q0 + 5]),
+                                            cvt_pk_bf16(sacc[kh][q0 + 6], sacc[kh][q0 + 7]));
+                if (MASK && bad) {
+                    for (int j = 0; j < 16; ++j) {
+                        const uint4 one = keep_one(j & 7, (j >> 3) == lh);
+                        const bool sees = kb + 16 * s4 + j <= limit;
+#pragma unroll
+                        for (int db = 0; db < Gm::DB; ++db) {
+                            const uint4 v = and4(*reinterpret_cast<const uint4 *>(V + sa_vswz(32 * db + li, c)), one);
+                            const f32x16_t t = mfma32x32x16(as_bf16x8(v), as_bf16x8(and4(pw, one)), o[db]);
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) o[db][r] = sees ? t[r] : o[db][r];
+                        }
+                    }
+                    continue;
+                }
+                uint4 mk = make_uint4(~0u, ~0u, ~0u, ~0u);
+                if (MASK) mk = keep_below(kb + 8 * c, end);
+#pragma unroll
+                for (int db = 0; db < Gm::DB; ++db) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(V + sa_vswz(32 * db + li, c));
+                    o[db] = mfma32x32x16(as_bf16x8(MASK ? and4(v, mk) : v), as_bf16x8(pw), o[db]);
+                }
+            }
+        };
+        int ids = load_ids(b0 * SA_KB), next = load_ids((b0 + 1) * SA_KB);
+        stage_blk(b0 * SA_KB, 0, ids);
+        dma::wait_vm<0>();
+        __syncthreads();
+        for (int blk = b0; blk < b1; ++blk) {
+            const int after = load_ids((blk + 2) * SA_KB);
+            if (blk * SA_KB + SA_KB - 1 <= lo) block(blk, next, std::false_type{});
+            else block(blk, next, std::true_type{});
+            next = after;
+            dma::wait_vm<0>();
+            __syncthreads();
+        }
+    };
+
+    // q's loads end here: a wait at their first use, in the loop, would also wait for the
+    // copies in flight, which the compiler does not see
+#pragma unroll
+    for (int ks = 0; ks < Gm::KSTEPS; ++ks) asm volatile("" ::"v"(qv[ks]));
+    const int pb = (P + SA_KB - 1) / SA_KB;
+    segment(a.prefix_table, a.prefix_width, P, min(t0, pb), min(t1, pb), P - 1);
+    if (a.any_big) {
+        int at = pb;
+        for (int r = r0; r < a.R && at < t1; ++r) {
+            const Seq s = seq_of(a, r, rows);
+            if (s.first > row1) break;
+            const int nb = own_blocks(s);
+            const int limit = col_ok && row >= s.first && row < s.first + s.n ? s.len - s.n + row - s.first : -1;
+            segment(a.tables + (size_t)r * a.width, a.width, s.len, clampi(t0 - at, 0, nb), clampi(t1 - at, 0, nb), limit);
+            at += nb;
+        }
+    }
+
+    const float ltot = lsum + __shfl_xor(lsum, 32);
+    if (!col_ok) return;
+    if (big && a.nsplit == 1) {
+        const float inv = ltot == 0.f ? 0.f : 1.f / ltot;      // (a row without a key: 0)
+        uint16_t *orow = a.out + (size_t)row * a.out_stride + (size_t)h * D;
+#pragma unroll
+        for (int db = 0; db < Gm::DB; ++db)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4)
+                *reinterpret_cast<uint2 *>(orow + 32 * db + 8 * r4 + 4 * lh) =
+                    make_uint2(cvt_pk_bf16(o[db][4 * r4] * inv, o[db][4 * r4 + 1] * inv),
+                               cvt_pk_bf16(o[db][4 * r4 + 2] * inv, o[db][4 * r4 + 3] * inv));
+        return;
+    }
+    const size_t part = (size_t)split * a.N * a.H + (size_t)row * a.H + h;
+    float *po = a.tile_o + part * D;
+#pragma unroll
+    for (int db = 0; db < Gm::DB; ++db)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4)
+            *reinterpret_cast<float4 *>(po + 32 * db + 8 * r4 + 4 * lh) =
+                make_float4(o[db][4 * r4], o[db][4 * r4 + 1], o[db][4 * r4 + 2], o[db][4 * r4 + 3]);
+    if (lh == 0) a.tile_ml[part] = make_float2(m * sc, ltot);
+}
+
+// ---------------------------------------------------------------- 16 columns
+//
+// A unit is 16 columns (row i, q head g: column i G + g) of one sequence and kv head; its
+// keys are tiles of 128.  All units' tiles in a line (sequence, kv head, 16 columns, key
+// tile) are cut into own_wgs equal runs, one a workgroup, whatever the lengths are; a
+// run's share of a unit is one part, number unit + workgroup (two consecutive runs meet
+// in one unit at most, so the numbers differ).  "Sequence" R is the prefix, with all rows.
+template <typename F>
+__device__ __forceinline__ void own_shape(const SaArgs &a, int r, int rows, int P, F &&f) {
+    // f(first row, rows, keys)
+    if (r < a.R) {
+        const Seq s = seq_of(a, r, rows);
+        f(s.first, s.n <= a.small_rows ? s.n : 0, s.len);
+    } else {
+        f(0, a.own_prefix ? rows : 0, P);
+    }
+}
+__device__ __forceinline__ int own_coltiles(const SaArgs &a, int n) { return (n * a.G + 15) >> 4; }
+__device__ __forceinline__ int own_keytiles(int len) { return (len + SO_TILE - 1) / SO_TILE; }
+// tiles a workgroup takes of `total`
+__device__ __forceinline__ int own_run(const SaArgs &a, int total) { return max((total + a.own_wgs - 1) / a.own_wgs, 1); }
+
+template <int D>
+struct OwnBlock {
+    uint4 k[2][D / 32];
+    uint4 v[D / 16];
+};
+
+template <int D>
+__global__ void __launch_bounds__(64 * SO_WAVES) attn_own_kernel(SaArgs a) {
+    constexpr int U = D / 32, DT = D / 16;
+    extern __shared__ int32_t seq_lds[];                 // off[R + 2], unit[R + 2]
+    __shared__ float sm_m[SO_WAVES][16], sm_l[SO_WAVES][16];
+    __shared__ float sm_o[SO_WAVES][D][17];
+    __shared__ int wsum[2][SO_WAVES];
+    int32_t *off = seq_lds, *unit = seq_lds + a.R + 2;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int c = lane & 15, g = lane >> 4;
+    const int rows = live_rows(a), P = prefix_keys(a);
+    const int sh = a.shift, bs = 1 << sh;
+
+    // first tile and unit of every sequence
+    {
+        int t_before = 0, u_before = 0;
+        for (int r0 = 0; r0 <= a.R; r0 += 64 * SO_WAVES) {
+            const int r = r0 + tid;
+            int t = 0, u = 0;
+            if (r <= a.R)
+                own_shape(a, r, rows, P, [&](int, int n, int len) {
+                    const int kt = own_keytiles(len);
+                    u = kt ? a.Hkv * own_coltiles(a, n) : 0;
+                    t = u * kt;
+                });
+            int ts = t, us = u;
+#pragma unroll
+            for (int x = 1; x < 64; x <<= 1) {
+                const int t2 = __shfl_up(ts, x), u2 = __shfl_up(us, x);
+                if (lane >= x) { ts += t2; us += u2; }
+            }
+            if (lane == 63) { wsum[0][w] = ts; wsum[1][w] = us; }
+            __syncthreads();
+            int tb = t_before, ub = u_before;
+            for (int i = 0; i < SO_WAVES; ++i) {
+                if (i < w) { tb += wsum[0][i]; ub += wsum[1][i]; }
+                t_before += wsum[0][i];
+                u_before += wsum[1][i];
+            }
+            if (r <= a.R) { off[r] = tb + ts - t; unit[r] = ub + us - u; }
+            __syncthreads();
+        }
+        if (tid == 0) { off[a.R + 1] = t_before; unit[a.R + 1] = u_before; }
+        __syncthreads();
+        if (blockIdx.x == 0)
+            for (int r = tid; r < a.R + 2; r += 64 * SO_WAVES) { a.own_off[r] = off[r]; a.own_unit[r] = unit[r]; }
+    }
+    const int total = off[a.R + 1], run = own_run(a, total);
+    int t = (int)min((long)blockIdx.x * run, (long)total);
+    const int t_end = min(t + run, total);
+    int r = 0;
+    if (t < t_end) {
+        int n = a.R + 1;
+        while (n > 1) {
+            const int half = n >> 1;
+            if (off[r + half] <= t) { r += half; n -= half; }
+            else n = half;
+        }
+    }
+    for (; t < t_end;) {
+        while (off[r + 1] <= t) ++r;
+        int first = 0, n = 0, len = 0;
+        own_shape(a, r, rows, P, [&](int f, int nn, int l) { first = f; n = nn; len = l; });
+        const int kt = own_keytiles(len), ct = own_coltiles(a, n);
+        const int lt = t - off[r], u = lt / kt, tile0 = lt - u * kt, tile1 = min(kt, tile0 + t_end - t);
+        const int hk = u / ct, cols0 = (u - hk * ct) * 16;
+        const bool pre = r == a.R;
+        const int32_t *table = pre ? a.prefix_table : a.tables + (size_t)r * a.width;
+        const int width = pre ? a.prefix_width : a.width;
+        const int part = unit[r] + u + (int)blockIdx.x;
+        t += tile1 - tile0;
+
+        const int i = (cols0 + c) / a.G, gq = cols0 + c - i * a.G;
+        const bool col_ok = i < n;
+        const int row = first + i, h = hk * a.G + gq;
+        const int last = min((cols0 + 15) / a.G, n - 1);              // the last row of the unit
+        const int limit = !col_ok ? -1 : pre ? P - 1 : len - n + i;
+        const int seen = pre ? P : clampi(len - n + last + 1, 0, len);         // keys some column sees
+        const int all = pre ? P : clampi(len - n + cols0 / a.G + 1, 0, len);   // keys every column sees
+        bf16x8_t qv[U];
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (col_ok) v = *reinterpret_cast<const uint4 *>(a.q + (size_t)row * a.q_stride + (size_t)h * D + 32 * x + 8 * g);
+            qv[x] = as_bf16x8(v);
+        }
+        const size_t blk_elems = (size_t)a.Hkv * D << sh;
+        const uint16_t *kbase = a.kc + ((size_t)hk * D << sh), *vbase = a.vt + ((size_t)hk * D << sh);
+        float m = -INFINITY, lsum = 0.f;
+        f4 o[DT];
+#pragma unroll
+        for (int x = 0; x < DT; ++x) o[x] = f4{0.f, 0.f, 0.f, 0.f};
+
+        const int k_end = min(tile1 * SO_TILE, seen);
+        struct Ids { int k, v; };
+        // the cache blocks of this lane's keys (two 16-key groups a block of 32)
+        auto load_ids = [&](int kb) {
+            kb = min(kb, max(k_end - 1, 0));
+            Ids x;
+            x.k = table[min((kb + 16 * (c >> 3)) >> sh, width - 1)];
+            x.v = table[min((kb + 16 * (g >> 1)) >> sh, width - 1)];
+            return x;
+        };
+        auto load = [&](OwnBlock<D> &b, int kb, Ids x) {
+            const uint16_t *kp = kbase + (size_t)clampi(x.k, 0, a.n_blocks - 1) * blk_elems;
+            const int k0 = kb + 8 * (c >> 2) + (c & 3);
+            const uint16_t *ka = kp + (size_t)(k0 & (bs - 1)) * D + 8 * g, *kb4 = kp + (size_t)((k0 + 4) & (bs - 1)) * D + 8 * g;
+#pragma unroll
+            for (int y = 0; y < U; ++y) {
+                b.k[0][y] = *reinterpret_cast<const uint4 *>(ka + 32 * y);
+                b.k[1][y] = *reinterpret_cast<const uint4 *>(kb4 + 32 * y);
+            }
+            const uint16_t *vp = vbase + (size_t)clampi(x.v, 0, a.n_blocks - 1) * blk_elems + ((kb + 8 * g) & (bs - 1));
+#pragma unroll
+            for (int y = 0; y < DT; ++y) b.v[y] = *reinterpret_cast<const uint4 *>(vp + ((size_t)(16 * y + c) << sh));
+        };
+        auto compute = [&](const OwnBlock<D> &b, int kb) {
+            f4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int y = 0; y < U; ++y) {
+                s0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(b.k[0][y]), qv[y], s0, 0, 0, 0);
+                s1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(b.k[1][y]), qv[y], s1, 0, 0, 0);
+            }
+            float sv[8];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                sv[x] = kb + 8 * g + x <= limit ? s0[x] * a.scale_log2 : -INFINITY;
+                sv[4 + x] = kb + 8 * g + 4 + x <= limit ? s1[x] * a.scale_log2 : -INFINITY;
+            }
+            float bm = sv[0];
+#pragma unroll
+            for (int x = 1; x < 8; ++x) bm = fmaxf(bm, sv[x]);
+            bm = fmaxf(bm, __shfl_xor(bm, 16));
+            bm = fmaxf(bm, __shfl_xor(bm, 32));
+            const float mn = fmaxf(m, bm);
+            const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            float p[8], ps = 0.f;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                p[x] = sv[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sv[x] - mn);
+                ps += p[x];
+            }
+            lsum = lsum * alpha + ps;
+            m = mn;
+            const uint4 pw = make_uint4(cvt_pk_bf16(p[0], p[1]), cvt_pk_bf16(p[2], p[3]), cvt_pk_bf16(p[4], p[5]),
+                                        cvt_pk_bf16(p[6], p[7]));
+            const bool edge = kb + SO_KB > all;
+            uint4 mk = make_uint4(~0u, ~0u, ~0u, ~0u);
+            bool bad = false;
+            if (edge) {                                  // as in attn_tile_kernel
+                mk = keep_below(kb + 8 * g, seen);
+#pragma unroll
+                for (int y = 0; y < DT; ++y) bad = bad || nonfinite8(and4(b.v[y], mk));
+                bad = __ballot(bad) != 0ull;
+            }
+#pragma unroll
+            for (int y = 0; y < DT; ++y) {
+                f4 acc = o[y];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) acc[x] *= alpha;
+                if (!bad) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(and4(b.v[y], mk)), as_bf16x8(pw), acc, 0, 0, 0);
+                o[y] = acc;
+            }
+            if (bad)
+                for (int j = 0; j < 32; ++j) {
+                    const uint4 one = keep_one(j & 7, (j >> 3) == g);
+                    const bool sees = kb + j <= limit;
+#pragma unroll
+                    for (int y = 0; y < DT; ++y) {
+                        const f4 z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(and4(b.v[y], one)), as_bf16x8(and4(pw, one)),
+                                                                             o[y], 0, 0, 0);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) o[y][x] = sees ? z[x] : o[y][x];
+                    }
+                }
+        };
+        // 32-key blocks of the run, the four waves in turn; the next block's keys and the
+        // one's after it block numbers are on their way while one is computed
+        int kb = tile0 * SO_TILE + SO_KB * w;
+        if (kb < k_end) {
+            OwnBlock<D> cur, nxt;
+            Ids x = load_ids(kb), x1 = load_ids(kb + SO_TILE);
+            load(cur, kb, x);
+            while (true) {
+                const int kn = kb + SO_TILE;
+                x = load_ids(kn + SO_TILE);
+                load(nxt, kn < k_end ? kn : kb, x1);
+                compute(cur, kb);
+                if (kn >= k_end) break;
+                const int kn2 = kn + SO_TILE;
+                x1 = load_ids(kn2 + SO_TILE);
+                load(cur, kn2 < k_end ? kn2 : kn, x);
+                compute(nxt, kn);
+                if (kn2 >= k_end) break;
+                kb = kn2;
+            }
+        }
+        float ltot = lsum + __shfl_xor(lsum, 16);
+        ltot += __shfl_xor(ltot, 32);
+        if (g == 0) { sm_m[w][c] = m; sm_l[w][c] = ltot; }
+#pragma unroll
+        for (int y = 0; y < DT; ++y)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) sm_o[w][16 * y + 4 * g + x][c] = o[y][x];
+        __syncthreads();
+        const int cc = tid & 15, d0 = tid >> 4;
+        if (part < a.own_parts) {
+            float M = sm_m[0][cc];
+#pragma unroll
+            for (int x = 1; x < SO_WAVES; ++x) M = fmaxf(M, sm_m[x][cc]);
+            float wt[SO_WAVES], L = 0.f;
+#pragma unroll
+            for (int x = 0; x < SO_WAVES; ++x) {
+                wt[x] = sm_m[x][cc] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm_m[x][cc] - M);
+                L += wt[x] * sm_l[x][cc];
+            }
+            float *po = a.own_o + ((size_t)part * 16 + cc) * D;
+#pragma unroll
+            for (int y = 0; y < D / 16; ++y) {
+                float acc = 0.f;
+#pragma unroll
+                for (int x = 0; x < SO_WAVES; ++x) acc += wt[x] * sm_o[x][d0 + 16 * y][cc];
+                po[d0 + 16 * y] = acc;
+            }
+            if (d0 == 0) a.own_ml[(size_t)part * 16 + cc] = make_float2(M, L);
+        }
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------- merge
+//
+// One wave a row and q head: the parts of attn_tile_kernel (nsplit), then those of
+// attn_own_kernel for the row's sequence and for the prefix.  out = sum_i 2^(m_i - M) O_i /
+// sum_i 2^(m_i - M) l_i; parts of no key have m = -inf and weight 0, a row of no key at
+// all is 0.
+template <int D>
+__global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_parts) {
+    constexpr int PER = D / 64;
+    const long wid = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const int rows = live_rows(a);
+    if (wid >= (long)rows * a.H) return;
+    const int row = (int)(wid / a.H), h = (int)(wid - (long)row * a.H);
+    const int hk = h / a.G, gq = h - hk * a.G;
+    const int r = find_seq(a, row);
+    const Seq s = seq_of(a, r, rows);
+    if (s.n > a.small_rows && a.nsplit == 1) return;           // written by attn_tile_kernel
+    const int total = a.own_off[a.R + 1], run = own_run(a, total);
+    float M = -INFINITY, L = 0.f, acc[PER] = {};
+    // n parts: (m, l) of part i at ml[i * step], its values at o + i * step * D
+    auto take = [&](const float2 *ml, const float *o, long step, int n) {
+        for (int i0 = 0; i0 < n; i0 += 64) {
+            const int k = min(64, n - i0);
+            float2 x = make_float2(-INFINITY, 0.f);
+            if (lane < k) x = ml[(i0 + lane) * step];
+            float bm = x.x;
+#pragma unroll
+            for (int y = 32; y >= 1; y >>= 1) bm = fmaxf(bm, __shfl_xor(bm, y));
+            if (bm == -INFINITY) continue;
+            const float mn = fmaxf(M, bm), alpha = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mn);
+            const float wi = x.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x.x - mn);
+            M = mn;
+            L = L * alpha + wave_sum(wi * x.y);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) acc[e] *= alpha;
+            for (int i = 0; i < k; ++i) {
+                const float wk = __shfl(wi, i);
+                if (wk == 0.f) continue;
+                const float *po = o + (size_t)(i0 + i) * step * D;
+#pragma unroll
+                for (int e = 0; e < PER; ++e) acc[e] += wk * po[lane + 64 * e];
+            }
+        }
+    };
+    if (tile_parts) take(a.tile_ml + wid, a.tile_o + (size_t)wid * D, (long)a.N * a.H, tile_parts);
+    auto own = [&](int q, int n, int len, int i) {
+        const int kt = own_keytiles(len), ct = own_coltiles(a, n);
+        if (!kt) return;
+        const int col = i * a.G + gq, u = hk * ct + (col >> 4);
+        const int t0 = a.own_off[q] + u * kt, w0 = t0 / run, w1 = (t0 + kt - 1) / run;
+        const int part = a.own_unit[q] + u + w0;
+        if (part + w1 - w0 >= a.own_parts) return;
+        take(a.own_ml + (size_t)part * 16 + (col & 15), a.own_o + ((size_t)part * 16 + (col & 15)) * D, 16, w1 - w0 + 1);
+    };
+    if (s.n <= a.small_rows) own(r, s.n, s.len, row - s.first);
+    if (a.own_prefix) own(a.R, rows, prefix_keys(a), row);
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    uint16_t *po = a.out + (size_t)row * a.out_stride + (size_t)h * D;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) po[lane + 64 * e] = (uint16_t)f2bf(acc[e] * inv);
+}
+
+// ---------------------------------------------------------------- host side
+
+struct SaPlan {
+    int small_rows, any_big, nsplit, own_prefix, own_wgs, use_tile;
+    long tiles, own_parts;
+    long tile_o, tile_ml, own_o, own_ml, own_idx, bytes;       // workspace offsets
+};
+
+// own_cap, prefix_cap: positions the tables have room for; max_new: at least the rows of
+// the sequence with the most
+SaPlan plan_shared(long N, long R, long H, long Hkv, long D, long own_cap, long prefix_cap, long max_new) {
+    SaPlan p = {};
+    const long G = H / Hkv, cols = N * G, cus = device_info().num_cus;
+    if (max_new > N) max_new = N;
+    p.small_rows = (int)(64 / G > 1 ? 64 / G : 1);
+    p.any_big = max_new > p.small_rows;
+    p.own_prefix = prefix_cap > 0 && cols <= 32 && !p.any_big;
+    p.use_tile = p.any_big || (prefix_cap > 0 && !p.own_prefix);
+    p.tiles = (cols + SA_COLS - 1) / SA_COLS;
+    // attn_tile_kernel: two workgroups a CU
+    const long wgs = p.tiles * Hkv;
+    const long blocks = ((p.own_prefix ? 0 : prefix_cap) + (p.any_big ? own_cap : 0) + SA_KB - 1) / SA_KB;
+    long ns = wgs ? 2 * cus / wgs : 1;
+    if (ns > blocks / 2) ns = blocks / 2;
+    p.nsplit = (int)(ns < 1 ? 1 : ns > 64 ? 64 : ns);
+    // attn_own_kernel: at most R coltiles of the most rows a sequence has here, and no more
+    // than the rows make
+    const long rows_max = max_new < p.small_rows ? max_new : p.small_rows;
+    long coltiles = R * ((rows_max * G + 15) / 16);
+    if (coltiles > R + cols / 16) coltiles = R + cols / 16;
+    const long pre = p.own_prefix ? (cols + 15) / 16 : 0;
+    const long keytiles = coltiles * ((own_cap + SO_TILE - 1) / SO_TILE) + pre * ((prefix_cap + SO_TILE - 1) / SO_TILE);
+    long ow = 2 * cus;
+    if (ow > Hkv * keytiles) ow = Hkv * keytiles;
+    p.own_wgs = (int)(ow < 1 ? 1 : ow);
+    p.own_parts = Hkv * (coltiles + pre) + p.own_wgs;
+    auto up = [](long v) { return (v + 255) / 256 * 256; };
+    long at = 0;
+    const long tparts = p.use_tile ? p.nsplit * N * H : 0;
+    p.tile_o = at; at += up(tparts * D * 4);
+    p.tile_ml = at; at += up(tparts * 8);
+    p.own_o = at; at += up(p.own_parts * 16 * D * 4);
+    p.own_ml = at; at += up(p.own_parts * 16 * 8);
+    p.own_idx = at; at += up((R + 2) * 2 * 4);
+    p.bytes = at;
+    return p;
+}
+
+template <int D>
+int run_shared(const SaArgs &a, const SaPlan &p, hipStream_t stream) {
+    if (p.use_tile) {
+        hipLaunchKernelGGL(attn_tile_kernel<D>, dim3((unsigned)(p.tiles * p.nsplit * a.Hkv)), dim3(SA_THREADS),
+                           SaGeo<D>::LDS, stream, a);
+        SC_HIP_CHECK(hipGetLastError());
+    }
+    hipLaunchKernelGGL(attn_own_kernel<D>, dim3((unsigned)p.own_wgs), dim3(64 * SO_WAVES), (a.R + 2) * 8, stream, a);
+    SC_HIP_CHECK(hipGetLastError());
+    hipLaunchKernelGGL(attn_merge_kernel<D>, dim3((unsigned)(((long)a.N * a.H + 3) / 4)), dim3(256), 0, stream, a,
+                       p.use_tile ? p.nsplit : 0);
+    SC_HIP_CHECK(hipGetLastError());
+    return SC_OK;
+}
+
+bool bad_shape(long N, long R, long H, long Hkv, long D, long own_cap, long prefix_cap, long max_new) {
+    return N < 0 || N >= (1L << 24) || R <= 0 || R > SA_MAX_SEQ || H <= 0 || Hkv <= 0 || H % Hkv || H > 4096 ||
+           (D != 64 && D != 128) || own_cap <= 0 || own_cap >= (1L << 30) || prefix_cap < 0 || prefix_cap >= (1L << 30) ||
+           max_new < 0;
+}
+
+}  // namespace
+
+long attention_shared_workspace_bytes(long N, long R, long H, long Hkv, long D, long own_cap, long prefix_cap,
+                                      long max_new) {
+    if (bad_shape(N, R, H, Hkv, D, own_cap, prefix_cap, max_new) || N == 0) return 0;
+    return plan_shared(N, R, H, Hkv, D, own_cap, prefix_cap, max_new).bytes;
+}
+
+int launch_attention_shared(const uint16_t *q, long q_stride, const uint16_t *kc, const uint16_t *vt, long n_blocks,
+                            long bs, const int32_t *row_starts, const int32_t *lengths, const int32_t *tables,
+                            long width, const int32_t *prefix_table, long prefix_width, const int32_t *prefix_len,
+                            uint16_t *out, long out_stride, long N, long R, long H, long Hkv, long D, float scale,
+                            long max_new, void *workspace, long workspace_bytes, hipStream_t stream) {
+    if (N == 0) return SC_OK;
+    if (!q || !kc || !vt || !row_starts || !lengths || !tables || !out || (prefix_width > 0 && (!prefix_table || !prefix_len)))
+        return set_error(SC_EINVAL, "attention_shared: null pointer");
+    if (D != 64 && D != 128) return set_error(SC_EUNSUPPORTED, "attention_shared: head_dim %ld (64 or 128 supported)", D);
+    const int shift = block_shift(bs);
+    if (shift < 0) return set_error(SC_EINVAL, "attention_shared: block size %ld (16, 32, 64, 128 or 256)", bs);
+    if (width <= 0 || width >= (1L << 26) || prefix_width < 0 || prefix_width >= (1L << 26) ||
+        bad_shape(N, R, H, Hkv, D, width * bs, prefix_width * bs, max_new))
+        return set_error(SC_EINVAL, "attention_shared: bad shape rows=%ld sequences=%ld (at most %d) H=%ld Hkv=%ld tables=%ld/%ld",
+                         N, R, SA_MAX_SEQ, H, Hkv, width, prefix_width);
+    if (n_blocks <= 0 || n_blocks * bs >= (1L << 31)) return set_error(SC_EINVAL, "attention_shared: bad pool size");
+    // the maximum is taken of the unscaled scores
+    if (!(scale >= 1e-30f && scale <= 1e30f)) return set_error(SC_EINVAL, "attention_shared: scale must be positive (1e-30 to 1e30)");
+    if (q_stride < H * D || out_stride < H * D || q_stride % 8 || out_stride % 4)
+        return set_error(SC_EINVAL, "attention_shared: bad row strides");
+    if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vt) % 16 || (uintptr_t)out % 8)
+        return set_error(SC_EINVAL, "attention_shared: misaligned pointers");
+    const SaPlan p = plan_shared(N, R, H, Hkv, D, width * bs, prefix_width * bs, max_new);
+    if (!workspace || workspace_bytes < p.bytes || (uintptr_t)workspace % 16)
+        return set_error(SC_EINVAL, "attention_shared: a 16-byte aligned workspace of %ld bytes required", p.bytes);
+    if (p.tiles * p.nsplit * Hkv >= (1L << 31) || N * H >= (1L << 31))
+        return set_error(SC_EINVAL, "attention_shared: too many rows");
+    SaArgs a;
+    a.q = q; a.q_stride = q_stride; a.kc = kc; a.vt = vt; a.out = out; a.out_stride = out_stride;
+    a.row_starts = row_starts; a.lengths = lengths; a.tables = tables;
+    a.prefix_table = prefix_table; a.prefix_len = prefix_len;
+    a.N = (int)N; a.R = (int)R; a.H = (int)H; a.Hkv = (int)Hkv; a.G = (int)(H / Hkv);
+    a.width = (int)width; a.shift = shift; a.n_blocks = (int)n_blocks; a.prefix_width = (int)prefix_width;
+    a.small_rows = p.small_rows; a.any_big = p.any_big; a.nsplit = p.nsplit; a.own_prefix = p.own_prefix;
+    a.own_wgs = p.own_wgs;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    char *ws = static_cast<char *>(workspace);
+    a.tile_o = reinterpret_cast<float *>(ws + p.tile_o);
+    a.tile_ml = reinterpret_cast<float2 *>(ws + p.tile_ml);
+    a.own_o = reinterpret_cast<float *>(ws + p.own_o);
+    a.own_ml = reinterpret_cast<float2 *>(ws + p.own_ml);
+    a.own_parts = (int)p.own_parts;
+    a.own_off = reinterpret_cast<int32_t *>(ws + p.own_idx);
+    a.own_unit = a.own_off + R + 2;
+    return D == 128 ? run_shared<128>(a, p, stream) : run_shared<64>(a, p, stream);
+}
+
+}  // namespace sc

@@ -1,0 +1,87 @@
+"""Refusals of the block cache's entry points (argument checks only, no GPU calls)."""
+import ctypes
+import os
+
+import pytest
+import torch
+
+from shardcompute_amd import _lib
+from shardcompute_amd.build import LIB_PATH
+
+pytestmark = pytest.mark.skipif(not os.path.exists(LIB_PATH), reason="library not built")
+A = 1 << 12                     # a 16-byte aligned address nothing reads
+
+
+def _tables(**kw):
+    a = dict(lengths=A, new=A, release=None, tables=A, free=A, n_free=A, prefix=None, R=4, width=8, bs=64, cap=40, rows=4,
+             lengths_out=A, n_free_out=A, row_starts=A, slots=A, positions=A, status=A)
+    a.update(kw)
+    return _lib.load().sc_block_tables_i32(*a.values(), None)
+
+
+def _append(**kw):
+    a = dict(qkv=A, qkv_stride=1536, q=A, q_stride=1024, N=3, H=8, Hkv=2, D=128, cos=A, sin=A, length=99, k=A, vt=A,
+             n_blocks=10, bs=64, slots=A, positions=A)
+    a.update(kw)
+    return _lib.load().sc_rope_append_blocks_bf16(*a.values(), None)
+
+
+def _attend(**kw):
+    a = dict(q=A, q_stride=1024, k=A, vt=A, n_blocks=10, bs=64, row_starts=A, lengths=A, tables=A, width=4, prefix_table=A,
+             prefix_width=5, prefix_len=A, out=A, out_stride=1024, N=3, R=3, H=8, Hkv=2, D=128, scale=0.1, max_new=1,
+             workspace=A, workspace_bytes=1 << 30)
+    a.update(kw)
+    return _lib.load().sc_attention_shared_bf16(*a.values(), None)
+
+
+@pytest.mark.parametrize("call,kw,message", [
+    (_tables, dict(lengths=None), "null pointer"), (_tables, dict(tables=None), "null pointer"),
+    (_tables, dict(status=None), "null pointer"), (_tables, dict(slots=None), "null pointer"),
+    (_tables, dict(bs=48), "block size 48"), (_tables, dict(bs=8), "block size 8"), (_tables, dict(bs=512), "block size"),
+    (_tables, dict(R=0), "sequences"), (_tables, dict(R=65537), "sequences"), (_tables, dict(width=0), "width"),
+    (_tables, dict(width=1 << 25), "width"), (_tables, dict(cap=0), "stack"), (_tables, dict(cap=1 << 26), "stack"),
+    (_tables, dict(rows=-1), "row count"),
+    (_append, dict(qkv=None), "null pointer"), (_append, dict(slots=None), "null pointer"),
+    (_append, dict(D=96), "head_dim 96"), (_append, dict(bs=20), "block size 20"), (_append, dict(Hkv=3), "bad shape"),
+    (_append, dict(N=-1), "bad shape"), (_append, dict(n_blocks=0), "pool"), (_append, dict(n_blocks=1 << 25), "pool"),
+    (_append, dict(qkv_stride=1528), "strides"), (_append, dict(qkv_stride=1540), "strides"),
+    (_append, dict(q_stride=1020), "strides"), (_append, dict(k=A + 2), "aligned"), (_append, dict(cos=A + 4), "aligned"),
+    (_attend, dict(q=None), "null pointer"), (_attend, dict(prefix_table=None), "null pointer"),
+    (_attend, dict(prefix_len=None), "null pointer"), (_attend, dict(D=80), "head_dim 80"),
+    (_attend, dict(bs=0), "block size 0"), (_attend, dict(H=9), "bad shape"), (_attend, dict(R=0), "bad shape"),
+    (_attend, dict(R=2049), "bad shape"), (_attend, dict(width=0), "bad shape"), (_attend, dict(max_new=-1), "bad shape"),
+    (_attend, dict(prefix_width=1 << 26), "bad shape"), (_attend, dict(n_blocks=0), "pool"),
+    (_attend, dict(scale=0.0), "scale"), (_attend, dict(scale=-0.1), "scale"),
+    (_attend, dict(scale=float("nan")), "scale"), (_attend, dict(scale=float("inf")), "scale"),
+    (_attend, dict(q_stride=1023), "strides"), (_attend, dict(q_stride=1028), "strides"),
+    (_attend, dict(out_stride=1000), "strides"), (_attend, dict(q=A + 8), "misaligned"),
+    (_attend, dict(out=A + 4), "misaligned"), (_attend, dict(workspace=None), "workspace"),
+    (_attend, dict(workspace_bytes=64), "workspace"), (_attend, dict(workspace=A + 8), "workspace"),
+])
+def test_refused(call, kw, message):
+    assert call(**kw) in (-1, -2)
+    assert message in _lib.load().sc_last_error().decode()
+
+
+def test_no_rows_is_no_work():
+    assert _append(N=0, qkv=None) == 0 and _attend(N=0, q=None) == 0
+    lib = _lib.load()
+    assert lib.sc_attention_shared_workspace_bytes(0, 3, 8, 2, 128, 256, 320, 1) == 0
+    assert lib.sc_attention_shared_workspace_bytes(5, 3, 8, 3, 128, 256, 320, 1) == 0
+
+
+def test_workspace_grows_with_rows_not_with_table_width():
+    lib = _lib.load()
+    small = lib.sc_attention_shared_workspace_bytes(64, 64, 32, 8, 128, 1 << 10, 1 << 13, 1)
+    assert 0 < small <= lib.sc_attention_shared_workspace_bytes(128, 128, 32, 8, 128, 1 << 10, 1 << 13, 1)
+    wide = lib.sc_attention_shared_workspace_bytes(64, 64, 32, 8, 128, 1 << 20, 1 << 13, 1)
+    assert wide <= 2 * small + (16 << 20)
+
+
+def test_wrappers_need_gpu_tensors():
+    z = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="GPU"):
+        _lib.block_tables(z, z, z.view(4, 1), z, z, 64, 4)
+    with pytest.raises(RuntimeError, match="GPU"):
+        _lib.attention_shared(torch.zeros(1, 64, dtype=torch.bfloat16), 1, 1, 64, z, z, z, z, z, 1.0)
+    assert ctypes.c_int64 in _lib.load().sc_attention_shared_bf16.argtypes
