@@ -34,6 +34,7 @@ namespace {
 using f4 = dma::f4;
 
 constexpr int SA_COLS = 128, SA_KB = 64, SA_THREADS = 256;
+constexpr int SA_AHEAD = 4;                              // operand reads in flight ahead of the MFMAs
 constexpr int SO_WAVES = 4, SO_KB = 32, SO_TILE = SO_WAVES * SO_KB;      // keys a workgroup takes at a time
 constexpr int SA_MAX_SEQ = 2048;         // attn_own_kernel keeps two numbers of each in LDS
 
@@ -111,7 +112,9 @@ struct SaGeo {
     static constexpr int LDS = 2 * STAGE;
     static constexpr int KSTEPS = D / 16;
     static constexpr int DB = D / 32;
-    static constexpr int DMA = KTILE / 1024 / 4;
+    static constexpr int DMA = KTILE / 1024 / 4;         // K (and Vt) copies of a wave, a key block
+    // the growth of a column's maximum (log2) that moves it, as in the dense kernel
+    static constexpr float LAZY = D == 64 ? 0.f : 8.f;
 };
 
 __device__ __forceinline__ int sa_swap23(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }
@@ -137,6 +140,13 @@ __device__ __forceinline__ uint4 keep_below(int k0, int end) {
     m.w = (k0 + 6 < end ? 0xFFFFu : 0u) | (k0 + 7 < end ? 0xFFFF0000u : 0u);
     return m;
 }
+// non-finite values replaced by 0
+__device__ __forceinline__ uint4 finite8(uint4 v) {
+    auto keep = [](uint32_t x) {
+        return ((x & 0x7F80u) == 0x7F80u ? 0u : x & 0xFFFFu) | ((x & 0x7F800000u) == 0x7F800000u ? 0u : x & 0xFFFF0000u);
+    };
+    return make_uint4(keep(v.x), keep(v.y), keep(v.z), keep(v.w));
+}
 // key e of 8 alone
 __device__ __forceinline__ uint4 keep_one(int e, bool on) {
     const uint32_t h = on ? ((e & 1) ? 0xFFFF0000u : 0xFFFFu) : 0u;
@@ -145,8 +155,9 @@ __device__ __forceinline__ uint4 keep_one(int e, bool on) {
 }
 __device__ __forceinline__ uint4 and4(uint4 v, uint4 m) { return make_uint4(v.x & m.x, v.y & m.y, v.z & m.z, v.w & m.w); }
 
-template <int D>
-__global__ void __launch_bounds__(SA_THREADS) attn_tile_kernel(SaArgs a) {
+// ONE: a key block lies in one cache block (block sizes from 64 up)
+template <int D, bool ONE>
+__global__ void __launch_bounds__(SA_THREADS) __attribute__((amdgpu_waves_per_eu(2))) attn_tile_kernel(SaArgs a) {
     using Gm = SaGeo<D>;
     extern __shared__ __align__(16) uint8_t smem[];
     static_assert(Gm::LDS <= 65536, "no larger dynamic LDS is asked for at the launch");
@@ -196,37 +207,52 @@ __global__ void __launch_bounds__(SA_THREADS) attn_tile_kernel(SaArgs a) {
     float m = -INFINITY, lsum = 0.f;
     const float sc = a.scale_log2;
     const int arow = sa_swap23(li);
-    const size_t blk_elems = (size_t)a.Hkv * D << sh;
-    const uint16_t *kbase = a.kc + ((size_t)hk * D << sh), *vbase = a.vt + ((size_t)hk * D << sh);
+    const size_t blk_bytes = (size_t)a.Hkv * D * 2 << sh;
+    const char *kpool = reinterpret_cast<const char *>(a.kc) + ((size_t)hk * D * 2 << sh);
+    const char *vpool = reinterpret_cast<const char *>(a.vt) + ((size_t)hk * D * 2 << sh);
+
+    // This lane's share of a key block's copies.  Wave w issues K instructions of the block's
+    // 16 keys 16 w .. 16 w + 15 and Vt instructions of D / 4 dims; a lane's dim row d and
+    // chunk c of Vt instruction qq differ between even and odd qq only in bit 2 of c.
+    const int kr = D == 128 ? 16 * w + (lane >> 4) : 16 * w + (lane >> 3);    // key row at qq = 0
+    const int vd = Gm::DMA * 8 * w + (lane >> 3);                             // dim at qq = 0
+    const int vc = (lane & 7) ^ ((vd >> 1) & 7);                              // chunk at even qq; ^ 4 at odd
 
     // key blocks [b0, b1) of one table with `end` keys; the column sees keys <= limit
     auto segment = [&](const int32_t *table, int width, int end, int b0, int b1, int limit) {
         if (b0 >= b1) return;
-        // the cache blocks of a key block's four 16-key groups: lane l loads group l % 4's
-        // number, one key block before its copies are issued
-        auto load_ids = [&](int kb) { return table[min((kb + 16 * (lane & 3)) >> sh, width - 1)]; };
-        auto stage_blk = [&](int kb, int st, int ids) {
-            ids = clampi(ids, 0, a.n_blocks - 1);
-            const int i0 = __builtin_amdgcn_readlane(ids, 0), i1 = __builtin_amdgcn_readlane(ids, 1);
-            const int i2 = __builtin_amdgcn_readlane(ids, 2), i3 = __builtin_amdgcn_readlane(ids, 3);
-            auto pick = [&](int g) { return g < 2 ? (g == 0 ? i0 : i1) : (g == 2 ? i2 : i3); };
-            const uint32_t kl = (uint32_t)(uintptr_t)(smem + st * Gm::STAGE);
+        // the cache blocks of a key block, one ahead of its copies: ONE, its block's number;
+        // else those of the wave's 16 keys of K and of the lane's two chunks of Vt
+        struct Ids { int k, v0, v1; };
+        auto id_at = [&](int key) { return table[min(key >> sh, width - 1)]; };
+        auto load_ids = [&](int kb) {
+            Ids x;
+            x.k = id_at(ONE ? kb : kb + 16 * w);
+            if (!ONE) { x.v0 = id_at(kb + 8 * vc); x.v1 = id_at(kb + 8 * (vc ^ 4)); }
+            return x;
+        };
+        auto stage_blk = [&](int kb, int st, const Ids &x) {
+            const uint32_t kl = (uint32_t)(uintptr_t)(smem + st * Gm::STAGE) + 1024 * Gm::DMA * w;
             const uint32_t vl = kl + Gm::KTILE;
+            const int kid = clampi(__builtin_amdgcn_readfirstlane(x.k), 0, a.n_blocks - 1);
+            const char *kp = kpool + kid * blk_bytes + (size_t)((ONE ? kb : kb + 16 * w) & (bs - 1)) * Gm::KROW;
 #pragma unroll
             for (int qq = 0; qq < Gm::DMA; ++qq) {
-                const int qi = Gm::DMA * w + qq;
-                const int r = D == 128 ? 4 * qi + (lane >> 4) : 8 * qi + (lane >> 3);
+                const int r = kr + (D == 128 ? 4 : 8) * qq;          // key row in the key block
                 const int c = D == 128 ? (lane & 15) ^ (sa_swap23(r) & 15) : (lane & 7) ^ ((r >> 1) & 7);
-                dma::dma16(kbase + (size_t)pick(r >> 4) * blk_elems + (size_t)((kb + r) & (bs - 1)) * D + 8 * c,
-                           kl + 1024 * qi);
+                dma::dma16s(kp, (uint32_t)((ONE ? r : r - 16 * w) * Gm::KROW + 16 * c), kl + 1024 * qq);
             }
+            const char *vp = vpool + kid * blk_bytes + (ONE ? (size_t)(kb & (bs - 1)) * 2 : 0);
 #pragma unroll
             for (int qq = 0; qq < Gm::DMA; ++qq) {
-                const int qi = Gm::DMA * w + qq;
-                const int d = 8 * qi + (lane >> 3);
-                const int c = (lane & 7) ^ ((d >> 1) & 7);
-                dma::dma16(vbase + (size_t)pick(c >> 1) * blk_elems + ((size_t)d << sh) + ((kb + 8 * c) & (bs - 1)),
-                           vl + 1024 * qi);
+                const int c = (qq & 1) ? vc ^ 4 : vc;
+                const uint32_t voff = ((uint32_t)(vd + 8 * qq) << sh) * 2;
+                if (ONE) {
+                    dma::dma16s(vp, voff + 16 * c, vl + 1024 * qq);
+                } else {
+                    const int vid = clampi((qq & 1) ? x.v1 : x.v0, 0, a.n_blocks - 1);
+                    dma::dma16(vpool + vid * blk_bytes + voff + ((kb + 8 * c) & (bs - 1)) * 2, vl + 1024 * qq);
+                }
             }
         };
         // of the wave's columns: the fewest and the most keys one of them sees
@@ -236,116 +262,164 @@ __global__ void __launch_bounds__(SA_THREADS) attn_tile_kernel(SaArgs a) {
             lo = min(lo, __shfl_xor(lo, x));
             hi = max(hi, __shfl_xor(hi, x));
         }
-        auto block = [&](int blk, int ids_next, auto mask_tag) {
+        lo = __builtin_amdgcn_readfirstlane(lo);
+        hi = __builtin_amdgcn_readfirstlane(hi);
+        Ids ids;
+        // the stage is a compile-time constant in each copy of the body, so that every
+        // operand read is a loop-invariant lane offset plus an immediate
+        auto block = [&](int blk, auto mask_tag, auto stage_tag) {
             constexpr bool MASK = decltype(mask_tag)::value;
-            const int kb = blk * SA_KB, st = (blk - b0) & 1;
+            constexpr int st = decltype(stage_tag)::value;
+            const int kb = blk * SA_KB;
             const uint8_t *K = smem + st * Gm::STAGE;
             const uint8_t *V = K + Gm::KTILE;
-            if (blk + 1 < b1) stage_blk(kb + SA_KB, st ^ 1, ids_next);
-            if (MASK && kb > hi) return;                 // nothing of it is seen by the wave
-            f32x16_t sacc[2] = {f32x16_t{}, f32x16_t{}};
+            if (blk + 1 < b1) {
+                stage_blk(kb + SA_KB, st ^ 1, ids);
+                ids = load_ids(kb + 2 * SA_KB);
+            }
+            if (!MASK || kb <= hi) {                     // else: nothing of it is seen by the wave
+                f32x16_t sacc[2] = {f32x16_t{}, f32x16_t{}};
+                // operand reads SA_AHEAD ahead of their MFMAs (the scheduler, left alone,
+                // issues each read just before its MFMA)
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int ks = 0; ks < Gm::KSTEPS; ++ks)
+                for (int ks = 0; ks < Gm::KSTEPS; ++ks)
 #pragma unroll
-                for (int kh = 0; kh < 2; ++kh) {
-                    const bf16x8_t ka = as_bf16x8(*reinterpret_cast<const uint4 *>(K + sa_kswz<D>(32 * kh + arow, 2 * ks + lh)));
-                    sacc[kh] = mfma32x32x16(ka, qv[ks], sacc[kh]);
+                    for (int kh = 0; kh < 2; ++kh) {
+                        const bf16x8_t ka = as_bf16x8(*reinterpret_cast<const uint4 *>(K + sa_kswz<D>(32 * kh + arow, 2 * ks + lh)));
+                        sacc[kh] = mfma32x32x16(ka, qv[ks], sacc[kh]);
+                    }
+                __builtin_amdgcn_sched_group_barrier(0x100, SA_AHEAD, 0);
+#pragma unroll
+                for (int i = 0; i < 2 * Gm::KSTEPS - SA_AHEAD; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
                 }
-            if (MASK) {
-                const int rel = limit - kb - 8 * lh;
+                __builtin_amdgcn_sched_group_barrier(0x008, SA_AHEAD, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                if (MASK) {
+                    const int rel = limit - kb - 8 * lh;
+#pragma unroll
+                    for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (32 * kh + 16 * (r >> 3) + (r & 7) > rel) sacc[kh][r] = -INFINITY;
+                }
+                float bm = -INFINITY;
 #pragma unroll
                 for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (32 * kh + 16 * (r >> 3) + (r & 7) > rel) sacc[kh][r] = -INFINITY;
-            }
-            float bm = -INFINITY;
-#pragma unroll
-            for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) bm = fmaxf(bm, sacc[kh][r]);
-            bm = fmaxf(bm, __shfl_xor(bm, 32));
-            float alpha = 1.f;
-            if (bm > m) {
-                alpha = __builtin_amdgcn_exp2f((m - bm) * sc);
-                m = bm;
-            }
-            const float nms = -m * sc;
-            float ps = 0.f;
-#pragma unroll
-            for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    float p = __builtin_amdgcn_exp2f(fmaf(sacc[kh][r], sc, nms));
-                    // a column that has seen no key yet has m = -inf: 0, not NaN
-                    if (MASK && sacc[kh][r] == -INFINITY) p = 0.f;
-                    sacc[kh][r] = p;
-                    ps += p;
+                    for (int r = 0; r < 16; ++r) bm = fmaxf(bm, sacc[kh][r]);
+                bm = fmaxf(bm, __shfl_xor(bm, 32));
+                float alpha = 1.f;
+                if ((bm - m) * sc > Gm::LAZY) {
+                    alpha = __builtin_amdgcn_exp2f((m - bm) * sc);
+                    m = bm;
                 }
-            lsum = lsum * alpha + ps;
-            if (__ballot(alpha != 1.f) != 0ull) {
+                const float nms = -m * sc;
+                float ps = 0.f;
 #pragma unroll
-                for (int db = 0; db < Gm::DB; ++db)
+                for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
-            }
-            // keys at or past `end` may hold anything: their V is dropped.  Keys of the
-            // sequence that only some of the columns see (a later row's, or another
-            // sequence's keys) meet zero probabilities, which an inf or NaN would turn into
-            // NaN: where there is one, key by key, each column taking the keys it sees
-            bool bad = false;
-            if (MASK) {
-#pragma unroll
-                for (int s4 = 0; s4 < 4; ++s4) {
-                    const int c = 2 * s4 + lh;
-                    const uint4 mk = keep_below(kb + 8 * c, end);
+                    for (int r = 0; r < 16; ++r) {
+                        float p = __builtin_amdgcn_exp2f(fmaf(sacc[kh][r], sc, nms));
+                        // a column that has seen no key yet has m = -inf: 0, not NaN
+                        if (MASK && sacc[kh][r] == -INFINITY) p = 0.f;
+                        sacc[kh][r] = p;
+                        ps += p;
+                    }
+                lsum = lsum * alpha + ps;
+                if (__ballot(alpha != 1.f) != 0ull) {
 #pragma unroll
                     for (int db = 0; db < Gm::DB; ++db)
-                        bad = bad || nonfinite8(and4(*reinterpret_cast<const uint4 *>(V + sa_vswz(32 * db + li, c)), mk));
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
                 }
-                bad = __ballot(bad) != 0ull;
-            }
+                // keys at or past `end` may hold anything: their V is dropped.  Keys that only
+                // some of the columns see (a later row's, another sequence's) meet zero
+                // probabilities, which an inf or NaN among their values would turn into NaN
+                // for every column: such values are dropped here and added afterwards to the
+                // columns that see them
+                bool bad = false;
+                if (MASK) {
+#pragma unroll 1                                         // (few registers: this block's P is live)
+                    for (int s4 = 0; s4 < 4; ++s4) {
+                        const uint4 mk = keep_below(kb + 16 * s4 + 8 * lh, end);
 #pragma unroll
-            for (int s4 = 0; s4 < 4; ++s4) {
-                const int kh = s4 >> 1, q0 = 8 * (s4 & 1), c = 2 * s4 + lh;
-                const uint4 pw = make_uint4(cvt_pk_bf16(sacc[kh][q0], sacc[kh][q0 + 1]),
-                                            cvt_pk_bf16(sacc[kh][q0 + 2], sacc[kh][q0 + 3]),
-                                            cvt_pk_bf16(sacc[kh][q0 + 4], sacc[kh][q0 + 5]),
-                                            cvt_pk_bf16(sacc[kh][q0 + 6], sacc[kh][q0 + 7]));
-                if (MASK && bad) {
-                    for (int j = 0; j < 16; ++j) {
-                        const uint4 one = keep_one(j & 7, (j >> 3) == lh);
-                        const bool sees = kb + 16 * s4 + j <= limit;
-#pragma unroll
-                        for (int db = 0; db < Gm::DB; ++db) {
-                            const uint4 v = and4(*reinterpret_cast<const uint4 *>(V + sa_vswz(32 * db + li, c)), one);
-                            const f32x16_t t = mfma32x32x16(as_bf16x8(v), as_bf16x8(and4(pw, one)), o[db]);
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) o[db][r] = sees ? t[r] : o[db][r];
-                        }
+                        for (int db = 0; db < Gm::DB; ++db)
+                            bad = bad || nonfinite8(and4(*reinterpret_cast<const uint4 *>(V + sa_vswz(32 * db + li, 2 * s4 + lh)), mk));
                     }
-                    continue;
+                    bad = __ballot(bad) != 0ull;
                 }
-                uint4 mk = make_uint4(~0u, ~0u, ~0u, ~0u);
-                if (MASK) mk = keep_below(kb + 8 * c, end);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int db = 0; db < Gm::DB; ++db) {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(V + sa_vswz(32 * db + li, c));
-                    o[db] = mfma32x32x16(as_bf16x8(MASK ? and4(v, mk) : v), as_bf16x8(pw), o[db]);
+                for (int s4 = 0; s4 < 4; ++s4) {
+                    const int kh = s4 >> 1, q0 = 8 * (s4 & 1), c = 2 * s4 + lh;
+                    const bf16x8_t pb = as_bf16x8(cvt_pk_bf16(sacc[kh][q0], sacc[kh][q0 + 1]),
+                                                  cvt_pk_bf16(sacc[kh][q0 + 2], sacc[kh][q0 + 3]),
+                                                  cvt_pk_bf16(sacc[kh][q0 + 4], sacc[kh][q0 + 5]),
+                                                  cvt_pk_bf16(sacc[kh][q0 + 6], sacc[kh][q0 + 7]));
+                    uint4 mk;
+                    if (MASK) mk = keep_below(kb + 8 * c, end);
+#pragma unroll
+                    for (int db = 0; db < Gm::DB; ++db) {
+                        uint4 v = *reinterpret_cast<const uint4 *>(V + sa_vswz(32 * db + li, c));
+                        if (MASK) {
+                            v = and4(v, mk);
+                            if (bad) v = finite8(v);
+                        }
+                        o[db] = mfma32x32x16(as_bf16x8(v), pb, o[db]);
+                    }
+                }
+                if (!MASK) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, SA_AHEAD, 0);
+#pragma unroll
+                    for (int i = 0; i < 4 * Gm::DB - SA_AHEAD; ++i) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    }
+                    __builtin_amdgcn_sched_group_barrier(0x008, SA_AHEAD, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (MASK && bad) {
+                    // register r of o[db] is dim 32 db + 8 (r / 4) + 4 lh + r % 4; the weight
+                    // of an inf is positive whatever it is
+                    for (int j = 0; j < SA_KB && kb + j < end; ++j) {
+                        const bool sees = kb + j <= limit;
+                        int half = lh;                   // opaque: no addresses of this rare loop are kept
+                        asm volatile("" : "+v"(half));
+#pragma unroll
+                        for (int db = 0; db < Gm::DB; ++db)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) {
+                                const int d = 32 * db + 8 * (r >> 2) + 4 * half + (r & 3);
+                                const uint32_t x = *reinterpret_cast<const uint16_t *>(V + sa_vswz(d, j >> 3) + 2 * (j & 7));
+                                if (sees && (x & 0x7F80u) == 0x7F80u) o[db][r] += bf2f(x);
+                            }
+                    }
                 }
             }
-        };
-        int ids = load_ids(b0 * SA_KB), next = load_ids((b0 + 1) * SA_KB);
-        stage_blk(b0 * SA_KB, 0, ids);
-        dma::wait_vm<0>();
-        __syncthreads();
-        for (int blk = b0; blk < b1; ++blk) {
-            const int after = load_ids((blk + 2) * SA_KB);
-            if (blk * SA_KB + SA_KB - 1 <= lo) block(blk, next, std::false_type{});
-            else block(blk, next, std::true_type{});
-            next = after;
+            // key block blk + 1 has landed, and this one is read, before the next is begun
             dma::wait_vm<0>();
             __syncthreads();
+        };
+        ids = load_ids(b0 * SA_KB);
+        stage_blk(b0 * SA_KB, 0, ids);
+        ids = load_ids(b0 * SA_KB + SA_KB);
+        dma::wait_vm<0>();
+        __syncthreads();
+        using S0 = std::integral_constant<int, 0>;
+        using S1 = std::integral_constant<int, 1>;
+        const int bf = min(b1, (lo + 1) / SA_KB);        // key blocks below it need no mask
+        int blk = b0;
+        for (; blk + 1 < bf; blk += 2) {
+            block(blk, std::false_type{}, S0{});
+            block(blk + 1, std::false_type{}, S1{});
+        }
+        if (blk < bf) block(blk++, std::false_type{}, S0{});
+        for (; blk < b1; ++blk) {
+            if ((blk - b0) & 1) block(blk, std::true_type{}, S1{});
+            else block(blk, std::true_type{}, S0{});
         }
     };
 
@@ -353,18 +427,24 @@ __global__ void __launch_bounds__(SA_THREADS) attn_tile_kernel(SaArgs a) {
     // copies in flight, which the compiler does not see
 #pragma unroll
     for (int ks = 0; ks < Gm::KSTEPS; ++ks) asm volatile("" ::"v"(qv[ks]));
+    // the prefix, then the sequences, in one loop (the body is compiled once)
     const int pb = (P + SA_KB - 1) / SA_KB;
-    segment(a.prefix_table, a.prefix_width, P, min(t0, pb), min(t1, pb), P - 1);
-    if (a.any_big) {
-        int at = pb;
-        for (int r = r0; r < a.R && at < t1; ++r) {
+    for (int r = r0 - 1, at = 0; r < a.R && at < t1; ++r) {
+        const bool pre = r < r0;
+        int nb = pb, end = P, limit = P - 1, width = a.prefix_width;
+        const int32_t *table = a.prefix_table;
+        if (!pre) {
+            if (!a.any_big) break;
             const Seq s = seq_of(a, r, rows);
             if (s.first > row1) break;
-            const int nb = own_blocks(s);
-            const int limit = col_ok && row >= s.first && row < s.first + s.n ? s.len - s.n + row - s.first : -1;
-            segment(a.tables + (size_t)r * a.width, a.width, s.len, clampi(t0 - at, 0, nb), clampi(t1 - at, 0, nb), limit);
-            at += nb;
+            nb = own_blocks(s);
+            end = s.len;
+            limit = row >= s.first && row < s.first + s.n ? s.len - s.n + row - s.first : -1;
+            table = a.tables + (size_t)r * a.width;
+            width = a.width;
         }
+        segment(table, width, end, clampi(t0 - at, 0, nb), clampi(t1 - at, 0, nb), limit);
+        at += nb;
     }
 
     const float ltot = lsum + __shfl_xor(lsum, 32);
@@ -764,8 +844,9 @@ SaPlan plan_shared(long N, long R, long H, long Hkv, long D, long own_cap, long 
 template <int D>
 int run_shared(const SaArgs &a, const SaPlan &p, hipStream_t stream) {
     if (p.use_tile) {
-        hipLaunchKernelGGL(attn_tile_kernel<D>, dim3((unsigned)(p.tiles * p.nsplit * a.Hkv)), dim3(SA_THREADS),
-                           SaGeo<D>::LDS, stream, a);
+        auto kern = a.shift >= 6 ? attn_tile_kernel<D, true> : attn_tile_kernel<D, false>;
+        hipLaunchKernelGGL(kern, dim3((unsigned)(p.tiles * p.nsplit * a.Hkv)), dim3(SA_THREADS), SaGeo<D>::LDS, stream,
+                           a);
         SC_HIP_CHECK(hipGetLastError());
     }
     hipLaunchKernelGGL(attn_own_kernel<D>, dim3((unsigned)p.own_wgs), dim3(64 * SO_WAVES), (a.R + 2) * 8, stream, a);
