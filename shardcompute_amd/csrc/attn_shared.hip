@@ -125,10 +125,14 @@ __device__ __forceinline__ uint32_t sa_kswz(int r, int c) {
 }
 __device__ __forceinline__ uint32_t sa_vswz(int d, int c) { return (uint32_t)(d * 128 + ((c ^ ((d >> 1) & 7)) << 4)); }
 
-// any bf16 of 8 is inf or NaN
-__device__ __forceinline__ bool nonfinite8(uint4 v) {
-    auto bad = [](uint32_t x) { return (x & 0x7F80u) == 0x7F80u || (x & 0x7F800000u) == 0x7F800000u; };
-    return bad(v.x) || bad(v.y) || bad(v.z) || bad(v.w);
+// bits 15 and 31 are set if the pair's low or high bf16 is inf or NaN (its exponent is all ones)
+__device__ __forceinline__ uint32_t nonfinite_bits(uint32_t x) { return (x & 0x7F807F80u) + 0x00800080u; }
+__device__ __forceinline__ uint32_t nonfinite_bits(uint4 v) {
+    return nonfinite_bits(v.x) | nonfinite_bits(v.y) | nonfinite_bits(v.z) | nonfinite_bits(v.w);
+}
+// of the wave's lanes, some one's bits are set (a scalar)
+__device__ __forceinline__ bool any_nonfinite(uint32_t bits) {
+    return __builtin_amdgcn_readfirstlane((int)(__ballot((bits & 0x80008000u) != 0u) != 0ull)) != 0;
 }
 
 // word masks of 8 consecutive keys k0 .. k0 + 7, of which those below end are kept
@@ -146,12 +150,6 @@ __device__ __forceinline__ uint4 finite8(uint4 v) {
         return ((x & 0x7F80u) == 0x7F80u ? 0u : x & 0xFFFFu) | ((x & 0x7F800000u) == 0x7F800000u ? 0u : x & 0xFFFF0000u);
     };
     return make_uint4(keep(v.x), keep(v.y), keep(v.z), keep(v.w));
-}
-// key e of 8 alone
-__device__ __forceinline__ uint4 keep_one(int e, bool on) {
-    const uint32_t h = on ? ((e & 1) ? 0xFFFF0000u : 0xFFFFu) : 0u;
-    const int w = e >> 1;
-    return make_uint4(w == 0 ? h : 0u, w == 1 ? h : 0u, w == 2 ? h : 0u, w == 3 ? h : 0u);
 }
 __device__ __forceinline__ uint4 and4(uint4 v, uint4 m) { return make_uint4(v.x & m.x, v.y & m.y, v.z & m.z, v.w & m.w); }
 
@@ -265,11 +263,11 @@ __global__ void __launch_bounds__(SA_THREADS) __attribute__((amdgpu_waves_per_eu
         lo = __builtin_amdgcn_readfirstlane(lo);
         hi = __builtin_amdgcn_readfirstlane(hi);
         Ids ids;
-        // the stage is a compile-time constant in each copy of the body, so that every
+        // the stage is a compile-time constant in the copies without a mask, so that every
         // operand read is a loop-invariant lane offset plus an immediate
-        auto block = [&](int blk, auto mask_tag, auto stage_tag) {
+        auto block = [&](int blk, auto mask_tag, auto stage) {
             constexpr bool MASK = decltype(mask_tag)::value;
-            constexpr int st = decltype(stage_tag)::value;
+            const int st = stage;
             const int kb = blk * SA_KB;
             const uint8_t *K = smem + st * Gm::STAGE;
             const uint8_t *V = K + Gm::KTILE;
@@ -316,15 +314,14 @@ __global__ void __launch_bounds__(SA_THREADS) __attribute__((amdgpu_waves_per_eu
                     alpha = __builtin_amdgcn_exp2f((m - bm) * sc);
                     m = bm;
                 }
-                const float nms = -m * sc;
+                // (a column that has seen no key yet has m = -inf: probabilities 0, not NaN)
+                const float nms = m == -INFINITY ? 0.f : -m * sc;
                 float ps = 0.f;
 #pragma unroll
                 for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        float p = __builtin_amdgcn_exp2f(fmaf(sacc[kh][r], sc, nms));
-                        // a column that has seen no key yet has m = -inf: 0, not NaN
-                        if (MASK && sacc[kh][r] == -INFINITY) p = 0.f;
+                        const float p = __builtin_amdgcn_exp2f(fmaf(sacc[kh][r], sc, nms));
                         sacc[kh][r] = p;
                         ps += p;
                     }
@@ -342,14 +339,15 @@ __global__ void __launch_bounds__(SA_THREADS) __attribute__((amdgpu_waves_per_eu
                 // columns that see them
                 bool bad = false;
                 if (MASK) {
+                    uint32_t bits = 0;
 #pragma unroll 1                                         // (few registers: this block's P is live)
                     for (int s4 = 0; s4 < 4; ++s4) {
                         const uint4 mk = keep_below(kb + 16 * s4 + 8 * lh, end);
 #pragma unroll
                         for (int db = 0; db < Gm::DB; ++db)
-                            bad = bad || nonfinite8(and4(*reinterpret_cast<const uint4 *>(V + sa_vswz(32 * db + li, 2 * s4 + lh)), mk));
+                            bits |= nonfinite_bits(and4(*reinterpret_cast<const uint4 *>(V + sa_vswz(32 * db + li, 2 * s4 + lh)), mk));
                     }
-                    bad = __ballot(bad) != 0ull;
+                    bad = any_nonfinite(bits);
                 }
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -417,10 +415,7 @@ __global__ void __launch_bounds__(SA_THREADS) __attribute__((amdgpu_waves_per_eu
             block(blk + 1, std::false_type{}, S1{});
         }
         if (blk < bf) block(blk++, std::false_type{}, S0{});
-        for (; blk < b1; ++blk) {
-            if ((blk - b0) & 1) block(blk, std::true_type{}, S1{});
-            else block(blk, std::true_type{}, S0{});
-        }
+        for (; blk < b1; ++blk) block(blk, std::true_type{}, (blk - b0) & 1);
     };
 
     // q's loads end here: a wait at their first use, in the loop, would also wait for the
@@ -500,15 +495,16 @@ struct OwnBlock {
     uint4 v[D / 16];
 };
 
-template <int D>
-__global__ void __launch_bounds__(64 * SO_WAVES) attn_own_kernel(SaArgs a) {
+// ONE: 32 keys lie in one cache block (block sizes from 32 up)
+template <int D, bool ONE>
+__global__ void __launch_bounds__(64 * SO_WAVES) __attribute__((amdgpu_waves_per_eu(2))) attn_own_kernel(SaArgs a) {
     constexpr int U = D / 32, DT = D / 16;
     extern __shared__ int32_t seq_lds[];                 // off[R + 2], unit[R + 2]
     __shared__ float sm_m[SO_WAVES][16], sm_l[SO_WAVES][16];
-    __shared__ float sm_o[SO_WAVES][D][17];
+    __shared__ __align__(16) float sm_o[SO_WAVES][D][17];
     __shared__ int wsum[2][SO_WAVES];
     int32_t *off = seq_lds, *unit = seq_lds + a.R + 2;
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
     const int rows = live_rows(a), P = prefix_keys(a);
     const int sh = a.shift, bs = 1 << sh;
@@ -559,17 +555,25 @@ __global__ void __launch_bounds__(64 * SO_WAVES) attn_own_kernel(SaArgs a) {
             else n = half;
         }
     }
+    const size_t blk_bytes = (size_t)a.Hkv * D * 2 << sh;
+    // byte offsets of this lane within a cache block of one kv head: key 8 (c / 4) + c % 4
+    // of K (the key 4 further on is 8 D bytes on), dim c of Vt (16 dims on: 32 << sh bytes)
+    const int krow = 8 * (c >> 2) + (c & 3);
+    const uint32_t koff = (uint32_t)((ONE ? krow : krow & 15) * D * 2 + 16 * g);
+    const uint32_t voff = ((uint32_t)c << sh) * 2 + (ONE ? 16 * g : 16 * (g & 1));
     for (; t < t_end;) {
         while (off[r + 1] <= t) ++r;
+        r = __builtin_amdgcn_readfirstlane(r);
         int first = 0, n = 0, len = 0;
         own_shape(a, r, rows, P, [&](int f, int nn, int l) { first = f; n = nn; len = l; });
         const int kt = own_keytiles(len), ct = own_coltiles(a, n);
-        const int lt = t - off[r], u = lt / kt, tile0 = lt - u * kt, tile1 = min(kt, tile0 + t_end - t);
+        const int lt = t - __builtin_amdgcn_readfirstlane(off[r]), u = lt / kt, tile0 = lt - u * kt;
+        const int tile1 = min(kt, tile0 + t_end - t);
         const int hk = u / ct, cols0 = (u - hk * ct) * 16;
         const bool pre = r == a.R;
         const int32_t *table = pre ? a.prefix_table : a.tables + (size_t)r * a.width;
         const int width = pre ? a.prefix_width : a.width;
-        const int part = unit[r] + u + (int)blockIdx.x;
+        const int part = __builtin_amdgcn_readfirstlane(unit[r]) + u + (int)blockIdx.x;
         t += tile1 - tile0;
 
         const int i = (cols0 + c) / a.G, gq = cols0 + c - i * a.G;
@@ -586,116 +590,153 @@ __global__ void __launch_bounds__(64 * SO_WAVES) attn_own_kernel(SaArgs a) {
             if (col_ok) v = *reinterpret_cast<const uint4 *>(a.q + (size_t)row * a.q_stride + (size_t)h * D + 32 * x + 8 * g);
             qv[x] = as_bf16x8(v);
         }
-        const size_t blk_elems = (size_t)a.Hkv * D << sh;
-        const uint16_t *kbase = a.kc + ((size_t)hk * D << sh), *vbase = a.vt + ((size_t)hk * D << sh);
+        const char *kpool = reinterpret_cast<const char *>(a.kc) + ((size_t)hk * D * 2 << sh);
+        const char *vpool = reinterpret_cast<const char *>(a.vt) + ((size_t)hk * D * 2 << sh);
         float m = -INFINITY, lsum = 0.f;
         f4 o[DT];
 #pragma unroll
         for (int x = 0; x < DT; ++x) o[x] = f4{0.f, 0.f, 0.f, 0.f};
 
         const int k_end = min(tile1 * SO_TILE, seen);
+        // the cache blocks of 32 keys (one, or those of this lane's K and Vt halves)
         struct Ids { int k, v; };
-        // the cache blocks of this lane's keys (two 16-key groups a block of 32)
         auto load_ids = [&](int kb) {
             kb = min(kb, max(k_end - 1, 0));
             Ids x;
-            x.k = table[min((kb + 16 * (c >> 3)) >> sh, width - 1)];
-            x.v = table[min((kb + 16 * (g >> 1)) >> sh, width - 1)];
+            x.k = table[min((ONE ? kb : kb + 16 * (c >> 3)) >> sh, width - 1)];
+            x.v = ONE ? 0 : table[min((kb + 16 * (g >> 1)) >> sh, width - 1)];
             return x;
         };
         auto load = [&](OwnBlock<D> &b, int kb, Ids x) {
-            const uint16_t *kp = kbase + (size_t)clampi(x.k, 0, a.n_blocks - 1) * blk_elems;
-            const int k0 = kb + 8 * (c >> 2) + (c & 3);
-            const uint16_t *ka = kp + (size_t)(k0 & (bs - 1)) * D + 8 * g, *kb4 = kp + (size_t)((k0 + 4) & (bs - 1)) * D + 8 * g;
+            auto take = [&](const char *kp, const char *vp) {
 #pragma unroll
-            for (int y = 0; y < U; ++y) {
-                b.k[0][y] = *reinterpret_cast<const uint4 *>(ka + 32 * y);
-                b.k[1][y] = *reinterpret_cast<const uint4 *>(kb4 + 32 * y);
+                for (int y = 0; y < U; ++y) {
+                    b.k[0][y] = *reinterpret_cast<const uint4 *>(kp + koff + 64 * y);
+                    b.k[1][y] = *reinterpret_cast<const uint4 *>(kp + koff + 64 * y + 8 * D);
+                }
+#pragma unroll
+                for (int y = 0; y < DT; ++y) b.v[y] = *reinterpret_cast<const uint4 *>(vp + (voff + ((uint32_t)y << (sh + 5))));
+            };
+            if (ONE) {
+                const size_t at = (size_t)clampi(__builtin_amdgcn_readfirstlane(x.k), 0, a.n_blocks - 1) * blk_bytes;
+                const int k0 = kb & (bs - 1);
+                take(kpool + at + (size_t)k0 * (D * 2), vpool + at + (size_t)k0 * 2);
+            } else {
+                take(kpool + (size_t)clampi(x.k, 0, a.n_blocks - 1) * blk_bytes,
+                     vpool + (size_t)clampi(x.v, 0, a.n_blocks - 1) * blk_bytes);
             }
-            const uint16_t *vp = vbase + (size_t)clampi(x.v, 0, a.n_blocks - 1) * blk_elems + ((kb + 8 * g) & (bs - 1));
-#pragma unroll
-            for (int y = 0; y < DT; ++y) b.v[y] = *reinterpret_cast<const uint4 *>(vp + ((size_t)(16 * y + c) << sh));
         };
-        auto compute = [&](const OwnBlock<D> &b, int kb) {
+        // EDGE: some column does not see all the 32 keys
+        auto compute = [&](OwnBlock<D> &b, int kb, auto edge_tag) {
+            constexpr bool EDGE = decltype(edge_tag)::value;
             f4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int y = 0; y < U; ++y) {
                 s0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(b.k[0][y]), qv[y], s0, 0, 0, 0);
                 s1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(b.k[1][y]), qv[y], s1, 0, 0, 0);
             }
-            float sv[8];
+            float p[8];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                sv[x] = kb + 8 * g + x <= limit ? s0[x] * a.scale_log2 : -INFINITY;
-                sv[4 + x] = kb + 8 * g + 4 + x <= limit ? s1[x] * a.scale_log2 : -INFINITY;
+                p[x] = s0[x] * a.scale_log2;
+                p[4 + x] = s1[x] * a.scale_log2;
             }
-            float bm = sv[0];
+            if (EDGE)
 #pragma unroll
-            for (int x = 1; x < 8; ++x) bm = fmaxf(bm, sv[x]);
+                for (int x = 0; x < 8; ++x)
+                    if (kb + 8 * g + x > limit) p[x] = -INFINITY;
+            float bm = p[0];
+#pragma unroll
+            for (int x = 1; x < 8; ++x) bm = fmaxf(bm, p[x]);
             bm = fmaxf(bm, __shfl_xor(bm, 16));
             bm = fmaxf(bm, __shfl_xor(bm, 32));
             const float mn = fmaxf(m, bm);
-            const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-            float p[8], ps = 0.f;
+            const float ref = mn == -INFINITY ? 0.f : mn;          // (no key seen yet: probabilities 0, not NaN)
+            const float alpha = __builtin_amdgcn_exp2f(m - ref);
+            float ps = 0.f;
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
-                p[x] = sv[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sv[x] - mn);
+                p[x] = __builtin_amdgcn_exp2f(p[x] - ref);
                 ps += p[x];
             }
             lsum = lsum * alpha + ps;
             m = mn;
-            const uint4 pw = make_uint4(cvt_pk_bf16(p[0], p[1]), cvt_pk_bf16(p[2], p[3]), cvt_pk_bf16(p[4], p[5]),
-                                        cvt_pk_bf16(p[6], p[7]));
-            const bool edge = kb + SO_KB > all;
-            uint4 mk = make_uint4(~0u, ~0u, ~0u, ~0u);
-            bool bad = false;
-            if (edge) {                                  // as in attn_tile_kernel
-                mk = keep_below(kb + 8 * g, seen);
+            const bf16x8_t pb = as_bf16x8(cvt_pk_bf16(p[0], p[1]), cvt_pk_bf16(p[2], p[3]), cvt_pk_bf16(p[4], p[5]),
+                                          cvt_pk_bf16(p[6], p[7]));
 #pragma unroll
-                for (int y = 0; y < DT; ++y) bad = bad || nonfinite8(and4(b.v[y], mk));
-                bad = __ballot(bad) != 0ull;
-            }
+            for (int y = 0; y < DT; ++y)
 #pragma unroll
-            for (int y = 0; y < DT; ++y) {
-                f4 acc = o[y];
+                for (int x = 0; x < 4; ++x) o[y][x] *= alpha;
+            // V of keys nobody sees is dropped, and values that are not finite where some
+            // column does not see their key are added to those that do (attn_tile_kernel)
+            if (EDGE) {
+                const uint4 mk = keep_below(kb + 8 * g, seen);
+                uint32_t bits = 0;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) acc[x] *= alpha;
-                if (!bad) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(and4(b.v[y], mk)), as_bf16x8(pw), acc, 0, 0, 0);
-                o[y] = acc;
-            }
-            if (bad)
-                for (int j = 0; j < 32; ++j) {
-                    const uint4 one = keep_one(j & 7, (j >> 3) == g);
-                    const bool sees = kb + j <= limit;
-#pragma unroll
-                    for (int y = 0; y < DT; ++y) {
-                        const f4 z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(and4(b.v[y], one)), as_bf16x8(and4(pw, one)),
-                                                                             o[y], 0, 0, 0);
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) o[y][x] = sees ? z[x] : o[y][x];
-                    }
+                for (int y = 0; y < DT; ++y) {
+                    b.v[y] = and4(b.v[y], mk);
+                    bits |= nonfinite_bits(b.v[y]);
                 }
+                if (any_nonfinite(bits)) {
+                    // through the wave's part of sm_o, free until the run's end: [D][32] values
+                    uint16_t *vs = reinterpret_cast<uint16_t *>(&sm_o[w][0][0]);
+#pragma unroll
+                    for (int y = 0; y < DT; ++y) *reinterpret_cast<uint4 *>(vs + (16 * y + c) * SO_KB + 8 * g) = b.v[y];
+#pragma unroll 1
+                    for (int j = 0; j < SO_KB; ++j) {
+                        const bool sees = kb + j <= limit;
+                        int quad = g;                    // opaque: no addresses of this rare loop are kept
+                        asm volatile("" : "+v"(quad));
+#pragma unroll
+                        for (int y = 0; y < DT; ++y) {
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                const uint32_t z = vs[(16 * y + 4 * quad + x) * SO_KB + j];
+                                if (sees && (z & 0x7F80u) == 0x7F80u) o[y][x] += bf2f(z);
+                            }
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+#pragma unroll
+                    for (int y = 0; y < DT; ++y)
+                        b.v[y] = finite8(*reinterpret_cast<const uint4 *>(vs + (16 * y + c) * SO_KB + 8 * g));
+                }
+            }
+#pragma unroll
+            for (int y = 0; y < DT; ++y)
+                o[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(b.v[y]), pb, o[y], 0, 0, 0);
         };
-        // 32-key blocks of the run, the four waves in turn; the next block's keys and the
-        // one's after it block numbers are on their way while one is computed
+        // 32-key blocks of the run, the four waves in turn.  At most one of a wave's blocks, its
+        // last, reaches past the keys that every column sees (16 columns are 16 rows at most,
+        // and a wave's blocks are 128 keys apart): that one goes first, on its own copy of the
+        // code.  While a block is computed the next one's keys and the block numbers of the
+        // one after it are on their way
         int kb = tile0 * SO_TILE + SO_KB * w;
         if (kb < k_end) {
-            OwnBlock<D> cur, nxt;
-            Ids x = load_ids(kb), x1 = load_ids(kb + SO_TILE);
-            load(cur, kb, x);
-            while (true) {
-                const int kn = kb + SO_TILE;
-                x = load_ids(kn + SO_TILE);
-                load(nxt, kn < k_end ? kn : kb, x1);
-                compute(cur, kb);
-                if (kn >= k_end) break;
-                const int kn2 = kn + SO_TILE;
-                x1 = load_ids(kn2 + SO_TILE);
-                load(cur, kn2 < k_end ? kn2 : kn, x);
-                compute(nxt, kn);
-                if (kn2 >= k_end) break;
-                kb = kn2;
-            }
+            using Full = std::false_type;
+            const int kl = kb + (k_end - 1 - kb) / SO_TILE * SO_TILE;
+            const bool edge = kl + SO_KB > all;
+            const int stop = edge ? kl : k_end;              // the others end here
+            OwnBlock<D> one, two;
+            Ids x = load_ids(edge ? kl : kb), x1 = load_ids(kb), x2 = load_ids(kb + SO_TILE);
+            if (edge) load(one, kl, x);
+            load(two, min(kb, kl), x1);
+            if (edge) compute(one, kl, std::true_type{});
+            if (kb < stop)
+                while (true) {
+                    const int kn = kb + SO_TILE;
+                    x = load_ids(kn + SO_TILE);
+                    load(one, kn < stop ? kn : kb, kn < stop ? x2 : x1);
+                    compute(two, kb, Full{});
+                    if (kn >= stop) break;
+                    const int kn2 = kn + SO_TILE;
+                    x1 = x;
+                    x2 = load_ids(kn2 + SO_TILE);
+                    load(two, kn2 < stop ? kn2 : kn, x);
+                    compute(one, kn, Full{});
+                    if (kn2 >= stop) break;
+                    kb = kn2;
+                }
         }
         float ltot = lsum + __shfl_xor(lsum, 16);
         ltot += __shfl_xor(ltot, 32);
@@ -735,20 +776,32 @@ __global__ void __launch_bounds__(64 * SO_WAVES) attn_own_kernel(SaArgs a) {
 // One wave a row and q head: the parts of attn_tile_kernel (nsplit), then those of
 // attn_own_kernel for the row's sequence and for the prefix.  out = sum_i 2^(m_i - M) O_i /
 // sum_i 2^(m_i - M) l_i; parts of no key have m = -inf and weight 0, a row of no key at
-// all is 0.
+// all is 0.  The waves go over every row, or, where only sequences of few rows have parts,
+// over per_seq rows of every sequence, if that is less (prompts are then passed over).
 template <int D>
-__global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_parts) {
+__global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_parts, int per_seq) {
     constexpr int PER = D / 64;
-    const long wid = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    constexpr int AHEAD = 8;                 // parts whose values are on their way together
+    const long wid = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     const int rows = live_rows(a);
-    if (wid >= (long)rows * a.H) return;
-    const int row = (int)(wid / a.H), h = (int)(wid - (long)row * a.H);
+    int row = (int)(wid / a.H), r;
+    const int h = (int)(wid - (long)row * a.H);
+    Seq s;
+    if (per_seq) {
+        r = row / per_seq;
+        if (r >= a.R) return;
+        s = seq_of(a, r, rows);
+        const int i = row - r * per_seq;
+        if (i >= s.n || s.n > a.small_rows) return;
+        row = s.first + i;
+    } else {
+        if (row >= rows) return;
+        r = find_seq(a, row);
+        s = seq_of(a, r, rows);
+        if (s.n > a.small_rows && a.nsplit == 1) return;       // written by attn_tile_kernel
+    }
     const int hk = h / a.G, gq = h - hk * a.G;
-    const int r = find_seq(a, row);
-    const Seq s = seq_of(a, r, rows);
-    if (s.n > a.small_rows && a.nsplit == 1) return;           // written by attn_tile_kernel
-    const int total = a.own_off[a.R + 1], run = own_run(a, total);
     float M = -INFINITY, L = 0.f, acc[PER] = {};
     // n parts: (m, l) of part i at ml[i * step], its values at o + i * step * D
     auto take = [&](const float2 *ml, const float *o, long step, int n) {
@@ -756,6 +809,14 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
             const int k = min(64, n - i0);
             float2 x = make_float2(-INFINITY, 0.f);
             if (lane < k) x = ml[(i0 + lane) * step];
+            float v[AHEAD][PER];
+            auto fetch = [&](int i) {
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+                    for (int e = 0; e < PER; ++e) v[j][e] = o[(size_t)(i0 + min(i + j, k - 1)) * step * D + lane + 64 * e];
+            };
+            fetch(0);
             float bm = x.x;
 #pragma unroll
             for (int y = 32; y >= 1; y >>= 1) bm = fmaxf(bm, __shfl_xor(bm, y));
@@ -766,19 +827,30 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
             L = L * alpha + wave_sum(wi * x.y);
 #pragma unroll
             for (int e = 0; e < PER; ++e) acc[e] *= alpha;
-            for (int i = 0; i < k; ++i) {
-                const float wk = __shfl(wi, i);
-                if (wk == 0.f) continue;
-                const float *po = o + (size_t)(i0 + i) * step * D;
+            for (int i = 0; i < k; i += AHEAD) {
+                float u[AHEAD][PER];
 #pragma unroll
-                for (int e = 0; e < PER; ++e) acc[e] += wk * po[lane + 64 * e];
+                for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+                    for (int e = 0; e < PER; ++e) u[j][e] = v[j][e];
+                if (i + AHEAD < k) fetch(i + AHEAD);
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) {
+                    const float wk = i + j < k ? __shfl(wi, i + j) : 0.f;
+#pragma unroll
+                    for (int e = 0; e < PER; ++e) acc[e] += wk == 0.f ? 0.f : wk * u[j][e];
+                }
             }
         }
     };
-    if (tile_parts) take(a.tile_ml + wid, a.tile_o + (size_t)wid * D, (long)a.N * a.H, tile_parts);
+    if (tile_parts) {
+        const long at = (long)row * a.H + h;
+        take(a.tile_ml + at, a.tile_o + (size_t)at * D, (long)a.N * a.H, tile_parts);
+    }
     auto own = [&](int q, int n, int len, int i) {
         const int kt = own_keytiles(len), ct = own_coltiles(a, n);
         if (!kt) return;
+        const int run = own_run(a, a.own_off[a.R + 1]);
         const int col = i * a.G + gq, u = hk * ct + (col >> 4);
         const int t0 = a.own_off[q] + u * kt, w0 = t0 / run, w1 = (t0 + kt - 1) / run;
         const int part = a.own_unit[q] + u + w0;
@@ -796,7 +868,7 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
 // ---------------------------------------------------------------- host side
 
 struct SaPlan {
-    int small_rows, any_big, nsplit, own_prefix, own_wgs, use_tile;
+    int small_rows, rows_max, any_big, nsplit, own_prefix, own_wgs, use_tile;
     long tiles, own_parts;
     long tile_o, tile_ml, own_o, own_ml, own_idx, bytes;       // workspace offsets
 };
@@ -821,6 +893,7 @@ SaPlan plan_shared(long N, long R, long H, long Hkv, long D, long own_cap, long 
     // attn_own_kernel: at most R coltiles of the most rows a sequence has here, and no more
     // than the rows make
     const long rows_max = max_new < p.small_rows ? max_new : p.small_rows;
+    p.rows_max = (int)rows_max;
     long coltiles = R * ((rows_max * G + 15) / 16);
     if (coltiles > R + cols / 16) coltiles = R + cols / 16;
     const long pre = p.own_prefix ? (cols + 15) / 16 : 0;
@@ -849,10 +922,13 @@ int run_shared(const SaArgs &a, const SaPlan &p, hipStream_t stream) {
                            a);
         SC_HIP_CHECK(hipGetLastError());
     }
-    hipLaunchKernelGGL(attn_own_kernel<D>, dim3((unsigned)p.own_wgs), dim3(64 * SO_WAVES), (a.R + 2) * 8, stream, a);
+    auto own = a.shift >= 5 ? attn_own_kernel<D, true> : attn_own_kernel<D, false>;
+    hipLaunchKernelGGL(own, dim3((unsigned)p.own_wgs), dim3(64 * SO_WAVES), (a.R + 2) * 8, stream, a);
     SC_HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL(attn_merge_kernel<D>, dim3((unsigned)(((long)a.N * a.H + 3) / 4)), dim3(256), 0, stream, a,
-                       p.use_tile ? p.nsplit : 0);
+    const bool by_seq = (p.nsplit == 1 || !p.any_big) && (long)a.R * p.rows_max < a.N;
+    const long merge_rows = by_seq ? (long)a.R * p.rows_max : a.N;
+    hipLaunchKernelGGL(attn_merge_kernel<D>, dim3((unsigned)((merge_rows * a.H + 3) / 4)), dim3(256), 0, stream, a,
+                       p.use_tile ? p.nsplit : 0, by_seq ? p.rows_max : 0);
     SC_HIP_CHECK(hipGetLastError());
     return SC_OK;
 }
