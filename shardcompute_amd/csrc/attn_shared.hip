@@ -8,12 +8,12 @@
 // instructions, keys through LDS); read once for all instead of once per sequence.  A
 // sequence's own keys serve its rows alone: few rows (a decoded token, a few guessed ones)
 // make it a stream of memory, many rows (a prompt) a product again.  So:
-//   attn_tile_kernel   128 columns: the prefix, then the own keys of sequences with many
+//   attn_tile    128 columns: the prefix, then the own keys of sequences with many
 //                      rows; over several workgroups where there are few
-//   attn_own_kernel    16 columns: the own keys of sequences with few rows (and the prefix
+//   attn_own     16 columns: the own keys of sequences with few rows (and the prefix
 //                      where all the rows are few), the work cut evenly over the
 //                      workgroups whatever the lengths are
-//   attn_merge_kernel  joins the parts of a row by their softmax maxima and sums
+//   attn_merge_kernel   joins the parts of a row by their softmax maxima and sums
 // Parts are fp32 (O unnormalised, maximum in log2 units, sum).
 //
 // Pool layout as in blocks.hip: K [n_blocks, Hkv, bs, D], Vt [n_blocks, Hkv, D, bs].
@@ -35,8 +35,8 @@ using f4 = dma::f4;
 
 constexpr int SA_COLS = 128, SA_KB = 64, SA_THREADS = 256;
 constexpr int SA_AHEAD = 4;                              // operand reads in flight ahead of the MFMAs
-constexpr int SO_WAVES = 4, SO_KB = 32, SO_TILE = SO_WAVES * SO_KB;      // keys a workgroup takes at a time
-constexpr int SA_MAX_SEQ = 2048;         // attn_own_kernel keeps two numbers of each in LDS
+constexpr int SO_WAVES = 4, SO_KB = 32;
+constexpr int SA_MAX_SEQ = 2048;         // attn_own keeps two numbers of each in LDS
 
 struct SaArgs {
     const uint16_t *q;
@@ -46,13 +46,14 @@ struct SaArgs {
     long out_stride;
     const int32_t *row_starts, *lengths, *tables, *prefix_table, *prefix_len;
     int N, R, H, Hkv, G, width, shift, n_blocks, prefix_width;
-    int small_rows;          // a sequence of at most this many rows is attn_own_kernel's
+    int small_rows;          // a sequence of at most this many rows is attn_own's
     int any_big;             // some sequence may have more
     int nsplit;              // workgroups a column tile's keys are cut into
-    int own_prefix;          // the prefix is attn_own_kernel's
-    int own_wgs;             // attn_own_kernel's workgroups
+    int own_prefix;          // the prefix is attn_own's
+    int tile_wgs, own_wgs;   // their workgroups
+    int tiles, pair_half;    // attn_tile's column tiles; > 0: workgroups of a round, paired with the next round's
     float scale_log2;
-    // parts: of attn_tile_kernel [nsplit][N * H] rows, of attn_own_kernel [own_parts][16] columns
+    // parts: of attn_tile [nsplit][N * H] rows, of attn_own [own_parts][16] columns
     float *tile_o;
     float2 *tile_ml;
     float *own_o;
@@ -155,16 +156,16 @@ __device__ __forceinline__ uint4 and4(uint4 v, uint4 m) { return make_uint4(v.x 
 
 // ONE: a key block lies in one cache block (block sizes from 64 up)
 template <int D, bool ONE>
-__global__ void __launch_bounds__(SA_THREADS) __attribute__((amdgpu_waves_per_eu(2))) attn_tile_kernel(SaArgs a) {
+__device__ __forceinline__ void attn_tile(const SaArgs &a, int id, uint8_t *smem) {
     using Gm = SaGeo<D>;
-    extern __shared__ __align__(16) uint8_t smem[];
-    static_assert(Gm::LDS <= 65536, "no larger dynamic LDS is asked for at the launch");
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 31, lh = lane >> 5;
-    int id = (int)blockIdx.x;
+    // later column tiles (of prompts: more keys) are dispatched first, the first two rounds,
+    // resident together, in heavy and light pairs (an order only: results do not depend on it)
+    if (a.pair_half > 0 && id < 2 * a.pair_half && id >= a.pair_half) id = 3 * a.pair_half - 1 - id;
     const int hk = id % a.Hkv;
     id /= a.Hkv;
-    const int split = id % a.nsplit, tile = id / a.nsplit;
+    const int split = id % a.nsplit, tile = a.tiles - 1 - id / a.nsplit;
     const int rows = live_rows(a);
     const int col = tile * SA_COLS + 32 * w + li;
     const int row = col / a.G, h = hk * a.G + col - row * a.G;
@@ -470,10 +471,16 @@ __global__ void __launch_bounds__(SA_THREADS) __attribute__((amdgpu_waves_per_eu
 // ---------------------------------------------------------------- 16 columns
 //
 // A unit is 16 columns (row i, q head g: column i G + g) of one sequence and kv head; its
-// keys are tiles of 128.  All units' tiles in a line (sequence, kv head, 16 columns, key
-// tile) are cut into own_wgs equal runs, one a workgroup, whatever the lengths are; a
-// run's share of a unit is one part, number unit + workgroup (two consecutive runs meet
-// in one unit at most, so the numbers differ).  "Sequence" R is the prefix, with all rows.
+// keys are blocks of 32, each one wave's work: S^T[32 keys x 16] = K Q^T and O^T[D x 16] +=
+// Vt P^T on v_mfma_f32_16x16x32_bf16, K and Vt straight into registers, the keys permuted on
+// their way so that lane group g = lane / 16 holds the 8 consecutive keys 8 g .. 8 g + 7
+// of the block (as the dense decode attention does).  All units' blocks in a line (sequence,
+// kv head, 16 columns, key block) are cut into equal runs, one a wave, whatever the lengths
+// are.  A run's share of a unit is one part, number unit + wave (two consecutive runs meet in
+// one unit at most, so the numbers differ).  "Sequence" R is the prefix, with all rows.
+//
+// Bound by memory: a wave has the next block's loads (16 KB at head_dim 128) in flight
+// while it computes one, also from one unit into the next, and no wave waits for another.
 template <typename F>
 __device__ __forceinline__ void own_shape(const SaArgs &a, int r, int rows, int P, F &&f) {
     // f(first row, rows, keys)
@@ -485,9 +492,12 @@ __device__ __forceinline__ void own_shape(const SaArgs &a, int r, int rows, int 
     }
 }
 __device__ __forceinline__ int own_coltiles(const SaArgs &a, int n) { return (n * a.G + 15) >> 4; }
-__device__ __forceinline__ int own_keytiles(int len) { return (len + SO_TILE - 1) / SO_TILE; }
-// tiles a workgroup takes of `total`
-__device__ __forceinline__ int own_run(const SaArgs &a, int total) { return max((total + a.own_wgs - 1) / a.own_wgs, 1); }
+__device__ __forceinline__ int own_keyblocks(int len) { return (len + SO_KB - 1) / SO_KB; }
+// blocks a wave takes of `total`
+__device__ __forceinline__ int own_run(const SaArgs &a, int total) {
+    const int waves = a.own_wgs * SO_WAVES;
+    return max((total + waves - 1) / waves, 1);
+}
 
 template <int D>
 struct OwnBlock {
@@ -495,21 +505,25 @@ struct OwnBlock {
     uint4 v[D / 16];
 };
 
-// ONE: 32 keys lie in one cache block (block sizes from 32 up)
+// LDS of a workgroup, off[R + 2] and unit[R + 2] behind it
+template <int D>
+struct OwnLds {
+    uint16_t v[SO_WAVES][D][SO_KB];          // a wave's Vt block, where it holds values that are not finite
+    int wsum[2][SO_WAVES];
+};
+
+// ONE: 32 keys lie in one cache block
 template <int D, bool ONE>
-__global__ void __launch_bounds__(64 * SO_WAVES) __attribute__((amdgpu_waves_per_eu(2))) attn_own_kernel(SaArgs a) {
+__device__ __forceinline__ void attn_own(const SaArgs &a, int wg, uint8_t *smem) {
     constexpr int U = D / 32, DT = D / 16;
-    extern __shared__ int32_t seq_lds[];                 // off[R + 2], unit[R + 2]
-    __shared__ float sm_m[SO_WAVES][16], sm_l[SO_WAVES][16];
-    __shared__ __align__(16) float sm_o[SO_WAVES][D][17];
-    __shared__ int wsum[2][SO_WAVES];
-    int32_t *off = seq_lds, *unit = seq_lds + a.R + 2;
+    OwnLds<D> &lds = *reinterpret_cast<OwnLds<D> *>(smem);
+    int32_t *off = reinterpret_cast<int32_t *>(smem + sizeof(OwnLds<D>)), *unit = off + a.R + 2;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
     const int rows = live_rows(a), P = prefix_keys(a);
     const int sh = a.shift, bs = 1 << sh;
 
-    // first tile and unit of every sequence
+    // first block and unit of every sequence
     {
         int t_before = 0, u_before = 0;
         for (int r0 = 0; r0 <= a.R; r0 += 64 * SO_WAVES) {
@@ -517,7 +531,7 @@ __global__ void __launch_bounds__(64 * SO_WAVES) __attribute__((amdgpu_waves_per
             int t = 0, u = 0;
             if (r <= a.R)
                 own_shape(a, r, rows, P, [&](int, int n, int len) {
-                    const int kt = own_keytiles(len);
+                    const int kt = own_keyblocks(len);
                     u = kt ? a.Hkv * own_coltiles(a, n) : 0;
                     t = u * kt;
                 });
@@ -527,33 +541,32 @@ __global__ void __launch_bounds__(64 * SO_WAVES) __attribute__((amdgpu_waves_per
                 const int t2 = __shfl_up(ts, x), u2 = __shfl_up(us, x);
                 if (lane >= x) { ts += t2; us += u2; }
             }
-            if (lane == 63) { wsum[0][w] = ts; wsum[1][w] = us; }
+            if (lane == 63) { lds.wsum[0][w] = ts; lds.wsum[1][w] = us; }
             __syncthreads();
             int tb = t_before, ub = u_before;
             for (int i = 0; i < SO_WAVES; ++i) {
-                if (i < w) { tb += wsum[0][i]; ub += wsum[1][i]; }
-                t_before += wsum[0][i];
-                u_before += wsum[1][i];
+                if (i < w) { tb += lds.wsum[0][i]; ub += lds.wsum[1][i]; }
+                t_before += lds.wsum[0][i];
+                u_before += lds.wsum[1][i];
             }
             if (r <= a.R) { off[r] = tb + ts - t; unit[r] = ub + us - u; }
             __syncthreads();
         }
         if (tid == 0) { off[a.R + 1] = t_before; unit[a.R + 1] = u_before; }
         __syncthreads();
-        if (blockIdx.x == 0)
+        if (wg == 0)
             for (int r = tid; r < a.R + 2; r += 64 * SO_WAVES) { a.own_off[r] = off[r]; a.own_unit[r] = unit[r]; }
     }
-    const int total = off[a.R + 1], run = own_run(a, total);
-    int t = (int)min((long)blockIdx.x * run, (long)total);
+    const int wave = wg * SO_WAVES + w;
+    const int total = __builtin_amdgcn_readfirstlane(off[a.R + 1]), run = own_run(a, total);
+    int t = (int)min((long)wave * run, (long)total);
     const int t_end = min(t + run, total);
+    if (t >= t_end) return;
     int r = 0;
-    if (t < t_end) {
-        int n = a.R + 1;
-        while (n > 1) {
-            const int half = n >> 1;
-            if (off[r + half] <= t) { r += half; n -= half; }
-            else n = half;
-        }
+    for (int n = a.R + 1; n > 1;) {
+        const int half = n >> 1;
+        if (off[r + half] <= t) { r += half; n -= half; }
+        else n = half;
     }
     const size_t blk_bytes = (size_t)a.Hkv * D * 2 << sh;
     // byte offsets of this lane within a cache block of one kv head: key 8 (c / 4) + c % 4
@@ -561,227 +574,239 @@ __global__ void __launch_bounds__(64 * SO_WAVES) __attribute__((amdgpu_waves_per
     const int krow = 8 * (c >> 2) + (c & 3);
     const uint32_t koff = (uint32_t)((ONE ? krow : krow & 15) * D * 2 + 16 * g);
     const uint32_t voff = ((uint32_t)c << sh) * 2 + (ONE ? 16 * g : 16 * (g & 1));
-    for (; t < t_end;) {
+
+    // the wave's share of one unit
+    struct Run {
+        const int32_t *table;
+        int width, hk, part, first, cols0, n;
+        int kb, stop;            // the next key block, and the key its blocks end at
+        int all, seen;           // keys that every, that some column sees
+        int rel;                 // the unit's row i sees keys up to rel + i (the prefix: up to rel)
+        bool pre;
+    };
+    auto open = [&]() {          // at block t; t moves to the end of the share
         while (off[r + 1] <= t) ++r;
         r = __builtin_amdgcn_readfirstlane(r);
-        int first = 0, n = 0, len = 0;
-        own_shape(a, r, rows, P, [&](int f, int nn, int l) { first = f; n = nn; len = l; });
-        const int kt = own_keytiles(len), ct = own_coltiles(a, n);
-        const int lt = t - __builtin_amdgcn_readfirstlane(off[r]), u = lt / kt, tile0 = lt - u * kt;
-        const int tile1 = min(kt, tile0 + t_end - t);
-        const int hk = u / ct, cols0 = (u - hk * ct) * 16;
-        const bool pre = r == a.R;
-        const int32_t *table = pre ? a.prefix_table : a.tables + (size_t)r * a.width;
-        const int width = pre ? a.prefix_width : a.width;
-        const int part = __builtin_amdgcn_readfirstlane(unit[r]) + u + (int)blockIdx.x;
-        t += tile1 - tile0;
-
-        const int i = (cols0 + c) / a.G, gq = cols0 + c - i * a.G;
-        const bool col_ok = i < n;
-        const int row = first + i, h = hk * a.G + gq;
-        const int last = min((cols0 + 15) / a.G, n - 1);              // the last row of the unit
-        const int limit = !col_ok ? -1 : pre ? P - 1 : len - n + i;
-        const int seen = pre ? P : clampi(len - n + last + 1, 0, len);         // keys some column sees
-        const int all = pre ? P : clampi(len - n + cols0 / a.G + 1, 0, len);   // keys every column sees
-        bf16x8_t qv[U];
+        int len = 0;
+        Run s;
+        own_shape(a, r, rows, P, [&](int f, int nn, int l) { s.first = f; s.n = nn; len = l; });
+        const int kt = own_keyblocks(len), ct = own_coltiles(a, s.n);
+        const int lt = t - __builtin_amdgcn_readfirstlane(off[r]), u = lt / kt, b0 = lt - u * kt;
+        const int b1 = min(kt, b0 + t_end - t);
+        s.pre = r == a.R;
+        s.hk = u / ct;
+        s.cols0 = (u - s.hk * ct) * 16;
+        s.table = s.pre ? a.prefix_table : a.tables + (size_t)r * a.width;
+        s.width = s.pre ? a.prefix_width : a.width;
+        s.part = __builtin_amdgcn_readfirstlane(unit[r]) + u + wave;
+        s.kb = b0 * SO_KB;
+        s.stop = b1 * SO_KB;
+        s.rel = s.pre ? P - 1 : len - s.n;
+        const int last = min((s.cols0 + 15) / a.G, s.n - 1);                 // the unit's last row
+        s.seen = s.pre ? P : clampi(s.rel + last + 1, 0, len);
+        s.all = s.pre ? P : clampi(s.rel + s.cols0 / a.G + 1, 0, len);
+        t += b1 - b0;
+        return s;
+    };
+    bf16x8_t qv[U];
+    float m, lsum;
+    f4 o[DT];
+    int limit;                   // the last key this lane's column sees
+    auto begin = [&](const Run &s) {
+        const int i = (s.cols0 + c) / a.G, h = s.hk * a.G + s.cols0 + c - i * a.G;
+        const bool ok = i < s.n;
+        limit = !ok ? -1 : s.pre ? s.rel : s.rel + i;
 #pragma unroll
         for (int x = 0; x < U; ++x) {
             uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (col_ok) v = *reinterpret_cast<const uint4 *>(a.q + (size_t)row * a.q_stride + (size_t)h * D + 32 * x + 8 * g);
+            if (ok) v = *reinterpret_cast<const uint4 *>(a.q + (size_t)(s.first + i) * a.q_stride + (size_t)h * D + 32 * x + 8 * g);
             qv[x] = as_bf16x8(v);
         }
-        const char *kpool = reinterpret_cast<const char *>(a.kc) + ((size_t)hk * D * 2 << sh);
-        const char *vpool = reinterpret_cast<const char *>(a.vt) + ((size_t)hk * D * 2 << sh);
-        float m = -INFINITY, lsum = 0.f;
-        f4 o[DT];
+        m = -INFINITY;
+        lsum = 0.f;
 #pragma unroll
         for (int x = 0; x < DT; ++x) o[x] = f4{0.f, 0.f, 0.f, 0.f};
-
-        const int k_end = min(tile1 * SO_TILE, seen);
-        // the cache blocks of 32 keys (one, or those of this lane's K and Vt halves)
-        struct Ids { int k, v; };
-        auto load_ids = [&](int kb) {
-            kb = min(kb, max(k_end - 1, 0));
-            Ids x;
-            x.k = table[min((ONE ? kb : kb + 16 * (c >> 3)) >> sh, width - 1)];
-            x.v = ONE ? 0 : table[min((kb + 16 * (g >> 1)) >> sh, width - 1)];
-            return x;
-        };
-        auto load = [&](OwnBlock<D> &b, int kb, Ids x) {
-            auto take = [&](const char *kp, const char *vp) {
-#pragma unroll
-                for (int y = 0; y < U; ++y) {
-                    b.k[0][y] = *reinterpret_cast<const uint4 *>(kp + koff + 64 * y);
-                    b.k[1][y] = *reinterpret_cast<const uint4 *>(kp + koff + 64 * y + 8 * D);
-                }
-#pragma unroll
-                for (int y = 0; y < DT; ++y) b.v[y] = *reinterpret_cast<const uint4 *>(vp + (voff + ((uint32_t)y << (sh + 5))));
-            };
-            if (ONE) {
-                const size_t at = (size_t)clampi(__builtin_amdgcn_readfirstlane(x.k), 0, a.n_blocks - 1) * blk_bytes;
-                const int k0 = kb & (bs - 1);
-                take(kpool + at + (size_t)k0 * (D * 2), vpool + at + (size_t)k0 * 2);
-            } else {
-                take(kpool + (size_t)clampi(x.k, 0, a.n_blocks - 1) * blk_bytes,
-                     vpool + (size_t)clampi(x.v, 0, a.n_blocks - 1) * blk_bytes);
-            }
-        };
-        // EDGE: some column does not see all the 32 keys
-        auto compute = [&](OwnBlock<D> &b, int kb, auto edge_tag) {
-            constexpr bool EDGE = decltype(edge_tag)::value;
-            f4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
+    };
+    // the cache blocks of 32 keys (one, or those of this lane's K and Vt halves)
+    struct Ids { int k, v; };
+    auto load_ids = [&](const Run &s, int kb) {
+        kb = min(kb, s.stop - SO_KB);
+        Ids x;
+        x.k = s.table[min((ONE ? kb : kb + 16 * (c >> 3)) >> sh, s.width - 1)];
+        x.v = ONE ? 0 : s.table[min((kb + 16 * (g >> 1)) >> sh, s.width - 1)];
+        return x;
+    };
+    auto load = [&](OwnBlock<D> &b, const Run &s, Ids x) {
+        const char *kpool = reinterpret_cast<const char *>(a.kc) + ((size_t)s.hk * D * 2 << sh);
+        const char *vpool = reinterpret_cast<const char *>(a.vt) + ((size_t)s.hk * D * 2 << sh);
+        auto take = [&](const char *kp, const char *vp) {
 #pragma unroll
             for (int y = 0; y < U; ++y) {
-                s0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(b.k[0][y]), qv[y], s0, 0, 0, 0);
-                s1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(b.k[1][y]), qv[y], s1, 0, 0, 0);
-            }
-            float p[8];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                p[x] = s0[x] * a.scale_log2;
-                p[4 + x] = s1[x] * a.scale_log2;
-            }
-            if (EDGE)
-#pragma unroll
-                for (int x = 0; x < 8; ++x)
-                    if (kb + 8 * g + x > limit) p[x] = -INFINITY;
-            float bm = p[0];
-#pragma unroll
-            for (int x = 1; x < 8; ++x) bm = fmaxf(bm, p[x]);
-            bm = fmaxf(bm, __shfl_xor(bm, 16));
-            bm = fmaxf(bm, __shfl_xor(bm, 32));
-            const float mn = fmaxf(m, bm);
-            const float ref = mn == -INFINITY ? 0.f : mn;          // (no key seen yet: probabilities 0, not NaN)
-            const float alpha = __builtin_amdgcn_exp2f(m - ref);
-            float ps = 0.f;
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {
-                p[x] = __builtin_amdgcn_exp2f(p[x] - ref);
-                ps += p[x];
-            }
-            lsum = lsum * alpha + ps;
-            m = mn;
-            const bf16x8_t pb = as_bf16x8(cvt_pk_bf16(p[0], p[1]), cvt_pk_bf16(p[2], p[3]), cvt_pk_bf16(p[4], p[5]),
-                                          cvt_pk_bf16(p[6], p[7]));
-#pragma unroll
-            for (int y = 0; y < DT; ++y)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) o[y][x] *= alpha;
-            // V of keys nobody sees is dropped, and values that are not finite where some
-            // column does not see their key are added to those that do (attn_tile_kernel)
-            if (EDGE) {
-                const uint4 mk = keep_below(kb + 8 * g, seen);
-                uint32_t bits = 0;
-#pragma unroll
-                for (int y = 0; y < DT; ++y) {
-                    b.v[y] = and4(b.v[y], mk);
-                    bits |= nonfinite_bits(b.v[y]);
-                }
-                if (any_nonfinite(bits)) {
-                    // through the wave's part of sm_o, free until the run's end: [D][32] values
-                    uint16_t *vs = reinterpret_cast<uint16_t *>(&sm_o[w][0][0]);
-#pragma unroll
-                    for (int y = 0; y < DT; ++y) *reinterpret_cast<uint4 *>(vs + (16 * y + c) * SO_KB + 8 * g) = b.v[y];
-#pragma unroll 1
-                    for (int j = 0; j < SO_KB; ++j) {
-                        const bool sees = kb + j <= limit;
-                        int quad = g;                    // opaque: no addresses of this rare loop are kept
-                        asm volatile("" : "+v"(quad));
-#pragma unroll
-                        for (int y = 0; y < DT; ++y) {
-#pragma unroll
-                            for (int x = 0; x < 4; ++x) {
-                                const uint32_t z = vs[(16 * y + 4 * quad + x) * SO_KB + j];
-                                if (sees && (z & 0x7F80u) == 0x7F80u) o[y][x] += bf2f(z);
-                            }
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
-                    }
-#pragma unroll
-                    for (int y = 0; y < DT; ++y)
-                        b.v[y] = finite8(*reinterpret_cast<const uint4 *>(vs + (16 * y + c) * SO_KB + 8 * g));
-                }
+                b.k[0][y] = *reinterpret_cast<const uint4 *>(kp + koff + 64 * y);
+                b.k[1][y] = *reinterpret_cast<const uint4 *>(kp + koff + 64 * y + 8 * D);
             }
 #pragma unroll
-            for (int y = 0; y < DT; ++y)
-                o[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(b.v[y]), pb, o[y], 0, 0, 0);
+            for (int y = 0; y < DT; ++y) b.v[y] = *reinterpret_cast<const uint4 *>(vp + (voff + ((uint32_t)y << (sh + 5))));
         };
-        // 32-key blocks of the run, the four waves in turn.  At most one of a wave's blocks, its
-        // last, reaches past the keys that every column sees (16 columns are 16 rows at most,
-        // and a wave's blocks are 128 keys apart): that one goes first, on its own copy of the
-        // code.  While a block is computed the next one's keys and the block numbers of the
-        // one after it are on their way
-        int kb = tile0 * SO_TILE + SO_KB * w;
-        if (kb < k_end) {
-            using Full = std::false_type;
-            const int kl = kb + (k_end - 1 - kb) / SO_TILE * SO_TILE;
-            const bool edge = kl + SO_KB > all;
-            const int stop = edge ? kl : k_end;              // the others end here
-            OwnBlock<D> one, two;
-            Ids x = load_ids(edge ? kl : kb), x1 = load_ids(kb), x2 = load_ids(kb + SO_TILE);
-            if (edge) load(one, kl, x);
-            load(two, min(kb, kl), x1);
-            if (edge) compute(one, kl, std::true_type{});
-            if (kb < stop)
-                while (true) {
-                    const int kn = kb + SO_TILE;
-                    x = load_ids(kn + SO_TILE);
-                    load(one, kn < stop ? kn : kb, kn < stop ? x2 : x1);
-                    compute(two, kb, Full{});
-                    if (kn >= stop) break;
-                    const int kn2 = kn + SO_TILE;
-                    x1 = x;
-                    x2 = load_ids(kn2 + SO_TILE);
-                    load(two, kn2 < stop ? kn2 : kn, x);
-                    compute(one, kn, Full{});
-                    if (kn2 >= stop) break;
-                    kb = kn2;
-                }
+        if (ONE) {
+            const size_t at = (size_t)clampi(__builtin_amdgcn_readfirstlane(x.k), 0, a.n_blocks - 1) * blk_bytes;
+            const int k0 = s.kb & (bs - 1);
+            take(kpool + at + (size_t)k0 * (D * 2), vpool + at + (size_t)k0 * 2);
+        } else {
+            const int kk = (s.kb + 16 * (c >> 3)) & (bs - 1), kv = (s.kb + 16 * (g >> 1)) & (bs - 1);
+            take(kpool + (size_t)clampi(x.k, 0, a.n_blocks - 1) * blk_bytes + kk * (D * 2),
+                 vpool + (size_t)clampi(x.v, 0, a.n_blocks - 1) * blk_bytes + kv * 2);
         }
-        float ltot = lsum + __shfl_xor(lsum, 16);
-        ltot += __shfl_xor(ltot, 32);
-        if (g == 0) { sm_m[w][c] = m; sm_l[w][c] = ltot; }
+    };
+    // EDGE: some column does not see all the 32 keys
+    auto compute = [&](OwnBlock<D> &b, const Run &s, auto edge_tag) {
+        constexpr bool EDGE = decltype(edge_tag)::value;
+        const int kb = s.kb;
+        f4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int y = 0; y < U; ++y) {
+            s0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(b.k[0][y]), qv[y], s0, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(b.k[1][y]), qv[y], s1, 0, 0, 0);
+        }
+        float p[8];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            p[x] = s0[x] * a.scale_log2;
+            p[4 + x] = s1[x] * a.scale_log2;
+        }
+        if (EDGE)
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+                if (kb + 8 * g + x > limit) p[x] = -INFINITY;
+        float bm = p[0];
+#pragma unroll
+        for (int x = 1; x < 8; ++x) bm = fmaxf(bm, p[x]);
+        bm = fmaxf(bm, __shfl_xor(bm, 16));
+        bm = fmaxf(bm, __shfl_xor(bm, 32));
+        const float mn = fmaxf(m, bm);
+        const float ref = mn == -INFINITY ? 0.f : mn;          // (no key seen yet: probabilities 0, not NaN)
+        const float alpha = __builtin_amdgcn_exp2f(m - ref);
+        float ps = 0.f;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            p[x] = __builtin_amdgcn_exp2f(p[x] - ref);
+            ps += p[x];
+        }
+        lsum = lsum * alpha + ps;
+        m = mn;
+        const bf16x8_t pb = as_bf16x8(cvt_pk_bf16(p[0], p[1]), cvt_pk_bf16(p[2], p[3]), cvt_pk_bf16(p[4], p[5]),
+                                      cvt_pk_bf16(p[6], p[7]));
 #pragma unroll
         for (int y = 0; y < DT; ++y)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) sm_o[w][16 * y + 4 * g + x][c] = o[y][x];
-        __syncthreads();
-        const int cc = tid & 15, d0 = tid >> 4;
-        if (part < a.own_parts) {
-            float M = sm_m[0][cc];
+            for (int x = 0; x < 4; ++x) o[y][x] *= alpha;
+        // V of keys nobody sees is dropped, and values that are not finite where some
+        // column does not see their key are added to those that do (as in attn_tile)
+        if (EDGE) {
+            const uint4 mk = keep_below(kb + 8 * g, s.seen);
+            uint32_t bits = 0;
 #pragma unroll
-            for (int x = 1; x < SO_WAVES; ++x) M = fmaxf(M, sm_m[x][cc]);
-            float wt[SO_WAVES], L = 0.f;
-#pragma unroll
-            for (int x = 0; x < SO_WAVES; ++x) {
-                wt[x] = sm_m[x][cc] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm_m[x][cc] - M);
-                L += wt[x] * sm_l[x][cc];
+            for (int y = 0; y < DT; ++y) {
+                b.v[y] = and4(b.v[y], mk);
+                bits |= nonfinite_bits(b.v[y]);
             }
-            float *po = a.own_o + ((size_t)part * 16 + cc) * D;
+            if (any_nonfinite(bits)) {
+                uint16_t *vs = &lds.v[w][0][0];
 #pragma unroll
-            for (int y = 0; y < D / 16; ++y) {
-                float acc = 0.f;
+                for (int y = 0; y < DT; ++y) *reinterpret_cast<uint4 *>(vs + (16 * y + c) * SO_KB + 8 * g) = b.v[y];
+#pragma unroll 1
+                for (int j = 0; j < SO_KB; ++j) {
+                    const bool sees = kb + j <= limit;
+                    int quad = g;                        // opaque: no addresses of this rare loop are kept
+                    asm volatile("" : "+v"(quad));
 #pragma unroll
-                for (int x = 0; x < SO_WAVES; ++x) acc += wt[x] * sm_o[x][d0 + 16 * y][cc];
-                po[d0 + 16 * y] = acc;
+                    for (int y = 0; y < DT; ++y) {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const uint32_t z = vs[(16 * y + 4 * quad + x) * SO_KB + j];
+                            if (sees && (z & 0x7F80u) == 0x7F80u) o[y][x] += bf2f(z);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+#pragma unroll
+                for (int y = 0; y < DT; ++y)
+                    b.v[y] = finite8(*reinterpret_cast<const uint4 *>(vs + (16 * y + c) * SO_KB + 8 * g));
             }
-            if (d0 == 0) a.own_ml[(size_t)part * 16 + cc] = make_float2(M, L);
         }
-        __syncthreads();
-    }
+#pragma unroll
+        for (int y = 0; y < DT; ++y)
+            o[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(b.v[y]), pb, o[y], 0, 0, 0);
+    };
+    auto end = [&](const Run &s) {           // the part: the unit's columns that are there
+        float ltot = lsum + __shfl_xor(lsum, 16);
+        ltot += __shfl_xor(ltot, 32);
+        if ((s.cols0 + c) / a.G >= s.n || s.part >= a.own_parts) return;
+        const size_t at = (size_t)s.part * 16 + c;
+        float *po = a.own_o + at * D + 4 * g;
+#pragma unroll
+        for (int y = 0; y < DT; ++y) *reinterpret_cast<f4 *>(po + 16 * y) = o[y];
+        if (g == 0) a.own_ml[at] = make_float2(m, ltot);
+    };
+
+    // two blocks in turn: while one is computed the next one's loads (of the next unit's,
+    // after a unit's last) and the cache block numbers of the one after it are on their way.
+    // The loads are unconditional (past the run's end the last block again): with loads on
+    // some paths only the compiler would wait for all of them before it computes
+    OwnBlock<D> one, two;
+    Run s = open();
+    Ids ids = load_ids(s, s.kb), ids1 = load_ids(s, s.kb + SO_KB);
+    begin(s);
+    load(one, s, ids);
+    auto half = [&](OwnBlock<D> &cur, OwnBlock<D> &nxt) {
+        const bool last = s.kb + SO_KB >= s.stop, done = last && t >= t_end;
+        Run n = s;
+        if (!last) n.kb += SO_KB;
+        else if (!done) {
+            n = open();
+            ids1 = load_ids(n, n.kb);
+        }
+        ids = ids1;
+        ids1 = load_ids(n, n.kb + SO_KB);
+        load(nxt, n, ids);
+        if (s.kb + SO_KB <= s.all) compute(cur, s, std::false_type{});
+        else compute(cur, s, std::true_type{});
+        if (last) {
+            end(s);
+            if (!done) begin(n);
+        }
+        s = n;
+        return done;
+    };
+    while (!half(one, two) && !half(two, one)) {}
+}
+
+// ---------------------------------------------------------------- both
+//
+// One launch: the own workgroups, which wait for memory, run beside tile workgroups, which
+// keep the matrix units busy.
+template <int D, bool ONE>
+__global__ void __launch_bounds__(SA_THREADS) __attribute__((amdgpu_waves_per_eu(2))) attn_shared_kernel(SaArgs a) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    if ((int)blockIdx.x < a.tile_wgs) attn_tile<D, ONE>(a, (int)blockIdx.x, smem);
+    else attn_own<D, ONE>(a, (int)blockIdx.x - a.tile_wgs, smem);
 }
 
 // ---------------------------------------------------------------- merge
 //
-// One wave a row and q head: the parts of attn_tile_kernel (nsplit), then those of
-// attn_own_kernel for the row's sequence and for the prefix.  out = sum_i 2^(m_i - M) O_i /
+// One wave a row and q head: the parts of attn_tile (nsplit), then those of
+// attn_own for the row's sequence and for the prefix.  out = sum_i 2^(m_i - M) O_i /
 // sum_i 2^(m_i - M) l_i; parts of no key have m = -inf and weight 0, a row of no key at
 // all is 0.  The waves go over every row, or, where only sequences of few rows have parts,
 // over per_seq rows of every sequence, if that is less (prompts are then passed over).
+//
+// Bound by the latency of dependent loads, so there are two rounds of them: what says where
+// the parts are, then the parts, lane i holding part i's place and (m, l), the values of
+// AHEAD parts on their way together.
 template <int D>
 __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_parts, int per_seq) {
     constexpr int PER = D / 64;
-    constexpr int AHEAD = 8;                 // parts whose values are on their way together
+    constexpr int AHEAD = 8;
     const long wid = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     const int rows = live_rows(a);
@@ -799,66 +824,71 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
         if (row >= rows) return;
         r = find_seq(a, row);
         s = seq_of(a, r, rows);
-        if (s.n > a.small_rows && a.nsplit == 1) return;       // written by attn_tile_kernel
+        if (s.n > a.small_rows && a.nsplit == 1) return;       // written by attn_tile
     }
     const int hk = h / a.G, gq = h - hk * a.G;
-    float M = -INFINITY, L = 0.f, acc[PER] = {};
-    // n parts: (m, l) of part i at ml[i * step], its values at o + i * step * D
-    auto take = [&](const float2 *ml, const float *o, long step, int n) {
-        for (int i0 = 0; i0 < n; i0 += 64) {
-            const int k = min(64, n - i0);
-            float2 x = make_float2(-INFINITY, 0.f);
-            if (lane < k) x = ml[(i0 + lane) * step];
-            float v[AHEAD][PER];
-            auto fetch = [&](int i) {
-#pragma unroll
-                for (int j = 0; j < AHEAD; ++j)
-#pragma unroll
-                    for (int e = 0; e < PER; ++e) v[j][e] = o[(size_t)(i0 + min(i + j, k - 1)) * step * D + lane + 64 * e];
-            };
-            fetch(0);
-            float bm = x.x;
-#pragma unroll
-            for (int y = 32; y >= 1; y >>= 1) bm = fmaxf(bm, __shfl_xor(bm, y));
-            if (bm == -INFINITY) continue;
-            const float mn = fmaxf(M, bm), alpha = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mn);
-            const float wi = x.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x.x - mn);
-            M = mn;
-            L = L * alpha + wave_sum(wi * x.y);
-#pragma unroll
-            for (int e = 0; e < PER; ++e) acc[e] *= alpha;
-            for (int i = 0; i < k; i += AHEAD) {
-                float u[AHEAD][PER];
-#pragma unroll
-                for (int j = 0; j < AHEAD; ++j)
-#pragma unroll
-                    for (int e = 0; e < PER; ++e) u[j][e] = v[j][e];
-                if (i + AHEAD < k) fetch(i + AHEAD);
-#pragma unroll
-                for (int j = 0; j < AHEAD; ++j) {
-                    const float wk = i + j < k ? __shfl(wi, i + j) : 0.f;
-#pragma unroll
-                    for (int e = 0; e < PER; ++e) acc[e] += wk == 0.f ? 0.f : wk * u[j][e];
-                }
-            }
-        }
-    };
-    if (tile_parts) {
-        const long at = (long)row * a.H + h;
-        take(a.tile_ml + at, a.tile_o + (size_t)at * D, (long)a.N * a.H, tile_parts);
-    }
-    auto own = [&](int q, int n, int len, int i) {
-        const int kt = own_keytiles(len), ct = own_coltiles(a, n);
-        if (!kt) return;
-        const int run = own_run(a, a.own_off[a.R + 1]);
+    const int run = own_run(a, a.own_off[a.R + 1]);
+    // attn_own's parts of row i of n: the first one's number, and how many
+    auto own = [&](int q, int n, int len, int i, int &first, int &count, int &c) {
+        const int kt = own_keyblocks(len), ct = own_coltiles(a, n);
         const int col = i * a.G + gq, u = hk * ct + (col >> 4);
         const int t0 = a.own_off[q] + u * kt, w0 = t0 / run, w1 = (t0 + kt - 1) / run;
-        const int part = a.own_unit[q] + u + w0;
-        if (part + w1 - w0 >= a.own_parts) return;
-        take(a.own_ml + (size_t)part * 16 + (col & 15), a.own_o + ((size_t)part * 16 + (col & 15)) * D, 16, w1 - w0 + 1);
+        first = a.own_unit[q] + u + w0;
+        count = kt && first + w1 - w0 < a.own_parts ? w1 - w0 + 1 : 0;
+        c = col & 15;
     };
-    if (s.n <= a.small_rows) own(r, s.n, s.len, row - s.first);
-    if (a.own_prefix) own(a.R, rows, prefix_keys(a), row);
+    int f1 = 0, n1 = 0, c1 = 0, f2 = 0, n2 = 0, c2 = 0;
+    if (s.n <= a.small_rows) own(r, s.n, s.len, row - s.first, f1, n1, c1);
+    if (a.own_prefix) own(a.R, rows, prefix_keys(a), row, f2, n2, c2);
+    const int parts = tile_parts + n1 + n2;
+    float M = -INFINITY, L = 0.f, acc[PER] = {};
+    for (int i0 = 0; i0 < parts; i0 += 64) {
+        // part i0 + lane: its number among attn_tile's or attn_own's parts
+        const int i = min(i0 + lane, parts - 1), j = i - tile_parts;
+        const bool t = j < 0;
+        const long at = t ? ((long)i * a.N + row) * a.H + h : j < n1 ? (f1 + j) * 16L + c1 : (f2 + j - n1) * 16L + c2;
+        const int k = min(64, parts - i0);
+        float2 x = (t ? a.tile_ml : a.own_ml)[at];
+        if (lane >= k) x = make_float2(-INFINITY, 0.f);
+        const float *const po = (t ? a.tile_o : a.own_o) + at * D;
+        const uint32_t plo = (uint32_t)(uintptr_t)po, phi = (uint32_t)((uintptr_t)po >> 32);
+        float v[AHEAD][PER];
+        auto fetch = [&](int i) {
+#pragma unroll
+            for (int e = 0; e < AHEAD; ++e) {
+                const int y = min(i + e, k - 1);
+                const uintptr_t p = (uintptr_t)__builtin_amdgcn_readlane(plo, y) & 0xFFFFFFFFu;
+                const float *o = reinterpret_cast<const float *>(p | (uintptr_t)(uint32_t)__builtin_amdgcn_readlane(phi, y) << 32);
+#pragma unroll
+                for (int z = 0; z < PER; ++z) v[e][z] = o[lane + 64 * z];
+            }
+        };
+        fetch(0);
+        float bm = x.x;
+#pragma unroll
+        for (int y = 32; y >= 1; y >>= 1) bm = fmaxf(bm, __shfl_xor(bm, y));
+        if (bm == -INFINITY) continue;
+        const float mn = fmaxf(M, bm), alpha = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mn);
+        const float wi = x.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x.x - mn);
+        M = mn;
+        L = L * alpha + wave_sum(wi * x.y);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[e] *= alpha;
+        for (int i = 0; i < k; i += AHEAD) {
+            float u[AHEAD][PER];
+#pragma unroll
+            for (int e = 0; e < AHEAD; ++e)
+#pragma unroll
+                for (int z = 0; z < PER; ++z) u[e][z] = v[e][z];
+            if (i + AHEAD < k) fetch(i + AHEAD);
+#pragma unroll
+            for (int e = 0; e < AHEAD; ++e) {
+                const float wk = i + e < k ? __shfl(wi, min(i + e, 63)) : 0.f;
+#pragma unroll
+                for (int z = 0; z < PER; ++z) acc[z] += wk == 0.f ? 0.f : wk * u[e][z];
+            }
+        }
+    }
     const float inv = L == 0.f ? 0.f : 1.f / L;
     uint16_t *po = a.out + (size_t)row * a.out_stride + (size_t)h * D;
 #pragma unroll
@@ -884,24 +914,24 @@ SaPlan plan_shared(long N, long R, long H, long Hkv, long D, long own_cap, long 
     p.own_prefix = prefix_cap > 0 && cols <= 32 && !p.any_big;
     p.use_tile = p.any_big || (prefix_cap > 0 && !p.own_prefix);
     p.tiles = (cols + SA_COLS - 1) / SA_COLS;
-    // attn_tile_kernel: two workgroups a CU
+    // attn_tile: a workgroup a CU, and four key blocks at least
     const long wgs = p.tiles * Hkv;
     const long blocks = ((p.own_prefix ? 0 : prefix_cap) + (p.any_big ? own_cap : 0) + SA_KB - 1) / SA_KB;
-    long ns = wgs ? 2 * cus / wgs : 1;
-    if (ns > blocks / 2) ns = blocks / 2;
+    long ns = wgs ? cus / wgs : 1;
+    if (ns > blocks / 4) ns = blocks / 4;
     p.nsplit = (int)(ns < 1 ? 1 : ns > 64 ? 64 : ns);
-    // attn_own_kernel: at most R coltiles of the most rows a sequence has here, and no more
+    // attn_own: at most R coltiles of the most rows a sequence has here, and no more
     // than the rows make
     const long rows_max = max_new < p.small_rows ? max_new : p.small_rows;
     p.rows_max = (int)rows_max;
     long coltiles = R * ((rows_max * G + 15) / 16);
     if (coltiles > R + cols / 16) coltiles = R + cols / 16;
     const long pre = p.own_prefix ? (cols + 15) / 16 : 0;
-    const long keytiles = coltiles * ((own_cap + SO_TILE - 1) / SO_TILE) + pre * ((prefix_cap + SO_TILE - 1) / SO_TILE);
+    const long keyblocks = coltiles * ((own_cap + SO_KB - 1) / SO_KB) + pre * ((prefix_cap + SO_KB - 1) / SO_KB);
     long ow = 2 * cus;
-    if (ow > Hkv * keytiles) ow = Hkv * keytiles;
+    if (ow > (Hkv * keyblocks + SO_WAVES - 1) / SO_WAVES) ow = (Hkv * keyblocks + SO_WAVES - 1) / SO_WAVES;
     p.own_wgs = (int)(ow < 1 ? 1 : ow);
-    p.own_parts = Hkv * (coltiles + pre) + p.own_wgs;
+    p.own_parts = Hkv * (coltiles + pre) + (long)p.own_wgs * SO_WAVES;
     auto up = [](long v) { return (v + 255) / 256 * 256; };
     long at = 0;
     const long tparts = p.use_tile ? p.nsplit * N * H : 0;
@@ -916,16 +946,14 @@ SaPlan plan_shared(long N, long R, long H, long Hkv, long D, long own_cap, long 
 
 template <int D>
 int run_shared(const SaArgs &a, const SaPlan &p, hipStream_t stream) {
-    if (p.use_tile) {
-        auto kern = a.shift >= 6 ? attn_tile_kernel<D, true> : attn_tile_kernel<D, false>;
-        hipLaunchKernelGGL(kern, dim3((unsigned)(p.tiles * p.nsplit * a.Hkv)), dim3(SA_THREADS), SaGeo<D>::LDS, stream,
-                           a);
-        SC_HIP_CHECK(hipGetLastError());
-    }
-    auto own = a.shift >= 5 ? attn_own_kernel<D, true> : attn_own_kernel<D, false>;
-    hipLaunchKernelGGL(own, dim3((unsigned)p.own_wgs), dim3(64 * SO_WAVES), (a.R + 2) * 8, stream, a);
+    const int own_lds = (int)sizeof(OwnLds<D>) + (a.R + 2) * 8;
+    const int lds = a.tile_wgs && SaGeo<D>::LDS > own_lds ? SaGeo<D>::LDS : own_lds;
+    static_assert(SaGeo<D>::LDS <= 65536 && sizeof(OwnLds<D>) + (SA_MAX_SEQ + 2) * 8 <= 65536,
+                  "no larger dynamic LDS is asked for");
+    auto kern = a.shift >= 6 ? attn_shared_kernel<D, true> : attn_shared_kernel<D, false>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(a.own_wgs + a.tile_wgs)), dim3(SA_THREADS), lds, stream, a);
     SC_HIP_CHECK(hipGetLastError());
-    const bool by_seq = (p.nsplit == 1 || !p.any_big) && (long)a.R * p.rows_max < a.N;
+    const bool by_seq = (p.nsplit == 1 || !p.any_big) && (long)a.R * p.rows_max <= a.N;
     const long merge_rows = by_seq ? (long)a.R * p.rows_max : a.N;
     hipLaunchKernelGGL(attn_merge_kernel<D>, dim3((unsigned)((merge_rows * a.H + 3) / 4)), dim3(256), 0, stream, a,
                        p.use_tile ? p.nsplit : 0, by_seq ? p.rows_max : 0);
@@ -972,7 +1000,7 @@ int launch_attention_shared(const uint16_t *q, long q_stride, const uint16_t *kc
     const SaPlan p = plan_shared(N, R, H, Hkv, D, width * bs, prefix_width * bs, max_new);
     if (!workspace || workspace_bytes < p.bytes || (uintptr_t)workspace % 16)
         return set_error(SC_EINVAL, "attention_shared: a 16-byte aligned workspace of %ld bytes required", p.bytes);
-    if (p.tiles * p.nsplit * Hkv >= (1L << 31) || N * H >= (1L << 31))
+    if (p.tiles * p.nsplit * Hkv >= (1L << 30) || N * H >= (1L << 31))
         return set_error(SC_EINVAL, "attention_shared: too many rows");
     SaArgs a;
     a.q = q; a.q_stride = q_stride; a.kc = kc; a.vt = vt; a.out = out; a.out_stride = out_stride;
@@ -982,6 +1010,9 @@ int launch_attention_shared(const uint16_t *q, long q_stride, const uint16_t *kc
     a.width = (int)width; a.shift = shift; a.n_blocks = (int)n_blocks; a.prefix_width = (int)prefix_width;
     a.small_rows = p.small_rows; a.any_big = p.any_big; a.nsplit = p.nsplit; a.own_prefix = p.own_prefix;
     a.own_wgs = p.own_wgs;
+    a.tile_wgs = p.use_tile ? (int)(p.tiles * p.nsplit * Hkv) : 0;
+    a.tiles = (int)p.tiles;
+    a.pair_half = p.any_big && a.tile_wgs >= 2 * device_info().num_cus ? device_info().num_cus : 0;
     a.scale_log2 = scale * 1.4426950408889634f;
     char *ws = static_cast<char *>(workspace);
     a.tile_o = reinterpret_cast<float *>(ws + p.tile_o);
