@@ -8,12 +8,11 @@
 // instructions, keys through LDS); read once for all instead of once per sequence.  A
 // sequence's own keys serve its rows alone: few rows (a decoded token, a few guessed ones)
 // make it a stream of memory, many rows (a prompt) a product again.  So:
-//   attn_tile    128 columns: the prefix, then the own keys of sequences with many
+//   attn_tile          128 columns: the prefix, then the own keys of sequences with many
 //                      rows; over several workgroups where there are few
-//   attn_own     16 columns: the own keys of sequences with few rows (and the prefix
-//                      where all the rows are few), the work cut evenly over the
-//                      workgroups whatever the lengths are
-//   attn_merge_kernel   joins the parts of a row by their softmax maxima and sums
+//   attn_own           16 columns: the own keys of sequences with few rows, the work cut
+//                      evenly over the workgroups whatever the lengths are
+//   attn_merge_kernel  joins the parts of a row by their softmax maxima and sums
 // Parts are fp32 (O unnormalised, maximum in log2 units, sum).
 //
 // Pool layout as in blocks.hip: K [n_blocks, Hkv, bs, D], Vt [n_blocks, Hkv, D, bs].
@@ -23,6 +22,7 @@
 #include "dma_util.h"
 
 #include <math.h>
+#include <atomic>
 #include <type_traits>
 
 namespace sc {
@@ -35,7 +35,6 @@ using f4 = dma::f4;
 
 constexpr int SA_COLS = 128, SA_KB = 64, SA_THREADS = 256;
 constexpr int SA_AHEAD = 4;                              // operand reads in flight ahead of the MFMAs
-constexpr int SO_WAVES = 4, SO_KB = 32;
 constexpr int SA_MAX_SEQ = 2048;         // attn_own keeps two numbers of each in LDS
 
 struct SaArgs {
@@ -49,7 +48,6 @@ struct SaArgs {
     int small_rows;          // a sequence of at most this many rows is attn_own's
     int any_big;             // some sequence may have more
     int nsplit;              // workgroups a column tile's keys are cut into
-    int own_prefix;          // the prefix is attn_own's
     int tile_wgs, own_wgs;   // their workgroups
     int tiles, pair_half;    // attn_tile's column tiles; > 0: workgroups of a round, paired with the next round's
     float scale_log2;
@@ -59,7 +57,7 @@ struct SaArgs {
     float *own_o;
     float2 *own_ml;
     int own_parts;
-    int32_t *own_off, *own_unit;         // [R + 2]: first key tile and first unit of a sequence
+    int32_t *own_off, *own_unit;         // [R + 1]: a sequence's first block (and all of them), its first unit
 };
 
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return min(max(v, lo), hi); }
@@ -146,15 +144,76 @@ __device__ __forceinline__ uint4 keep_below(int k0, int end) {
     return m;
 }
 // non-finite values replaced by 0
+__device__ __forceinline__ uint32_t finite2(uint32_t x) {
+    return ((x & 0x7F80u) == 0x7F80u ? 0u : x & 0xFFFFu) | ((x & 0x7F800000u) == 0x7F800000u ? 0u : x & 0xFFFF0000u);
+}
 __device__ __forceinline__ uint4 finite8(uint4 v) {
-    auto keep = [](uint32_t x) {
-        return ((x & 0x7F80u) == 0x7F80u ? 0u : x & 0xFFFFu) | ((x & 0x7F800000u) == 0x7F800000u ? 0u : x & 0xFFFF0000u);
-    };
-    return make_uint4(keep(v.x), keep(v.y), keep(v.z), keep(v.w));
+    return make_uint4(finite2(v.x), finite2(v.y), finite2(v.z), finite2(v.w));
 }
 __device__ __forceinline__ uint4 and4(uint4 v, uint4 m) { return make_uint4(v.x & m.x, v.y & m.y, v.z & m.z, v.w & m.w); }
 
-// ONE: a key block lies in one cache block (block sizes from 64 up)
+// The copies of a key block (64 keys of one kv head) into a stage of the ring, by every wave
+// of the workgroup.  ONE: a key block lies in one cache block (block sizes from 64 up).
+template <int D, bool ONE>
+struct Stager {
+    using Gm = SaGeo<D>;
+    // cache blocks of a key block: ONE, its block's number; else those of the wave's 16
+    // keys of K and of the lane's two chunks of Vt
+    struct Ids { int k, v0, v1; };
+    const SaArgs &a;
+    uint8_t *smem;
+    int lane, w, sh, kr, vd, vc;
+    size_t blk_bytes;
+
+    // This lane's share.  Wave w issues K instructions of the keys 16 w .. 16 w + 15 and Vt
+    // instructions of D / 4 dims; a lane's dim row and chunk of Vt instruction qq differ
+    // between even and odd qq only in bit 2 of the chunk.
+    __device__ __forceinline__ Stager(const SaArgs &a_, uint8_t *smem_, int lane_, int w_)
+        : a(a_), smem(smem_), lane(lane_), w(w_), sh(a_.shift) {
+        kr = D == 128 ? 16 * w + (lane >> 4) : 16 * w + (lane >> 3);    // key row at qq = 0
+        vd = Gm::DMA * 8 * w + (lane >> 3);                             // dim at qq = 0
+        vc = (lane & 7) ^ ((vd >> 1) & 7);                              // chunk at even qq; ^ 4 at odd
+        blk_bytes = (size_t)a.Hkv * D * 2 << sh;
+    }
+    __device__ __forceinline__ Ids ids(const int32_t *table, int width, int kb) const {
+        auto at = [&](int key) { return table[min(key >> sh, width - 1)]; };
+        Ids x;
+        x.k = at(ONE ? kb : kb + 16 * w);
+        if (!ONE) { x.v0 = at(kb + 8 * vc); x.v1 = at(kb + 8 * (vc ^ 4)); }
+        return x;
+    }
+    // CLAMP (with ONE): keys past kb + lim read that key's row (or chunk) again, so that no
+    // memory is read for them
+    template <bool CLAMP>
+    __device__ __forceinline__ void copy(int hk, int kb, int lim, int st, const Ids &x) const {
+        const int bs = 1 << sh;
+        const char *kpool = reinterpret_cast<const char *>(a.kc) + ((size_t)hk * D * 2 << sh);
+        const char *vpool = reinterpret_cast<const char *>(a.vt) + ((size_t)hk * D * 2 << sh);
+        const uint32_t kl = (uint32_t)(uintptr_t)(smem + st * Gm::STAGE) + 1024 * Gm::DMA * w;
+        const uint32_t vl = kl + Gm::KTILE;
+        const int kid = clampi(__builtin_amdgcn_readfirstlane(x.k), 0, a.n_blocks - 1);
+        const char *kp = kpool + kid * blk_bytes + (size_t)((ONE ? kb : kb + 16 * w) & (bs - 1)) * Gm::KROW;
+#pragma unroll
+        for (int qq = 0; qq < Gm::DMA; ++qq) {
+            const int r = kr + (D == 128 ? 4 : 8) * qq;          // key row in the key block
+            const int c = D == 128 ? (lane & 15) ^ (sa_swap23(r) & 15) : (lane & 7) ^ ((r >> 1) & 7);
+            dma::dma16s(kp, (uint32_t)((ONE ? (CLAMP ? min(r, lim) : r) : r - 16 * w) * Gm::KROW + 16 * c), kl + 1024 * qq);
+        }
+        const char *vp = vpool + kid * blk_bytes + (ONE ? (size_t)(kb & (bs - 1)) * 2 : 0);
+#pragma unroll
+        for (int qq = 0; qq < Gm::DMA; ++qq) {
+            const int c = (qq & 1) ? vc ^ 4 : vc;
+            const uint32_t voff = ((uint32_t)(vd + 8 * qq) << sh) * 2;
+            if (ONE) {
+                dma::dma16s(vp, voff + 16 * (CLAMP ? min(c, lim >> 3) : c), vl + 1024 * qq);
+            } else {
+                const int vid = clampi((qq & 1) ? x.v1 : x.v0, 0, a.n_blocks - 1);
+                dma::dma16(vpool + vid * blk_bytes + voff + ((kb + 8 * c) & (bs - 1)) * 2, vl + 1024 * qq);
+            }
+        }
+    }
+};
+
 template <int D, bool ONE>
 __device__ __forceinline__ void attn_tile(const SaArgs &a, int id, uint8_t *smem) {
     using Gm = SaGeo<D>;
@@ -172,8 +231,7 @@ __device__ __forceinline__ void attn_tile(const SaArgs &a, int id, uint8_t *smem
     const int row0 = tile * SA_COLS / a.G, row1 = min((tile * SA_COLS + SA_COLS - 1) / a.G, rows - 1);
     if (row0 >= rows) return;
     const bool col_ok = row < rows;
-    const int P = a.own_prefix ? 0 : prefix_keys(a);
-    const int sh = a.shift, bs = 1 << sh;
+    const int P = prefix_keys(a);
 
     // the column tile's keys: the prefix, then the own keys of its sequences with many
     // rows; this workgroup takes key blocks [t0, t1) of them
@@ -206,54 +264,11 @@ __device__ __forceinline__ void attn_tile(const SaArgs &a, int id, uint8_t *smem
     float m = -INFINITY, lsum = 0.f;
     const float sc = a.scale_log2;
     const int arow = sa_swap23(li);
-    const size_t blk_bytes = (size_t)a.Hkv * D * 2 << sh;
-    const char *kpool = reinterpret_cast<const char *>(a.kc) + ((size_t)hk * D * 2 << sh);
-    const char *vpool = reinterpret_cast<const char *>(a.vt) + ((size_t)hk * D * 2 << sh);
-
-    // This lane's share of a key block's copies.  Wave w issues K instructions of the block's
-    // 16 keys 16 w .. 16 w + 15 and Vt instructions of D / 4 dims; a lane's dim row d and
-    // chunk c of Vt instruction qq differ between even and odd qq only in bit 2 of c.
-    const int kr = D == 128 ? 16 * w + (lane >> 4) : 16 * w + (lane >> 3);    // key row at qq = 0
-    const int vd = Gm::DMA * 8 * w + (lane >> 3);                             // dim at qq = 0
-    const int vc = (lane & 7) ^ ((vd >> 1) & 7);                              // chunk at even qq; ^ 4 at odd
+    const Stager<D, ONE> stager(a, smem, lane, w);
 
     // key blocks [b0, b1) of one table with `end` keys; the column sees keys <= limit
     auto segment = [&](const int32_t *table, int width, int end, int b0, int b1, int limit) {
         if (b0 >= b1) return;
-        // the cache blocks of a key block, one ahead of its copies: ONE, its block's number;
-        // else those of the wave's 16 keys of K and of the lane's two chunks of Vt
-        struct Ids { int k, v0, v1; };
-        auto id_at = [&](int key) { return table[min(key >> sh, width - 1)]; };
-        auto load_ids = [&](int kb) {
-            Ids x;
-            x.k = id_at(ONE ? kb : kb + 16 * w);
-            if (!ONE) { x.v0 = id_at(kb + 8 * vc); x.v1 = id_at(kb + 8 * (vc ^ 4)); }
-            return x;
-        };
-        auto stage_blk = [&](int kb, int st, const Ids &x) {
-            const uint32_t kl = (uint32_t)(uintptr_t)(smem + st * Gm::STAGE) + 1024 * Gm::DMA * w;
-            const uint32_t vl = kl + Gm::KTILE;
-            const int kid = clampi(__builtin_amdgcn_readfirstlane(x.k), 0, a.n_blocks - 1);
-            const char *kp = kpool + kid * blk_bytes + (size_t)((ONE ? kb : kb + 16 * w) & (bs - 1)) * Gm::KROW;
-#pragma unroll
-            for (int qq = 0; qq < Gm::DMA; ++qq) {
-                const int r = kr + (D == 128 ? 4 : 8) * qq;          // key row in the key block
-                const int c = D == 128 ? (lane & 15) ^ (sa_swap23(r) & 15) : (lane & 7) ^ ((r >> 1) & 7);
-                dma::dma16s(kp, (uint32_t)((ONE ? r : r - 16 * w) * Gm::KROW + 16 * c), kl + 1024 * qq);
-            }
-            const char *vp = vpool + kid * blk_bytes + (ONE ? (size_t)(kb & (bs - 1)) * 2 : 0);
-#pragma unroll
-            for (int qq = 0; qq < Gm::DMA; ++qq) {
-                const int c = (qq & 1) ? vc ^ 4 : vc;
-                const uint32_t voff = ((uint32_t)(vd + 8 * qq) << sh) * 2;
-                if (ONE) {
-                    dma::dma16s(vp, voff + 16 * c, vl + 1024 * qq);
-                } else {
-                    const int vid = clampi((qq & 1) ? x.v1 : x.v0, 0, a.n_blocks - 1);
-                    dma::dma16(vpool + vid * blk_bytes + voff + ((kb + 8 * c) & (bs - 1)) * 2, vl + 1024 * qq);
-                }
-            }
-        };
         // of the wave's columns: the fewest and the most keys one of them sees
         int lo = limit, hi = limit;
 #pragma unroll
@@ -263,7 +278,8 @@ __device__ __forceinline__ void attn_tile(const SaArgs &a, int id, uint8_t *smem
         }
         lo = __builtin_amdgcn_readfirstlane(lo);
         hi = __builtin_amdgcn_readfirstlane(hi);
-        Ids ids;
+        // cache block numbers, one key block ahead of its copies
+        typename Stager<D, ONE>::Ids ids;
         // the stage is a compile-time constant in the copies without a mask, so that every
         // operand read is a loop-invariant lane offset plus an immediate
         auto block = [&](int blk, auto mask_tag, auto stage) {
@@ -273,8 +289,8 @@ __device__ __forceinline__ void attn_tile(const SaArgs &a, int id, uint8_t *smem
             const uint8_t *K = smem + st * Gm::STAGE;
             const uint8_t *V = K + Gm::KTILE;
             if (blk + 1 < b1) {
-                stage_blk(kb + SA_KB, st ^ 1, ids);
-                ids = load_ids(kb + 2 * SA_KB);
+                stager.template copy<false>(hk, kb + SA_KB, 0, st ^ 1, ids);
+                ids = stager.ids(table, width, kb + 2 * SA_KB);
             }
             if (!MASK || kb <= hi) {                     // else: nothing of it is seen by the wave
                 f32x16_t sacc[2] = {f32x16_t{}, f32x16_t{}};
@@ -402,9 +418,9 @@ __device__ __forceinline__ void attn_tile(const SaArgs &a, int id, uint8_t *smem
             dma::wait_vm<0>();
             __syncthreads();
         };
-        ids = load_ids(b0 * SA_KB);
-        stage_blk(b0 * SA_KB, 0, ids);
-        ids = load_ids(b0 * SA_KB + SA_KB);
+        ids = stager.ids(table, width, b0 * SA_KB);
+        stager.template copy<false>(hk, b0 * SA_KB, 0, 0, ids);
+        ids = stager.ids(table, width, b0 * SA_KB + SA_KB);
         dma::wait_vm<0>();
         __syncthreads();
         using S0 = std::integral_constant<int, 0>;
@@ -468,219 +484,183 @@ __device__ __forceinline__ void attn_tile(const SaArgs &a, int id, uint8_t *smem
     if (lh == 0) a.tile_ml[part] = make_float2(m * sc, ltot);
 }
 
-// ---------------------------------------------------------------- 16 columns
+// ---------------------------------------------------------------- few columns
 //
-// A unit is 16 columns (row i, q head g: column i G + g) of one sequence and kv head; its
-// keys are blocks of 32, each one wave's work: S^T[32 keys x 16] = K Q^T and O^T[D x 16] +=
-// Vt P^T on v_mfma_f32_16x16x32_bf16, K and Vt straight into registers, the keys permuted on
-// their way so that lane group g = lane / 16 holds the 8 consecutive keys 8 g .. 8 g + 7
-// of the block (as the dense decode attention does).  All units' blocks in a line (sequence,
-// kv head, 16 columns, key block) are cut into equal runs, one a wave, whatever the lengths
-// are.  A run's share of a unit is one part, number unit + wave (two consecutive runs meet in
-// one unit at most, so the numbers differ).  "Sequence" R is the prefix, with all rows.
+// A unit is up to 64 columns (row i, q head g: column i G + g) of one sequence and kv head;
+// its keys are blocks of 64.  All units' blocks in a line (sequence, kv head, 64 columns, key
+// block) are cut into equal runs, one a workgroup, whatever the lengths are.  A block is
+// staged as attn_tile stages it, one ahead, also from one unit into the next.  A wave takes
+// 16 keys x 16 columns at a time: S^T[16 x 16] = K Q^T on v_mfma_f32_16x16x32_bf16, whose result
+// is operand B of O^T[D x 16] += Vt P^T on v_mfma_f32_16x16x16_bf16 as it lies in the registers.
+// Of a sequence with at most 16 columns wave w takes keys 16 w .. 16 w + 15 of every block,
+// with a maximum, a sum and an O of its own; of one with more, all the keys for columns 16 w ..
+// 16 w + 15, so that the keys are read once for them all.  A wave's share of a unit is one
+// part, number 4 (unit + workgroup) + wave (two consecutive runs meet in one unit at most, so
+// the numbers differ).
 //
-// Bound by memory: a wave has the next block's loads (16 KB at head_dim 128) in flight
-// while it computes one, also from one unit into the next, and no wave waits for another.
-template <typename F>
-__device__ __forceinline__ void own_shape(const SaArgs &a, int r, int rows, int P, F &&f) {
-    // f(first row, rows, keys)
-    if (r < a.R) {
-        const Seq s = seq_of(a, r, rows);
-        f(s.first, s.n <= a.small_rows ? s.n : 0, s.len);
-    } else {
-        f(0, a.own_prefix ? rows : 0, P);
-    }
-}
-__device__ __forceinline__ int own_coltiles(const SaArgs &a, int n) { return (n * a.G + 15) >> 4; }
-__device__ __forceinline__ int own_keyblocks(int len) { return (len + SO_KB - 1) / SO_KB; }
-// blocks a wave takes of `total`
-__device__ __forceinline__ int own_run(const SaArgs &a, int total) {
-    const int waves = a.own_wgs * SO_WAVES;
-    return max((total + waves - 1) / waves, 1);
-}
+// Bound by memory.  The copies read whole cache lines, 256 bytes a K row and 128 a Vt row:
+// 5.5 TB/s (64 sequences of 4096 positions, 194 us; operands loaded straight into the
+// registers in the MFMA's order, 64 bytes of 16 rows an instruction, 250 us).
+__device__ __forceinline__ int own_coltiles(const SaArgs &a, int n) { return (n * a.G + 63) >> 6; }
+__device__ __forceinline__ int own_keyblocks(int len) { return (len + SA_KB - 1) / SA_KB; }
+// blocks a workgroup takes of `total`
+__device__ __forceinline__ int own_run(const SaArgs &a, int total) { return max((total + a.own_wgs - 1) / a.own_wgs, 1); }
 
-template <int D>
-struct OwnBlock {
-    uint4 k[2][D / 32];
-    uint4 v[D / 16];
-};
+typedef __attribute__((__vector_size__(4 * sizeof(short)))) short s16x4_t;
 
-// LDS of a workgroup, off[R + 2] and unit[R + 2] behind it
-template <int D>
-struct OwnLds {
-    uint16_t v[SO_WAVES][D][SO_KB];          // a wave's Vt block, where it holds values that are not finite
-    int wsum[2][SO_WAVES];
-};
-
-// ONE: 32 keys lie in one cache block
 template <int D, bool ONE>
 __device__ __forceinline__ void attn_own(const SaArgs &a, int wg, uint8_t *smem) {
     constexpr int U = D / 32, DT = D / 16;
-    OwnLds<D> &lds = *reinterpret_cast<OwnLds<D> *>(smem);
-    int32_t *off = reinterpret_cast<int32_t *>(smem + sizeof(OwnLds<D>)), *unit = off + a.R + 2;
+    using Gm = SaGeo<D>;
+    // behind the ring, of every sequence: its first row (and the rows' number), and its keys;
+    // in the ring, before it is used: the sequences' first blocks and units
+    int32_t *first_row = reinterpret_cast<int32_t *>(smem + Gm::LDS), *keys = first_row + a.R + 1;
+    int32_t *off = reinterpret_cast<int32_t *>(smem), *unit = off + a.R, *wsum = unit + a.R;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
-    const int rows = live_rows(a), P = prefix_keys(a);
-    const int sh = a.shift, bs = 1 << sh;
+    const int rows = live_rows(a);
 
-    // first block and unit of every sequence
-    {
-        int t_before = 0, u_before = 0;
-        for (int r0 = 0; r0 <= a.R; r0 += 64 * SO_WAVES) {
-            const int r = r0 + tid;
-            int t = 0, u = 0;
-            if (r <= a.R)
-                own_shape(a, r, rows, P, [&](int, int n, int len) {
-                    const int kt = own_keyblocks(len);
-                    u = kt ? a.Hkv * own_coltiles(a, n) : 0;
-                    t = u * kt;
-                });
-            int ts = t, us = u;
-#pragma unroll
-            for (int x = 1; x < 64; x <<= 1) {
-                const int t2 = __shfl_up(ts, x), u2 = __shfl_up(us, x);
-                if (lane >= x) { ts += t2; us += u2; }
-            }
-            if (lane == 63) { lds.wsum[0][w] = ts; lds.wsum[1][w] = us; }
-            __syncthreads();
-            int tb = t_before, ub = u_before;
-            for (int i = 0; i < SO_WAVES; ++i) {
-                if (i < w) { tb += lds.wsum[0][i]; ub += lds.wsum[1][i]; }
-                t_before += lds.wsum[0][i];
-                u_before += lds.wsum[1][i];
-            }
-            if (r <= a.R) { off[r] = tb + ts - t; unit[r] = ub + us - u; }
-            __syncthreads();
+    int t_before = 0, u_before = 0;
+    for (int r0 = 0; r0 < a.R; r0 += SA_THREADS) {
+        const int r = r0 + tid;
+        int t = 0, u = 0;
+        if (r < a.R) {
+            const Seq s = seq_of(a, r, rows);
+            const int kt = own_keyblocks(s.len);
+            u = kt && s.n <= a.small_rows ? a.Hkv * own_coltiles(a, s.n) : 0;
+            t = u * kt;
+            first_row[r] = s.first;
+            keys[r] = s.len;
         }
-        if (tid == 0) { off[a.R + 1] = t_before; unit[a.R + 1] = u_before; }
+        int ts = t, us = u;
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) {
+            const int t2 = __shfl_up(ts, x), u2 = __shfl_up(us, x);
+            if (lane >= x) { ts += t2; us += u2; }
+        }
+        if (lane == 63) { wsum[w] = ts; wsum[4 + w] = us; }
         __syncthreads();
-        if (wg == 0)
-            for (int r = tid; r < a.R + 2; r += 64 * SO_WAVES) { a.own_off[r] = off[r]; a.own_unit[r] = unit[r]; }
+        int tb = t_before, ub = u_before;
+        for (int i = 0; i < 4; ++i) {
+            if (i < w) { tb += wsum[i]; ub += wsum[4 + i]; }
+            t_before += wsum[i];
+            u_before += wsum[4 + i];
+        }
+        if (r < a.R) { off[r] = tb + ts - t; unit[r] = ub + us - u; }
+        if (tid == 0 && r0 == 0) first_row[a.R] = rows;
+        __syncthreads();
     }
-    const int wave = wg * SO_WAVES + w;
-    const int total = __builtin_amdgcn_readfirstlane(off[a.R + 1]), run = own_run(a, total);
-    int t = (int)min((long)wave * run, (long)total);
+    if (wg == 0) {
+        for (int r = tid; r < a.R; r += SA_THREADS) { a.own_off[r] = off[r]; a.own_unit[r] = unit[r]; }
+        if (tid == 0) a.own_off[a.R] = t_before;
+    }
+    const int total = t_before, run = own_run(a, total);
+    int t = (int)min((long)wg * run, (long)total);
     const int t_end = min(t + run, total);
     if (t >= t_end) return;
+    // the sequence of block t: the last one that starts at or before it
     int r = 0;
-    for (int n = a.R + 1; n > 1;) {
+    for (int n = a.R; n > 1;) {
         const int half = n >> 1;
         if (off[r + half] <= t) { r += half; n -= half; }
         else n = half;
     }
-    const size_t blk_bytes = (size_t)a.Hkv * D * 2 << sh;
-    // byte offsets of this lane within a cache block of one kv head: key 8 (c / 4) + c % 4
-    // of K (the key 4 further on is 8 D bytes on), dim c of Vt (16 dims on: 32 << sh bytes)
-    const int krow = 8 * (c >> 2) + (c & 3);
-    const uint32_t koff = (uint32_t)((ONE ? krow : krow & 15) * D * 2 + 16 * g);
-    const uint32_t voff = ((uint32_t)c << sh) * 2 + (ONE ? 16 * g : 16 * (g & 1));
+    r = __builtin_amdgcn_readfirstlane(r);
+    int u_next = __builtin_amdgcn_readfirstlane(unit[r]);      // unit number of the next unit opened
+    int in_seq = t - __builtin_amdgcn_readfirstlane(off[r]);   // block t within sequence r
+    __syncthreads();                                           // off and unit have been read: the ring is free
 
-    // the wave's share of one unit
-    struct Run {
+    struct Run {                 // the workgroup's share of one unit
         const int32_t *table;
-        int width, hk, part, first, cols0, n;
-        int kb, stop;            // the next key block, and the key its blocks end at
+        int hk, part, first, n;
+        int col0;                // this wave's first column
+        bool wide;               // a wave takes 16 columns and every key, not all columns and 16 keys
+        int kb, stop;            // the key block, and the key its blocks end at
         int all, seen;           // keys that every, that some column sees
-        int rel;                 // the unit's row i sees keys up to rel + i (the prefix: up to rel)
-        bool pre;
+        int rel;                 // the unit's row i sees keys up to rel + i
+        bool fresh;              // the unit's first block here
     };
-    auto open = [&]() {          // at block t; t moves to the end of the share
-        while (off[r + 1] <= t) ++r;
-        r = __builtin_amdgcn_readfirstlane(r);
-        int len = 0;
-        Run s;
-        own_shape(a, r, rows, P, [&](int f, int nn, int l) { s.first = f; s.n = nn; len = l; });
-        const int kt = own_keyblocks(len), ct = own_coltiles(a, s.n);
-        const int lt = t - __builtin_amdgcn_readfirstlane(off[r]), u = lt / kt, b0 = lt - u * kt;
-        const int b1 = min(kt, b0 + t_end - t);
-        s.pre = r == a.R;
-        s.hk = u / ct;
-        s.cols0 = (u - s.hk * ct) * 16;
-        s.table = s.pre ? a.prefix_table : a.tables + (size_t)r * a.width;
-        s.width = s.pre ? a.prefix_width : a.width;
-        s.part = __builtin_amdgcn_readfirstlane(unit[r]) + u + wave;
-        s.kb = b0 * SO_KB;
-        s.stop = b1 * SO_KB;
-        s.rel = s.pre ? P - 1 : len - s.n;
-        const int last = min((s.cols0 + 15) / a.G, s.n - 1);                 // the unit's last row
-        s.seen = s.pre ? P : clampi(s.rel + last + 1, 0, len);
-        s.all = s.pre ? P : clampi(s.rel + s.cols0 / a.G + 1, 0, len);
+    bool first_unit = true;
+    auto open = [&](Run &s) {    // the unit of block t; t moves to its end in the run
+        if (t >= t_end) return false;
+        int first, len, n, kt, ct;
+        for (;; ++r, in_seq = 0) {
+            first = __builtin_amdgcn_readfirstlane(first_row[r]);
+            len = __builtin_amdgcn_readfirstlane(keys[r]);
+            n = __builtin_amdgcn_readfirstlane(first_row[r + 1]) - first;
+            if (n > a.small_rows) n = 0;
+            kt = own_keyblocks(len);
+            ct = own_coltiles(a, n);
+            if (in_seq < a.Hkv * ct * kt || r == a.R - 1) break;
+        }
+        const int u = in_seq / kt, b0 = in_seq - u * kt, b1 = min(kt, b0 + t_end - t);
         t += b1 - b0;
-        return s;
+        in_seq += b1 - b0;
+        if (first_unit) u_next += u;
+        first_unit = false;
+        s.fresh = true;
+        s.first = first;
+        s.n = n;
+        s.hk = u / ct;
+        s.wide = n * a.G > 16;
+        s.col0 = s.wide ? (u - s.hk * ct) * 64 + 16 * w : 0;
+        s.table = a.tables + (size_t)r * a.width;
+        s.part = 4 * (u_next + wg) + w;
+        ++u_next;
+        s.kb = b0 * SA_KB;
+        s.stop = b1 * SA_KB;
+        s.rel = len - n;
+        const int c0 = (u - s.hk * ct) * 64, last = min((c0 + 63) / a.G, n - 1);     // the unit's last row
+        s.seen = clampi(s.rel + last + 1, 0, len);
+        s.all = clampi(s.rel + c0 / a.G + 1, 0, len);
+        return true;
     };
-    bf16x8_t qv[U];
-    float m, lsum;
-    f4 o[DT];
-    int limit;                   // the last key this lane's column sees
-    auto begin = [&](const Run &s) {
-        const int i = (s.cols0 + c) / a.G, h = s.hk * a.G + s.cols0 + c - i * a.G;
-        const bool ok = i < s.n;
-        limit = !ok ? -1 : s.pre ? s.rel : s.rel + i;
+    auto advance = [&](Run &s) {
+        s.kb += SA_KB;
+        s.fresh = false;
+        return s.kb < s.stop || open(s);
+    };
+    const Stager<D, ONE> stager(a, smem, lane, w);
+    auto stage = [&](const Run &s, int st, const typename Stager<D, ONE>::Ids &ids) {
+        const int lim = max(s.seen - 1 - s.kb, 0);
+        if (ONE && lim < SA_KB - 1) stager.template copy<true>(s.hk, s.kb, lim, st, ids);
+        else stager.template copy<false>(s.hk, s.kb, 0, st, ids);
+    };
+    auto load_q = [&](const Run &s, uint4 (&q)[U]) {
+        const int i = (s.col0 + c) / a.G, h = s.hk * a.G + s.col0 + c - i * a.G;
 #pragma unroll
         for (int x = 0; x < U; ++x) {
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (ok) v = *reinterpret_cast<const uint4 *>(a.q + (size_t)(s.first + i) * a.q_stride + (size_t)h * D + 32 * x + 8 * g);
-            qv[x] = as_bf16x8(v);
-        }
-        m = -INFINITY;
-        lsum = 0.f;
-#pragma unroll
-        for (int x = 0; x < DT; ++x) o[x] = f4{0.f, 0.f, 0.f, 0.f};
-    };
-    // the cache blocks of 32 keys (one, or those of this lane's K and Vt halves)
-    struct Ids { int k, v; };
-    auto load_ids = [&](const Run &s, int kb) {
-        kb = min(kb, s.stop - SO_KB);
-        Ids x;
-        x.k = s.table[min((ONE ? kb : kb + 16 * (c >> 3)) >> sh, s.width - 1)];
-        x.v = ONE ? 0 : s.table[min((kb + 16 * (g >> 1)) >> sh, s.width - 1)];
-        return x;
-    };
-    auto load = [&](OwnBlock<D> &b, const Run &s, Ids x) {
-        const char *kpool = reinterpret_cast<const char *>(a.kc) + ((size_t)s.hk * D * 2 << sh);
-        const char *vpool = reinterpret_cast<const char *>(a.vt) + ((size_t)s.hk * D * 2 << sh);
-        auto take = [&](const char *kp, const char *vp) {
-#pragma unroll
-            for (int y = 0; y < U; ++y) {
-                b.k[0][y] = *reinterpret_cast<const uint4 *>(kp + koff + 64 * y);
-                b.k[1][y] = *reinterpret_cast<const uint4 *>(kp + koff + 64 * y + 8 * D);
-            }
-#pragma unroll
-            for (int y = 0; y < DT; ++y) b.v[y] = *reinterpret_cast<const uint4 *>(vp + (voff + ((uint32_t)y << (sh + 5))));
-        };
-        if (ONE) {
-            const size_t at = (size_t)clampi(__builtin_amdgcn_readfirstlane(x.k), 0, a.n_blocks - 1) * blk_bytes;
-            const int k0 = s.kb & (bs - 1);
-            take(kpool + at + (size_t)k0 * (D * 2), vpool + at + (size_t)k0 * 2);
-        } else {
-            const int kk = (s.kb + 16 * (c >> 3)) & (bs - 1), kv = (s.kb + 16 * (g >> 1)) & (bs - 1);
-            take(kpool + (size_t)clampi(x.k, 0, a.n_blocks - 1) * blk_bytes + kk * (D * 2),
-                 vpool + (size_t)clampi(x.v, 0, a.n_blocks - 1) * blk_bytes + kv * 2);
+            q[x] = make_uint4(0u, 0u, 0u, 0u);
+            if (i < s.n) q[x] = *reinterpret_cast<const uint4 *>(a.q + (size_t)(s.first + i) * a.q_stride + (size_t)h * D + 32 * x + 8 * g);
         }
     };
-    // EDGE: some column does not see all the 32 keys
-    auto compute = [&](OwnBlock<D> &b, const Run &s, auto edge_tag) {
-        constexpr bool EDGE = decltype(edge_tag)::value;
-        const int kb = s.kb;
-        f4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
+    bf16x8_t qv[U];
+    float m = -INFINITY, lsum = 0.f;
+    f4 o[DT];
+    int limit = -1;              // the last key this lane's column sees
+    // keys 16 sub .. 16 sub + 15 of the block
+    auto compute = [&](const Run &s, int st, int sub) {
+        const uint8_t *K = smem + st * Gm::STAGE, *V = K + Gm::KTILE;
+        const int k0 = s.kb + 16 * sub + 4 * g;            // this lane's keys: k0 .. k0 + 3
+        f4 sv = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int y = 0; y < U; ++y) {
-            s0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(b.k[0][y]), qv[y], s0, 0, 0, 0);
-            s1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(b.k[1][y]), qv[y], s1, 0, 0, 0);
-        }
-        float p[8];
+        for (int y = 0; y < U; ++y)
+            sv = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                as_bf16x8(*reinterpret_cast<const uint4 *>(K + sa_kswz<D>(16 * sub + c, 4 * y + g))), qv[y], sv, 0, 0, 0);
+        // Vt of the 16 keys: dim 16 y + c, keys 4 g .. 4 g + 3
+        uint2 v[DT];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            p[x] = s0[x] * a.scale_log2;
-            p[4 + x] = s1[x] * a.scale_log2;
-        }
-        if (EDGE)
+        for (int y = 0; y < DT; ++y)
+            v[y] = *reinterpret_cast<const uint2 *>(V + sa_vswz(16 * y + c, 2 * sub + (g >> 1)) + 8 * (g & 1));
+        float p[4];
 #pragma unroll
-            for (int x = 0; x < 8; ++x)
-                if (kb + 8 * g + x > limit) p[x] = -INFINITY;
-        float bm = p[0];
+        for (int x = 0; x < 4; ++x) p[x] = sv[x] * a.scale_log2;
+        const bool edge = s.kb + SA_KB > s.all;          // some column does not see all of the keys
+        if (edge)
 #pragma unroll
-        for (int x = 1; x < 8; ++x) bm = fmaxf(bm, p[x]);
+            for (int x = 0; x < 4; ++x)
+                if (k0 + x > limit) p[x] = -INFINITY;
+        float bm = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
         bm = fmaxf(bm, __shfl_xor(bm, 16));
         bm = fmaxf(bm, __shfl_xor(bm, 32));
         const float mn = fmaxf(m, bm);
@@ -688,60 +668,57 @@ __device__ __forceinline__ void attn_own(const SaArgs &a, int wg, uint8_t *smem)
         const float alpha = __builtin_amdgcn_exp2f(m - ref);
         float ps = 0.f;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
+        for (int x = 0; x < 4; ++x) {
             p[x] = __builtin_amdgcn_exp2f(p[x] - ref);
             ps += p[x];
         }
         lsum = lsum * alpha + ps;
         m = mn;
-        const bf16x8_t pb = as_bf16x8(cvt_pk_bf16(p[0], p[1]), cvt_pk_bf16(p[2], p[3]), cvt_pk_bf16(p[4], p[5]),
-                                      cvt_pk_bf16(p[6], p[7]));
+        const s16x4_t pb = __builtin_bit_cast(s16x4_t, make_uint2(cvt_pk_bf16(p[0], p[1]), cvt_pk_bf16(p[2], p[3])));
 #pragma unroll
         for (int y = 0; y < DT; ++y)
 #pragma unroll
             for (int x = 0; x < 4; ++x) o[y][x] *= alpha;
         // V of keys nobody sees is dropped, and values that are not finite where some
         // column does not see their key are added to those that do (as in attn_tile)
-        if (EDGE) {
-            const uint4 mk = keep_below(kb + 8 * g, s.seen);
+        if (edge) {
+            const uint32_t m0 = (k0 + 0 < s.seen ? 0xFFFFu : 0u) | (k0 + 1 < s.seen ? 0xFFFF0000u : 0u);
+            const uint32_t m1 = (k0 + 2 < s.seen ? 0xFFFFu : 0u) | (k0 + 3 < s.seen ? 0xFFFF0000u : 0u);
             uint32_t bits = 0;
 #pragma unroll
             for (int y = 0; y < DT; ++y) {
-                b.v[y] = and4(b.v[y], mk);
-                bits |= nonfinite_bits(b.v[y]);
+                v[y].x &= m0;
+                v[y].y &= m1;
+                bits |= nonfinite_bits(v[y].x) | nonfinite_bits(v[y].y);
             }
             if (any_nonfinite(bits)) {
-                uint16_t *vs = &lds.v[w][0][0];
-#pragma unroll
-                for (int y = 0; y < DT; ++y) *reinterpret_cast<uint4 *>(vs + (16 * y + c) * SO_KB + 8 * g) = b.v[y];
 #pragma unroll 1
-                for (int j = 0; j < SO_KB; ++j) {
-                    const bool sees = kb + j <= limit;
+                for (int j = 0; j < 16; ++j) {
+                    const int key = s.kb + 16 * sub + j;
+                    const bool sees = key <= limit;
                     int quad = g;                        // opaque: no addresses of this rare loop are kept
                     asm volatile("" : "+v"(quad));
 #pragma unroll
-                    for (int y = 0; y < DT; ++y) {
+                    for (int y = 0; y < DT; ++y)
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
-                            const uint32_t z = vs[(16 * y + 4 * quad + x) * SO_KB + j];
+                            const int d = 16 * y + 4 * quad + x;
+                            const uint32_t z = *reinterpret_cast<const uint16_t *>(V + sa_vswz(d, 2 * sub + (j >> 3)) + 2 * (j & 7));
                             if (sees && (z & 0x7F80u) == 0x7F80u) o[y][x] += bf2f(z);
                         }
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
                 }
 #pragma unroll
-                for (int y = 0; y < DT; ++y)
-                    b.v[y] = finite8(*reinterpret_cast<const uint4 *>(vs + (16 * y + c) * SO_KB + 8 * g));
+                for (int y = 0; y < DT; ++y) v[y] = make_uint2(finite2(v[y].x), finite2(v[y].y));
             }
         }
 #pragma unroll
         for (int y = 0; y < DT; ++y)
-            o[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(b.v[y]), pb, o[y], 0, 0, 0);
+            o[y] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4_t, v[y]), pb, o[y], 0, 0, 0);
     };
     auto end = [&](const Run &s) {           // the part: the unit's columns that are there
         float ltot = lsum + __shfl_xor(lsum, 16);
         ltot += __shfl_xor(ltot, 32);
-        if ((s.cols0 + c) / a.G >= s.n || s.part >= a.own_parts) return;
+        if ((s.col0 + c) / a.G >= s.n || s.part >= a.own_parts) return;
         const size_t at = (size_t)s.part * 16 + c;
         float *po = a.own_o + at * D + 4 * g;
 #pragma unroll
@@ -749,36 +726,44 @@ __device__ __forceinline__ void attn_own(const SaArgs &a, int wg, uint8_t *smem)
         if (g == 0) a.own_ml[at] = make_float2(m, ltot);
     };
 
-    // two blocks in turn: while one is computed the next one's loads (of the next unit's,
-    // after a unit's last) and the cache block numbers of the one after it are on their way.
-    // The loads are unconditional (past the run's end the last block again): with loads on
-    // some paths only the compiler would wait for all of them before it computes
-    OwnBlock<D> one, two;
-    Run s = open();
-    Ids ids = load_ids(s, s.kb), ids1 = load_ids(s, s.kb + SO_KB);
-    begin(s);
-    load(one, s, ids);
-    auto half = [&](OwnBlock<D> &cur, OwnBlock<D> &nxt) {
-        const bool last = s.kb + SO_KB >= s.stop, done = last && t >= t_end;
-        Run n = s;
-        if (!last) n.kb += SO_KB;
-        else if (!done) {
-            n = open();
-            ids1 = load_ids(n, n.kb);
+    Run f, n;                    // the block staged last, and the one after it
+    uint4 qn[U];                 // q of the unit of block f, where f is its first
+    open(f);
+    stage(f, 0, stager.ids(f.table, a.width, f.kb));
+    load_q(f, qn);
+    n = f;
+    bool more = advance(n);
+    typename Stager<D, ONE>::Ids ids = stager.ids(n.table, a.width, n.kb);
+    for (int st = 0;; st ^= 1) {
+        // block f has landed, and the other stage has been read
+        dma::wait_vm<0>();
+        __syncthreads();
+        const Run s = f;
+        if (s.fresh) {
+            const int i = (s.col0 + c) / a.G;
+            limit = i >= s.n ? -1 : s.rel + i;
+#pragma unroll
+            for (int x = 0; x < U; ++x) qv[x] = as_bf16x8(qn[x]);
+            m = -INFINITY;
+            lsum = 0.f;
+#pragma unroll
+            for (int y = 0; y < DT; ++y) o[y] = f4{0.f, 0.f, 0.f, 0.f};
         }
-        ids = ids1;
-        ids1 = load_ids(n, n.kb + SO_KB);
-        load(nxt, n, ids);
-        if (s.kb + SO_KB <= s.all) compute(cur, s, std::false_type{});
-        else compute(cur, s, std::true_type{});
-        if (last) {
-            end(s);
-            if (!done) begin(n);
+        const bool go = more;
+        if (go) {
+            f = n;
+            stage(f, st ^ 1, ids);
+            if (f.fresh) load_q(f, qn);
+            more = advance(n);
+            ids = stager.ids(n.table, a.width, n.kb);
         }
-        s = n;
-        return done;
-    };
-    while (!half(one, two) && !half(two, one)) {}
+        if (s.col0 < s.n * a.G) {                        // (a wave of a wide unit may have no column)
+            const int sub1 = s.wide ? 4 : w + 1;
+            for (int sub = s.wide ? 0 : w; sub < sub1; ++sub) compute(s, st, sub);
+            if (s.kb + SA_KB >= s.stop) end(s);
+        }
+        if (!go) break;
+    }
 }
 
 // ---------------------------------------------------------------- both
@@ -794,8 +779,7 @@ __global__ void __launch_bounds__(SA_THREADS) __attribute__((amdgpu_waves_per_eu
 
 // ---------------------------------------------------------------- merge
 //
-// One wave a row and q head: the parts of attn_tile (nsplit), then those of
-// attn_own for the row's sequence and for the prefix.  out = sum_i 2^(m_i - M) O_i /
+// One wave a row and q head: the parts of attn_tile (nsplit), then those of attn_own.  out = sum_i 2^(m_i - M) O_i /
 // sum_i 2^(m_i - M) l_i; parts of no key have m = -inf and weight 0, a row of no key at
 // all is 0.  The waves go over every row, or, where only sequences of few rows have parts,
 // over per_seq rows of every sequence, if that is less (prompts are then passed over).
@@ -803,12 +787,16 @@ __global__ void __launch_bounds__(SA_THREADS) __attribute__((amdgpu_waves_per_eu
 // Bound by the latency of dependent loads, so there are two rounds of them: what says where
 // the parts are, then the parts, lane i holding part i's place and (m, l), the values of
 // AHEAD parts on their way together.
-template <int D>
+// Few rows: WPR = 4, a workgroup a row and q head, its waves taking the parts in turn.
+template <int D, int WPR>
 __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_parts, int per_seq) {
     constexpr int PER = D / 64;
-    constexpr int AHEAD = 8;
-    const long wid = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
+    constexpr int AHEAD = 16;
+    __shared__ float2 sm_ml[WPR];
+    __shared__ float sm_o[WPR][D];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long wid = WPR == 4 ? (long)blockIdx.x : (long)blockIdx.x * 4 + w;
+    const int turn = WPR == 4 ? w : 0;
     const int rows = live_rows(a);
     int row = (int)(wid / a.H), r;
     const int h = (int)(wid - (long)row * a.H);
@@ -827,27 +815,29 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
         if (s.n > a.small_rows && a.nsplit == 1) return;       // written by attn_tile
     }
     const int hk = h / a.G, gq = h - hk * a.G;
-    const int run = own_run(a, a.own_off[a.R + 1]);
-    // attn_own's parts of row i of n: the first one's number, and how many
-    auto own = [&](int q, int n, int len, int i, int &first, int &count, int &c) {
-        const int kt = own_keyblocks(len), ct = own_coltiles(a, n);
-        const int col = i * a.G + gq, u = hk * ct + (col >> 4);
-        const int t0 = a.own_off[q] + u * kt, w0 = t0 / run, w1 = (t0 + kt - 1) / run;
-        first = a.own_unit[q] + u + w0;
-        count = kt && first + w1 - w0 < a.own_parts ? w1 - w0 + 1 : 0;
-        c = col & 15;
-    };
-    int f1 = 0, n1 = 0, c1 = 0, f2 = 0, n2 = 0, c2 = 0;
-    if (s.n <= a.small_rows) own(r, s.n, s.len, row - s.first, f1, n1, c1);
-    if (a.own_prefix) own(a.R, rows, prefix_keys(a), row, f2, n2, c2);
-    const int parts = tile_parts + n1 + n2;
+    // attn_own's parts: of the workgroups that have blocks of the row's unit, the four waves'
+    // or (a wide unit) that of the wave whose column it is
+    int own_part = 0, own_n = 0, own_c = 0, own_step = 1;
+    {
+        const int run = own_run(a, a.own_off[a.R]), kt = own_keyblocks(s.len), ct = own_coltiles(a, s.n);
+        const int col = (row - s.first) * a.G + gq, u = hk * ct + (col >> 6);
+        const int t0 = a.own_off[r] + u * kt, w0 = t0 / run, wgs = (t0 + kt - 1) / run - w0 + 1;
+        const bool wide = s.n * a.G > 16;
+        own_part = 4 * (a.own_unit[r] + u + w0) + (wide ? (col >> 4) & 3 : 0);
+        own_step = wide ? 4 : 1;
+        own_c = col & 15;
+        if (kt && s.n <= a.small_rows) own_n = wide ? wgs : 4 * wgs;
+        if (own_part + own_step * own_n > a.own_parts + 3) own_n = 0;
+    }
+    const int parts = tile_parts + own_n;
     float M = -INFINITY, L = 0.f, acc[PER] = {};
-    for (int i0 = 0; i0 < parts; i0 += 64) {
-        // part i0 + lane: its number among attn_tile's or attn_own's parts
-        const int i = min(i0 + lane, parts - 1), j = i - tile_parts;
-        const bool t = j < 0;
-        const long at = t ? ((long)i * a.N + row) * a.H + h : j < n1 ? (f1 + j) * 16L + c1 : (f2 + j - n1) * 16L + c2;
-        const int k = min(64, parts - i0);
+    for (int i0 = 0; i0 * WPR + turn < parts; i0 += 64) {
+        // this lane's part
+        const int k = min(64, (parts - turn + WPR - 1) / WPR - i0);
+        const int i = (i0 + min(lane, k - 1)) * WPR + turn;
+        const bool t = i < tile_parts;
+        long at = ((long)i * a.N + row) * a.H + h;
+        if (!t) at = (own_part + own_step * (i - tile_parts)) * 16L + own_c;
         float2 x = (t ? a.tile_ml : a.own_ml)[at];
         if (lane >= k) x = make_float2(-INFINITY, 0.f);
         const float *const po = (t ? a.tile_o : a.own_o) + at * D;
@@ -857,7 +847,7 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
 #pragma unroll
             for (int e = 0; e < AHEAD; ++e) {
                 const int y = min(i + e, k - 1);
-                const uintptr_t p = (uintptr_t)__builtin_amdgcn_readlane(plo, y) & 0xFFFFFFFFu;
+                const uintptr_t p = (uintptr_t)(uint32_t)__builtin_amdgcn_readlane(plo, y);
                 const float *o = reinterpret_cast<const float *>(p | (uintptr_t)(uint32_t)__builtin_amdgcn_readlane(phi, y) << 32);
 #pragma unroll
                 for (int z = 0; z < PER; ++z) v[e][z] = o[lane + 64 * z];
@@ -889,6 +879,26 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
             }
         }
     }
+    if (WPR == 4) {
+        if (lane == 0) sm_ml[w] = make_float2(M, L);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) sm_o[w][lane + 64 * e] = acc[e];
+        __syncthreads();
+        if (w != 0) return;
+        float M4 = M;
+#pragma unroll
+        for (int q = 1; q < WPR; ++q) M4 = fmaxf(M4, sm_ml[q].x);
+        L = 0.f;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+#pragma unroll
+        for (int q = 0; q < WPR; ++q) {
+            const float f = sm_ml[q].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm_ml[q].x - M4);
+            L += f * sm_ml[q].y;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) acc[e] += f * sm_o[q][lane + 64 * e];
+        }
+    }
     const float inv = L == 0.f ? 0.f : 1.f / L;
     uint16_t *po = a.out + (size_t)row * a.out_stride + (size_t)h * D;
 #pragma unroll
@@ -898,7 +908,7 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
 // ---------------------------------------------------------------- host side
 
 struct SaPlan {
-    int small_rows, rows_max, any_big, nsplit, own_prefix, own_wgs, use_tile;
+    int small_rows, rows_max, any_big, nsplit, own_wgs, use_tile;
     long tiles, own_parts;
     long tile_o, tile_ml, own_o, own_ml, own_idx, bytes;       // workspace offsets
 };
@@ -911,12 +921,11 @@ SaPlan plan_shared(long N, long R, long H, long Hkv, long D, long own_cap, long 
     if (max_new > N) max_new = N;
     p.small_rows = (int)(64 / G > 1 ? 64 / G : 1);
     p.any_big = max_new > p.small_rows;
-    p.own_prefix = prefix_cap > 0 && cols <= 32 && !p.any_big;
-    p.use_tile = p.any_big || (prefix_cap > 0 && !p.own_prefix);
+    p.use_tile = p.any_big || prefix_cap > 0;
     p.tiles = (cols + SA_COLS - 1) / SA_COLS;
     // attn_tile: a workgroup a CU, and four key blocks at least
     const long wgs = p.tiles * Hkv;
-    const long blocks = ((p.own_prefix ? 0 : prefix_cap) + (p.any_big ? own_cap : 0) + SA_KB - 1) / SA_KB;
+    const long blocks = (prefix_cap + (p.any_big ? own_cap : 0) + SA_KB - 1) / SA_KB;
     long ns = wgs ? cus / wgs : 1;
     if (ns > blocks / 4) ns = blocks / 4;
     p.nsplit = (int)(ns < 1 ? 1 : ns > 64 ? 64 : ns);
@@ -924,14 +933,13 @@ SaPlan plan_shared(long N, long R, long H, long Hkv, long D, long own_cap, long 
     // than the rows make
     const long rows_max = max_new < p.small_rows ? max_new : p.small_rows;
     p.rows_max = (int)rows_max;
-    long coltiles = R * ((rows_max * G + 15) / 16);
-    if (coltiles > R + cols / 16) coltiles = R + cols / 16;
-    const long pre = p.own_prefix ? (cols + 15) / 16 : 0;
-    const long keyblocks = coltiles * ((own_cap + SO_KB - 1) / SO_KB) + pre * ((prefix_cap + SO_KB - 1) / SO_KB);
+    long coltiles = R * ((rows_max * G + 63) / 64);
+    if (coltiles > R + cols / 64) coltiles = R + cols / 64;
+    const long keyblocks = coltiles * ((own_cap + SA_KB - 1) / SA_KB);
     long ow = 2 * cus;
-    if (ow > (Hkv * keyblocks + SO_WAVES - 1) / SO_WAVES) ow = (Hkv * keyblocks + SO_WAVES - 1) / SO_WAVES;
+    if (ow > Hkv * keyblocks) ow = Hkv * keyblocks;
     p.own_wgs = (int)(ow < 1 ? 1 : ow);
-    p.own_parts = Hkv * (coltiles + pre) + (long)p.own_wgs * SO_WAVES;
+    p.own_parts = 4 * (Hkv * coltiles + p.own_wgs);
     auto up = [](long v) { return (v + 255) / 256 * 256; };
     long at = 0;
     const long tparts = p.use_tile ? p.nsplit * N * H : 0;
@@ -939,23 +947,33 @@ SaPlan plan_shared(long N, long R, long H, long Hkv, long D, long own_cap, long 
     p.tile_ml = at; at += up(tparts * 8);
     p.own_o = at; at += up(p.own_parts * 16 * D * 4);
     p.own_ml = at; at += up(p.own_parts * 16 * 8);
-    p.own_idx = at; at += up((R + 2) * 2 * 4);
+    p.own_idx = at; at += up((R + 1) * 2 * 4);
     p.bytes = at;
     return p;
 }
 
 template <int D>
 int run_shared(const SaArgs &a, const SaPlan &p, hipStream_t stream) {
-    const int own_lds = (int)sizeof(OwnLds<D>) + (a.R + 2) * 8;
-    const int lds = a.tile_wgs && SaGeo<D>::LDS > own_lds ? SaGeo<D>::LDS : own_lds;
-    static_assert(SaGeo<D>::LDS <= 65536 && sizeof(OwnLds<D>) + (SA_MAX_SEQ + 2) * 8 <= 65536,
-                  "no larger dynamic LDS is asked for");
+    const int lds = SaGeo<D>::LDS + (2 * a.R + 1) * 4;
     auto kern = a.shift >= 6 ? attn_shared_kernel<D, true> : attn_shared_kernel<D, false>;
+    // more than 64 KB of LDS has to be allowed, once a device
+    static std::atomic<uint64_t> allowed[2];
+    int dev = 0;
+    SC_HIP_CHECK(hipGetDevice(&dev));
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(allowed[a.shift >= 6].load() & bit)) {
+        SC_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                         SaGeo<D>::LDS + (2 * SA_MAX_SEQ + 1) * 4));
+        allowed[a.shift >= 6].fetch_or(bit);
+    }
     hipLaunchKernelGGL(kern, dim3((unsigned)(a.own_wgs + a.tile_wgs)), dim3(SA_THREADS), lds, stream, a);
     SC_HIP_CHECK(hipGetLastError());
     const bool by_seq = (p.nsplit == 1 || !p.any_big) && (long)a.R * p.rows_max <= a.N;
     const long merge_rows = by_seq ? (long)a.R * p.rows_max : a.N;
-    hipLaunchKernelGGL(attn_merge_kernel<D>, dim3((unsigned)((merge_rows * a.H + 3) / 4)), dim3(256), 0, stream, a,
+    const long heads = merge_rows * a.H;
+    const bool wide = heads <= 4L * device_info().num_cus;
+    auto merge = wide ? attn_merge_kernel<D, 4> : attn_merge_kernel<D, 1>;
+    hipLaunchKernelGGL(merge, dim3((unsigned)(wide ? heads : (heads + 3) / 4)), dim3(256), 0, stream, a,
                        p.use_tile ? p.nsplit : 0, by_seq ? p.rows_max : 0);
     SC_HIP_CHECK(hipGetLastError());
     return SC_OK;
@@ -1008,7 +1026,7 @@ int launch_attention_shared(const uint16_t *q, long q_stride, const uint16_t *kc
     a.prefix_table = prefix_table; a.prefix_len = prefix_len;
     a.N = (int)N; a.R = (int)R; a.H = (int)H; a.Hkv = (int)Hkv; a.G = (int)(H / Hkv);
     a.width = (int)width; a.shift = shift; a.n_blocks = (int)n_blocks; a.prefix_width = (int)prefix_width;
-    a.small_rows = p.small_rows; a.any_big = p.any_big; a.nsplit = p.nsplit; a.own_prefix = p.own_prefix;
+    a.small_rows = p.small_rows; a.any_big = p.any_big; a.nsplit = p.nsplit;
     a.own_wgs = p.own_wgs;
     a.tile_wgs = p.use_tile ? (int)(p.tiles * p.nsplit * Hkv) : 0;
     a.tiles = (int)p.tiles;
@@ -1021,7 +1039,7 @@ int launch_attention_shared(const uint16_t *q, long q_stride, const uint16_t *kc
     a.own_ml = reinterpret_cast<float2 *>(ws + p.own_ml);
     a.own_parts = (int)p.own_parts;
     a.own_off = reinterpret_cast<int32_t *>(ws + p.own_idx);
-    a.own_unit = a.own_off + R + 2;
+    a.own_unit = a.own_off + R + 1;
     return D == 128 ? run_shared<128>(a, p, stream) : run_shared<64>(a, p, stream);
 }
 
