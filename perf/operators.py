@@ -207,6 +207,9 @@ def prepare(case, seed):
         from shardcompute_amd import _lib
         if st["kind"] == "step":
             st["out"] = _lib.block_step_buffers(case["R"], st["rows"], torch.device("cuda"))
+            # a sequence that gives its blocks back gets others in their place: a further pass
+            # starts from the tables as they were
+            st["before"] = None if st["release"] is None else st["tables"].clone()
         if st["kind"] == "attend":
             need = _lib.attention_shared_workspace_bytes(
                 st["rows"], case["R"], st["H"], st["Hkv"], st["D"], st["tables"].shape[1] * st["bs"],
@@ -225,6 +228,8 @@ def run(state):
 def _run_own(st):
     from shardcompute_amd import _lib
     if st["kind"] == "step":
+        if st["before"] is not None:
+            st["tables"].copy_(st["before"])
         s = _lib.block_tables(st["lengths"], st["new"], st["tables"], st["free"], st["n_free"], st["bs"], st["rows"],
                               prefix_len=st["prefix_len"], release=st["release"], out=st["out"])
         return dict(lengths=s.lengths, n_free=s.n_free, row_starts=s.row_starts, slots=s.slots, positions=s.positions,
