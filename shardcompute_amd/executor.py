@@ -15,17 +15,21 @@ slot are device counters, so the same graph serves every step.  Stop tokens are
 checked on the host every ``check_every`` tokens; tokens generated past a stop
 token are discarded, so the output matches a per-token check.
 
+``generate_batch`` decodes prompts of different lengths behind one shared prefix, from a
+cache in blocks (:class:`~shardcompute_amd.block_cache.BlockKVCache`).
+
 Sampling (``temperature > 0``: temperature, top-p, categorical draw, as in
 ``executor.py:280-305``) runs eagerly with torch ops on the device and is not
 part of the measured greedy path.
 """
 import time
 from dataclasses import dataclass, field
-from typing import Any, Callable, Dict, List, Optional
+from typing import Any, Callable, Dict, List, Optional, Sequence
 
 import torch
 
 from . import _lib
+from .block_cache import BlockBatch, BlockKVCache
 from .decode_plan import maybe_plan
 from .kv_cache import KVCache, round_capacity
 from .parallel.transformer import ParallelTransformer, StepBuffers, run_sync
@@ -138,6 +142,45 @@ class DecodeGraph:
             for _ in range(steps):
                 self._step()
         return g, self.logits
+
+
+class BlockDecodeGraph:
+    """Greedy decode steps of every sequence of a block cache, as a replayable graph of one
+    step: lengths, tables and positions advance on the device, so it replays unchanged."""
+
+    def __init__(self, model: ParallelTransformer, cache: BlockKVCache, tokens: torch.Tensor, use_graph: bool = True):
+        B = cache.max_sequences
+        self.model, self.cache, self.tokens, self.use_graph = model, cache, tokens, use_graph
+        self.bufs = StepBuffers(model, B, 1, 0)
+        self.new = torch.ones(B, dtype=torch.int32, device=cache.device)
+        self.step = torch.zeros(1, dtype=torch.int32, device=cache.device)
+        self.batch = BlockBatch(cache, cache._buffers(B, B, cache.lengths), cache.tables, B, 1, cache.host_prefix > 0)
+        att = model.layers[0].attention
+        need = self.batch.workspace_bytes(att.local_num_heads, att.local_num_kv_heads, att.head_dim)
+        self.bufs.workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=cache.device)
+        self.graph = None           # (graph, logits of its step)
+        self.logits = None          # logits of the most recent step
+
+    def _step(self):
+        return self.model.decode_step_blocks(self.bufs, self.batch, self.new, self.tokens, self.step)
+
+    def run(self, n: int):
+        """Advance every sequence by ``n`` tokens (the first call runs one step eagerly, then captures)."""
+        one = [1] * self.cache.max_sequences
+        for _ in range(n):
+            lengths, free = self.cache._plan(one, None)
+            if self.graph is not None:
+                self.graph[0].replay()
+                self.logits = self.graph[1]
+            else:
+                self.logits = self._step()
+                if self.use_graph:
+                    torch.cuda.synchronize()
+                    g = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(g):
+                        logits = self._step()
+                    self.graph = (g, logits)
+            self.cache.host_lengths, self.cache.host_free = lengths, free
 
 
 class ParallelExecutor:
@@ -321,6 +364,60 @@ class ParallelExecutor:
         self.last_metrics = ExecutionMetrics(total_time_ms=(time.perf_counter() - t0) * 1000, input_tokens=n_gen,
                                              output_shape=[1, n_gen])
         return torch.cat([ids, tokens[:, :n_gen].to(out_dtype)], dim=1)
+
+    async def generate_batch(self, prompts: Sequence[Sequence[int]], prefix: Optional[Sequence[int]] = None,
+                             max_new_tokens: int = 100, temperature: float = 0.0, top_p: float = 0.9,
+                             stop_tokens: Optional[List[int]] = None, block_size: int = 64) -> List[List[int]]:
+        """Tokens for several prompts of any lengths behind one shared ``prefix`` (the same
+        prompt several times gives several samples of it at ``temperature`` > 0).
+
+        The prefix is computed and held once, in a :class:`BlockKVCache`; the prompts' own
+        tokens are taken in as one ragged step, then all sequences decode together
+        (``temperature`` 0: the greedy step as a replayed HIP graph).  Returns each prompt's
+        new tokens, up to its first stop token, which is included.  Sequences that have
+        stopped run on until all have; their further tokens are dropped."""
+        stop = set(stop_tokens or [])
+        prompts = [[int(t) for t in p] for p in prompts]
+        if not prompts or any(not p for p in prompts):
+            raise ValueError("every prompt needs at least one token of its own")
+        if max_new_tokens <= 0:
+            return [[] for _ in prompts]
+        t0 = time.perf_counter()
+        m, R, prefix = self.model, len(prompts), list(prefix or [])
+        own = [-(-(len(p) + max_new_tokens) // block_size) for p in prompts]
+        cache = m.new_block_cache(R, max(own) * block_size, sum(own) + -(-len(prefix) // block_size), block_size,
+                                  len(prefix))
+        if prefix:
+            await m.forward_blocks(prefix, cache.begin_prefix(len(prefix)))
+        logits = await m.forward_blocks([t for p in prompts for t in p], cache.begin([len(p) for p in prompts]))
+        tokens = torch.zeros((R, max_new_tokens), dtype=torch.int32, device=m.device)
+
+        def finished(n):             # every sequence has a stop token among its first n
+            return bool(stop) and all(stop & set(row) for row in tokens[:, :n].tolist())
+
+        n = 1
+        if temperature == 0:
+            dec = BlockDecodeGraph(m, cache, tokens, use_graph=self.use_graphs)
+            _lib.argmax(logits, ids=dec.bufs.ids.view(-1), tokens=tokens, step=dec.step)
+            _lib.add_i32(dec.step, 1)
+            while n < max_new_tokens and not finished(n):
+                k = min(self.check_every, max_new_tokens - n)
+                dec.run(k)
+                n += k
+            cache.check_status()
+        else:
+            tokens[:, 0] = nxt = self._sample(logits, temperature, top_p)
+            while n < max_new_tokens and not finished(n):
+                logits = await m.forward_blocks(nxt, cache.begin([1] * R))
+                tokens[:, n] = nxt = self._sample(logits, temperature, top_p)
+                n += 1
+        out = []
+        for row in tokens[:, :n].tolist():
+            end = next((i + 1 for i, t in enumerate(row) if t in stop), n)
+            out.append(row[:end])
+        self.last_metrics = ExecutionMetrics(total_time_ms=(time.perf_counter() - t0) * 1000,
+                                             input_tokens=sum(map(len, out)), output_shape=[R, n])
+        return out
 
     def reset_cache(self):
         self._past_key_values = None

@@ -26,6 +26,7 @@ import numpy as np
 import torch
 
 from .. import _lib
+from ..block_cache import BlockLayerKV
 from ..kv_cache import KVCache, LayerKV, round_capacity
 from ._fused import FusedColumns
 from .column_linear import ColumnParallelLinear
@@ -171,8 +172,23 @@ class ParallelAttention:
         (RoPE, append and attention in one launch, plus the range merge), with the
         mask when one is given.  ``mask``
         is the reference's additive ``attention_mask``, broadcastable to
-        ``[B, local heads, S, cached + S keys]`` (``attention.py:449-450``)."""
+        ``[B, local heads, S, cached + S keys]`` (``attention.py:449-450``).
+
+        With a :class:`~shardcompute_amd.block_cache.BlockLayerKV` the rows are those of its
+        step: a ragged batch behind a shared prefix, q rotated in place."""
         H, Hk, D = self.local_num_heads, self.local_num_kv_heads, self.head_dim
+        if isinstance(kv, BlockLayerKV):
+            if mask is not None or pos_offset:
+                raise ValueError("a block cache takes no attention mask and no position offset")
+            b, st = kv.batch, kv.batch.step
+            if qkv.shape[0] != b.rows:
+                raise ValueError(f"the step has {b.rows} rows, got {qkv.shape[0]}")
+            cos_t, sin_t = self.rope.tables(b.cache.max_positions, qkv.device)
+            q = _lib.rope_append_blocks(qkv, H, Hk, D, cos_t, sin_t, kv.k, kv.vt, st.slots, st.positions,
+                                        out=qkv[:, :H * D])
+            return _lib.attention_shared(q, H, Hk, D, kv.k, kv.vt, st.row_starts, st.lengths, b.tables, self.scale,
+                                         prefix_table=b.prefix_table, prefix_len=b.prefix_len, max_new=b.max_new,
+                                         out=out, workspace=workspace)
         cos_t, sin_t = self.rope.tables(kv.cache.capacity + pos_offset, qkv.device)
         n_keys = kv.length + S
         if S == 1 and H // Hk <= 16:

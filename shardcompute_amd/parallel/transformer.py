@@ -30,6 +30,7 @@ from typing import List, Optional, Tuple
 import torch
 
 from .. import _lib
+from ..block_cache import BlockBatch, BlockKVCache
 from ..communicator import IdentityCommunicator
 from ..kv_cache import KVCache, LayerKV, round_capacity
 from .attention import ParallelAttention
@@ -277,6 +278,16 @@ class ParallelTransformer:
         att = self.layers[0].attention
         return KVCache(self.num_layers, batch, att.local_num_kv_heads, att.head_dim, capacity, device=self.device)
 
+    def new_block_cache(self, max_sequences: int, max_length: int, num_blocks: Optional[int] = None,
+                        block_size: int = 64, max_prefix: int = 0) -> BlockKVCache:
+        """A cache in blocks for ``max_sequences`` sequences of up to ``max_length`` own positions
+        behind a shared prefix of up to ``max_prefix`` (default: blocks for all of them)."""
+        att = self.layers[0].attention
+        if num_blocks is None:
+            num_blocks = max_sequences * -(-max_length // block_size) + -(-max_prefix // block_size)
+        return BlockKVCache(self.num_layers, att.local_num_kv_heads, att.head_dim, num_blocks, max_sequences,
+                            max_length, block_size=block_size, max_prefix=max_prefix, device=self.device)
+
     def _embed_sync(self, input_ids, out=None):
         if isinstance(self.embed_tokens, VocabParallelEmbedding):
             return self.embed_tokens.forward_sync(input_ids, out=out)
@@ -415,6 +426,36 @@ class ParallelTransformer:
         new_cache = (cache.as_tuples() if tuples else cache) if use_cache else None
         return logits.reshape(B, 1 if (last_only and S > 1) else S, -1), new_cache
 
+    async def forward_blocks(self, input_ids, batch: BlockBatch, *, all_rows: bool = False):
+        """One step of a ragged batch over a block cache: ``input_ids`` ``[rows]``, the new
+        positions' tokens of the sequences of ``batch`` in order.  Returns the logits of each
+        sequence's last row ``[sequences, vocab]`` (of a sequence without rows: some row's), or
+        of every row with ``all_rows``."""
+        ids = input_ids if isinstance(input_ids, torch.Tensor) else torch.as_tensor(input_ids)
+        ids = ids.to(self.device)
+        if ids.dim() != 1 or ids.shape[0] != batch.rows:
+            raise ValueError(f"input_ids must be [{batch.rows}], the step's rows")
+        N = batch.rows
+        h = (await self._embed(ids.view(1, N))).reshape(N, self.hidden_size).contiguous()
+        h, pending = await self._trunk(h, batch, 1, N)
+        if not all_rows:
+            rows = batch.last_rows
+            h = h[rows]
+            pending = pending[rows] if pending is not None else None
+        return (await self._head(h, pending, h.shape[0], 1, False)).reshape(h.shape[0], -1)
+
+    def decode_step_blocks(self, bufs: StepBuffers, batch: BlockBatch, new, tokens: torch.Tensor, step: torch.Tensor):
+        """One greedy decode step of every sequence of a block cache on device, no host
+        synchronisation: the step's tables (``new``: one position each), embed ``bufs.ids``, every
+        layer, argmax into ``bufs.ids`` and ``tokens[:, step]``, then advance ``step``.  Captured
+        once, replayed per token."""
+        c, st, B = batch.cache, batch.step, bufs.B
+        _lib.block_tables(c.lengths, new, c.tables, c.free_blocks, c.n_free, c.block_size, batch.rows,
+                          prefix_len=c.prefix_len, out=st)
+        h = self._embed_sync(bufs.ids, out=bufs.h.view(B, 1, self.hidden_size)).view(B, self.hidden_size)
+        h, pending = run_sync(self._trunk(h, batch, B, 1, bufs))
+        return self._greedy(h, pending, bufs, tokens, step, step, 1)
+
     def decode_step(self, bufs: StepBuffers, cache: KVCache, tokens: torch.Tensor, logits_out=None):
         """One greedy decode step on device, no host synchronisation: embed
         ``bufs.ids``, run every layer (appending at ``cache.counters[0]``), argmax the
@@ -427,6 +468,11 @@ class ParallelTransformer:
         else:
             h = self._embed_sync(bufs.ids, out=bufs.h.view(B, 1, self.hidden_size)).view(B, self.hidden_size)
             h, pending = run_sync(self._trunk(h, cache, B, 1, bufs))
+        return self._greedy(h, pending, bufs, tokens, cache.counters[1:], cache.counters, 2)
+
+    def _greedy(self, h, pending, bufs: StepBuffers, tokens, step, counters, n_counters: int):
+        """The greedy tail of a decode step: logits of ``h + pending``, their argmax into
+        ``bufs.ids`` and ``tokens[:, step]``, ``counters[:n_counters] += 1``."""
         lm = self.lm_head
         if (isinstance(lm, QuantizedColumnParallelLinear) and (not lm.gather_output or self.world_size == 1)
                 and self.norm.fusable):
@@ -438,12 +484,12 @@ class ParallelTransformer:
             logits, _ = _lib.decode_head(h, self.norm.weight, self.norm.eps, lm.quantized_weight, lm.scales,
                                          lm.biases_quant, bufs.ids.view(-1), bufs.head_ws, residual=pending,
                                          xn_out=bufs.hn, bias=lm.bias if lm.has_bias else None, bits=lm.bits,
-                                         group_size=lm.group_size, tokens=tokens, step=cache.counters[1:],
-                                         counters=cache.counters, n_counters=2)
+                                         group_size=lm.group_size, tokens=tokens, step=step,
+                                         counters=counters, n_counters=n_counters)
             return logits
-        logits = run_sync(self._head(h, pending, B, 1, True, hn_out=bufs.hn))
-        _lib.argmax(logits.reshape(B, -1), ids=bufs.ids.view(-1), tokens=tokens, step=cache.counters[1:])
-        _lib.add_i32(cache.counters, 1, n=2)
+        logits = run_sync(self._head(h, pending, bufs.B, 1, True, hn_out=bufs.hn))
+        _lib.argmax(logits.reshape(bufs.B, -1), ids=bufs.ids.view(-1), tokens=tokens, step=step)
+        _lib.add_i32(counters, 1, n=n_counters)
         return logits
 
     @property

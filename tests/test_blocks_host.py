@@ -85,3 +85,26 @@ def test_wrappers_need_gpu_tensors():
     with pytest.raises(RuntimeError, match="GPU"):
         _lib.attention_shared(torch.zeros(1, 64, dtype=torch.bfloat16), 1, 1, 64, z, z, z, z, z, 1.0)
     assert ctypes.c_int64 in _lib.load().sc_attention_shared_bf16.argtypes
+
+
+def test_cache_bookkeeping_on_the_host():
+    from shardcompute_amd.block_cache import BlockKVCache
+    c = BlockKVCache(2, 2, 64, num_blocks=5, max_sequences=3, max_length=40, block_size=16, max_prefix=20,
+                     device=torch.device("cpu"))
+    assert c.k.shape == (2, 5, 2, 16, 64) and c.vt.shape == (2, 5, 2, 64, 16) and c.tables.shape == (3, 3)
+    assert c.prefix_table.shape == (2,) and c.max_positions == 60 and c.free_blocks.tolist() == [4, 3, 2, 1, 0]
+    lengths, free = c._plan([17, 0, 16], None)
+    assert lengths == [17, 0, 16] and free == 2
+    c.host_lengths, c.host_free = lengths, free
+    assert c._plan([15, 16, 16], None) == ([32, 16, 32], 0)
+    assert c._plan([1, 40, 1], [True, False, True]) == ([1, 40, 1], 0)
+    with pytest.raises(RuntimeError, match="full: the step needs 1 blocks more"):
+        c.check_room([16, 16, 16])
+    with pytest.raises(RuntimeError, match="sequence 0 would hold 49 positions"):
+        c.check_room([32, 0, 0])
+    with pytest.raises(ValueError, match="-1 new positions"):
+        c.check_room([0, -1, 0])
+    with pytest.raises(ValueError, match="block_size"):
+        BlockKVCache(1, 1, 64, 4, 1, 64, block_size=48, device=torch.device("cpu"))
+    with pytest.raises(ValueError, match="at least one"):
+        BlockKVCache(1, 1, 64, 0, 1, 64, device=torch.device("cpu"))
