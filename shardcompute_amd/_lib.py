@@ -851,35 +851,35 @@ def block_step_buffers(R, rows, device):
     return BlockStep(i32(R), i32(1), i32(R + 1), i32(rows), i32(rows), torch.zeros(1, dtype=torch.int32, device=device))
 
 
-def _i32_flat(t, n, name):
-    if t.dtype != torch.int32 or t.numel() < n or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor of at least {n} entries")
-    return t
+_INT32, _BF16 = torch.int32, torch.bfloat16
 
 
-def _same_device(t, *others):
+def _gpu_of(t):
     dev = t.get_device()
-    for x in others:
-        if x is not None and x.get_device() != dev:
-            raise RuntimeError("all tensors of a call must be on one GPU")
+    if dev < 0:
+        raise RuntimeError("shardcompute_amd kernels need GPU tensors (no CPU fallback)")
+    return dev
 
 
-class _on_device:
-    """Makes a tensor's GPU the current one for a launch, when it is not already."""
+def _i32_flat(t, n, name, dev):
+    """A contiguous int32 tensor of at least ``n`` entries on GPU ``dev``."""
+    if t.dtype is not _INT32 or t.numel() < n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of at least {n} entries")
+    if t.get_device() != dev:
+        _gpu_of(t)
+        raise RuntimeError(f"{name} must be on the GPU of the call's other tensors")
 
-    def __init__(self, t):
-        self.dev = t.get_device()
-        self.back = None
 
-    def __enter__(self):
-        cur = torch.cuda.current_device()
-        if cur != self.dev:
-            torch.cuda.set_device(self.dev)
-            self.back = cur
+def _on_gpu(dev, fn, *args):
+    """``fn(*args, stream)`` with GPU ``dev`` current and its current stream."""
+    if torch.cuda.current_device() == dev:
+        return fn(*args, _stream_of(dev))
+    with torch.cuda.device(dev):
+        return fn(*args, _stream_of(dev))
 
-    def __exit__(self, *exc):
-        if self.back is not None:
-            torch.cuda.set_device(self.back)
+
+def _stream_of(dev):
+    return torch.cuda.current_stream(dev).cuda_stream if _raw_stream is None else _raw_stream(dev)
 
 
 def block_tables(lengths, new, tables, free_blocks, n_free, block_size, rows, prefix_len=None, release=None, out=None):
@@ -893,53 +893,65 @@ def block_tables(lengths, new, tables, free_blocks, n_free, block_size, rows, pr
     may be the ones passed in); without it a new one is allocated.  A step that does not fit
     changes nothing, has no rows and sets ``status`` (see ``sc_block_tables_i32``)."""
     lib = load()
-    _require_gpu(lengths, new, tables, free_blocks, n_free, prefix_len, release)
-    R = lengths.numel()
-    _i32_flat(lengths, 1, "lengths"), _i32_flat(new, R, "new"), _i32_flat(n_free, 1, "n_free")
-    _i32_flat(free_blocks, 1, "free_blocks")
-    if tables.dtype != torch.int32 or tables.dim() != 2 or tables.shape[0] != R or not tables.is_contiguous():
-        raise ValueError(f"tables must be a contiguous int32 [{R}, width] tensor")
+    dev, R = _gpu_of(lengths), lengths.numel()
     if block_size not in BLOCK_SIZES:
         raise ValueError(f"block_size must be one of {BLOCK_SIZES}, got {block_size}")
     if new.numel() != R:
         raise ValueError(f"new must hold {R} entries")
-    if prefix_len is not None:
-        _i32_flat(prefix_len, 1, "prefix_len")
-    if release is not None and (release.dtype not in (torch.bool, torch.uint8) or release.numel() != R
-                                or not release.is_contiguous()):
-        raise ValueError(f"release must be a contiguous bool tensor of {R} entries")
+    if tables.dim() != 2 or tables.shape[0] != R:
+        raise ValueError(f"tables must be a contiguous int32 [{R}, width] tensor")
     if out is None:
         out = block_step_buffers(R, rows, lengths.device)
-    else:
-        _require_gpu(*out)
-        _i32_flat(out.lengths, R, "out.lengths"), _i32_flat(out.n_free, 1, "out.n_free")
-        _i32_flat(out.row_starts, R + 1, "out.row_starts"), _i32_flat(out.slots, rows, "out.slots")
-        _i32_flat(out.positions, rows, "out.positions"), _i32_flat(out.status, 1, "out.status")
-    _same_device(lengths, new, tables, free_blocks, n_free, prefix_len, release, *out)
-    with _on_device(lengths):
-        rc = lib.sc_block_tables_i32(_ptr(lengths), _ptr(new), _ptr(release), _ptr(tables), _ptr(free_blocks),
-                                     _ptr(n_free), _ptr(prefix_len), R, tables.shape[1], block_size,
-                                     free_blocks.numel(), rows, _ptr(out.lengths), _ptr(out.n_free),
-                                     _ptr(out.row_starts), _ptr(out.slots), _ptr(out.positions), _ptr(out.status),
-                                     _stream(lengths))
+    lengths_out, n_free_out, row_starts, slots, positions, status = out
+    _i32_flat(lengths, 1, "lengths", dev), _i32_flat(new, R, "new", dev), _i32_flat(tables, 0, "tables", dev)
+    _i32_flat(free_blocks, 1, "free_blocks", dev), _i32_flat(n_free, 1, "n_free", dev)
+    _i32_flat(lengths_out, R, "out.lengths", dev), _i32_flat(n_free_out, 1, "out.n_free", dev)
+    _i32_flat(row_starts, R + 1, "out.row_starts", dev), _i32_flat(slots, rows, "out.slots", dev)
+    _i32_flat(positions, rows, "out.positions", dev), _i32_flat(status, 1, "out.status", dev)
+    if prefix_len is not None:
+        _i32_flat(prefix_len, 1, "prefix_len", dev)
+    if release is not None and (release.dtype not in (torch.bool, torch.uint8) or release.numel() != R
+                                or not release.is_contiguous() or release.get_device() != dev):
+        raise ValueError(f"release must be a contiguous bool tensor of {R} entries on the call's GPU")
+    rc = _on_gpu(dev, lib.sc_block_tables_i32, lengths.data_ptr(), new.data_ptr(), _ptr(release), tables.data_ptr(),
+                 free_blocks.data_ptr(), n_free.data_ptr(), _ptr(prefix_len), R, tables.shape[1], block_size,
+                 free_blocks.numel(), rows, lengths_out.data_ptr(), n_free_out.data_ptr(), row_starts.data_ptr(),
+                 slots.data_ptr(), positions.data_ptr(), status.data_ptr())
     if rc:
         _check(rc, "sc_block_tables_i32")
     return out
 
 
-def _pool(k_blocks, vt_blocks, Hkv, D):
+def _pool(k_blocks, vt_blocks, Hkv, D, dev):
     """(blocks, block size) of a pool's layer."""
-    _bf16(k_blocks, "k_blocks"), _bf16(vt_blocks, "vt_blocks")
-    if k_blocks.dim() != 4 or k_blocks.shape[1] != Hkv or k_blocks.shape[3] != D:
-        raise ValueError(f"k_blocks must be [blocks, {Hkv}, block_size, {D}], got {tuple(k_blocks.shape)}")
-    nb, _, bs, _ = k_blocks.shape
-    if tuple(vt_blocks.shape) != (nb, Hkv, D, bs):
+    if k_blocks.dtype is not _BF16 or vt_blocks.dtype is not _BF16:
+        raise TypeError("k_blocks and vt_blocks must be bfloat16")
+    ks = k_blocks.shape
+    if len(ks) != 4 or ks[1] != Hkv or ks[3] != D:
+        raise ValueError(f"k_blocks must be [blocks, {Hkv}, block_size, {D}], got {tuple(ks)}")
+    nb, bs = ks[0], ks[2]
+    if vt_blocks.shape != (nb, Hkv, D, bs):
         raise ValueError(f"vt_blocks must be [{nb}, {Hkv}, {D}, {bs}], got {tuple(vt_blocks.shape)}")
     if not (k_blocks.is_contiguous() and vt_blocks.is_contiguous()):
         raise ValueError("the pool's tensors must be contiguous")
     if bs not in BLOCK_SIZES:
         raise ValueError(f"block_size must be one of {BLOCK_SIZES}, got {bs}")
+    if k_blocks.get_device() != dev or vt_blocks.get_device() != dev:
+        _gpu_of(k_blocks), _gpu_of(vt_blocks)
+        raise RuntimeError("the pool must be on the GPU of the call's other tensors")
     return nb, bs
+
+
+def _row_matrix(t, cols, name, dev):
+    """Row stride of a row-major bf16 matrix [rows, >= cols] on GPU ``dev``."""
+    if t.dtype is not _BF16:
+        raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
+    if t.dim() != 2 or t.shape[1] < cols or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be a row-major [rows, >= {cols}] matrix")
+    if t.get_device() != dev:
+        _gpu_of(t)
+        raise RuntimeError(f"{name} must be on the GPU of the call's other tensors")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def rope_append_blocks(qkv, H, Hkv, D, cos_t, sin_t, k_blocks, vt_blocks, slots, positions, out=None):
@@ -949,28 +961,26 @@ def rope_append_blocks(qkv, H, Hkv, D, cos_t, sin_t, k_blocks, vt_blocks, slots,
     be the q part of qkv).  Rows whose slot is outside the pool (-1) or whose position is
     outside the tables are left alone.  The slots of different rows must differ."""
     lib = load()
-    _require_gpu(qkv, cos_t, sin_t, k_blocks, vt_blocks, slots, positions, out)
-    _bf16(qkv, "qkv")
-    if qkv.dim() != 2 or qkv.shape[1] < (H + 2 * Hkv) * D or qkv.stride(1) != 1:
-        raise ValueError(f"qkv must be a row-major [N, >= {(H + 2 * Hkv) * D}] matrix")
-    N = qkv.shape[0]
-    nb, bs = _pool(k_blocks, vt_blocks, Hkv, D)
-    _i32_flat(slots, N, "slots"), _i32_flat(positions, N, "positions")
-    if (cos_t.dtype != torch.float32 or sin_t.dtype != torch.float32 or cos_t.shape != sin_t.shape
-            or cos_t.dim() != 2 or cos_t.shape[1] != D // 2 or not cos_t.is_contiguous() or not sin_t.is_contiguous()):
+    dev = _gpu_of(qkv)
+    stride, N = _row_matrix(qkv, (H + 2 * Hkv) * D, "qkv", dev), qkv.shape[0]
+    nb, bs = _pool(k_blocks, vt_blocks, Hkv, D, dev)
+    _i32_flat(slots, N, "slots", dev), _i32_flat(positions, N, "positions", dev)
+    ts = cos_t.shape
+    if (cos_t.dtype is not torch.float32 or sin_t.dtype is not torch.float32 or ts != sin_t.shape
+            or len(ts) != 2 or ts[1] != D // 2 or not cos_t.is_contiguous() or not sin_t.is_contiguous()):
         raise ValueError("cos/sin tables must be contiguous fp32 [L, D/2]")
+    if cos_t.get_device() != dev or sin_t.get_device() != dev:
+        raise RuntimeError("the tables must be on the GPU of the call's other tensors")
     if out is None:
-        out = torch.empty((N, H * D), dtype=torch.bfloat16, device=qkv.device)
-    elif out.dtype != torch.bfloat16 or out.dim() != 2 or tuple(out.shape) != (N, H * D) or out.stride(1) != 1:
-        raise ValueError(f"out must be a row-major bf16 [{N}, {H * D}] matrix")
-    _same_device(qkv, cos_t, sin_t, k_blocks, vt_blocks, slots, positions, out)
+        out = torch.empty((N, H * D), dtype=_BF16, device=qkv.device)
+    out_stride = _row_matrix(out, H * D, "out", dev)
+    if out.shape != (N, H * D):
+        raise ValueError(f"out must be [{N}, {H * D}], got {tuple(out.shape)}")
     if N == 0:
         return out
-    with _on_device(qkv):
-        rc = lib.sc_rope_append_blocks_bf16(_ptr(qkv), qkv.stride(0) if N > 1 else qkv.shape[1], _ptr(out),
-                                            out.stride(0) if N > 1 else H * D, N, H, Hkv, D, _ptr(cos_t), _ptr(sin_t),
-                                            cos_t.shape[0], _ptr(k_blocks), _ptr(vt_blocks), nb, bs, _ptr(slots),
-                                            _ptr(positions), _stream(qkv))
+    rc = _on_gpu(dev, lib.sc_rope_append_blocks_bf16, qkv.data_ptr(), stride, out.data_ptr(), out_stride, N, H, Hkv, D,
+                 cos_t.data_ptr(), sin_t.data_ptr(), ts[0], k_blocks.data_ptr(), vt_blocks.data_ptr(), nb, bs,
+                 slots.data_ptr(), positions.data_ptr())
     if rc:
         _check(rc, "sc_rope_append_blocks_bf16")
     return out
@@ -993,44 +1003,43 @@ def attention_shared(q, H, Hkv, D, k_blocks, vt_blocks, row_starts, lengths, tab
     the rows of one sequence (default N).  Returns out [N, H*D] bf16; rows past the last
     sequence's are left as they were."""
     lib = load()
-    _require_gpu(q, k_blocks, vt_blocks, row_starts, lengths, tables, prefix_table, prefix_len, out, workspace)
-    _bf16(q, "q")
-    if q.dim() != 2 or q.shape[1] < H * D or q.stride(1) != 1:
-        raise ValueError(f"q must be a row-major [N, >= {H * D}] matrix")
-    N = q.shape[0]
-    nb, bs = _pool(k_blocks, vt_blocks, Hkv, D)
-    if tables.dtype != torch.int32 or tables.dim() != 2 or not tables.is_contiguous():
+    dev = _gpu_of(q)
+    stride, N = _row_matrix(q, H * D, "q", dev), q.shape[0]
+    nb, bs = _pool(k_blocks, vt_blocks, Hkv, D, dev)
+    if tables.dim() != 2:
         raise ValueError("tables must be a contiguous int32 [R, width] tensor")
     R, width = tables.shape
-    _i32_flat(lengths, R, "lengths"), _i32_flat(row_starts, R + 1, "row_starts")
+    _i32_flat(tables, 0, "tables", dev), _i32_flat(lengths, R, "lengths", dev)
+    _i32_flat(row_starts, R + 1, "row_starts", dev)
     pw = 0
     if prefix_table is not None:
         if prefix_len is None:
             raise ValueError("a prefix table needs prefix_len")
-        _i32_flat(prefix_len, 1, "prefix_len")
-        pw = _i32_flat(prefix_table, 0, "prefix_table").numel()
+        _i32_flat(prefix_len, 1, "prefix_len", dev), _i32_flat(prefix_table, 0, "prefix_table", dev)
+        pw = prefix_table.numel()
     if out is None:
-        out = torch.empty((N, H * D), dtype=torch.bfloat16, device=q.device)
-    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (N, H * D) or out.stride(1) != 1:
-        raise ValueError(f"out must be a row-major bf16 [{N}, {H * D}] matrix")
+        out = torch.empty((N, H * D), dtype=_BF16, device=q.device)
+    out_stride = _row_matrix(out, H * D, "out", dev)
+    if out.shape != (N, H * D):
+        raise ValueError(f"out must be [{N}, {H * D}], got {tuple(out.shape)}")
     if max_new is None:
         max_new = N
     elif max_new < 0:
         raise ValueError("max_new must not be negative")
-    _same_device(q, k_blocks, vt_blocks, row_starts, lengths, tables, prefix_table, prefix_len, out, workspace)
     if N == 0:
         return out
-    with _on_device(q):
-        need = lib.sc_attention_shared_workspace_bytes(N, R, H, Hkv, D, width * bs, pw * bs, max_new)
-        ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-        if ws_bytes < need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-            ws_bytes = need
-        rc = lib.sc_attention_shared_bf16(_ptr(q), q.stride(0) if N > 1 else H * D, _ptr(k_blocks), _ptr(vt_blocks), nb,
-                                          bs, _ptr(row_starts), _ptr(lengths), _ptr(tables), width,
-                                          _ptr(prefix_table) if pw else None, pw, _ptr(prefix_len) if pw else None,
-                                          _ptr(out), out.stride(0) if N > 1 else H * D, N, R, H, Hkv, D, float(scale),
-                                          int(max_new), _ptr(workspace), ws_bytes, _stream(q))
+    need = lib.sc_attention_shared_workspace_bytes(N, R, H, Hkv, D, width * bs, pw * bs, max_new)
+    ws_bytes = 0
+    if workspace is not None:
+        if workspace.get_device() != dev or not workspace.is_contiguous():
+            raise RuntimeError("the workspace must be contiguous and on the GPU of the call's other tensors")
+        ws_bytes = workspace.numel() * workspace.element_size()
+    if ws_bytes < need:
+        workspace, ws_bytes = torch.empty(need, dtype=torch.uint8, device=q.device), need
+    rc = _on_gpu(dev, lib.sc_attention_shared_bf16, q.data_ptr(), stride, k_blocks.data_ptr(), vt_blocks.data_ptr(), nb,
+                 bs, row_starts.data_ptr(), lengths.data_ptr(), tables.data_ptr(), width,
+                 prefix_table.data_ptr() if pw else None, pw, prefix_len.data_ptr() if pw else None, out.data_ptr(),
+                 out_stride, N, R, H, Hkv, D, float(scale), int(max_new), _ptr(workspace), ws_bytes)
     if rc:
         _check(rc, "sc_attention_shared_bf16")
     return out

@@ -23,7 +23,9 @@ namespace {
 // Integer work of a few bytes per sequence and row, so what counts is the chain of
 // dependent loads and launches.  One workgroup sums, checks and fills the tables; where
 // rows are few it writes them too (STEP_ROWS), else a second launch does, whose
-// workgroups read the finished tables.
+// workgroups read the finished tables.  Up to STEP_THREADS sequences, a thread each, take
+// one pass (block_step_kernel: every sum in one exchange between the waves, a decoded
+// token's slot from registers); more go through in chunks, three times (block_step_many_kernel).
 constexpr int STEP_THREADS = 1024;
 constexpr int STEP_ROWS = 4096;
 
@@ -71,7 +73,140 @@ __device__ __forceinline__ int last_at_most(const int32_t *start, int n, int x) 
     return lo;
 }
 
+// One thread a sequence.  Sums saturate at STEP_MOST, above every limit they are compared
+// with, so none wraps.
+constexpr int STEP_MOST = (1 << 30) - 1;
+
 __global__ void __launch_bounds__(STEP_THREADS) block_step_kernel(StepArgs a) {
+    struct Sums { int back, need, fresh; };
+    __shared__ Sums wave_sum_[STEP_THREADS / 64];
+    __shared__ int wave_flags[STEP_THREADS / 64];
+    __shared__ int first_back[STEP_THREADS], first_need[STEP_THREADS], first_row[STEP_THREADS], held[STEP_THREADS];
+    const int r = threadIdx.x, lane = r & 63, w = r >> 6, n = blockDim.x, nw = n >> 6, R = a.R;
+    const int bs = 1 << a.shift;
+    const long most = (long)a.width << a.shift;                // positions a table has room for
+    const int32_t *table = a.tables + (long)r * a.width;
+
+    int len = 0, fresh = 0, gone = 0;
+    if (r < R) {
+        len = a.lengths[r];
+        fresh = a.fresh[r];
+        gone = a.release ? a.release[r] : 0;
+    }
+    const int n_free = a.n_free[0], prefix = a.prefix_len ? a.prefix_len[0] : 0;
+    len = (int)min((long)max(len, 0), most);
+    fresh = max(fresh, 0);
+    const int old = gone ? 0 : len;
+    int last = 0;                                              // the block an unfilled last one goes on in
+    if (old & (bs - 1)) last = table[old >> a.shift];
+    enum { FLAG_TABLE = STEP_NO_TABLE, FLAG_ROWS = STEP_NO_ROWS, FLAG_MANY = 256 };
+    int flags = 0;
+    if ((long)old + fresh > most) flags |= FLAG_TABLE;
+    else if (fresh > a.rows) flags |= FLAG_ROWS;
+    if (fresh > 1) flags |= FLAG_MANY;
+    if (flags & (FLAG_TABLE | FLAG_ROWS)) fresh = 0;           // (the step is refused)
+    const int have = (old + bs - 1) >> a.shift, need = ((old + fresh + bs - 1) >> a.shift) - have;
+    Sums x = {gone ? (len + bs - 1) >> a.shift : 0, need, fresh};
+    const Sums mine = x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int b = __shfl_up(x.back, o), d = __shfl_up(x.need, o), f = __shfl_up(x.fresh, o);
+        if (lane >= o) {
+            x.back = min(x.back + b, STEP_MOST);
+            x.need = min(x.need + d, STEP_MOST);
+            x.fresh = min(x.fresh + f, STEP_MOST);
+        }
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) flags |= __shfl_xor(flags, o);
+    if (lane == 63) {
+        wave_sum_[w] = x;
+        wave_flags[w] = flags;
+    }
+    __syncthreads();
+    Sums before = {0, 0, 0}, all = {0, 0, 0};
+    for (int i = 0; i < nw; ++i) {
+        const Sums y = wave_sum_[i];
+        if (i == w) before = all;
+        all.back = min(all.back + y.back, STEP_MOST);
+        all.need = min(all.need + y.need, STEP_MOST);
+        all.fresh = min(all.fresh + y.fresh, STEP_MOST);
+        flags |= wave_flags[i];
+    }
+    const int stack = min(max(n_free, 0), a.cap);
+    const long top = (long)stack + all.back;
+    int bad = flags & (FLAG_TABLE | FLAG_ROWS);
+    if (all.fresh > a.rows) bad |= STEP_NO_ROWS;
+    if (all.need > top) bad |= STEP_NO_BLOCKS;
+    if (top > a.cap) bad |= STEP_NO_STACK;
+    if (bad) {
+        if (r == 0) {
+            a.status[0] |= bad;
+            a.n_free_out[0] = n_free;
+        }
+        if (r < R) a.lengths_out[r] = a.lengths[r];
+        for (int i = r; i <= R; i += n) a.row_starts[i] = 0;
+        if (a.rows_here)
+            for (int i = r; i < a.rows; i += n) a.slots[i] = a.positions[i] = -1;
+        return;
+    }
+    // exclusive sums of the sequences before this one
+    const int e_back = before.back + x.back - mine.back, e_need = before.need + x.need - need;
+    const int row = before.fresh + x.fresh - fresh;
+    if (r < R) {
+        a.lengths_out[r] = old + fresh;
+        a.row_starts[r] = row;
+    }
+    if (r == 0) {
+        a.row_starts[R] = all.fresh;
+        a.n_free_out[0] = (int)top - all.need;
+    }
+    const bool many = flags & FLAG_MANY;
+    if (many || all.back) {
+        first_back[r] = e_back;
+        first_need[r] = e_need;
+        first_row[r] = row;
+        held[r] = old;
+        __syncthreads();
+    }
+    // blocks given back
+    if (all.back) {
+        for (int e = r; e < all.back; e += n) {
+            const int i = last_at_most(first_back, R, e);
+            a.free_blocks[stack + e] = a.tables[(long)i * a.width + e - first_back[i]];
+        }
+        __syncthreads();                                       // before blocks are popped and tables written
+    }
+    if (!many) {
+        // decode: at most one new position, and one new block, a sequence
+        if (need) {
+            last = a.free_blocks[top - 1 - e_need];
+            a.tables[(long)r * a.width + have] = last;
+        }
+        if (fresh && a.rows_here) {
+            a.slots[row] = (last << a.shift) + (old & (bs - 1));
+            a.positions[row] = prefix + old;
+        }
+    } else if (a.rows_here) {                                  // (else block_rows_kernel's)
+        for (int e = r; e < all.need; e += n) {
+            const int i = last_at_most(first_need, R, e);
+            a.tables[(long)i * a.width + ((held[i] + bs - 1) >> a.shift) + e - first_need[i]] = a.free_blocks[top - 1 - e];
+        }
+        for (int e = r; e < all.fresh; e += n) {
+            // a position of the blocks held is in the table, of the new ones on the stack
+            const int i = last_at_most(first_row, R, e), p = held[i] + e - first_row[i];
+            const int j = (p >> a.shift) - ((held[i] + bs - 1) >> a.shift);
+            const int block = j < 0 ? a.tables[(long)i * a.width + (p >> a.shift)] : a.free_blocks[top - 1 - first_need[i] - j];
+            a.slots[e] = (block << a.shift) + (p & (bs - 1));
+            a.positions[e] = prefix + p;
+        }
+    }
+    if (a.rows_here)
+        for (int i = all.fresh + r; i < a.rows; i += n) a.slots[i] = a.positions[i] = -1;
+}
+
+// More sequences than threads.
+__global__ void __launch_bounds__(STEP_THREADS) block_step_many_kernel(StepArgs a) {
     __shared__ int wsum[STEP_THREADS / 64];
     __shared__ int start[STEP_THREADS], base[STEP_THREADS];     // of this chunk: exclusive sums, and held blocks
     __shared__ int row0[STEP_THREADS], held[STEP_THREADS];
@@ -124,7 +259,6 @@ __global__ void __launch_bounds__(STEP_THREADS) block_step_kernel(StepArgs a) {
     }
     __syncthreads();
     const bool refused = bad != 0;
-    const bool one = R <= n;                                   // the only chunk's values stay in registers
     if (refused) {
         for (int r = tid; r <= R; r += n) a.row_starts[r] = 0;
         for (int r = tid; r < R; r += n) a.lengths_out[r] = a.lengths[r];
@@ -138,7 +272,7 @@ __global__ void __launch_bounds__(STEP_THREADS) block_step_kernel(StepArgs a) {
     if (sums[2]) {
         int before = 0;
         for (int r0 = 0; r0 < R; r0 += n) {
-            if (!one) load(r0 + tid);
+            load(r0 + tid);
             int all;
             start[tid] = block_scan(back, wsum, all) - back;
             __syncthreads();
@@ -156,7 +290,7 @@ __global__ void __launch_bounds__(STEP_THREADS) block_step_kernel(StepArgs a) {
     int taken = 0, rows = 0;
     for (int r0 = 0; r0 < R; r0 += n) {
         const int r = r0 + tid, chunk = min(n, R - r0);
-        if (!one) load(r);
+        load(r);
         const int nd = need();
         int all, rall;
         start[tid] = block_scan(nd, wsum, all) - nd;
@@ -192,14 +326,42 @@ __global__ void __launch_bounds__(STEP_THREADS) block_step_kernel(StepArgs a) {
         for (int i = rows + tid; i < a.rows; i += n) a.slots[i] = a.positions[i] = -1;
 }
 
-// slots and positions of many rows from the finished tables, four rows a thread (one
-// search, 16-byte stores where the buffers are aligned)
+// Slots and positions of many rows, four rows a thread (one search, 16-byte stores where the
+// buffers are aligned).  FILL (up to STEP_THREADS sequences): block_step_kernel has left the
+// tables to this launch; a new position's block is popped here, by every row of it, and the
+// row that begins it writes the table's entry.  Otherwise the tables are whole.
+template <bool FILL>
 __global__ void __launch_bounds__(256) block_rows_kernel(StepArgs a) {
+    __shared__ int first_need[FILL ? STEP_THREADS + 1 : 1], wsum[4];
+    const int bs = 1 << a.shift;
+    if (FILL) {
+        // the exclusive sums of the blocks the sequences take, four sequences a thread
+        int need[4], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = 4 * (int)threadIdx.x + i;
+            need[i] = 0;
+            if (r < a.R) {
+                const int len = a.lengths_out[r], fresh = a.row_starts[r + 1] - a.row_starts[r];
+                need[i] = ((len + bs - 1) >> a.shift) - ((len - fresh + bs - 1) >> a.shift);
+            }
+            sum += need[i];
+        }
+        int all, at = block_scan(sum, wsum, all) - sum;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            first_need[4 * threadIdx.x + i] = at;
+            at += need[i];
+        }
+        if (threadIdx.x == 0) first_need[STEP_THREADS] = all;
+        __syncthreads();
+    }
     const int row = ((int)blockIdx.x * 256 + (int)threadIdx.x) * 4;
     if (row >= a.rows) return;
     const int total = a.row_starts[a.R], prefix = a.prefix_len ? a.prefix_len[0] : 0;
+    const int top = FILL ? a.n_free_out[0] + first_need[STEP_THREADS] : 0;
     int r = row < total ? last_at_most(a.row_starts, a.R, row) : 0;
-    int end = a.row_starts[r + 1], first = a.lengths_out[r] - end;      // position of row j: first + j
+    int begin = a.row_starts[r], end = a.row_starts[r + 1], first = a.lengths_out[r] - end;   // position of row j: first + j
     int sl[4], po[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -208,11 +370,21 @@ __global__ void __launch_bounds__(256) block_rows_kernel(StepArgs a) {
         if (j >= total) continue;
         while (j >= end) {
             ++r;
+            begin = end;
             end = a.row_starts[r + 1];
             first = a.lengths_out[r] - end;
         }
-        const int p = first + j;
-        sl[i] = (a.tables[(long)r * a.width + (p >> a.shift)] << a.shift) + (p & ((1 << a.shift) - 1));
+        const int p = first + j, b = p >> a.shift;
+        int32_t *entry = a.tables + (long)r * a.width + b;
+        int block;
+        const int have = (first + begin + bs - 1) >> a.shift;          // blocks held before the step
+        if (FILL && b >= have) {
+            block = a.free_blocks[top - 1 - first_need[r] - (b - have)];
+            if ((p & (bs - 1)) == 0) *entry = block;
+        } else {
+            block = *entry;
+        }
+        sl[i] = (block << a.shift) + (p & (bs - 1));
         po[i] = prefix + p;
     }
     if (row + 4 <= a.rows && (((uintptr_t)a.slots | (uintptr_t)a.positions) & 15) == 0) {
@@ -249,9 +421,11 @@ struct RopeBlocksArgs {
     int N, H, Hkv, shift, table_len;
     long n_slots;
     int v_blocks, heads_per_wave;
+    int v_heads;             // Hkv: the waves write v too (no v blocks)
 };
 
 constexpr int RB_ROWS = 64, RB_HALO = 8;
+constexpr long RB_FEW = 512;
 
 template <int D>
 __global__ void __launch_bounds__(256) rope_append_blocks_kernel(RopeBlocksArgs a) {
@@ -339,13 +513,21 @@ __global__ void __launch_bounds__(256) rope_append_blocks_kernel(RopeBlocksArgs 
         return;
     }
     constexpr int LPH = D / 16, HPW = 64 / LPH, HALF = D / 2;   // lanes a head, heads a wave at a time
-    const int heads = a.H + a.Hkv, parts = (heads + a.heads_per_wave - 1) / a.heads_per_wave;
+    const int heads = a.H + a.Hkv + a.v_heads, parts = (heads + a.heads_per_wave - 1) / a.heads_per_wave;
     const int wid = ((int)blockIdx.x - a.v_blocks) * 4 + ((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int tok = wid / parts, part = wid - tok * parts;
     if (tok >= a.N) return;
     const int slot = a.slots[tok], pos = a.positions[tok];
+    const int i0 = 8 * (lane % LPH), h0 = part * a.heads_per_wave + lane / LPH;
+    const uint16_t *row = a.qkv + (size_t)tok * a.qkv_stride + i0;
+    // the first head's values are on their way while the slot and the angles are read
+    uint4 a1, a2;
+    {
+        const uint16_t *hp = row + (size_t)min(h0, heads - 1) * D;
+        a1 = *reinterpret_cast<const uint4 *>(hp);
+        a2 = *reinterpret_cast<const uint4 *>(hp + HALF);
+    }
     if (slot < 0 || slot >= a.n_slots || pos < 0 || pos >= a.table_len) return;
-    const int i0 = 8 * (lane % LPH);
     float c[8], sn[8];
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
@@ -354,12 +536,25 @@ __global__ void __launch_bounds__(256) rope_append_blocks_kernel(RopeBlocksArgs 
         c[4 * q] = cv.x; c[4 * q + 1] = cv.y; c[4 * q + 2] = cv.z; c[4 * q + 3] = cv.w;
         sn[4 * q] = sv.x; sn[4 * q + 1] = sv.y; sn[4 * q + 2] = sv.z; sn[4 * q + 3] = sv.w;
     }
-    const uint16_t *row = a.qkv + (size_t)tok * a.qkv_stride + i0;
     const int h1 = min(heads, (part + 1) * a.heads_per_wave);
 #pragma unroll 4
-    for (int h = part * a.heads_per_wave + lane / LPH; h < h1; h += HPW) {
-        const uint16_t *hp = row + (size_t)h * D;
-        const uint4 a1 = *reinterpret_cast<const uint4 *>(hp), a2 = *reinterpret_cast<const uint4 *>(hp + HALF);
+    for (int h = h0; h < h1; h += HPW) {
+        if (h != h0) {
+            const uint16_t *hp = row + (size_t)h * D;
+            a1 = *reinterpret_cast<const uint4 *>(hp);
+            a2 = *reinterpret_cast<const uint4 *>(hp + HALF);
+        }
+        if (h >= a.H + a.Hkv) {                              // a v head: a slot's values lie bs apart
+            uint16_t *dst = a.vt + ((((size_t)(slot >> a.shift) * a.Hkv + (h - a.H - a.Hkv)) * D + i0) << a.shift) + (slot & (bs - 1));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t w1 = e < 2 ? a1.x : e < 4 ? a1.y : e < 6 ? a1.z : a1.w;
+                const uint32_t w2 = e < 2 ? a2.x : e < 4 ? a2.y : e < 6 ? a2.z : a2.w;
+                dst[(size_t)e << a.shift] = (uint16_t)((e & 1) ? w1 >> 16 : w1);
+                dst[(size_t)(e + HALF) << a.shift] = (uint16_t)((e & 1) ? w2 >> 16 : w2);
+            }
+            continue;
+        }
         uint32_t o1[4], o2[4];
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
@@ -410,10 +605,12 @@ int launch_block_tables(const int32_t *lengths, const int32_t *fresh, const uint
     a.rows_here = rows <= STEP_ROWS;
     const long want = R > rows / 4 ? R : rows / 4;
     const int threads = (int)(want >= STEP_THREADS || !a.rows_here ? STEP_THREADS : (want + 63) / 64 * 64);
-    hipLaunchKernelGGL(block_step_kernel, dim3(1), dim3(threads), 0, stream, a);
+    if (R <= threads) hipLaunchKernelGGL(block_step_kernel, dim3(1), dim3(threads), 0, stream, a);
+    else hipLaunchKernelGGL(block_step_many_kernel, dim3(1), dim3(threads), 0, stream, a);
     SC_HIP_CHECK(hipGetLastError());
     if (!a.rows_here) {
-        hipLaunchKernelGGL(block_rows_kernel, dim3((unsigned)((rows + 1023) / 1024)), dim3(256), 0, stream, a);
+        auto kern = R <= threads ? block_rows_kernel<true> : block_rows_kernel<false>;
+        hipLaunchKernelGGL(kern, dim3((unsigned)((rows + 1023) / 1024)), dim3(256), 0, stream, a);
         SC_HIP_CHECK(hipGetLastError());
     }
     return SC_OK;
@@ -442,13 +639,18 @@ int launch_rope_append_blocks(const uint16_t *qkv, long qkv_stride, uint16_t *q,
     a.cos_t = cos_t; a.sin_t = sin_t; a.slots = slots; a.positions = positions;
     a.N = (int)N; a.H = (int)H; a.Hkv = (int)Hkv; a.shift = shift; a.table_len = (int)table_len;
     a.n_slots = n_blocks * bs;
-    const long v_blocks = (N + RB_ROWS - 1) / RB_ROWS * Hkv;
+    // few rows: v in 2-byte stores by the rotation's waves, which spares the way through LDS
+    // (64 single rows of 32 + 8 heads of 128: 8.1 -> 4.0 us; at 1024 rows of a
+    // prompt 10.0 -> 15.5)
+    const bool few = N <= RB_FEW;
+    a.v_heads = few ? (int)Hkv : 0;
+    const long v_blocks = few ? 0 : (N + RB_ROWS - 1) / RB_ROWS * Hkv, heads = H + Hkv + a.v_heads;
     // a token's heads over several waves while tokens alone leave CUs idle
     const int hpw = (int)(64 / (D / 16));
-    long per = N >= 4L * device_info().num_cus ? H + Hkv : 2 * hpw;
-    if (per > H + Hkv) per = H + Hkv;
+    long per = N >= 4L * device_info().num_cus ? heads : N >= device_info().num_cus ? 2 * hpw : hpw;
+    if (per > heads) per = heads;
     a.heads_per_wave = (int)per;
-    const long waves = N * ((H + Hkv + per - 1) / per);
+    const long waves = N * ((heads + per - 1) / per);
     const long blocks = v_blocks + (waves + 3) / 4;
     if (blocks >= (1L << 31)) return set_error(SC_EINVAL, "rope_append_blocks: too many rows");
     a.v_blocks = (int)v_blocks;
