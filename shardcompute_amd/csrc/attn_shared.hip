@@ -791,7 +791,7 @@ __global__ void __launch_bounds__(SA_THREADS) __attribute__((amdgpu_waves_per_eu
 template <int D, int WPR>
 __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_parts, int per_seq) {
     constexpr int PER = D / 64;
-    constexpr int AHEAD = 16;
+    constexpr int AHEAD = WPR == 4 ? 16 : 8;
     __shared__ float2 sm_ml[WPR];
     __shared__ float sm_o[WPR][D];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -907,6 +907,27 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
 
 // ---------------------------------------------------------------- host side
 
+// Into how many workgroups a column tile's key blocks are cut (wgs: workgroups without a cut).
+// A key block takes a workgroup alone on its CU 1.5 us, 2.1 us where two share it, further
+// ones wait (head_dim 128, measured: 300 rows behind 30000 positions 222 us in 3 pieces of 80
+// workgroups, 16 prompts 633 us in 2117 workgroups of 72 blocks; head_dim 64 ~0.8 of it, the
+// softmax is the same), and the keys come at 5.3 TB/s at most; a row's part is written and read
+// at about 2.5 TB/s and lengthens the merge by 0.06 us.  The sum is least at the count returned: 16 rows behind 65536 positions 66 us
+// (in 32), 86 at 24; 768 rows behind 2048 71 us (whole), 86 in 2.
+int tile_splits(long wgs, long blocks, long Hkv, long D, double part_bytes, bool last_is_whole, long cus) {
+    const double stream = (double)Hkv * blocks * SA_KB * D * 4 / 5.3e6;
+    int best = 1;
+    double least = 1e30;
+    for (int n = 1; n <= 64 && (n == 1 || n <= blocks); ++n) {
+        const long w = wgs * n;
+        const double block = (D == 64 ? 0.8 : 1.0) * (w <= cus ? 1.5 : 2.1 * ((w + 2 * cus - 1) / (2 * cus)));
+        const double walk = (double)((blocks + n - 1) / n) * block;
+        const double us = (walk > stream ? walk : stream) + (n == 1 && last_is_whole ? 0 : n * (part_bytes / 2.5e6 + 0.06));
+        if (us < least) { least = us; best = n; }
+    }
+    return best;
+}
+
 struct SaPlan {
     int small_rows, rows_max, any_big, nsplit, own_wgs, use_tile;
     long tiles, own_parts;
@@ -923,12 +944,9 @@ SaPlan plan_shared(long N, long R, long H, long Hkv, long D, long own_cap, long 
     p.any_big = max_new > p.small_rows;
     p.use_tile = p.any_big || prefix_cap > 0;
     p.tiles = (cols + SA_COLS - 1) / SA_COLS;
-    // attn_tile: a workgroup a CU, and four key blocks at least
     const long wgs = p.tiles * Hkv;
     const long blocks = (prefix_cap + (p.any_big ? own_cap : 0) + SA_KB - 1) / SA_KB;
-    long ns = wgs ? cus / wgs : 1;
-    if (ns > blocks / 4) ns = blocks / 4;
-    p.nsplit = (int)(ns < 1 ? 1 : ns > 64 ? 64 : ns);
+    p.nsplit = p.use_tile ? tile_splits(wgs, blocks, Hkv, D, (double)N * H * (8 * D + 16), p.any_big, cus) : 1;
     // attn_own: at most R coltiles of the most rows a sequence has here, and no more
     // than the rows make
     const long rows_max = max_new < p.small_rows ? max_new : p.small_rows;
