@@ -830,6 +830,7 @@ def add_i32(counters, delta, n=None):
 # ---------------------------------------------------------------- key/value cache in blocks
 
 BLOCK_SIZES = (16, 32, 64, 128, 256)
+SHARED_MAX_SEQUENCES = 2048         # of one attention_shared call
 # bits of the status word of block_tables
 BLOCKS_NO_BLOCKS, BLOCKS_NO_TABLE, BLOCKS_NO_ROWS, BLOCKS_NO_STACK = 1, 2, 4, 8
 

@@ -74,6 +74,8 @@ class BlockKVCache:
             raise ValueError(f"block_size must be one of {_lib.BLOCK_SIZES}, got {block_size}")
         if min(num_layers, num_kv_heads, head_dim, num_blocks, max_sequences, max_length) < 1 or max_prefix < 0:
             raise ValueError("a block cache needs at least one layer, head, block, sequence and position")
+        if max_sequences > _lib.SHARED_MAX_SEQUENCES:
+            raise ValueError(f"at most {_lib.SHARED_MAX_SEQUENCES} sequences, got {max_sequences}")
         if device is None:
             device = torch.device("cuda", torch.cuda.current_device())
         self.num_layers, self.num_kv_heads, self.head_dim = num_layers, num_kv_heads, head_dim

@@ -49,9 +49,10 @@ struct SaArgs {
     int any_big;             // some sequence may have more
     int nsplit;              // workgroups a column tile's keys are cut into
     int tile_wgs, own_wgs;   // their workgroups
+    int part_rows, per_seq;  // attn_tile's parts: by row, or (per_seq > 0) by sequence, per_seq rows each
     int tiles, pair_half;    // attn_tile's column tiles; > 0: workgroups of a round, paired with the next round's
     float scale_log2;
-    // parts: of attn_tile [nsplit][N * H] rows, of attn_own [own_parts][16] columns
+    // parts: of attn_tile [nsplit][part_rows * H], of attn_own [own_parts][16] columns
     float *tile_o;
     float2 *tile_ml;
     float *own_o;
@@ -242,11 +243,15 @@ __device__ __forceinline__ void attn_tile(const SaArgs &a, int id, uint8_t *smem
     const int r0 = a.any_big ? find_seq(a, row0) : 0;
     int total = (P + SA_KB - 1) / SA_KB;
     bool big = false;                                   // this column's own keys are taken here
+    int part_row = row;                                 // where its part goes, if it has one
     if (a.any_big)
         for (int r = r0; r < a.R; ++r) {
             const Seq s = seq_of(a, r, rows);
             if (s.first > row1) break;
-            if (s.n > a.small_rows && row >= s.first && row < s.first + s.n) big = true;
+            if (row >= s.first && row < s.first + s.n) {
+                big = s.n > a.small_rows;
+                if (a.per_seq) part_row = r * a.per_seq + row - s.first;
+            }
             total += own_blocks(s);
         }
     const int t0 = (int)((long)total * split / a.nsplit), t1 = (int)((long)total * (split + 1) / a.nsplit);
@@ -473,7 +478,8 @@ __device__ __forceinline__ void attn_tile(const SaArgs &a, int id, uint8_t *smem
                                cvt_pk_bf16(o[db][4 * r4 + 2] * inv, o[db][4 * r4 + 3] * inv));
         return;
     }
-    const size_t part = (size_t)split * a.N * a.H + (size_t)row * a.H + h;
+    if (part_row >= a.part_rows) return;                // (a sequence of more rows than max_new)
+    const size_t part = ((size_t)split * a.part_rows + part_row) * a.H + h;
     float *po = a.tile_o + part * D;
 #pragma unroll
     for (int db = 0; db < Gm::DB; ++db)
@@ -481,7 +487,8 @@ __device__ __forceinline__ void attn_tile(const SaArgs &a, int id, uint8_t *smem
         for (int r4 = 0; r4 < 4; ++r4)
             *reinterpret_cast<float4 *>(po + 32 * db + 8 * r4 + 4 * lh) =
                 make_float4(o[db][4 * r4], o[db][4 * r4 + 1], o[db][4 * r4 + 2], o[db][4 * r4 + 3]);
-    if (lh == 0) a.tile_ml[part] = make_float2(m * sc, ltot);
+    if (lh == 0)     // (a sum that is no number: nor is the row)
+        a.tile_ml[part] = make_float2(ltot == ltot ? m * sc : INFINITY, ltot);
 }
 
 // ---------------------------------------------------------------- few columns
@@ -723,7 +730,7 @@ __device__ __forceinline__ void attn_own(const SaArgs &a, int wg, uint8_t *smem)
         float *po = a.own_o + at * D + 4 * g;
 #pragma unroll
         for (int y = 0; y < DT; ++y) *reinterpret_cast<f4 *>(po + 16 * y) = o[y];
-        if (g == 0) a.own_ml[at] = make_float2(m, ltot);
+        if (g == 0) a.own_ml[at] = make_float2(ltot == ltot ? m : INFINITY, ltot);
     };
 
     Run f, n;                    // the block staged last, and the one after it
@@ -782,14 +789,14 @@ __global__ void __launch_bounds__(SA_THREADS) __attribute__((amdgpu_waves_per_eu
 // One wave a row and q head: the parts of attn_tile (nsplit), then those of attn_own.  out = sum_i 2^(m_i - M) O_i /
 // sum_i 2^(m_i - M) l_i; parts of no key have m = -inf and weight 0, a row of no key at
 // all is 0.  The waves go over every row, or, where only sequences of few rows have parts,
-// over per_seq rows of every sequence, if that is less (prompts are then passed over).
+// over by_seq rows of every sequence, if that is less (prompts are then passed over).
 //
 // Bound by the latency of dependent loads, so there are two rounds of them: what says where
 // the parts are, then the parts, lane i holding part i's place and (m, l), the values of
 // AHEAD parts on their way together.
 // Few rows: WPR = 4, a workgroup a row and q head, its waves taking the parts in turn.
 template <int D, int WPR>
-__global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_parts, int per_seq) {
+__global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_parts, int by_seq) {
     constexpr int PER = D / 64;
     constexpr int AHEAD = WPR == 4 ? 16 : 8;
     __shared__ float2 sm_ml[WPR];
@@ -801,13 +808,15 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
     int row = (int)(wid / a.H), r;
     const int h = (int)(wid - (long)row * a.H);
     Seq s;
-    if (per_seq) {
-        r = row / per_seq;
+    int part_row = row;
+    if (by_seq) {
+        r = row / by_seq;
         if (r >= a.R) return;
         s = seq_of(a, r, rows);
-        const int i = row - r * per_seq;
+        const int i = row - r * by_seq;
         if (i >= s.n || s.n > a.small_rows) return;
         row = s.first + i;
+        if (!a.per_seq) part_row = row;
     } else {
         if (row >= rows) return;
         r = find_seq(a, row);
@@ -836,7 +845,7 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
         const int k = min(64, (parts - turn + WPR - 1) / WPR - i0);
         const int i = (i0 + min(lane, k - 1)) * WPR + turn;
         const bool t = i < tile_parts;
-        long at = ((long)i * a.N + row) * a.H + h;
+        long at = ((long)i * a.part_rows + part_row) * a.H + h;
         if (!t) at = (own_part + own_step * (i - tile_parts)) * 16L + own_c;
         float2 x = (t ? a.tile_ml : a.own_ml)[at];
         if (lane >= k) x = make_float2(-INFINITY, 0.f);
@@ -912,8 +921,9 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
 // ones wait (head_dim 128, measured: 300 rows behind 30000 positions 222 us in 3 pieces of 80
 // workgroups, 16 prompts 633 us in 2117 workgroups of 72 blocks; head_dim 64 ~0.8 of it, the
 // softmax is the same), and the keys come at 5.3 TB/s at most; a row's part is written and read
-// at about 2.5 TB/s and lengthens the merge by 0.06 us.  The sum is least at the count returned: 16 rows behind 65536 positions 66 us
-// (in 32), 86 at 24; 768 rows behind 2048 71 us (whole), 86 in 2.
+// at about 2.5 TB/s and lengthens the merge by 0.06 us.  The sum is least at the count
+// returned: 16 rows behind 65536 positions 66 us (in 32), 86 at 24; 768 rows behind 2048
+// 71 us (whole), 86 in 2.
 int tile_splits(long wgs, long blocks, long Hkv, long D, double part_bytes, bool last_is_whole, long cus) {
     const double stream = (double)Hkv * blocks * SA_KB * D * 4 / 5.3e6;
     int best = 1;
@@ -922,7 +932,8 @@ int tile_splits(long wgs, long blocks, long Hkv, long D, double part_bytes, bool
         const long w = wgs * n;
         const double block = (D == 64 ? 0.8 : 1.0) * (w <= cus ? 1.5 : 2.1 * ((w + 2 * cus - 1) / (2 * cus)));
         const double walk = (double)((blocks + n - 1) / n) * block;
-        const double us = (walk > stream ? walk : stream) + (n == 1 && last_is_whole ? 0 : n * (part_bytes / 2.5e6 + 0.06));
+        const double parts = n == 1 && last_is_whole ? 0 : n * (part_bytes / 2.5e6 + 0.06);
+        const double us = (walk > stream ? walk : stream) + parts;
         if (us < least) { least = us; best = n; }
     }
     return best;
@@ -930,7 +941,8 @@ int tile_splits(long wgs, long blocks, long Hkv, long D, double part_bytes, bool
 
 struct SaPlan {
     int small_rows, rows_max, any_big, nsplit, own_wgs, use_tile;
-    long tiles, own_parts;
+    long tiles, own_parts, part_rows;
+    int by_seq, per_seq;     // the merge, and attn_tile's parts, by sequence: rows of each
     long tile_o, tile_ml, own_o, own_ml, own_idx, bytes;       // workspace offsets
 };
 
@@ -954,13 +966,22 @@ SaPlan plan_shared(long N, long R, long H, long Hkv, long D, long own_cap, long 
     long coltiles = R * ((rows_max * G + 63) / 64);
     if (coltiles > R + cols / 64) coltiles = R + cols / 64;
     const long keyblocks = coltiles * ((own_cap + SA_KB - 1) / SA_KB);
-    long ow = 2 * cus;
+    // Equal runs of key blocks, two workgroups a CU; one where the other is attn_tile's (128
+    // sequences of up to 600 behind 8192 positions 73 us, 78 at two) and no tile takes own
+    // keys as well (the mixed batch 75 us at one, 72 at two)
+    long ow = p.use_tile && !p.any_big ? cus : 2 * cus;
     if (ow > Hkv * keyblocks) ow = Hkv * keyblocks;
     p.own_wgs = (int)(ow < 1 ? 1 : ow);
     p.own_parts = 4 * (Hkv * coltiles + p.own_wgs);
     auto up = [](long v) { return (v + 255) / 256 * 256; };
     long at = 0;
-    const long tparts = p.use_tile ? p.nsplit * N * H : 0;
+    // With whole tiles only sequences of few rows have parts.  Where they can be few of the
+    // batch's rows the parts are kept, and merged, by sequence
+    const bool few = R * rows_max < N && p.any_big && p.nsplit == 1;
+    p.by_seq = few || (!p.any_big && R * rows_max <= N) ? (int)rows_max : 0;
+    p.per_seq = few ? (int)rows_max : 0;
+    p.part_rows = few ? R * rows_max : N;
+    const long tparts = p.use_tile ? p.nsplit * p.part_rows * H : 0;
     p.tile_o = at; at += up(tparts * D * 4);
     p.tile_ml = at; at += up(tparts * 8);
     p.own_o = at; at += up(p.own_parts * 16 * D * 4);
@@ -986,13 +1007,12 @@ int run_shared(const SaArgs &a, const SaPlan &p, hipStream_t stream) {
     }
     hipLaunchKernelGGL(kern, dim3((unsigned)(a.own_wgs + a.tile_wgs)), dim3(SA_THREADS), lds, stream, a);
     SC_HIP_CHECK(hipGetLastError());
-    const bool by_seq = (p.nsplit == 1 || !p.any_big) && (long)a.R * p.rows_max <= a.N;
-    const long merge_rows = by_seq ? (long)a.R * p.rows_max : a.N;
+    const long merge_rows = p.by_seq ? (long)a.R * p.by_seq : a.N;
     const long heads = merge_rows * a.H;
     const bool wide = heads <= 4L * device_info().num_cus;
     auto merge = wide ? attn_merge_kernel<D, 4> : attn_merge_kernel<D, 1>;
     hipLaunchKernelGGL(merge, dim3((unsigned)(wide ? heads : (heads + 3) / 4)), dim3(256), 0, stream, a,
-                       p.use_tile ? p.nsplit : 0, by_seq ? p.rows_max : 0);
+                       p.use_tile ? p.nsplit : 0, p.by_seq);
     SC_HIP_CHECK(hipGetLastError());
     return SC_OK;
 }
@@ -1048,6 +1068,7 @@ int launch_attention_shared(const uint16_t *q, long q_stride, const uint16_t *kc
     a.own_wgs = p.own_wgs;
     a.tile_wgs = p.use_tile ? (int)(p.tiles * p.nsplit * Hkv) : 0;
     a.tiles = (int)p.tiles;
+    a.part_rows = (int)p.part_rows; a.per_seq = p.per_seq;
     a.pair_half = p.any_big && a.tile_wgs >= 2 * device_info().num_cus ? device_info().num_cus : 0;
     a.scale_log2 = scale * 1.4426950408889634f;
     char *ws = static_cast<char *>(workspace);

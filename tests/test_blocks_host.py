@@ -108,3 +108,5 @@ def test_cache_bookkeeping_on_the_host():
         BlockKVCache(1, 1, 64, 4, 1, 64, block_size=48, device=torch.device("cpu"))
     with pytest.raises(ValueError, match="at least one"):
         BlockKVCache(1, 1, 64, 0, 1, 64, device=torch.device("cpu"))
+    with pytest.raises(ValueError, match="at most 2048 sequences, got 2049"):
+        BlockKVCache(1, 1, 64, 4, 2049, 64, device=torch.device("cpu"))

@@ -233,6 +233,17 @@ def test_attention(device, held, new, prefix, bs, H, Hkv, D, pad):
         assert torch.equal(got, c.attend(max_new=max_new, out=torch.full_like(out, 5.0)))       # same bits again
 
 
+@pytest.mark.parametrize("new", [[1, 3, 0, 1700, 2, 16, 17, 1], [2000] + [1] * 20, [1] * 5 + [900, 1, 900]])
+def test_attention_of_few_decoded_rows_beside_prompts(device, new):
+    """Sequences of few rows among long prompts, behind a prefix."""
+    held = [(37 * i) % 200 for i in range(len(new))]
+    c = Cache(held, new, 300, 64, 32, 8, 64, pad=3)
+    exact, mag = c.exact()
+    got = c.attend(max_new=c.max_new, out=torch.full_like(c.q, 5.0))
+    assert_attention(got, exact, mag, c.starts[-1])
+    assert (got[c.starts[-1]:] == 5).all()
+
+
 def test_attention_strides_scale_and_wide_tables(device):
     c = Cache([30, 2, 200], [1, 1, 40], 150, 32, 8, 2, 128, pad=2, width=50)
     wide = torch.zeros((c.N, 2 * 1024 + 8), dtype=torch.bfloat16, device="cuda")
@@ -268,6 +279,21 @@ def test_attention_keeps_values_that_are_not_attended_out(device, new, bs, D, va
     got = got.clone()
     got[sees], exact[sees], mag[sees] = 0, 0, 0
     assert_attention(got, exact, mag, c.N)
+
+
+@pytest.mark.parametrize("new,prefix,bs", [([1, 1, 1], 0, 64), ([1, 1, 1], 2000, 16), ([3, 9, 3], 100, 64),
+                                           ([1, 200, 2], 100, 32), ([90, 80, 2], 3000, 64)])
+def test_attention_of_a_query_that_is_no_number(device, new, prefix, bs):
+    """A query with a NaN makes its own row's head NaN and nothing else."""
+    H, D = 8, 64
+    c = Cache([40, 70, 9], new, prefix, bs, H, 2, D)
+    exact, mag = c.exact()
+    row, h = c.starts[2] - 1, 5
+    c.q[row, h * D + 3] = float("nan")
+    got = c.attend(max_new=c.max_new).clone().view(c.N, H, D)
+    assert torch.isnan(got[row, h]).all()
+    got[row, h], exact[row, h], mag[row, h] = 0, 0, 0
+    assert_attention(got.view(c.N, H * D), exact, mag, c.N)
 
 
 def test_attention_row_without_a_key_is_zero(device):
