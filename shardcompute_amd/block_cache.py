@@ -49,11 +49,17 @@ class BlockBatch:
         self.tables = tables
         self.rows = rows
         self.max_new = max_new
+        self.number = cache.steps
         self.prefix_table = cache.prefix_table if prefix else None
         self.prefix_len = cache.prefix_len if prefix else None
 
     def __getitem__(self, layer: int) -> BlockLayerKV:
         return BlockLayerKV(self, layer)
+
+    def check_current(self):
+        """Raise if the cache has begun another step since (its lengths are that step's)."""
+        if self.number != self.cache.steps:
+            raise RuntimeError("the block cache has begun another step since this one")
 
     @property
     def last_rows(self) -> torch.Tensor:
@@ -98,6 +104,7 @@ class BlockKVCache:
         self.host_lengths: List[int] = [0] * max_sequences
         self.host_prefix = 0
         self.host_free = num_blocks
+        self.steps = 0              # begun
 
     @property
     def max_positions(self) -> int:
@@ -148,6 +155,7 @@ class BlockKVCache:
                           self.free_blocks, self.n_free, self.block_size, rows, prefix_len=self.prefix_len,
                           release=rel, out=step)
         self.host_lengths, self.host_free = lengths, free
+        self.steps += 1
         return BlockBatch(self, step, self.tables, rows, max(new), self.host_prefix > 0)
 
     def begin_prefix(self, positions: int) -> BlockBatch:
@@ -167,6 +175,7 @@ class BlockKVCache:
                           self.free_blocks, self.n_free, self.block_size, positions, out=step)
         self.host_prefix += positions
         self.host_free -= need
+        self.steps += 1
         return BlockBatch(self, step, tables, positions, positions, False)
 
     def check_status(self):

@@ -1020,7 +1020,9 @@ int run_shared(const SaArgs &a, const SaPlan &p, hipStream_t stream) {
 bool bad_shape(long N, long R, long H, long Hkv, long D, long own_cap, long prefix_cap, long max_new) {
     return N < 0 || N >= (1L << 24) || R <= 0 || R > SA_MAX_SEQ || H <= 0 || Hkv <= 0 || H % Hkv || H > 4096 ||
            (D != 64 && D != 128) || own_cap <= 0 || own_cap >= (1L << 30) || prefix_cap < 0 || prefix_cap >= (1L << 30) ||
-           max_new < 0;
+           max_new < 0 ||
+           // attn_own numbers its key blocks in 32 bits
+           R * Hkv * ((H / Hkv + 63) / 64) * ((own_cap + SA_KB - 1) / SA_KB) >= (1L << 31);
 }
 
 }  // namespace

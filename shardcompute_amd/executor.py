@@ -154,7 +154,7 @@ class BlockDecodeGraph:
         self.bufs = StepBuffers(model, B, 1, 0)
         self.new = torch.ones(B, dtype=torch.int32, device=cache.device)
         self.step = torch.zeros(1, dtype=torch.int32, device=cache.device)
-        self.batch = BlockBatch(cache, cache._buffers(B, B, cache.lengths), cache.tables, B, 1, cache.host_prefix > 0)
+        self.batch = BlockBatch(cache, cache._buffers(B, B, cache.lengths), cache.tables, B, 1, cache.max_prefix > 0)
         att = model.layers[0].attention
         need = self.batch.workspace_bytes(att.local_num_heads, att.local_num_kv_heads, att.head_dim)
         self.bufs.workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=cache.device)
@@ -181,6 +181,7 @@ class BlockDecodeGraph:
                         logits = self._step()
                     self.graph = (g, logits)
             self.cache.host_lengths, self.cache.host_free = lengths, free
+            self.cache.steps += 1
 
 
 class ParallelExecutor:
@@ -383,7 +384,7 @@ class ParallelExecutor:
         if max_new_tokens <= 0:
             return [[] for _ in prompts]
         t0 = time.perf_counter()
-        m, R, prefix = self.model, len(prompts), list(prefix or [])
+        m, R, prefix = self.model, len(prompts), [int(t) for t in prefix] if prefix is not None else []
         own = [-(-(len(p) + max_new_tokens) // block_size) for p in prompts]
         cache = m.new_block_cache(R, max(own) * block_size, sum(own) + -(-len(prefix) // block_size), block_size,
                                   len(prefix))

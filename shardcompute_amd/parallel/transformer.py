@@ -435,6 +435,9 @@ class ParallelTransformer:
         ids = ids.to(self.device)
         if ids.dim() != 1 or ids.shape[0] != batch.rows:
             raise ValueError(f"input_ids must be [{batch.rows}], the step's rows")
+        if batch.rows == 0:
+            raise ValueError("the step has no rows")
+        batch.check_current()
         N = batch.rows
         h = (await self._embed(ids.view(1, N))).reshape(N, self.hidden_size).contiguous()
         h, pending = await self._trunk(h, batch, 1, N)

@@ -110,3 +110,10 @@ def test_cache_bookkeeping_on_the_host():
         BlockKVCache(1, 1, 64, 0, 1, 64, device=torch.device("cpu"))
     with pytest.raises(ValueError, match="at most 2048 sequences, got 2049"):
         BlockKVCache(1, 1, 64, 4, 2049, 64, device=torch.device("cpu"))
+
+
+def test_more_key_blocks_than_32_bits_count_are_refused():
+    """A workspace of 0 bytes is a refusal: 2048 sequences of 8 kv heads of 2^25 positions each."""
+    from shardcompute_amd import _lib
+    assert _lib.attention_shared_workspace_bytes(64, 2048, 32, 8, 128, 1 << 25, 0, 1) == 0
+    assert _lib.attention_shared_workspace_bytes(64, 2048, 2048, 1, 128, 1 << 25, 0, 1) == 0       # 32 columns' 64s

@@ -8,7 +8,7 @@ import torch
 
 from oracle.bf16 import bf16_to_f32
 from oracle.decoder import random_decoder_weights
-from shardcompute_amd.executor import ParallelExecutor
+from shardcompute_amd.executor import BlockDecodeGraph, ParallelExecutor
 from tests.gpu_util import host_u16
 from tests.test_gpu_model import LOGIT_TOL, SHAPE, build_model
 
@@ -145,3 +145,36 @@ def test_refusals(model):
         layer.attend_qkv(qkv, 1, 3, step[0], mask=torch.zeros((1, 3), device="cuda"))
     with pytest.raises(ValueError, match="3 rows"):
         layer.attend_qkv(qkv[:2], 1, 2, step[0])
+
+
+def test_a_step_that_only_gives_back_and_one_that_is_over(model):
+    cache = model.new_block_cache(3, 64, block_size=16)
+    free = cache.host_free
+    first = cache.begin([17, 1, 0])
+    run(model.forward_blocks([3] * 18, first))
+    second = cache.begin([1, 1, 1])
+    with pytest.raises(RuntimeError, match="another step"):
+        run(model.forward_blocks([3] * 18, first))
+    run(model.forward_blocks([3] * 3, second))
+    none = cache.begin([0, 0, 0], release=[True, False, True])
+    with pytest.raises(ValueError, match="no rows"):
+        run(model.forward_blocks([], none))
+    assert cache.lengths.tolist() == cache.host_lengths == [0, 2, 0]
+    assert cache.n_free.item() == cache.host_free == free - 1
+    cache.check_status()
+
+
+def test_decode_graph_made_before_its_prefix(model):
+    rng = np.random.default_rng(11)
+    pre, prompts, n = tokens(rng, 45), [tokens(rng, 5), tokens(rng, 2)], 12
+    want = run(ParallelExecutor(0, 1, None, model).generate_batch(prompts, prefix=pre, max_new_tokens=n))
+    cache = model.new_block_cache(2, 128, block_size=64, max_prefix=64)
+    out = torch.zeros((2, n), dtype=torch.int32, device="cuda")
+    dec = BlockDecodeGraph(model, cache, out)
+    run(model.forward_blocks(pre, cache.begin_prefix(len(pre))))
+    logits = run(model.forward_blocks(prompts[0] + prompts[1], cache.begin([5, 2])))
+    out[:, 0] = dec.bufs.ids[:, 0] = logits.float().argmax(-1).to(torch.int32)
+    dec.step.fill_(1)
+    dec.run(n - 1)
+    cache.check_status()
+    assert out.tolist() == want
