@@ -974,10 +974,13 @@ SaPlan plan_shared(long N, long R, long H, long Hkv, long D, long own_cap, long 
     long coltiles = R * ((rows_max * G + 63) / 64);
     if (coltiles > R + cols / 64) coltiles = R + cols / 64;
     const long keyblocks = coltiles * ((own_cap + SA_KB - 1) / SA_KB);
-    // Equal runs of key blocks, two workgroups a CU; one where the other is attn_tile's (128
-    // sequences of up to 600 behind 8192 positions 73 us, 78 at two) and no tile takes own
-    // keys as well (the mixed batch 75 us at one, 72 at two)
-    long ow = p.use_tile && !p.any_big ? cus : 2 * cus;
+    // Equal runs of key blocks over what the column tiles leave of two workgroups a CU, so that
+    // one round holds all (64 rows behind 2048 positions, 128 tile workgroups: 119 us with 384
+    // here, 123 with 256 or 512), but at least one a CU (128 rows behind 8192, 256 tile
+    // workgroups: 71 us, 77 with two a CU).  Where tiles take own keys as well they end at
+    // different times, and two a CU fill in (the mixed batch 72 us, 75 with one)
+    long ow = p.use_tile && !p.any_big ? 2 * cus - wgs * p.nsplit : 2 * cus;
+    if (ow < cus) ow = cus;
     if (ow > Hkv * keyblocks) ow = Hkv * keyblocks;
     p.own_wgs = (int)(ow < 1 ? 1 : ow);
     p.own_parts = 4 * (Hkv * coltiles + p.own_wgs);
