@@ -104,6 +104,8 @@ __device__ __forceinline__ int find_seq(const SaArgs &a, int row) {
 // Vt by LDS-DMA one block of 64 keys ahead into a 2-stage ring, chunks XOR-swizzled by row.
 // A key block takes its four 16-key groups from up to four cache blocks (block sizes below
 // 64) or one.
+//
+// Bound by the matrix units: 16 ragged prompts behind 4096 positions 620 us, 990 TFLOP/s.
 template <int D>
 struct SaGeo {
     static constexpr int KROW = D * 2;
@@ -527,6 +529,10 @@ __device__ __forceinline__ void attn_own(const SaArgs &a, int wg, uint8_t *smem)
     const int c = lane & 15, g = lane >> 4;
     const int rows = live_rows(a);
 
+    // a short burst between two waits, beside a column tile's waves that always have work: it
+    // goes first (64 rows behind 8192 positions 61.0 -> 58.8 us, 24 x 5 rows 24.4 -> 23.0)
+    if (!a.any_big) __builtin_amdgcn_s_setprio(2);
+
     int t_before = 0, u_before = 0;
     for (int r0 = 0; r0 < a.R; r0 += SA_THREADS) {
         const int r = r0 + tid;
@@ -794,14 +800,15 @@ __global__ void __launch_bounds__(SA_THREADS) __attribute__((amdgpu_waves_per_eu
 
 // ---------------------------------------------------------------- merge
 //
-// One wave a row and q head: the parts of attn_tile (nsplit), then those of attn_own.  out = sum_i 2^(m_i - M) O_i /
-// sum_i 2^(m_i - M) l_i; parts of no key have m = -inf and weight 0, a row of no key at
-// all is 0.  The waves go over every row, or, where only sequences of few rows have parts,
+// One wave a row and q head: the parts of attn_tile (nsplit), then those of attn_own.
+// out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i; parts of no key have m = -inf and
+// weight 0, a row of no key at all is 0.  The waves go over every row, or, where only sequences of few rows have parts,
 // over by_seq rows of every sequence, if that is less (prompts are then passed over).
 //
 // Bound by the latency of dependent loads, so there are two rounds of them: what says where
 // the parts are, then the parts, lane i holding part i's place and (m, l), the values of
 // AHEAD parts on their way together.
+// 64 rows of 32 heads behind 8192 positions, 27 MB of parts: 8.2 us.
 // Few rows: WPR = 4, a workgroup a row and q head, its waves taking the parts in turn.
 template <int D, int WPR>
 __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_parts, int by_seq) {
