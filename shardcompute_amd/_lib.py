@@ -1002,7 +1002,8 @@ def attention_shared(q, H, Hkv, D, k_blocks, vt_blocks, row_starts, lengths, tab
     blocks).  Each attends the ``prefix_len[0]`` positions of ``prefix_table`` [width'], read
     once for the batch, and its own sequence up to itself.  ``max_new``: an upper bound of
     the rows of one sequence (default N).  Returns out [N, H*D] bf16; rows past the last
-    sequence's are left as they were."""
+    sequence's are left as they were.  ``workspace``: a contiguous tensor of at least
+    ``attention_shared_workspace_bytes`` (a smaller one, or none, and one is allocated)."""
     lib = load()
     dev = _gpu_of(q)
     stride, N = _row_matrix(q, H * D, "q", dev), q.shape[0]

@@ -52,12 +52,12 @@ struct SaArgs {
     int part_rows, per_seq;  // attn_tile's parts: by row, or (per_seq > 0) by sequence, per_seq rows each
     int tiles, pair_half;    // attn_tile's column tiles; > 0: workgroups of a round, paired with the next round's
     float scale_log2;
-    // parts: of attn_tile [nsplit][part_rows * H], of attn_own [own_parts][16] columns
+    // parts: of attn_tile [nsplit][part_rows * H], of attn_own [own_parts][part_cols] columns
     float *tile_o;
     float2 *tile_ml;
     float *own_o;
     float2 *own_ml;
-    int own_parts;
+    int own_parts, part_cols;
     int32_t *own_off, *own_unit;         // [R + 1]: a sequence's first block (and all of them), its first unit
 };
 
@@ -739,8 +739,8 @@ __device__ __forceinline__ void attn_own(const SaArgs &a, int wg, uint8_t *smem)
     auto end = [&](const Run &s) {           // the part: the unit's columns that are there
         float ltot = lsum + __shfl_xor(lsum, 16);
         ltot += __shfl_xor(ltot, 32);
-        if ((s.col0 + c) / a.G >= s.n || s.part >= a.own_parts) return;
-        const size_t at = (size_t)s.part * 16 + c;
+        if ((s.col0 + c) / a.G >= s.n || s.part >= a.own_parts || c >= a.part_cols) return;
+        const size_t at = (size_t)s.part * a.part_cols + c;
         float *po = a.own_o + at * D + 4 * g;
 #pragma unroll
         for (int y = 0; y < DT; ++y) *reinterpret_cast<f4 *>(po + 16 * y) = o[y];
@@ -851,7 +851,7 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
         own_step = wide ? 4 : 1;
         own_c = col & 15;
         if (kt && s.n <= a.small_rows) own_n = wide ? wgs : 4 * wgs;
-        if (own_part + own_step * own_n > a.own_parts + 3) own_n = 0;
+        if (own_part + own_step * own_n > a.own_parts + 3 || own_c >= a.part_cols) own_n = 0;
     }
     const int parts = tile_parts + own_n;
     float M = -INFINITY, L = 0.f, acc[PER] = {};
@@ -861,7 +861,7 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
         const int i = (i0 + min(lane, k - 1)) * WPR + turn;
         const bool t = i < tile_parts;
         long at = ((long)i * a.part_rows + part_row) * a.H + h;
-        if (!t) at = (own_part + own_step * (i - tile_parts)) * 16L + own_c;
+        if (!t) at = (own_part + own_step * (i - tile_parts)) * (long)a.part_cols + own_c;
         float2 x = (t ? a.tile_ml : a.own_ml)[at];
         if (lane >= k) x = make_float2(-INFINITY, 0.f);
         const float *const po = (t ? a.tile_o : a.own_o) + at * D;
@@ -955,7 +955,7 @@ int tile_splits(long wgs, long blocks, long Hkv, long D, double part_bytes, bool
 }
 
 struct SaPlan {
-    int small_rows, rows_max, any_big, nsplit, own_wgs, use_tile;
+    int small_rows, rows_max, any_big, nsplit, own_wgs, use_tile, part_cols;
     long tiles, own_parts, part_rows;
     int by_seq, per_seq;     // the merge, and attn_tile's parts, by sequence: rows of each
     long tile_o, tile_ml, own_o, own_ml, own_idx, bytes;       // workspace offsets
@@ -991,6 +991,7 @@ SaPlan plan_shared(long N, long R, long H, long Hkv, long D, long own_cap, long 
     if (ow > Hkv * keyblocks) ow = Hkv * keyblocks;
     p.own_wgs = (int)(ow < 1 ? 1 : ow);
     p.own_parts = 4 * (Hkv * coltiles + p.own_wgs);
+    p.part_cols = (int)(rows_max * G < 16 ? (rows_max * G > 1 ? rows_max * G : 1) : 16);
     auto up = [](long v) { return (v + 255) / 256 * 256; };
     long at = 0;
     // With whole tiles only sequences of few rows have parts.  Where they can be few of the
@@ -1002,8 +1003,8 @@ SaPlan plan_shared(long N, long R, long H, long Hkv, long D, long own_cap, long 
     const long tparts = p.use_tile ? p.nsplit * p.part_rows * H : 0;
     p.tile_o = at; at += up(tparts * D * 4);
     p.tile_ml = at; at += up(tparts * 8);
-    p.own_o = at; at += up(p.own_parts * 16 * D * 4);
-    p.own_ml = at; at += up(p.own_parts * 16 * 8);
+    p.own_o = at; at += up(p.own_parts * p.part_cols * D * 4);
+    p.own_ml = at; at += up(p.own_parts * p.part_cols * 8);
     p.own_idx = at; at += up((R + 1) * 2 * 4);
     p.bytes = at;
     return p;
@@ -1096,7 +1097,7 @@ int launch_attention_shared(const uint16_t *q, long q_stride, const uint16_t *kc
     a.tile_ml = reinterpret_cast<float2 *>(ws + p.tile_ml);
     a.own_o = reinterpret_cast<float *>(ws + p.own_o);
     a.own_ml = reinterpret_cast<float2 *>(ws + p.own_ml);
-    a.own_parts = (int)p.own_parts;
+    a.own_parts = (int)p.own_parts; a.part_cols = p.part_cols;
     a.own_off = reinterpret_cast<int32_t *>(ws + p.own_idx);
     a.own_unit = a.own_off + R + 1;
     return D == 128 ? run_shared<128>(a, p, stream) : run_shared<64>(a, p, stream);
