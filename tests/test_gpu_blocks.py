@@ -244,6 +244,25 @@ def test_attention_of_few_decoded_rows_beside_prompts(device, new):
     assert (got[c.starts[-1]:] == 5).all()
 
 
+@pytest.mark.parametrize("max_new", [1, 3, 20])
+@pytest.mark.parametrize("prefix", [0, 700])
+def test_attention_beyond_max_new_harms_nobody(device, max_new, prefix):
+    """Sequences of more rows than max_new: the others' rows are right, and nothing is written
+    outside the rows and the workspace."""
+    new = [1, 5, 2, 40, 1, 16, 3]
+    c = Cache([50, 3, 200, 0, 129, 10, 64], new, prefix, 64, 8, 2, 128, pad=2)
+    exact, mag = c.exact()
+    pre = 0 if c.prefix_table is None else c.prefix_table.numel() * c.bs
+    need = _lib.attention_shared_workspace_bytes(c.N, len(new), 8, 2, 128, c.tables.shape[1] * c.bs, pre, max_new)
+    buf = torch.full((need + 4096,), 77, dtype=torch.uint8, device="cuda")
+    got = c.attend(max_new=max_new, out=torch.full_like(c.q, 5.0), workspace=buf[:need])
+    assert (buf[need:] == 77).all() and (got[c.starts[-1]:] == 5).all()
+    for r, n in enumerate(new):
+        if n <= max_new:
+            rows = slice(c.starts[r], c.starts[r + 1])
+            assert_attention(got[rows], exact[rows], mag[rows], n)
+
+
 def test_attention_strides_scale_and_wide_tables(device):
     c = Cache([30, 2, 200], [1, 1, 40], 150, 32, 8, 2, 128, pad=2, width=50)
     wide = torch.zeros((c.N, 2 * 1024 + 8), dtype=torch.bfloat16, device="cuda")
