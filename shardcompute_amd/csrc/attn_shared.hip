@@ -808,7 +808,7 @@ __global__ void __launch_bounds__(SA_THREADS) __attribute__((amdgpu_waves_per_eu
 // Bound by the latency of dependent loads, so there are two rounds of them: what says where
 // the parts are, then the parts, lane i holding part i's place and (m, l), the values of
 // AHEAD parts on their way together.
-// 64 rows of 32 heads behind 8192 positions, 27 MB of parts: 8.2 us.
+// 64 rows of 32 heads behind 8192 positions: 7.5 us.
 // Few rows: WPR = 4, a workgroup a row and q head, its waves taking the parts in turn.
 template <int D, int WPR>
 __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_parts, int by_seq) {
@@ -936,9 +936,11 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
 // ones wait (head_dim 128, measured: 300 rows behind 30000 positions 222 us in 3 pieces of 80
 // workgroups, 16 prompts 633 us in 2117 workgroups of 72 blocks; head_dim 64 ~0.8 of it, the
 // softmax is the same), and the keys come at 5.3 TB/s at most; a row's part is written and read
-// at about 2.5 TB/s and lengthens the merge by 0.06 us.  The sum is least at the count
-// returned: 16 rows behind 65536 positions 66 us (in 32), 86 at 24; 768 rows behind 2048
-// 71 us (whole), 86 in 2.
+// at about 2.5 TB/s and lengthens the merge by 0.06 us; at 1.3 TB/s where no tile takes own
+// keys (last_is_whole false), which then come by themselves beside it (200 rows behind 1000
+// positions 82 us, at 2.5 96, 64 rows behind 2048 35.5 and 38.5; but 300 rows of a prompt
+// behind 8000 80 us at 1.3, 69 at 2.5).  The sum is least at the count returned: 16 rows
+// behind 65536 positions 66 us (in 32), 86 at 24; 768 rows behind 2048 71 us (whole), 86 in 2.
 int tile_splits(long wgs, long blocks, long Hkv, long D, double part_bytes, bool last_is_whole, long cus) {
     const double stream = (double)Hkv * blocks * SA_KB * D * 4 / 5.3e6;
     int best = 1;
@@ -947,7 +949,7 @@ int tile_splits(long wgs, long blocks, long Hkv, long D, double part_bytes, bool
         const long w = wgs * n;
         const double block = (D == 64 ? 0.8 : 1.0) * (w <= cus ? 1.5 : 2.1 * ((w + 2 * cus - 1) / (2 * cus)));
         const double walk = (double)((blocks + n - 1) / n) * block;
-        const double parts = n == 1 && last_is_whole ? 0 : n * (part_bytes / 2.5e6 + 0.06);
+        const double parts = n == 1 && last_is_whole ? 0 : n * (part_bytes / (last_is_whole ? 2.5e6 : 1.3e6) + 0.06);
         const double us = (walk > stream ? walk : stream) + parts;
         if (us < least) { least = us; best = n; }
     }
