@@ -244,6 +244,22 @@ def test_attention_of_few_decoded_rows_beside_prompts(device, new):
     assert (got[c.starts[-1]:] == 5).all()
 
 
+@pytest.mark.parametrize("D,bs", [(64, 16), (128, 64)])
+def test_attention_of_the_most_sequences(device, D, bs):
+    """2048 sequences, one in three waiting, some without any position; one more is refused."""
+    print(f"2048 sequences D={D} bs={bs}", flush=True)
+    R = _lib.SHARED_MAX_SEQUENCES
+    c = Cache([(11 * i) % 70 if i % 5 else 0 for i in range(R)], [i % 3 for i in range(R)], 90, bs, 4, 2, D, pad=1)
+    exact, mag = c.exact()
+    got = c.attend(max_new=2, out=torch.full_like(c.q, 5.0))
+    assert_attention(got, exact, mag, c.starts[-1])
+    assert (got[c.starts[-1]:] == 5).all()
+    more = torch.cat([c.tables, c.tables[:1]])
+    with pytest.raises(RuntimeError, match="at most 2048"):
+        _lib.attention_shared(c.q, 4, 2, D, c.k, c.vt, torch.cat([c.row_starts, c.row_starts[-1:]]),
+                              torch.cat([c.lens, c.lens[:1]]), more, c.scale)
+
+
 @pytest.mark.parametrize("max_new", [1, 3, 20])
 @pytest.mark.parametrize("prefix", [0, 700])
 def test_attention_beyond_max_new_harms_nobody(device, max_new, prefix):
