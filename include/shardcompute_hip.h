@@ -372,10 +372,11 @@ int64_t sc_attention_shared_workspace_bytes(int64_t N, int64_t R, int64_t H, int
  * own positions 0 .. lengths[r] - n_r + i (lengths: with the new positions, which have been
  * appended): out = softmax(q k^T * scale) v, q head h reading KV head h / (H / Hkv).  The
  * prefix is read once for the whole batch.  q rows at q + row*q_stride + h*D, output rows
- * likewise with out_stride; rows at or past row_starts[R] are left as they were; a row with
- * no key is 0.  prefix_width 0: no prefix (null pointers).  max_new: at least the most new
- * positions of one sequence (N does; a smaller bound saves launches; below the truth the
- * rows of sequences above it are unspecified).  Slots that no row attends may hold anything.
+ * likewise with out_stride; rows before row_starts[0] and from row_starts[R] on are left as
+ * they were; a row with no key is 0.  prefix_width 0: no prefix (null pointers).  max_new: at
+ * least the most new positions of one sequence (N does; a smaller bound saves launches; below
+ * the truth the rows of sequences above it are unspecified).  Slots that no row attends may
+ * hold anything.
  * Block numbers, lengths and row starts out of range are clamped: the result is then
  * unspecified, the access in bounds.  scale must be positive; D 64 or 128; R <= 2048, and
  * R * Hkv * (width * block_size) below 2^37 (tables of more positions than any pool has).

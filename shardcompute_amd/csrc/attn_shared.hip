@@ -20,6 +20,7 @@
 // row starts to the rows, so nothing outside the buffers is touched whatever they hold.
 #include "sc_common.h"
 #include "dma_util.h"
+#include "attn_shared_parts.h"
 
 #include <math.h>
 #include <atomic>
@@ -510,10 +511,7 @@ __device__ __forceinline__ void attn_tile(const SaArgs &a, int id, uint8_t *smem
 // Bound by memory.  The copies read whole cache lines, 256 bytes a K row and 128 a Vt row:
 // 5.5 TB/s (64 sequences of 4096 positions, 194 us; operands loaded straight into the
 // registers in the MFMA's order, 64 bytes of 16 rows an instruction, 250 us).
-__device__ __forceinline__ int own_coltiles(const SaArgs &a, int n) { return (n * a.G + 63) >> 6; }
-__device__ __forceinline__ int own_keyblocks(int len) { return (len + SA_KB - 1) / SA_KB; }
-// blocks a workgroup takes of `total`
-__device__ __forceinline__ int own_run(const SaArgs &a, int total) { return max((total + a.own_wgs - 1) / a.own_wgs, 1); }
+static_assert(SA_KB == 64, "own_keyblocks counts blocks of 64 keys");
 
 typedef __attribute__((__vector_size__(4 * sizeof(short)))) short s16x4_t;
 
@@ -540,7 +538,7 @@ __device__ __forceinline__ void attn_own(const SaArgs &a, int wg, uint8_t *smem)
         if (r < a.R) {
             const Seq s = seq_of(a, r, rows);
             const int kt = own_keyblocks(s.len);
-            u = kt && s.n <= a.small_rows ? a.Hkv * own_coltiles(a, s.n) : 0;
+            u = kt && s.n <= a.small_rows ? a.Hkv * own_coltiles(s.n, a.G) : 0;
             t = u * kt;
             first_row[r] = s.first;
             keys[r] = s.len;
@@ -567,7 +565,7 @@ __device__ __forceinline__ void attn_own(const SaArgs &a, int wg, uint8_t *smem)
         for (int r = tid; r < a.R; r += SA_THREADS) { a.own_off[r] = off[r]; a.own_unit[r] = unit[r]; }
         if (tid == 0) a.own_off[a.R] = t_before;
     }
-    const int total = t_before, run = own_run(a, total);
+    const int total = t_before, run = own_run(total, a.own_wgs);
     int t = (int)min((long)wg * run, (long)total);
     const int t_end = min(t + run, total);
     if (t >= t_end) return;
@@ -603,7 +601,7 @@ __device__ __forceinline__ void attn_own(const SaArgs &a, int wg, uint8_t *smem)
             n = __builtin_amdgcn_readfirstlane(first_row[r + 1]) - first;
             if (n > a.small_rows) n = 0;
             kt = own_keyblocks(len);
-            ct = own_coltiles(a, n);
+            ct = own_coltiles(n, a.G);
             if (in_seq < a.Hkv * ct * kt || r == a.R - 1) break;
         }
         const int u = in_seq / kt, b0 = in_seq - u * kt, b1 = min(kt, b0 + t_end - t);
@@ -838,24 +836,13 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
         if (row >= rows) return;
         r = find_seq(a, row);
         s = seq_of(a, r, rows);
+        if (row < s.first || row >= s.first + s.n) return;     // no sequence's row
         if (s.n > a.small_rows && a.nsplit == 1) return;       // written by attn_tile
     }
     const int hk = h / a.G, gq = h - hk * a.G;
-    // attn_own's parts: of the workgroups that have blocks of the row's unit, the four waves'
-    // or (a wide unit) that of the wave whose column it is
-    int own_part = 0, own_n = 0, own_c = 0, own_step = 1;
-    {
-        const int run = own_run(a, a.own_off[a.R]), kt = own_keyblocks(s.len), ct = own_coltiles(a, s.n);
-        const int col = (row - s.first) * a.G + gq, u = hk * ct + (col >> 6);
-        const int t0 = a.own_off[r] + u * kt, w0 = t0 / run, wgs = (t0 + kt - 1) / run - w0 + 1;
-        const bool wide = s.n * a.G > 16;
-        own_part = 4 * (a.own_unit[r] + u + w0) + (wide ? (col >> 4) & 3 : 0);
-        own_step = wide ? 4 : 1;
-        own_c = col & 15;
-        if (kt && s.n <= a.small_rows) own_n = wide ? wgs : 4 * wgs;
-        if (own_part + own_step * own_n > a.own_parts + 3 || own_c >= a.part_cols) own_n = 0;
-    }
-    const int parts = tile_parts + own_n;
+    const OwnParts own = own_parts_of(row, s.first, s.n, s.len, hk, gq, a.G, a.small_rows, a.own_off[r], a.own_unit[r],
+                                      a.own_off[a.R], a.own_wgs, a.own_parts, a.part_cols);
+    const int parts = tile_parts + own.n;
     float M = -INFINITY, L = 0.f, acc[PER] = {};
     for (int i0 = 0; i0 * WPR + turn < parts; i0 += 64) {
         // this lane's part
@@ -863,7 +850,7 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
         const int i = (i0 + min(lane, k - 1)) * WPR + turn;
         const bool t = i < tile_parts;
         long at = ((long)i * a.part_rows + part_row) * a.H + h;
-        if (!t) at = (own_part + own_step * (i - tile_parts)) * (long)a.part_cols + own_c;
+        if (!t) at = (own.first + own.step * (i - tile_parts)) * (long)a.part_cols + own.col;
         float2 x = (t ? a.tile_ml : a.own_ml)[at];
         if (lane >= k) x = make_float2(-INFINITY, 0.f);
         const float *const po = (t ? a.tile_o : a.own_o) + at * D;

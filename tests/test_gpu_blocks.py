@@ -279,6 +279,30 @@ def test_attention_beyond_max_new_harms_nobody(device, max_new, prefix):
             assert_attention(got[rows], exact[rows], mag[rows], n)
 
 
+def attend_without_first(c, max_new):
+    """The call of c without its first sequence: row starts that begin above 0, and rows of nobody."""
+    pre = dict(prefix_table=c.prefix_table, prefix_len=c.prefix_len) if c.prefix_table is not None else {}
+    return _lib.attention_shared(c.q, c.H, c.Hkv, c.D, c.k, c.vt, c.row_starts[1:], c.lens[1:], c.tables[1:], c.scale,
+                                 max_new=max_new, out=torch.full_like(c.q, 5.0), **pre)
+
+
+# rows of the first sequence, which the call leaves out, and of the others; room of the tables in blocks
+@pytest.mark.parametrize("held,new,prefix,bs,H,Hkv,D,width,max_new", [
+    ([0, 700, 0], [299, 1, 0], 0, 64, 32, 8, 128, 128, None),       # cut tiles, merged row by row
+    ([0, 40, 300, 3], [40, 30, 2, 40], 9000, 64, 8, 2, 64, 10, None),
+    ([0, 40, 300, 3], [2, 1, 2, 1], 70, 16, 8, 2, 64, 30, 3),       # few rows, merged row by row
+    ([0, 40, 300, 3], [9, 3, 2, 1], 0, 32, 32, 8, 128, 30, 3),      # few rows, by sequence
+    ([0, 5], [700, 1], 33, 64, 4, 4, 64, 12, 1),                    # one row's slot behind 700 rows
+])
+def test_attention_leaves_rows_before_the_first_sequence(device, held, new, prefix, bs, H, Hkv, D, width, max_new):
+    print(f"rows from {new[0]}: {new[1:]} prefix={prefix} bs={bs} H={H} Hkv={Hkv} D={D}", flush=True)
+    c = Cache(held, new, prefix, bs, H, Hkv, D, pad=2, width=width)
+    exact, mag = c.exact()
+    got, rows = attend_without_first(c, max_new), slice(c.starts[1], c.starts[-1])
+    assert_attention(got[rows], exact[rows], mag[rows], rows.stop - rows.start)
+    assert (got[:rows.start] == 5).all() and (got[rows.stop:] == 5).all()
+
+
 def test_attention_strides_scale_and_wide_tables(device):
     c = Cache([30, 2, 200], [1, 1, 40], 150, 32, 8, 2, 128, pad=2, width=50)
     wide = torch.zeros((c.N, 2 * 1024 + 8), dtype=torch.bfloat16, device="cuda")
