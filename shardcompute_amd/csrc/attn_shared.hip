@@ -246,14 +246,14 @@ __device__ __forceinline__ void attn_tile(const SaArgs &a, int id, uint8_t *smem
     const int r0 = a.any_big ? find_seq(a, row0) : 0;
     int total = (P + SA_KB - 1) / SA_KB;
     bool big = false;                                   // this column's own keys are taken here
-    int part_row = row;                                 // where its part goes, if it has one
+    int part_row = tile_part_row(row, -1, 0, a.per_seq, a.part_rows);      // where its part goes, if it has one
     if (a.any_big)
         for (int r = r0; r < a.R; ++r) {
             const Seq s = seq_of(a, r, rows);
             if (s.first > row1) break;
             if (row >= s.first && row < s.first + s.n) {
                 big = s.n > a.small_rows;
-                if (a.per_seq) part_row = r * a.per_seq + row - s.first;
+                part_row = tile_part_row(row, r, row - s.first, a.per_seq, a.part_rows);
             }
             total += own_blocks(s);
         }
@@ -481,7 +481,7 @@ __device__ __forceinline__ void attn_tile(const SaArgs &a, int id, uint8_t *smem
                                cvt_pk_bf16(o[db][4 * r4 + 2] * inv, o[db][4 * r4 + 3] * inv));
         return;
     }
-    if (part_row >= a.part_rows) return;                // (a sequence of more rows than max_new)
+    if (part_row >= a.part_rows) return;
     const size_t part = ((size_t)split * a.part_rows + part_row) * a.H + h;
     float *po = a.tile_o + part * D;
 #pragma unroll

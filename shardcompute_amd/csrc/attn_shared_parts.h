@@ -1,5 +1,5 @@
-// Where attn_own (attn_shared.hip) leaves the parts of a row, for the merge that joins
-// them: whole numbers only, so that it also runs, and is tested, on the host.
+// Where attn_tile and attn_own (attn_shared.hip) leave the parts of a row, for the merge that
+// joins them: whole numbers only, so that it also runs, and is tested, on the host.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -11,6 +11,14 @@ __host__ __device__ __forceinline__ int own_keyblocks(int len) { return (len + 6
 // blocks a workgroup takes of `total`
 __host__ __device__ __forceinline__ int own_run(int total, int wgs) {
     return total > 0 ? (total - 1) / wgs + 1 : 1;
+}
+
+// Of part_rows rows' parts, attn_tile's of row `row`, the i-th of sequence r (-1: of none): the
+// row's number, or, where they are kept by sequence (per_seq > 0 each), the sequence's i-th.
+// part_rows: it has no part.
+__host__ __device__ __forceinline__ int tile_part_row(int row, int r, int i, int per_seq, int part_rows) {
+    if (per_seq == 0) return row;
+    return r < 0 || i >= per_seq ? part_rows : r * per_seq + i;
 }
 
 struct OwnParts {

@@ -16,11 +16,14 @@ extern "C" void parts_of(const int *a, int *out) {
                                             a[12], a[13]);
     out[0] = p.first; out[1] = p.n; out[2] = p.step; out[3] = p.col;
 }
+extern "C" int tile_part_row(int row, int r, int i, int per_seq, int part_rows) {
+    return sc::tile_part_row(row, r, i, per_seq, part_rows);
+}
 """
 
 
 @pytest.fixture(scope="module")
-def parts_of(tmp_path_factory):
+def library(tmp_path_factory):
     if not (shutil.which("hipcc") or shutil.os.path.exists("/opt/rocm/bin/hipcc")):
         pytest.skip("no hipcc")
     d = tmp_path_factory.mktemp("parts")
@@ -28,7 +31,12 @@ def parts_of(tmp_path_factory):
     src.write_text(SOURCE)
     subprocess.run([build.hipcc(), "--cuda-host-only", "-O1", "-std=c++17", "-shared", "-fPIC", "-I", build.CSRC, str(src),
                     "-o", str(lib)], check=True, capture_output=True)
-    fn = ctypes.CDLL(str(lib)).parts_of
+    return ctypes.CDLL(str(lib))
+
+
+@pytest.fixture(scope="module")
+def parts_of(library):
+    fn = library.parts_of
     I14, I4 = ctypes.c_int * 14, ctypes.c_int * 4
 
     def call(*a):
@@ -113,3 +121,16 @@ def test_rows_of_no_sequence_have_no_parts(parts_of):
         p = parts_of(*a)
         assert inside(p, parts, 16), (a, p)
         assert p[1] == 0 or first <= row < first + n
+
+
+def test_rows_of_no_sequence_take_no_sequences_part(library):
+    """attn_tile's parts by sequence, 3 of 16 rows each: every row of a sequence has a slot of its
+    own, a row of no sequence none of them."""
+    f = library.tile_part_row
+    owned = [f(100 + 20 * r + i, r, i, 16, 48) for r in range(3) for i in range(16)]
+    assert sorted(owned) == list(range(48))
+    assert all(f(row, -1, 0, 16, 48) >= 48 for row in range(200))
+    # a sequence of more rows keeps out of the next one's
+    assert all(f(row, 0, row, 16, 48) >= 48 for row in range(16, 60))
+    # by row: every row its own
+    assert [f(row, r, 1, 0, 200) for row in range(200) for r in (-1, 2)] == [row for row in range(200) for _ in (0, 1)]

@@ -292,6 +292,8 @@ def attend_without_first(c, max_new):
     ([0, 40, 300, 3], [40, 30, 2, 40], 9000, 64, 8, 2, 64, 10, None),
     ([0, 40, 300, 3], [2, 1, 2, 1], 70, 16, 8, 2, 64, 30, 3),       # few rows, merged row by row
     ([0, 40, 300, 3], [9, 3, 2, 1], 0, 32, 32, 8, 128, 30, 3),      # few rows, by sequence
+    ([0, 40, 30, 3], [120, 1, 50, 2], 100, 64, 32, 8, 128, 4, None),        # whole tiles, parts by sequence
+    ([0, 40, 30, 3], [90, 5, 70, 8], 20, 16, 32, 4, 64, 8, None),
     ([0, 5], [700, 1], 33, 64, 4, 4, 64, 12, 1),                    # one row's slot behind 700 rows
 ])
 def test_attention_leaves_rows_before_the_first_sequence(device, held, new, prefix, bs, H, Hkv, D, width, max_new):
