@@ -108,8 +108,14 @@ class BlockKVCache:
 
     @property
     def max_positions(self) -> int:
-        """Rotary positions the cache can reach."""
+        """Positions asked for: the longest prefix and the longest sequence behind it."""
         return self.max_prefix + self.max_length
+
+    @property
+    def rotary_positions(self) -> int:
+        """Positions the tables have room for, whole blocks: what the rotary tables must hold."""
+        blocks = self.tables.shape[1] + (0 if self.prefix_table is None else self.prefix_table.numel())
+        return blocks * self.block_size
 
     @property
     def nbytes(self) -> int:

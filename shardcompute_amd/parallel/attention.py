@@ -183,7 +183,7 @@ class ParallelAttention:
             b, st = kv.batch, kv.batch.step
             if qkv.shape[0] != b.rows:
                 raise ValueError(f"the step has {b.rows} rows, got {qkv.shape[0]}")
-            cos_t, sin_t = self.rope.tables(b.cache.max_positions, qkv.device)
+            cos_t, sin_t = self.rope.tables(b.cache.rotary_positions, qkv.device)
             q = _lib.rope_append_blocks(qkv, H, Hk, D, cos_t, sin_t, kv.k, kv.vt, st.slots, st.positions,
                                         out=qkv[:, :H * D])
             return _lib.attention_shared(q, H, Hk, D, kv.k, kv.vt, st.row_starts, st.lengths, b.tables, self.scale,

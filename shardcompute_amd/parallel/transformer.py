@@ -281,7 +281,8 @@ class ParallelTransformer:
     def new_block_cache(self, max_sequences: int, max_length: int, num_blocks: Optional[int] = None,
                         block_size: int = 64, max_prefix: int = 0) -> BlockKVCache:
         """A cache in blocks for ``max_sequences`` sequences of up to ``max_length`` own positions
-        behind a shared prefix of up to ``max_prefix`` (default: blocks for all of them)."""
+        (rounded up to whole blocks) behind a shared prefix of up to ``max_prefix`` (default:
+        blocks for all of them)."""
         att = self.layers[0].attention
         if num_blocks is None:
             num_blocks = max_sequences * -(-max_length // block_size) + -(-max_prefix // block_size)

@@ -117,3 +117,29 @@ def test_more_key_blocks_than_32_bits_count_are_refused():
     from shardcompute_amd import _lib
     assert _lib.attention_shared_workspace_bytes(64, 2048, 32, 8, 128, 1 << 25, 0, 1) == 0
     assert _lib.attention_shared_workspace_bytes(64, 2048, 2048, 1, 128, 1 << 25, 0, 1) == 0       # 32 columns' 64s
+
+
+@pytest.mark.parametrize("max_length,max_prefix,bs", [(2050, 0, 256), (2050, 300, 256), (17, 1, 16), (64, 128, 64)])
+def test_rotary_tables_reach_every_position_a_table_has_room_for(max_length, max_prefix, bs, monkeypatch):
+    """A sequence may grow to the room of its table, max_length rounded up to a block: the rotary
+    tables that its layers ask for hold the last of these positions."""
+    from types import SimpleNamespace
+
+    from shardcompute_amd.block_cache import BlockBatch, BlockKVCache
+    from shardcompute_amd.parallel import attention
+    cpu = torch.device("cpu")
+    c = BlockKVCache(1, 2, 64, num_blocks=40, max_sequences=1, max_length=max_length, block_size=bs,
+                     max_prefix=max_prefix, device=cpu)
+    room = c.tables.shape[1] * bs
+    assert c._plan([room], None)[0] == [room]
+    with pytest.raises(RuntimeError, match="room"):
+        c._plan([room + 1], None)
+    seen = []
+    monkeypatch.setattr(attention._lib, "rope_append_blocks", lambda qkv, H, Hk, D, cos, *a, **kw: seen.append(cos.shape[0]))
+    monkeypatch.setattr(attention._lib, "attention_shared", lambda *a, **kw: None)
+    att = SimpleNamespace(local_num_heads=4, local_num_kv_heads=2, head_dim=64, scale=0.125,
+                          rope=attention.RoPE(64, max_position_embeddings=1))
+    step = c._buffers(1, 1, c.lengths)
+    kv = BlockBatch(c, step, c.tables, 1, 1, False)[0]
+    attention.ParallelAttention.attend_qkv(att, torch.zeros((1, 8 * 64), dtype=torch.bfloat16), 1, 1, kv)
+    assert seen[0] >= max_prefix + room

@@ -178,3 +178,20 @@ def test_decode_graph_made_before_its_prefix(model):
     dec.run(n - 1)
     cache.check_status()
     assert out.tolist() == want
+
+
+@pytest.mark.parametrize("prefix", [0, 70])
+def test_positions_up_to_the_tables_room(device, prefix):
+    """A sequence past max_length, up to the room of its table, behind more positions than the
+    model's rotary tables hold by themselves."""
+    m = build_model(SHAPE, random_decoder_weights(SHAPE, seed=0))
+    rng = np.random.default_rng(5)
+    pre, own, more = tokens(rng, prefix), tokens(rng, 255), tokens(rng, 200)
+    cache = m.new_block_cache(1, 260, block_size=256, max_prefix=prefix)
+    if prefix:
+        run(m.forward_blocks(pre, cache.begin_prefix(prefix)))
+    run(m.forward_blocks(own, cache.begin([255])))
+    got = f32(run(m.forward_blocks(more, cache.begin([200]), all_rows=True)))
+    assert close(got, dense(m, pre + own + more)[prefix + 255:])
+    with pytest.raises(RuntimeError, match="room for 512"):
+        cache.begin([58])
