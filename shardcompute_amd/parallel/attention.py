@@ -61,13 +61,19 @@ class RoPE:
         self.inv_freq = (1.0 / (np.float32(base) ** (np.arange(0, head_dim, 2, dtype=np.float32)
                                                       / np.float32(head_dim)))).astype(np.float32)
         self._tables = {}
+        self._replaced = []
 
     def tables(self, length: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
-        """(cos, sin) fp32 ``[>= length, head_dim/2]`` on ``device`` (grown by doubling, min 256)."""
+        """(cos, sin) fp32 ``[>= length, head_dim/2]`` on ``device`` (grown by doubling, min 256).
+
+        Tables replaced by longer ones are kept: a captured graph goes on reading those it was
+        captured with.  As each at least doubles the last, they are no more than the newest."""
         key = str(device)
         cur = self._tables.get(key)
         if cur is None or cur[0].shape[0] < length:
             have = 0 if cur is None else cur[0].shape[0]
+            if cur is not None:
+                self._replaced.append(cur)
             n = max(int(length), 2 * have, 256, self.max_position_embeddings)
             c, s = rope_tables_np(self.head_dim, self.base, self.scaling_factor, n)
             cur = (torch.from_numpy(c).to(device), torch.from_numpy(s).to(device))
