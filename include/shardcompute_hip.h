@@ -17,10 +17,11 @@
  *    the products inside sc_qmm_rmsnorm_bf16 / sc_qmm_swiglu_bf16 / sc_qmm_add_rmsnorm_bf16:
  *    8-160 rows, and larger products whose 256-wide tiles fill at most a quarter of the GPU
  *    over K >= 4096) uses a
- *    library-owned scratch per device, allocated on first need and grown (with a
- *    device synchronisation) when a larger shape arrives: calls that overlap on one
+ *    library-owned scratch per device, allocated on first need and grown (which may
+ *    synchronise the device) when a larger shape arrives: calls that overlap on one
  *    device (concurrent streams) race on it, and the first call of a new largest
- *    shape must not happen under stream capture.  sc_qmm_bf16_noalloc is the
+ *    shape must not happen under stream capture.  What it grew out of stays allocated,
+ *    so that graphs captured before go on replaying.  sc_qmm_bf16_noalloc is the
  *    variant that never allocates.
  */
 #ifndef SHARDCOMPUTE_HIP_H

@@ -134,29 +134,30 @@ const DeviceInfo &device_info() {
 }
 
 // Grows (never shrinks) the calling device's split-K scratch.  Counters must
-// start at zero; the kernels return every counter they use to zero.  Growing
-// synchronises the device so no in-flight kernel still uses the old buffers.
+// start at zero; the kernels return every counter they use to zero.  The buffers grown
+// out of are kept: a captured graph goes on using those it was captured with.  As each at
+// least doubles the last, they are together no more than the newest.
 int splitk_scratch(size_t partial_floats, size_t n_counters, SplitKScratch *out) {
     int dev = 0;
     SC_HIP_CHECK(hipGetDevice(&dev));
     if (dev < 0 || dev >= kMaxDevices) return set_error(SC_EINVAL, "device id %d out of range", dev);
     std::lock_guard<std::mutex> lk(g_mu);
     ScratchSlot &sl = g_scratch[dev];
-    if (sl.partial_cap < partial_floats || sl.counter_cap < n_counters) {
-        const size_t pc = partial_floats > sl.partial_cap ? partial_floats : sl.partial_cap;
-        const size_t cc = n_counters > sl.counter_cap ? n_counters : sl.counter_cap;
+    if (sl.partial_cap < partial_floats) {
+        const size_t cap = partial_floats > 2 * sl.partial_cap ? partial_floats : 2 * sl.partial_cap;
+        float *p = nullptr;
+        SC_HIP_CHECK(hipMalloc(&p, cap * sizeof(float)));
+        sl.partials = p;
+        sl.partial_cap = cap;
+    }
+    if (sl.counter_cap < n_counters) {
+        const size_t cap = n_counters > 2 * sl.counter_cap ? n_counters : 2 * sl.counter_cap;
+        unsigned *c = nullptr;
+        SC_HIP_CHECK(hipMalloc(&c, cap * sizeof(unsigned)));
+        SC_HIP_CHECK(hipMemset(c, 0, cap * sizeof(unsigned)));
         SC_HIP_CHECK(hipDeviceSynchronize());
-        if (sl.partials) SC_HIP_CHECK(hipFree(sl.partials));
-        if (sl.counters) SC_HIP_CHECK(hipFree(sl.counters));
-        sl.partials = nullptr;
-        sl.counters = nullptr;
-        sl.partial_cap = sl.counter_cap = 0;
-        SC_HIP_CHECK(hipMalloc(&sl.partials, pc * sizeof(float)));
-        SC_HIP_CHECK(hipMalloc(&sl.counters, cc * sizeof(unsigned)));
-        SC_HIP_CHECK(hipMemset(sl.counters, 0, cc * sizeof(unsigned)));
-        SC_HIP_CHECK(hipDeviceSynchronize());
-        sl.partial_cap = pc;
-        sl.counter_cap = cc;
+        sl.counters = c;
+        sl.counter_cap = cap;
     }
     out->partials = sl.partials;
     out->counters = sl.counters;

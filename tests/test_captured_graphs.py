@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from oracle.decoder import random_decoder_weights
+from shardcompute_amd import _lib
 from shardcompute_amd.executor import BlockDecodeGraph, DecodeGraph
 from tests.test_gpu_model import SHAPE, build_model
 
@@ -67,3 +68,37 @@ def test_graph_outlives_longer_rotary_tables(device, weights, decoder):
     held = fill_memory(before, 4 * len(model.layers))
     dec.run(n - 10)
     assert torch.equal(out, want) and all(t.isnan().all() for t in held)
+
+
+def product(g, M, N, K):
+    x = torch.randn((M, K), generator=g, device="cuda").to(torch.bfloat16)
+    return x, _lib.quantize(torch.randn((N, K), generator=g, device="cuda").mul_(0.02), bits=4)
+
+
+def test_graph_outlives_a_larger_split_k_product(device):
+    """Products that split K in a graph (9-32 rows, the band kernel), then one whose partials
+    need more of the library's scratch, other allocations, and replays: the eager results."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    small = [product(g, 20, 128, 8192), product(g, 40, 256, 4096)]
+    want = [_lib.qmm(x, *w) for x, w in small]
+    outs = [torch.empty_like(y) for y in want]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for (x, w), y in zip(small, outs):
+            _lib.qmm(x, *w, out=y)
+    free = torch.cuda.mem_get_info()[0]
+    x, w = product(g, 1000, 4096, 14336)                      # 4 x 1000 x 4096 partials
+    big = _lib.qmm(x, *w)
+    torch.cuda.synchronize()
+    print(f"{(free - torch.cuda.mem_get_info()[0]) >> 20} MB more held", flush=True)
+    held = [torch.full((n,), 7.0, device="cuda") for n in (1 << 16, 1 << 20, 1 << 24, 1 << 26)]
+    for _ in range(3):
+        for y in outs:
+            y.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, z) for y, z in zip(outs, want))
+        assert torch.equal(_lib.qmm(x, *w), big)
+    assert all((t == 7).all() for t in held)
