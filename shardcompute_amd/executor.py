@@ -169,19 +169,21 @@ class BlockDecodeGraph:
         one = [1] * self.cache.max_sequences
         for _ in range(n):
             lengths, free = self.cache._plan(one, None)
-            if self.graph is not None:
+            eager = self.graph is None
+            if eager:
+                self.logits = self._step()
+            else:
                 self.graph[0].replay()
                 self.logits = self.graph[1]
-            else:
-                self.logits = self._step()
-                if self.use_graph:
-                    torch.cuda.synchronize()
-                    g = torch.cuda.CUDAGraph()
-                    with torch.cuda.graph(g):
-                        logits = self._step()
-                    self.graph = (g, logits)
+            # the step is on its way, also if it cannot be captured below
             self.cache.host_lengths, self.cache.host_free = lengths, free
             self.cache.steps += 1
+            if eager and self.use_graph:
+                torch.cuda.synchronize()
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g):
+                    logits = self._step()
+                self.graph = (g, logits)
 
 
 class ParallelExecutor:
