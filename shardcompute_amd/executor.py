@@ -125,23 +125,29 @@ class DecodeGraph:
             if self.graph is not None:
                 g, self.logits = self.graph
                 g.replay()
+                self.cache.length += 1
             else:
                 self._step()
-                if self.use_graph:
-                    eager = self.logits
-                    self.graph = self._capture(1)
-                    # capture only records: the step's logits are the eager run's
-                    self.logits = eager
-            self.cache.length += 1
+                try:
+                    if self.use_graph:
+                        self.graph = self._capture(1)
+                finally:
+                    # the step has run, also if it could not be captured
+                    self.cache.length += 1
             n -= 1
 
     def _capture(self, steps: int):
-        torch.cuda.synchronize()
-        g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
-            for _ in range(steps):
-                self._step()
-        return g, self.logits
+        # capture only records: the logits stay those of the step that ran
+        ran = self.logits
+        try:
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                for _ in range(steps):
+                    self._step()
+            return g, self.logits
+        finally:
+            self.logits = ran
 
 
 class BlockDecodeGraph:

@@ -7,7 +7,8 @@ import torch
 from shardcompute_amd import executor
 from shardcompute_amd.block_cache import BlockKVCache
 from shardcompute_amd.build import LIB_PATH
-from shardcompute_amd.executor import BlockDecodeGraph
+from shardcompute_amd.executor import BlockDecodeGraph, DecodeGraph
+from shardcompute_amd.kv_cache import KVCache
 
 pytestmark = pytest.mark.skipif(not os.path.exists(LIB_PATH), reason="library not built")
 
@@ -34,3 +35,23 @@ def test_block_cache_counts_the_step_before_a_capture_that_fails(monkeypatch):
     dec.use_graph = False
     dec.run(2)
     assert len(steps) == 3 and cache.host_lengths == [19, 6] and cache.steps == 3
+
+
+def test_dense_cache_counts_the_step_before_a_capture_that_fails(monkeypatch):
+    cache = KVCache(1, 1, 1, 64, 64, device=torch.device("cpu"))
+    cache.length = 5
+    dec = DecodeGraph.__new__(DecodeGraph)
+    dec.cache, dec.use_graph, dec.steps_per_graph, dec.graph, dec.graph_n = cache, True, 8, None, None
+    lengths = []
+
+    def step():
+        lengths.append(cache.length)
+        dec.logits = len(lengths)
+    dec._step = step
+    monkeypatch.setattr(executor.torch.cuda, "synchronize", no_memory)
+    with pytest.raises(RuntimeError, match="out of memory"):
+        dec.run(2)
+    assert lengths == [5] and dec.logits == 1 and cache.length == 6
+    dec.use_graph = False
+    dec.run(2)
+    assert lengths == [5, 6, 7] and cache.length == 8
