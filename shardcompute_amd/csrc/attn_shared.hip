@@ -37,6 +37,7 @@ using f4 = dma::f4;
 constexpr int SA_COLS = 128, SA_KB = 64, SA_THREADS = 256;
 constexpr int SA_AHEAD = 4;                              // operand reads in flight ahead of the MFMAs
 constexpr int SA_MAX_SEQ = 2048;         // attn_own keeps two numbers of each in LDS
+constexpr int SA_CU_LDS = 160 * 1024;    // of a CU
 
 struct SaArgs {
     const uint16_t *q;
@@ -519,9 +520,9 @@ template <int D, bool ONE>
 __device__ __forceinline__ void attn_own(const SaArgs &a, int wg, uint8_t *smem) {
     constexpr int U = D / 32, DT = D / 16;
     using Gm = SaGeo<D>;
-    // behind the ring, of every sequence: its first row (and the rows' number), and its keys;
-    // in the ring, before it is used: the sequences' first blocks and units
-    int32_t *first_row = reinterpret_cast<int32_t *>(smem + Gm::LDS), *keys = first_row + a.R + 1;
+    // behind the ring, of every sequence: its first row, and its keys; in the ring, before it
+    // is used: the sequences' first blocks and units
+    int32_t *first_row = reinterpret_cast<int32_t *>(smem + Gm::LDS), *keys = first_row + a.R;
     int32_t *off = reinterpret_cast<int32_t *>(smem), *unit = off + a.R, *wsum = unit + a.R;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
@@ -558,7 +559,6 @@ __device__ __forceinline__ void attn_own(const SaArgs &a, int wg, uint8_t *smem)
             u_before += wsum[4 + i];
         }
         if (r < a.R) { off[r] = tb + ts - t; unit[r] = ub + us - u; }
-        if (tid == 0 && r0 == 0) first_row[a.R] = rows;
         __syncthreads();
     }
     if (wg == 0) {
@@ -598,7 +598,7 @@ __device__ __forceinline__ void attn_own(const SaArgs &a, int wg, uint8_t *smem)
         for (;; ++r, in_seq = 0) {
             first = __builtin_amdgcn_readfirstlane(first_row[r]);
             len = __builtin_amdgcn_readfirstlane(keys[r]);
-            n = __builtin_amdgcn_readfirstlane(first_row[r + 1]) - first;
+            n = (r + 1 < a.R ? __builtin_amdgcn_readfirstlane(first_row[r + 1]) : rows) - first;
             if (n > a.small_rows) n = 0;
             kt = own_keyblocks(len);
             ct = own_coltiles(n, a.G);
@@ -1003,7 +1003,10 @@ SaPlan plan_shared(long N, long R, long H, long Hkv, long D, long own_cap, long 
 
 template <int D>
 int run_shared(const SaArgs &a, const SaPlan &p, hipStream_t stream) {
-    const int lds = SaGeo<D>::LDS + (2 * a.R + 1) * 4;
+    const int lds = SaGeo<D>::LDS + 2 * a.R * 4;
+    // plan_shared counts on two workgroups a CU, whatever the sequences are: 2048 of up to 200
+    // positions behind 4096, 32 heads of 128 on 8, 433 us, with one a CU 480
+    static_assert(2 * (SaGeo<D>::LDS + 2 * SA_MAX_SEQ * 4) <= SA_CU_LDS, "two workgroups on a CU");
     auto kern = a.shift >= 6 ? attn_shared_kernel<D, true> : attn_shared_kernel<D, false>;
     // more than 64 KB of LDS has to be allowed, once a device
     static std::atomic<uint64_t> allowed[2];
@@ -1012,7 +1015,7 @@ int run_shared(const SaArgs &a, const SaPlan &p, hipStream_t stream) {
     const uint64_t bit = 1ull << (dev & 63);
     if (!(allowed[a.shift >= 6].load() & bit)) {
         SC_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                         SaGeo<D>::LDS + (2 * SA_MAX_SEQ + 1) * 4));
+                                         SaGeo<D>::LDS + 2 * SA_MAX_SEQ * 4));
         allowed[a.shift >= 6].fetch_or(bit);
     }
     hipLaunchKernelGGL(kern, dim3((unsigned)(a.own_wgs + a.tile_wgs)), dim3(SA_THREADS), lds, stream, a);
