@@ -379,8 +379,9 @@ int64_t sc_attention_shared_workspace_bytes(int64_t N, int64_t R, int64_t H, int
  * the truth the rows of sequences above it are unspecified).  Slots that no row attends may
  * hold anything.
  * Block numbers, lengths and row starts out of range are clamped: the result is then
- * unspecified, the access in bounds.  scale must be positive; D 64 or 128; R <= 2048, and
- * R * Hkv * (width * block_size) below 2^37 (tables of more positions than any pool has).
+ * unspecified, the access in bounds.  scale must be positive; D 64 or 128; H <= 4096,
+ * N < 2^24, N * H < 2^31, R <= 2048, and R * Hkv * (width * block_size), times
+ * ceil(H / Hkv / 64), below 2^37 (tables of more positions than any pool has).
  */
 int sc_attention_shared_bf16(const uint16_t *q, int64_t q_stride, const uint16_t *k_blocks, const uint16_t *vt_blocks,
                              int64_t n_blocks, int64_t block_size, const int32_t *row_starts, const int32_t *lengths,

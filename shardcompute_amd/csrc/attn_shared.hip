@@ -10,10 +10,15 @@
 // make it a stream of memory, many rows (a prompt) a product again.  So:
 //   attn_tile          128 columns: the prefix, then the own keys of sequences with many
 //                      rows; over several workgroups where there are few
-//   attn_own           16 columns: the own keys of sequences with few rows, the work cut
-//                      evenly over the workgroups whatever the lengths are
+//   attn_own           units of up to 64 columns: the own keys of sequences with few rows
+//                      (at most max(64 / (H / Hkv), 1), small_rows), the work cut evenly
+//                      over the workgroups whatever the lengths are
 //   attn_merge_kernel  joins the parts of a row by their softmax maxima and sums
 // Parts are fp32 (O unnormalised, maximum in log2 units, sum).
+// Scores, maxima, exponents and sums are fp32.  The probabilities are rounded to bf16 for the
+// product with v, whose matrix instructions take 16-bit operands: half a step, 2^-8 of
+// softmax |v| at most, beside the output's own 2^-8.  Against 64 bits 0.0019 to 0.0024 of the
+// output's size (rms), where one rounding of the output alone gives 0.0017.
 //
 // Pool layout as in blocks.hip: K [n_blocks, Hkv, bs, D], Vt [n_blocks, Hkv, D, bs].
 // Block numbers outside the pool are clamped into it; lengths to the tables' width and
@@ -107,7 +112,8 @@ __device__ __forceinline__ int find_seq(const SaArgs &a, int row) {
 // A key block takes its four 16-key groups from up to four cache blocks (block sizes below
 // 64) or one.
 //
-// Bound by the matrix units: 16 ragged prompts behind 4096 positions 620 us, 990 TFLOP/s.
+// Bound by the matrix units: 16 ragged prompts behind 4096 positions 617 to 651 us with the
+// card's clock, 945 to 1000 TFLOP/s.
 template <int D>
 struct SaGeo {
     static constexpr int KROW = D * 2;
@@ -510,8 +516,8 @@ __device__ __forceinline__ void attn_tile(const SaArgs &a, int id, uint8_t *smem
 // the numbers differ).
 //
 // Bound by memory.  The copies read whole cache lines, 256 bytes a K row and 128 a Vt row:
-// 5.5 TB/s (64 sequences of 4096 positions, 194 us; operands loaded straight into the
-// registers in the MFMA's order, 64 bytes of 16 rows an instruction, 250 us).
+// 5.6 TB/s (64 sequences of 4096 positions, no prefix, 191 us; operands loaded straight into
+// the registers in the MFMA's order, 64 bytes of 16 rows an instruction, 250 us).
 static_assert(SA_KB == 64, "own_keyblocks counts blocks of 64 keys");
 
 typedef __attribute__((__vector_size__(4 * sizeof(short)))) short s16x4_t;
@@ -529,7 +535,8 @@ __device__ __forceinline__ void attn_own(const SaArgs &a, int wg, uint8_t *smem)
     const int rows = live_rows(a);
 
     // a short burst between two waits, beside a column tile's waves that always have work: it
-    // goes first (64 rows behind 8192 positions 61.0 -> 58.8 us, 24 x 5 rows 24.4 -> 23.0)
+    // goes first (64 rows of up to 1023 own positions behind 8192 61.0 -> 58.8 us, host-timed;
+    // 24 x 5 rows 24.4 -> 23.0)
     if (!a.any_big) __builtin_amdgcn_s_setprio(2);
 
     int t_before = 0, u_before = 0;
@@ -648,8 +655,8 @@ __device__ __forceinline__ void attn_own(const SaArgs &a, int wg, uint8_t *smem)
     bf16x8_t qv[U];
     // Of this lane's column: the exponents' reference (m = -inf: no key seen yet, 0 taken).  It
     // follows the maximum only when that is more than LAG above, so that most blocks spare
-    // the two exchanges and the scaling of O: 64 rows behind 8192 61.8 -> 60.0 us, 24 x 5 rows
-    // 24.7 -> 24.1
+    // the two exchanges and the scaling of O: 64 rows of up to 1023 own positions behind 8192
+    // 61.8 -> 60.0 us, host-timed, 24 x 5 rows 24.7 -> 24.1
     constexpr float LAG = 8.f;
     float m = -INFINITY, ref = 0.f, lsum = 0.f;
     f4 o[DT];
@@ -808,8 +815,8 @@ __global__ void __launch_bounds__(SA_THREADS) __attribute__((amdgpu_waves_per_eu
 // AHEAD parts on their way together.
 // 64 rows of 32 heads behind 8192 positions: 7.5 us.
 // Few rows (up to four a CU): WPR = 4, a workgroup a row and q head, its waves taking the parts
-// in turn: 8 rows of 32 heads behind 32768 positions 40 us in all, 42 with one wave; but 64
-// rows behind 2048 39 us, 34 with one.
+// in turn: 8 rows of 32 heads, up to 300 own positions, behind 32768 33 us in all, 35 with one
+// wave; but 64 rows, up to 1023 own, behind 2048 45 us, 40 with one.
 template <int D, int WPR>
 __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_parts, int by_seq) {
     constexpr int PER = D / 64;
@@ -922,14 +929,16 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
 
 // Into how many workgroups a column tile's key blocks are cut (wgs: workgroups without a cut).
 // A key block takes a workgroup alone on its CU 1.5 us, 2.1 us where two share it, further
-// ones wait (head_dim 128, measured: 300 rows behind 30000 positions 222 us in 3 pieces of 80
-// workgroups, 16 prompts 633 us in 2117 workgroups of 72 blocks; head_dim 64 ~0.8 of it, the
-// softmax is the same), and the keys come at 5.3 TB/s at most; a row's part is written and read
-// at about 2.5 TB/s and lengthens the merge by 0.06 us; at 1.3 TB/s where no tile takes own
-// keys (last_is_whole false), which then come by themselves beside it (200 rows behind 1000
-// positions 82 us, at 2.5 96, 64 rows behind 2048 35.5 and 38.5; but 300 rows of a prompt
-// behind 8000 80 us at 1.3, 69 at 2.5).  The sum is least at the count returned: 16 rows
-// behind 65536 positions 66 us (in 32), 86 at 24; 768 rows behind 2048 71 us (whole), 86 in 2.
+// ones wait (head_dim 128, measured: 300 rows behind 30000 positions 199 to 222 us in 3 pieces
+// of 80 workgroups, 16 prompts 633 us in 2117 workgroups of 72 blocks; head_dim 64 ~0.8 of it,
+// the softmax is the same), and the keys come at 5.3 TB/s at most; a row's part is written and
+// read at about 2.5 TB/s and lengthens the merge by 0.06 us; at 1.3 TB/s where no tile takes own
+// keys (last_is_whole false), which then come by themselves beside it.  Measured, 32 heads of
+// 128 on 8: 200 rows of up to 500 own positions behind 1000 60 us, at 2.5 69; 64 of up to 1023
+// behind 2048 40.3 and 41.5; but 300 rows of a prompt behind 8000 77 us at 1.3, 64 at 2.5.  The
+// sum is least at the count returned: 16 rows of up to 300 own positions behind 65536 58 us (in
+// 31), 65 in 24, 64 in 64; a prompt's 768 rows behind 2048 60 us (whole), 62 in 2.  64 pieces are
+// what the merge's lanes take in one round; more have not been measured.
 int tile_splits(long wgs, long blocks, long Hkv, long D, double part_bytes, bool last_is_whole, long cus) {
     const double stream = (double)Hkv * blocks * SA_KB * D * 4 / 5.3e6;
     int best = 1;
@@ -973,10 +982,10 @@ SaPlan plan_shared(long N, long R, long H, long Hkv, long D, long own_cap, long 
     if (coltiles > R + cols / 64) coltiles = R + cols / 64;
     const long keyblocks = coltiles * ((own_cap + SA_KB - 1) / SA_KB);
     // Equal runs of key blocks over what the column tiles leave of two workgroups a CU, so that
-    // one round holds all (64 rows behind 2048 positions, 128 tile workgroups: 119 us with 384
-    // here, 123 with 256 or 512), but at least one a CU (128 rows behind 8192, 256 tile
-    // workgroups: 71 us, 77 with two a CU).  Where tiles take own keys as well they end at
-    // different times, and two a CU fill in (the mixed batch 72 us, 75 with one)
+    // one round holds all (64 rows of up to 1023 own positions behind 2048, 64 tile workgroups:
+    // 40 us with 448 here, 47 with 256 or 512), but at least one a CU (128 such rows behind 8192,
+    // 256 tile workgroups: 87 us, 95 with two a CU).  Where tiles take own keys as well they end
+    // at different times, and two a CU fill in (the mixed batch 70 us, 72 with one)
     long ow = p.use_tile && !p.any_big ? 2 * cus - wgs * p.nsplit : 2 * cus;
     if (ow < cus) ow = cus;
     if (ow > Hkv * keyblocks) ow = Hkv * keyblocks;

@@ -27,7 +27,8 @@ namespace {
 // one pass (block_step_kernel: every sum in one exchange between the waves, a decoded
 // token's slot from registers); more go through in chunks, three times (block_step_many_kernel).
 // One decoded sequence 2.3 us, 256 with 32 of them starting anew 5.0; 512 prompts of up to
-// 700 positions, 180 thousand rows, 4.3 + 6.1.
+// 700 positions, 180 thousand rows, 4.3 + 6.1.  With the host's call 1024 decoded sequences
+// 9.7 us, 2048 15.
 constexpr int STEP_THREADS = 1024;
 constexpr int STEP_ROWS = 4096;
 
@@ -413,7 +414,8 @@ __global__ void __launch_bounds__(256) block_rows_kernel(StepArgs a) {
 // sequence are consecutive slots within a block); rows that no whole piece covers,
 // single decoded tokens among them, in 2-byte stores.  24 prompts, 8.6 thousand rows of 32 + 4 + 4
 // heads of 64: 18 us, 4.9 TB/s.  Single rows are bound by their values' cache lines, D of
-// them a row and kv head: 2048 rows of 8 kv heads of 128 111 us.
+// them a row and kv head: 2048 rows of 8 kv heads of 128 111 us where no cache holds those lines
+// (blocks of 64), 38 where one does.
 struct RopeBlocksArgs {
     const uint16_t *qkv;
     long qkv_stride;
