@@ -102,12 +102,11 @@ __global__ void __launch_bounds__(STEP_THREADS) block_step_kernel(StepArgs a) {
     const int old = gone ? 0 : len;
     int last = 0;                                              // the block an unfilled last one goes on in
     if (old & (bs - 1)) last = table[old >> a.shift];
-    enum { FLAG_TABLE = STEP_NO_TABLE, FLAG_ROWS = STEP_NO_ROWS, FLAG_MANY = 256 };
+    enum { FLAG_TABLE = STEP_NO_TABLE, FLAG_MANY = 256 };
     int flags = 0;
     if ((long)old + fresh > most) flags |= FLAG_TABLE;
-    else if (fresh > a.rows) flags |= FLAG_ROWS;
     if (fresh > 1) flags |= FLAG_MANY;
-    if (flags & (FLAG_TABLE | FLAG_ROWS)) fresh = 0;           // (the step is refused)
+    if (flags & FLAG_TABLE) fresh = 0;                         // (the step is refused; in 32 bits from here)
     const int have = (old + bs - 1) >> a.shift, need = ((old + fresh + bs - 1) >> a.shift) - have;
     Sums x = {gone ? (len + bs - 1) >> a.shift : 0, need, fresh};
     const Sums mine = x;
@@ -138,7 +137,7 @@ __global__ void __launch_bounds__(STEP_THREADS) block_step_kernel(StepArgs a) {
     }
     const int stack = min(max(n_free, 0), a.cap);
     const long top = (long)stack + all.back;
-    int bad = flags & (FLAG_TABLE | FLAG_ROWS);
+    int bad = flags & FLAG_TABLE;
     if (all.fresh > a.rows) bad |= STEP_NO_ROWS;
     if (all.need > top) bad |= STEP_NO_BLOCKS;
     if (top > a.cap) bad |= STEP_NO_STACK;

@@ -104,6 +104,20 @@ def test_tables_refused_step_changes_nothing(device, what, R):
     assert ok.status.item() == bit and ok.lengths.tolist() == lengths
 
 
+@pytest.mark.parametrize("R", [1, 3, 1500])
+def test_tables_refused_step_names_every_reason(device, R):
+    """One sequence with more positions than rows and more blocks than the stack holds."""
+    bs, width, rows = 16, 80, 10
+    tables, free = [[-1] * width for _ in range(R)], list(range(40))
+    new = [1000] + [0] * (R - 1)
+    plain = PlainTables([0] * R, tables, free, 2, len(free), bs)
+    plain.step(new, rows)
+    out = _lib.block_tables(i32([0] * R), i32(new), i32(tables), i32(free), i32([2]), bs, rows)
+    assert out.status.item() == plain.status == _lib.BLOCKS_NO_ROWS | _lib.BLOCKS_NO_BLOCKS
+    assert out.slots.tolist() == [-1] * rows and out.row_starts.tolist() == [0] * (R + 1)
+    assert out.lengths.tolist() == [0] * R and out.n_free.item() == 2
+
+
 # ---------------------------------------------------------------- rotation and append
 
 # rows of each sequence, positions before them, block size, heads; single rows, runs at the edges
