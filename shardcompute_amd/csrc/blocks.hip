@@ -601,7 +601,7 @@ int launch_block_tables(const int32_t *lengths, const int32_t *fresh, const uint
     if (R <= 0 || R > 65536) return set_error(SC_EINVAL, "block_tables: %ld sequences (1 to 65536)", R);
     if (width <= 0 || width * bs >= (1L << 30)) return set_error(SC_EINVAL, "block_tables: bad table width %ld", width);
     if (cap <= 0 || cap * bs >= (1L << 31)) return set_error(SC_EINVAL, "block_tables: bad stack size %ld", cap);
-    if (rows < 0 || rows >= (1L << 30)) return set_error(SC_EINVAL, "block_tables: bad row count %ld", rows);
+    if (rows < 0 || rows >= STEP_MOST) return set_error(SC_EINVAL, "block_tables: bad row count %ld", rows);
     StepArgs a;
     a.lengths = lengths; a.fresh = fresh; a.release = release; a.tables = tables; a.free_blocks = free_blocks;
     a.n_free = n_free; a.prefix_len = prefix_len; a.lengths_out = lengths_out; a.n_free_out = n_free_out;

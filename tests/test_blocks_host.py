@@ -143,3 +143,10 @@ def test_rotary_tables_reach_every_position_a_table_has_room_for(max_length, max
     kv = BlockBatch(c, step, c.tables, 1, 1, False)[0]
     attention.ParallelAttention.attend_qkv(att, torch.zeros((1, 8 * 64), dtype=torch.bfloat16), 1, 1, kv)
     assert seen[0] >= max_prefix + room
+
+
+@pytest.mark.parametrize("rows", [(1 << 30) - 1, 1 << 30, 1 << 40])
+def test_more_rows_than_the_sums_count_are_refused(rows):
+    """Sums of new positions saturate at 2^30 - 1: only row counts below that can tell a step that
+    does not fit."""
+    assert _tables(rows=rows) == -1 and "row count" in _lib.load().sc_last_error().decode()
