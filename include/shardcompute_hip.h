@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define SC_ABI_VERSION 14
+#define SC_ABI_VERSION 15
 
 /* Kernel selection for sc_qmm_bf16_path. */
 #define SC_QMM_PATH_AUTO 0 /* M <= 16: GEMV or band kernel (8-16 rows, by shape);
@@ -389,6 +389,54 @@ int sc_attention_shared_bf16(const uint16_t *q, int64_t q_stride, const uint16_t
                              const int32_t *prefix_len, uint16_t *out, int64_t out_stride, int64_t N, int64_t R,
                              int64_t H, int64_t Hkv, int64_t D, float scale, int64_t max_new, void *workspace,
                              int64_t workspace_bytes, void *hip_stream);
+
+/* ------------------------------------------------------------------------------
+ * The cache in blocks held in 4 or 8 bits: keys and values as codes in groups of 64 dims
+ * with a bf16 scale and bias each, value = scale * code + bias, the affine format of the
+ * quantized weights.  Tables, slots, row starts and lengths as above (sc_block_tables_i32).
+ *
+ * Pool per layer: [n_blocks, Hkv, block_size / 16, sc_kv_cell_bytes(D, bits)] bytes, 16-byte
+ * aligned: 4.5 or 8.5 bits a value (a cell of 16 positions of a kv head: 2304 or 4352 bytes
+ * at D 128, 1152 or 2176 at D 64; how it lies is the library's, csrc/kv_cells.h).  Zeroed
+ * memory holds zeros.  A slot holds what sc_rope_append_quantized_bf16 last wrote there.
+ * ---------------------------------------------------------------------------- */
+
+/* Bytes of 16 positions of one kv head (D 64 or 128, bits 4 or 8; 0: not supported). */
+int64_t sc_kv_cell_bytes(int64_t D, int bits);
+
+/*
+ * sc_rope_append_blocks_bf16 into a quantized pool: q and the rotation alike, bit for bit;
+ * the rotated k (rounded to bf16) and v of row t are quantized as sc_quantize_affine quantizes
+ * a weight row, and written to slot slots[t].  A group with a value that is not finite stands
+ * for values of which none is.  Same conditions; the pool 16-byte aligned.
+ */
+int sc_rope_append_quantized_bf16(const uint16_t *qkv, int64_t qkv_stride, uint16_t *q_out, int64_t q_stride, int64_t N,
+                                  int64_t H, int64_t Hkv, int64_t D, const float *cos_t, const float *sin_t,
+                                  int64_t table_len, uint8_t *pool, int64_t n_blocks, int64_t block_size, int bits,
+                                  const int32_t *slots, const int32_t *positions, void *hip_stream);
+
+/*
+ * k_out, v_out [n, Hkv, D] bf16 (16-byte aligned): bf16(scale * code + bias) of the positions
+ * at slots[n], as sc_dequantize_bf16; 0 for a slot outside the pool.  A slot may come up more
+ * than once.  For a cache's keys and values in the reference's layout
+ * (src/shardcompute/parallel/attention.py:429-433).
+ */
+int sc_read_quantized_bf16(const uint8_t *pool, int64_t n_blocks, int64_t block_size, int bits, int64_t Hkv, int64_t D,
+                           const int32_t *slots, int64_t n, uint16_t *k_out, uint16_t *v_out, void *hip_stream);
+
+/*
+ * sc_attention_shared_bf16 over a quantized pool: the same rows, tables, prefix, clamping and
+ * limits, keys and values being scale * code + bias (their magnitudes below 2^100).  Slots that
+ * no row attends may hold anything.
+ */
+int64_t sc_attention_quantized_workspace_bytes(int64_t N, int64_t R, int64_t H, int64_t Hkv, int64_t D, int64_t own_cap,
+                                               int64_t prefix_cap, int64_t max_new, int bits);
+int sc_attention_quantized_bf16(const uint16_t *q, int64_t q_stride, const uint8_t *pool, int64_t n_blocks,
+                                int64_t block_size, int bits, const int32_t *row_starts, const int32_t *lengths,
+                                const int32_t *tables, int64_t width, const int32_t *prefix_table, int64_t prefix_width,
+                                const int32_t *prefix_len, uint16_t *out, int64_t out_stride, int64_t N, int64_t R,
+                                int64_t H, int64_t Hkv, int64_t D, float scale, int64_t max_new, void *workspace,
+                                int64_t workspace_bytes, void *hip_stream);
 
 /* Bytes of workspace sc_attention_bf16 needs for these sizes (0: none). */
 int64_t sc_attention_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t T_cap);

@@ -15,7 +15,7 @@ import torch
 
 from .build import LIB_PATH
 
-ABI_VERSION = 14
+ABI_VERSION = 15
 PATH_AUTO, PATH_GEMV, PATH_GEMM, PATH_BAND = 0, 1, 2, 3
 
 # Exported symbols (must match include/shardcompute_hip.h).
@@ -45,6 +45,11 @@ EXPORTS = (
     "sc_rope_append_blocks_bf16",
     "sc_attention_shared_workspace_bytes",
     "sc_attention_shared_bf16",
+    "sc_kv_cell_bytes",
+    "sc_rope_append_quantized_bf16",
+    "sc_read_quantized_bf16",
+    "sc_attention_quantized_workspace_bytes",
+    "sc_attention_quantized_bf16",
     "sc_attention_workspace_bytes",
     "sc_attention_bf16",
     "sc_attention_masked_bf16",
@@ -141,6 +146,18 @@ def load():
         lib.sc_attention_shared_bf16.argtypes = [p, i64, p, p, i64, i64, p, p, p, i64, p, i64, p, p, i64, i64, i64, i64,
                                                  i64, i64, f32, i64, p, i64, p]
         lib.sc_attention_shared_bf16.restype = i32
+        lib.sc_kv_cell_bytes.argtypes = [i64, i32]
+        lib.sc_kv_cell_bytes.restype = i64
+        lib.sc_rope_append_quantized_bf16.argtypes = [p, i64, p, i64, i64, i64, i64, i64, p, p, i64, p, i64, i64, i32, p,
+                                                      p, p]
+        lib.sc_rope_append_quantized_bf16.restype = i32
+        lib.sc_read_quantized_bf16.argtypes = [p, i64, i64, i32, i64, i64, p, i64, p, p, p]
+        lib.sc_read_quantized_bf16.restype = i32
+        lib.sc_attention_quantized_workspace_bytes.argtypes = [i64] * 8 + [i32]
+        lib.sc_attention_quantized_workspace_bytes.restype = i64
+        lib.sc_attention_quantized_bf16.argtypes = [p, i64, p, i64, i64, i32, p, p, p, i64, p, i64, p, p, i64, i64, i64,
+                                                    i64, i64, i64, f32, i64, p, i64, p]
+        lib.sc_attention_quantized_bf16.restype = i32
         lib.sc_attention_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i64]
         lib.sc_attention_workspace_bytes.restype = i64
         lib.sc_attention_bf16.argtypes = [p, i64, p, p, i64, p, p, i64, i64, i64, i64, i64, i64, f32, p, i64, p]
@@ -955,6 +972,17 @@ def _row_matrix(t, cols, name, dev):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _rope_tables(cos_t, sin_t, D, dev):
+    """Positions of the rotary tables."""
+    ts = cos_t.shape
+    if (cos_t.dtype is not torch.float32 or sin_t.dtype is not torch.float32 or ts != sin_t.shape
+            or len(ts) != 2 or ts[1] != D // 2 or not cos_t.is_contiguous() or not sin_t.is_contiguous()):
+        raise ValueError("cos/sin tables must be contiguous fp32 [L, D/2]")
+    if cos_t.get_device() != dev or sin_t.get_device() != dev:
+        raise RuntimeError("the tables must be on the GPU of the call's other tensors")
+    return ts[0]
+
+
 def rope_append_blocks(qkv, H, Hkv, D, cos_t, sin_t, k_blocks, vt_blocks, slots, positions, out=None):
     """RoPE of the rows qkv [N, >= (H+2Hkv)*D] for ``positions`` and append of their k and v
     at ``slots`` of the pool k_blocks [blocks, Hkv, block_size, D], vt_blocks
@@ -966,12 +994,7 @@ def rope_append_blocks(qkv, H, Hkv, D, cos_t, sin_t, k_blocks, vt_blocks, slots,
     stride, N = _row_matrix(qkv, (H + 2 * Hkv) * D, "qkv", dev), qkv.shape[0]
     nb, bs = _pool(k_blocks, vt_blocks, Hkv, D, dev)
     _i32_flat(slots, N, "slots", dev), _i32_flat(positions, N, "positions", dev)
-    ts = cos_t.shape
-    if (cos_t.dtype is not torch.float32 or sin_t.dtype is not torch.float32 or ts != sin_t.shape
-            or len(ts) != 2 or ts[1] != D // 2 or not cos_t.is_contiguous() or not sin_t.is_contiguous()):
-        raise ValueError("cos/sin tables must be contiguous fp32 [L, D/2]")
-    if cos_t.get_device() != dev or sin_t.get_device() != dev:
-        raise RuntimeError("the tables must be on the GPU of the call's other tensors")
+    length = _rope_tables(cos_t, sin_t, D, dev)
     if out is None:
         out = torch.empty((N, H * D), dtype=_BF16, device=qkv.device)
     out_stride = _row_matrix(out, H * D, "out", dev)
@@ -980,11 +1003,39 @@ def rope_append_blocks(qkv, H, Hkv, D, cos_t, sin_t, k_blocks, vt_blocks, slots,
     if N == 0:
         return out
     rc = _on_gpu(dev, lib.sc_rope_append_blocks_bf16, qkv.data_ptr(), stride, out.data_ptr(), out_stride, N, H, Hkv, D,
-                 cos_t.data_ptr(), sin_t.data_ptr(), ts[0], k_blocks.data_ptr(), vt_blocks.data_ptr(), nb, bs,
+                 cos_t.data_ptr(), sin_t.data_ptr(), length, k_blocks.data_ptr(), vt_blocks.data_ptr(), nb, bs,
                  slots.data_ptr(), positions.data_ptr())
     if rc:
         _check(rc, "sc_rope_append_blocks_bf16")
     return out
+
+
+def _attention_tables(row_starts, lengths, tables, prefix_table, prefix_len, dev):
+    """(sequences, table width, prefix table width) of an attention over blocks."""
+    if tables.dim() != 2:
+        raise ValueError("tables must be a contiguous int32 [R, width] tensor")
+    R, width = tables.shape
+    _i32_flat(tables, 0, "tables", dev), _i32_flat(lengths, R, "lengths", dev)
+    _i32_flat(row_starts, R + 1, "row_starts", dev)
+    pw = 0
+    if prefix_table is not None:
+        if prefix_len is None:
+            raise ValueError("a prefix table needs prefix_len")
+        _i32_flat(prefix_len, 1, "prefix_len", dev), _i32_flat(prefix_table, 0, "prefix_table", dev)
+        pw = prefix_table.numel()
+    return R, width, pw
+
+
+def _workspace(workspace, need, q, dev):
+    """(tensor, bytes): the caller's workspace if it is large enough, else a new one."""
+    ws_bytes = 0
+    if workspace is not None:
+        if workspace.get_device() != dev or not workspace.is_contiguous():
+            raise RuntimeError("the workspace must be contiguous and on the GPU of the call's other tensors")
+        ws_bytes = workspace.numel() * workspace.element_size()
+    if ws_bytes < need:
+        workspace, ws_bytes = torch.empty(need, dtype=torch.uint8, device=q.device), need
+    return workspace, ws_bytes
 
 
 def attention_shared_workspace_bytes(N, R, H, Hkv, D, own_cap, prefix_cap, max_new):
@@ -1008,17 +1059,7 @@ def attention_shared(q, H, Hkv, D, k_blocks, vt_blocks, row_starts, lengths, tab
     dev = _gpu_of(q)
     stride, N = _row_matrix(q, H * D, "q", dev), q.shape[0]
     nb, bs = _pool(k_blocks, vt_blocks, Hkv, D, dev)
-    if tables.dim() != 2:
-        raise ValueError("tables must be a contiguous int32 [R, width] tensor")
-    R, width = tables.shape
-    _i32_flat(tables, 0, "tables", dev), _i32_flat(lengths, R, "lengths", dev)
-    _i32_flat(row_starts, R + 1, "row_starts", dev)
-    pw = 0
-    if prefix_table is not None:
-        if prefix_len is None:
-            raise ValueError("a prefix table needs prefix_len")
-        _i32_flat(prefix_len, 1, "prefix_len", dev), _i32_flat(prefix_table, 0, "prefix_table", dev)
-        pw = prefix_table.numel()
+    R, width, pw = _attention_tables(row_starts, lengths, tables, prefix_table, prefix_len, dev)
     if out is None:
         out = torch.empty((N, H * D), dtype=_BF16, device=q.device)
     out_stride = _row_matrix(out, H * D, "out", dev)
@@ -1031,17 +1072,146 @@ def attention_shared(q, H, Hkv, D, k_blocks, vt_blocks, row_starts, lengths, tab
     if N == 0:
         return out
     need = lib.sc_attention_shared_workspace_bytes(N, R, H, Hkv, D, width * bs, pw * bs, max_new)
-    ws_bytes = 0
-    if workspace is not None:
-        if workspace.get_device() != dev or not workspace.is_contiguous():
-            raise RuntimeError("the workspace must be contiguous and on the GPU of the call's other tensors")
-        ws_bytes = workspace.numel() * workspace.element_size()
-    if ws_bytes < need:
-        workspace, ws_bytes = torch.empty(need, dtype=torch.uint8, device=q.device), need
+    workspace, ws_bytes = _workspace(workspace, need, q, dev)
     rc = _on_gpu(dev, lib.sc_attention_shared_bf16, q.data_ptr(), stride, k_blocks.data_ptr(), vt_blocks.data_ptr(), nb,
                  bs, row_starts.data_ptr(), lengths.data_ptr(), tables.data_ptr(), width,
                  prefix_table.data_ptr() if pw else None, pw, prefix_len.data_ptr() if pw else None, out.data_ptr(),
                  out_stride, N, R, H, Hkv, D, float(scale), int(max_new), _ptr(workspace), ws_bytes)
     if rc:
         _check(rc, "sc_attention_shared_bf16")
+    return out
+
+
+# ---------------------------------------------------------------- the same cache in 4 or 8 bits
+
+CACHE_BITS = (4, 8)
+_cell_bytes = {}                    # (head_dim, bits) -> bytes of a cell of 16 positions
+
+
+def _cell(D, bits):
+    n = _cell_bytes.get((D, bits))
+    if n is None:
+        if bits not in CACHE_BITS:
+            raise ValueError(f"a quantized cache holds {CACHE_BITS} bits, got {bits}")
+        n = int(load().sc_kv_cell_bytes(D, bits))
+        if n == 0:
+            raise ValueError(f"a quantized cache needs head_dim 64 or 128, got {D}")
+        _cell_bytes[(D, bits)] = n
+    return n
+
+
+def quantized_pool_shape(n_blocks, Hkv, block_size, D, bits=4):
+    """Shape of a quantized pool's uint8 tensor: [blocks, kv heads, cells of 16 positions, bytes]."""
+    if block_size not in BLOCK_SIZES:
+        raise ValueError(f"block_size must be one of {BLOCK_SIZES}, got {block_size}")
+    return (n_blocks, Hkv, block_size // 16, _cell(D, bits))
+
+
+def quantized_pool(n_blocks, Hkv, block_size, D, bits=4, device=None):
+    """A pool of ``n_blocks`` blocks of ``block_size`` positions, keys and values in ``bits`` bits
+    (4 or 8) in groups of 64 dims with a bf16 scale and bias each, every position zero."""
+    return torch.zeros(quantized_pool_shape(n_blocks, Hkv, block_size, D, bits), dtype=torch.uint8,
+                       device="cuda" if device is None else device)
+
+
+def _quantized(pool, Hkv, D, bits, dev):
+    """(blocks, block size) of a quantized pool's layer."""
+    cell, ps = _cell(D, bits), pool.shape
+    if pool.dtype is not torch.uint8:
+        raise TypeError(f"a quantized pool must be uint8, got {pool.dtype}")
+    if len(ps) != 4 or ps[1] != Hkv or ps[3] != cell:
+        raise ValueError(f"a pool of {bits} bits must be [blocks, {Hkv}, block_size / 16, {cell}], got {tuple(ps)}")
+    if not pool.is_contiguous():
+        raise ValueError("the pool must be contiguous")
+    if 16 * ps[2] not in BLOCK_SIZES:
+        raise ValueError(f"block_size must be one of {BLOCK_SIZES}, got {16 * ps[2]}")
+    if pool.get_device() != dev:
+        _gpu_of(pool)
+        raise RuntimeError("the pool must be on the GPU of the call's other tensors")
+    return ps[0], 16 * ps[2]
+
+
+def rope_append_quantized(qkv, H, Hkv, D, cos_t, sin_t, pool, slots, positions, bits=4, out=None):
+    """``rope_append_blocks`` into a quantized pool: RoPE of the rows qkv [N, >= (H+2Hkv)*D] for
+    ``positions``, their k and v quantized as ``quantize`` does (after the rotated k's rounding to
+    bf16) and written at ``slots``.  Returns the rotated q [N, H*D] (``out`` when given; it may be
+    the q part of qkv).  Rows whose slot is outside the pool (-1) or whose position is outside
+    the tables are left alone.  The slots of different rows must differ."""
+    lib = load()
+    dev = _gpu_of(qkv)
+    stride, N = _row_matrix(qkv, (H + 2 * Hkv) * D, "qkv", dev), qkv.shape[0]
+    nb, bs = _quantized(pool, Hkv, D, bits, dev)
+    _i32_flat(slots, N, "slots", dev), _i32_flat(positions, N, "positions", dev)
+    length = _rope_tables(cos_t, sin_t, D, dev)
+    if out is None:
+        out = torch.empty((N, H * D), dtype=_BF16, device=qkv.device)
+    out_stride = _row_matrix(out, H * D, "out", dev)
+    if out.shape != (N, H * D):
+        raise ValueError(f"out must be [{N}, {H * D}], got {tuple(out.shape)}")
+    if N == 0:
+        return out
+    rc = _on_gpu(dev, lib.sc_rope_append_quantized_bf16, qkv.data_ptr(), stride, out.data_ptr(), out_stride, N, H, Hkv, D,
+                 cos_t.data_ptr(), sin_t.data_ptr(), length, pool.data_ptr(), nb, bs, bits, slots.data_ptr(),
+                 positions.data_ptr())
+    if rc:
+        _check(rc, "sc_rope_append_quantized_bf16")
+    return out
+
+
+def read_quantized(pool, Hkv, D, slots, bits=4):
+    """(k, v) bf16 [n, Hkv, D] of the positions at ``slots`` [n] int32 of a quantized pool:
+    bf16(scale * code + bias); 0 for a slot outside the pool (-1)."""
+    lib = load()
+    dev = _gpu_of(pool)
+    nb, bs = _quantized(pool, Hkv, D, bits, dev)
+    n = slots.numel()
+    _i32_flat(slots, n, "slots", dev)
+    k = torch.empty((n, Hkv, D), dtype=_BF16, device=pool.device)
+    v = torch.empty_like(k)
+    rc = _on_gpu(dev, lib.sc_read_quantized_bf16, pool.data_ptr(), nb, bs, bits, Hkv, D, slots.data_ptr(), n,
+                 k.data_ptr(), v.data_ptr())
+    if rc:
+        _check(rc, "sc_read_quantized_bf16")
+    return k, v
+
+
+def attention_quantized_workspace_bytes(N, R, H, Hkv, D, own_cap, prefix_cap, max_new, bits=4):
+    """Workspace of ``attention_quantized`` for N rows of R sequences; ``own_cap`` and
+    ``prefix_cap``: positions the tables have room for."""
+    return int(load().sc_attention_quantized_workspace_bytes(N, R, H, Hkv, D, own_cap, prefix_cap, max_new, bits))
+
+
+def attention_quantized(q, H, Hkv, D, pool, row_starts, lengths, tables, scale, bits=4, prefix_table=None,
+                        prefix_len=None, max_new=None, out=None, workspace=None):
+    """``attention_shared`` over a quantized pool: the rows ``row_starts[r] .. row_starts[r + 1] - 1``
+    of q [N, >= H*D] are sequence r's new positions, the last of its ``lengths[r]`` own ones; each
+    attends the ``prefix_len[0]`` positions of ``prefix_table`` and its own sequence up to itself.
+    ``max_new``: an upper bound of the rows of one sequence (default N).  Returns out [N, H*D]
+    bf16; rows past the last sequence's are left as they were.  ``workspace``: a contiguous tensor
+    of at least ``attention_quantized_workspace_bytes`` (a smaller one, or none, and one is
+    allocated)."""
+    lib = load()
+    dev = _gpu_of(q)
+    stride, N = _row_matrix(q, H * D, "q", dev), q.shape[0]
+    nb, bs = _quantized(pool, Hkv, D, bits, dev)
+    R, width, pw = _attention_tables(row_starts, lengths, tables, prefix_table, prefix_len, dev)
+    if out is None:
+        out = torch.empty((N, H * D), dtype=_BF16, device=q.device)
+    out_stride = _row_matrix(out, H * D, "out", dev)
+    if out.shape != (N, H * D):
+        raise ValueError(f"out must be [{N}, {H * D}], got {tuple(out.shape)}")
+    if max_new is None:
+        max_new = N
+    elif max_new < 0:
+        raise ValueError("max_new must not be negative")
+    if N == 0:
+        return out
+    need = lib.sc_attention_quantized_workspace_bytes(N, R, H, Hkv, D, width * bs, pw * bs, max_new, bits)
+    workspace, ws_bytes = _workspace(workspace, need, q, dev)
+    rc = _on_gpu(dev, lib.sc_attention_quantized_bf16, q.data_ptr(), stride, pool.data_ptr(), nb, bs, bits,
+                 row_starts.data_ptr(), lengths.data_ptr(), tables.data_ptr(), width,
+                 prefix_table.data_ptr() if pw else None, pw, prefix_len.data_ptr() if pw else None, out.data_ptr(),
+                 out_stride, N, R, H, Hkv, D, float(scale), int(max_new), _ptr(workspace), ws_bytes)
+    if rc:
+        _check(rc, "sc_attention_quantized_bf16")
     return out

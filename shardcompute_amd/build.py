@@ -22,7 +22,7 @@ ARCH = os.environ.get("SC_OFFLOAD_ARCH", "gfx950")
 SOURCES = ["abi.hip", "qgemv_dma.hip", "qgemv_m1.hip", "qgemv16.hip", "qgemv.hip", "qgemm.hip",
            "qgemm_dense.hip", "qgemm_mid.hip", "qgemm_band.hip", "gather.hip",
            "quant.hip", "decode.hip", "attn_prefill.hip", "decode_step.hip", "act.hip", "blocks.hip",
-           "attn_shared.hip"]
+           "attn_shared.hip", "kv_quant.hip", "attn_quant.hip"]
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",
@@ -36,12 +36,13 @@ HIPCC_FLAGS = [
     "-I", os.path.join(ROOT, "include"),
 ]
 
-# per-source additions: the prefill attention kernels keep their MFMA accumulators in
+# per-source additions: the attention kernels over a cache keep their MFMA accumulators in
 # VGPRs (they rescale them in place every few blocks; in AGPRs each block would copy
 # them to VGPRs and back)
 EXTRA_FLAGS = {
     "attn_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "attn_shared.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "attn_quant.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -8,6 +8,7 @@
 #include <mutex>
 
 #include "sc_common.h"
+#include "kv_cells.h"
 #include "../../include/shardcompute_hip.h"
 
 namespace sc {
@@ -74,6 +75,19 @@ int launch_rope_append_blocks(const uint16_t *qkv, long qkv_stride, uint16_t *q,
                               hipStream_t stream);
 long attention_shared_workspace_bytes(long N, long R, long H, long Hkv, long D, long own_cap, long prefix_cap,
                                       long max_new);
+int launch_rope_append_quantized(const uint16_t *qkv, long qkv_stride, uint16_t *q, long q_stride, long N, long H,
+                                 long Hkv, long D, const float *cos_t, const float *sin_t, long table_len,
+                                 uint8_t *pool, long n_blocks, long bs, int bits, const int32_t *slots,
+                                 const int32_t *positions, hipStream_t stream);
+int launch_read_quantized(const uint8_t *pool, long n_blocks, long bs, int bits, long Hkv, long D,
+                          const int32_t *slots, long n, uint16_t *k, uint16_t *v, hipStream_t stream);
+long attention_quantized_workspace_bytes(long N, long R, long H, long Hkv, long D, long own_cap, long prefix_cap,
+                                         long max_new, int bits);
+int launch_attention_quantized(const uint16_t *q, long q_stride, const uint8_t *pool, long n_blocks, long bs, int bits,
+                               const int32_t *row_starts, const int32_t *lengths, const int32_t *tables, long width,
+                               const int32_t *prefix_table, long prefix_width, const int32_t *prefix_len, uint16_t *out,
+                               long out_stride, long N, long R, long H, long Hkv, long D, float scale, long max_new,
+                               void *workspace, long workspace_bytes, hipStream_t stream);
 int launch_attention_shared(const uint16_t *q, long q_stride, const uint16_t *kc, const uint16_t *vt, long n_blocks,
                             long bs, const int32_t *row_starts, const int32_t *lengths, const int32_t *tables,
                             long width, const int32_t *prefix_table, long prefix_width, const int32_t *prefix_len,
@@ -507,6 +521,39 @@ int sc_attention_shared_bf16(const uint16_t *q, int64_t q_stride, const uint16_t
                                    width, prefix_table, prefix_width, prefix_len, out, out_stride, N, R, H, Hkv, D,
                                    scale, max_new, workspace, workspace_bytes,
                                    reinterpret_cast<hipStream_t>(hip_stream));
+}
+
+int64_t sc_kv_cell_bytes(int64_t D, int bits) { return kv_cell_bytes(D, bits); }
+
+int sc_rope_append_quantized_bf16(const uint16_t *qkv, int64_t qkv_stride, uint16_t *q_out, int64_t q_stride, int64_t N,
+                                  int64_t H, int64_t Hkv, int64_t D, const float *cos_t, const float *sin_t,
+                                  int64_t table_len, uint8_t *pool, int64_t n_blocks, int64_t block_size, int bits,
+                                  const int32_t *slots, const int32_t *positions, void *hip_stream) {
+    return launch_rope_append_quantized(qkv, qkv_stride, q_out, q_stride, N, H, Hkv, D, cos_t, sin_t, table_len, pool,
+                                        n_blocks, block_size, bits, slots, positions,
+                                        reinterpret_cast<hipStream_t>(hip_stream));
+}
+
+int sc_read_quantized_bf16(const uint8_t *pool, int64_t n_blocks, int64_t block_size, int bits, int64_t Hkv, int64_t D,
+                           const int32_t *slots, int64_t n, uint16_t *k_out, uint16_t *v_out, void *hip_stream) {
+    return launch_read_quantized(pool, n_blocks, block_size, bits, Hkv, D, slots, n, k_out, v_out,
+                                 reinterpret_cast<hipStream_t>(hip_stream));
+}
+
+int64_t sc_attention_quantized_workspace_bytes(int64_t N, int64_t R, int64_t H, int64_t Hkv, int64_t D, int64_t own_cap,
+                                               int64_t prefix_cap, int64_t max_new, int bits) {
+    return attention_quantized_workspace_bytes(N, R, H, Hkv, D, own_cap, prefix_cap, max_new, bits);
+}
+
+int sc_attention_quantized_bf16(const uint16_t *q, int64_t q_stride, const uint8_t *pool, int64_t n_blocks,
+                                int64_t block_size, int bits, const int32_t *row_starts, const int32_t *lengths,
+                                const int32_t *tables, int64_t width, const int32_t *prefix_table, int64_t prefix_width,
+                                const int32_t *prefix_len, uint16_t *out, int64_t out_stride, int64_t N, int64_t R,
+                                int64_t H, int64_t Hkv, int64_t D, float scale, int64_t max_new, void *workspace,
+                                int64_t workspace_bytes, void *hip_stream) {
+    return launch_attention_quantized(q, q_stride, pool, n_blocks, block_size, bits, row_starts, lengths, tables, width,
+                                      prefix_table, prefix_width, prefix_len, out, out_stride, N, R, H, Hkv, D, scale,
+                                      max_new, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(hip_stream));
 }
 
 int64_t sc_attention_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t T_cap) {

@@ -1,0 +1,103 @@
+"""Refusals of the quantized cache's entry points (argument checks only, no GPU calls)."""
+import os
+
+import pytest
+import torch
+
+from shardcompute_amd import _lib
+from shardcompute_amd.build import LIB_PATH
+
+pytestmark = pytest.mark.skipif(not os.path.exists(LIB_PATH), reason="library not built")
+A = 1 << 12                     # a 16-byte aligned address nothing reads
+
+
+def _append(**kw):
+    a = dict(qkv=A, qkv_stride=1536, q=A, q_stride=1024, N=3, H=8, Hkv=2, D=128, cos=A, sin=A, length=99, pool=A,
+             n_blocks=10, bs=64, bits=4, slots=A, positions=A)
+    a.update(kw)
+    return _lib.load().sc_rope_append_quantized_bf16(*a.values(), None)
+
+
+def _read(**kw):
+    a = dict(pool=A, n_blocks=10, bs=64, bits=4, Hkv=2, D=128, slots=A, n=5, k=A, v=A)
+    a.update(kw)
+    return _lib.load().sc_read_quantized_bf16(*a.values(), None)
+
+
+def _attend(**kw):
+    a = dict(q=A, q_stride=1024, pool=A, n_blocks=10, bs=64, bits=8, row_starts=A, lengths=A, tables=A, width=4,
+             prefix_table=A, prefix_width=5, prefix_len=A, out=A, out_stride=1024, N=3, R=3, H=8, Hkv=2, D=128, scale=0.1,
+             max_new=1, workspace=A, workspace_bytes=1 << 30)
+    a.update(kw)
+    return _lib.load().sc_attention_quantized_bf16(*a.values(), None)
+
+
+@pytest.mark.parametrize("call,kw,message", [
+    (_append, dict(qkv=None), "null pointer"), (_append, dict(pool=None), "null pointer"),
+    (_append, dict(slots=None), "null pointer"), (_append, dict(D=96), "head_dim 96"), (_append, dict(bits=3), "3 bits"),
+    (_append, dict(bits=16), "16 bits"), (_append, dict(bs=20), "block size 20"), (_append, dict(bs=8), "block size 8"),
+    (_append, dict(Hkv=3), "bad shape"), (_append, dict(N=-1), "bad shape"), (_append, dict(n_blocks=0), "pool"),
+    (_append, dict(n_blocks=1 << 25), "pool"), (_append, dict(length=0), "table size"),
+    (_append, dict(qkv_stride=1528), "strides"), (_append, dict(qkv_stride=1540), "strides"),
+    (_append, dict(q_stride=1020), "strides"), (_append, dict(pool=A + 8), "aligned"), (_append, dict(cos=A + 4), "aligned"),
+    (_append, dict(N=1 << 29), "too many rows"),
+    (_read, dict(pool=None), "null pointer"), (_read, dict(k=None), "null pointer"), (_read, dict(D=32), "head_dim 32"),
+    (_read, dict(bits=2), "2 bits"), (_read, dict(bs=512), "block size 512"), (_read, dict(n=-1), "bad shape"),
+    (_read, dict(Hkv=0), "bad shape"), (_read, dict(n_blocks=0), "pool"), (_read, dict(v=A + 2), "aligned"),
+    (_read, dict(n=1 << 29), "too many rows"),
+    (_attend, dict(q=None), "null pointer"), (_attend, dict(pool=None), "null pointer"),
+    (_attend, dict(prefix_table=None), "null pointer"), (_attend, dict(prefix_len=None), "null pointer"),
+    (_attend, dict(D=80), "head_dim 80"), (_attend, dict(bits=5), "5 bits"), (_attend, dict(bs=0), "block size 0"),
+    (_attend, dict(H=9), "bad shape"), (_attend, dict(R=0), "bad shape"), (_attend, dict(R=2049), "bad shape"),
+    (_attend, dict(width=0), "bad shape"), (_attend, dict(max_new=-1), "bad shape"),
+    (_attend, dict(prefix_width=1 << 26), "bad shape"), (_attend, dict(n_blocks=0), "pool"),
+    (_attend, dict(scale=0.0), "scale"), (_attend, dict(scale=-0.1), "scale"),
+    (_attend, dict(scale=float("nan")), "scale"), (_attend, dict(scale=float("inf")), "scale"),
+    (_attend, dict(q_stride=1023), "strides"), (_attend, dict(q_stride=1028), "strides"),
+    (_attend, dict(out_stride=1000), "strides"), (_attend, dict(q=A + 8), "misaligned"),
+    (_attend, dict(out=A + 4), "misaligned"), (_attend, dict(pool=A + 4), "misaligned"),
+])
+def test_refused(call, kw, message):
+    assert call(**kw) in (-1, -2)
+    assert message in _lib.load().sc_last_error().decode()
+
+
+def test_no_rows_is_no_work():
+    assert _append(N=0, qkv=None) == 0 and _attend(N=0, q=None) == 0 and _read(n=0, k=None) == 0
+    lib = _lib.load()
+    assert lib.sc_attention_quantized_workspace_bytes(0, 3, 8, 2, 128, 256, 320, 1, 4) == 0
+    assert lib.sc_attention_quantized_workspace_bytes(5, 3, 8, 3, 128, 256, 320, 1, 4) == 0
+
+
+@pytest.mark.parametrize("D,bits", [(64, 4), (64, 8), (128, 4), (128, 8)])
+def test_a_cell_holds_the_codes_a_scale_and_a_bias_per_64_values(D, bits):
+    assert _lib.load().sc_kv_cell_bytes(D, bits) == 16 * (2 * D * bits // 8 + 2 * (D // 64) * 4)
+    assert _lib.quantized_pool_shape(5, 3, 32, D, bits) == (5, 3, 2, 16 * (2 * D * bits // 8 + 2 * (D // 64) * 4))
+
+
+def test_pools_refused():
+    with pytest.raises(ValueError, match="bits"):
+        _lib.quantized_pool_shape(5, 3, 32, 64, bits=6)
+    with pytest.raises(ValueError, match="head_dim"):
+        _lib.quantized_pool_shape(5, 3, 32, 96)
+    with pytest.raises(ValueError, match="block_size"):
+        _lib.quantized_pool_shape(5, 3, 48, 64)
+    good = torch.zeros(_lib.quantized_pool_shape(5, 3, 32, 64, 4), dtype=torch.uint8)
+    for pool, error, message in [(good.to(torch.int32), TypeError, "uint8"), (good[:, :2], ValueError, "must be"),
+                                 (good[..., :64], ValueError, "must be"), (good.transpose(0, 1).contiguous(), ValueError, "must be"),
+                                 (good[:, :, :1], ValueError, "contiguous"), (good, RuntimeError, "GPU")]:
+        with pytest.raises(error, match=message):
+            _lib._quantized(pool, 3, 64, 4, 0)
+    with pytest.raises(ValueError, match="8 bits must be"):
+        _lib._quantized(good, 3, 64, 8, 0)
+
+
+def test_wrappers_need_gpu_tensors():
+    z = torch.zeros(4, dtype=torch.int32)
+    pool = torch.zeros(_lib.quantized_pool_shape(1, 1, 16, 64), dtype=torch.uint8)
+    x = torch.zeros((4, 192), dtype=torch.bfloat16)
+    for call in (lambda: _lib.rope_append_quantized(x, 1, 1, 64, z, z, pool, z, z),
+                 lambda: _lib.read_quantized(pool, 1, 64, z),
+                 lambda: _lib.attention_quantized(x, 1, 1, 64, pool, z, z, z, 1.0)):
+        with pytest.raises(RuntimeError, match="GPU"):
+            call()
