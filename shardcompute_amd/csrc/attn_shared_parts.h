@@ -5,9 +5,11 @@
 
 namespace sc {
 
-// units of up to 64 columns of a sequence's n rows, and its blocks of 64 keys
+// units of up to 64 columns of a sequence's n rows, and its blocks of 2^shift keys
 __host__ __device__ __forceinline__ int own_coltiles(int n, int G) { return (n * G + 63) >> 6; }
-__host__ __device__ __forceinline__ int own_keyblocks(int len) { return (len + 63) / 64; }
+__host__ __device__ __forceinline__ int own_keyblocks(int len, int shift = 6) {
+    return (int)(((unsigned)len + (1u << shift) - 1) >> shift);
+}
 // blocks a workgroup takes of `total`
 __host__ __device__ __forceinline__ int own_run(int total, int wgs) {
     return total > 0 ? (total - 1) / wgs + 1 : 1;
@@ -30,12 +32,15 @@ struct OwnParts {
 // blocks of the row's unit, the four waves' or (a wide unit) that of the wave whose column
 // it is.  total: blocks of all sequences.  A row outside the sequence (row starts that begin
 // above 0 or do not ascend) has none, nor has one whose parts would not all be there.
+// shift: log2 of a block's keys; before: blocks that come before the sequence's own.
 __host__ __device__ __forceinline__ OwnParts own_parts_of(int row, int first, int n, int len, int hk, int gq, int G,
                                                           int small_rows, int off, int unit, int total, int own_wgs,
-                                                          int own_parts, int part_cols) {
+                                                          int own_parts, int part_cols, int shift = 6,
+                                                          int before = 0) {
     OwnParts p = {0, 0, 1, 0};
-    if (row < first || row >= first + n || n > small_rows || len <= 0) return p;
-    const int run = own_run(total, own_wgs), kt = own_keyblocks(len), ct = own_coltiles(n, G);
+    const int kt = before + (len > 0 ? own_keyblocks(len, shift) : 0);
+    if (row < first || row >= first + n || n > small_rows || kt <= 0) return p;
+    const int run = own_run(total, own_wgs), ct = own_coltiles(n, G);
     const int col = (row - first) * G + gq, u = hk * ct + (col >> 6);
     const int t0 = off + u * kt, w0 = t0 / run, wgs = (t0 + kt - 1) / run - w0 + 1;
     const bool wide = n * G > 16;
