@@ -25,8 +25,6 @@
 #include "attn_shared_core.h"
 #include "kv_cells.h"
 
-#include <atomic>
-
 namespace sc {
 
 namespace {
@@ -42,18 +40,32 @@ __device__ __forceinline__ const uint8_t *cell_at(const QuantArgs &a, int hk, in
     return a.pool + ((((size_t)clampi(block, 0, a.n_blocks - 1) * a.Hkv + hk) << per) + ((t >> 4) & ((1 << per) - 1))) * BYTES;
 }
 
-// lane 16 (lane / 16) + SRC's value
-template <int SRC>
-__device__ __forceinline__ float row_lane(float v) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + SRC, 0xF, 0xF, true));
+// nib_pair, the mask from a scalar and the 128s from a vector register: one instruction
+__device__ __forceinline__ bf16x8_t nibbles(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    uint32_t mask = 0x000F000Fu, one28 = 0x43004300u;
+    asm("" : "+s"(mask));
+    asm("" : "+v"(one28));
+    return as_bf16x8(dma::and_or(a, mask, one28), dma::and_or(b, mask, one28), dma::and_or(c, mask, one28), dma::and_or(d, mask, one28));
 }
 
-// What a wave reads of a cell.
+// lane 16 (lane / 16) + n's value, n below 16 and known when the loop around is unrolled
+__device__ __forceinline__ float row_lane(float v, int n) {
+    const int x = __float_as_int(v);
+#define SC_ROW_LANE(i) case i: return __int_as_float(__builtin_amdgcn_update_dpp(0, x, 0x150 + i, 0xF, 0xF, true));
+    switch (n) {
+        SC_ROW_LANE(0) SC_ROW_LANE(1) SC_ROW_LANE(2) SC_ROW_LANE(3) SC_ROW_LANE(4) SC_ROW_LANE(5) SC_ROW_LANE(6) SC_ROW_LANE(7)
+        SC_ROW_LANE(8) SC_ROW_LANE(9) SC_ROW_LANE(10) SC_ROW_LANE(11) SC_ROW_LANE(12) SC_ROW_LANE(13) SC_ROW_LANE(14)
+        default: SC_ROW_LANE(15)
+    }
+#undef SC_ROW_LANE
+}
+
+// What a wave reads of a cell's codes.
 template <int D, int BITS>
 struct CellRegs {
     using C = Cell<D, BITS>;
     static constexpr int WORDS = C::LANE / 4;
-    uint32_t k[WORDS], v[WORDS], meta;
+    uint32_t k[WORDS], v[WORDS];
     __device__ __forceinline__ void load(const uint8_t *cell, int lane) {
 #pragma unroll
         for (int p = 0; p < C::PLANES; ++p) {
@@ -67,43 +79,110 @@ struct CellRegs {
                 k[0] = x.x; k[1] = x.y; v[0] = y.x; v[1] = y.y;
             }
         }
-        // lane row g: positions 4 g .. 4 g + 3, item by item (64 dims: its lanes 8 .. 15 again)
-        constexpr int PER = 4 * C::ITEMS;
-        meta = *reinterpret_cast<const uint32_t *>(cell + 2 * C::CODES + ((lane >> 4) * PER + (lane & (PER - 1))) * 4);
     }
 };
 
-// Softmax over keys taken in, 32 at a time, for 16 columns (of which a lane has column lane & 15).
-template <int D, int BITS>
+// Softmax over keys taken in, two cells at a time, for up to CW columns.
+//
+// Of a step's sums q . code there are 2 GROUPS kinds: one of each cell and group of dims, to be
+// scaled apart.  With 16 columns each kind has a result of its own (the instruction's 16
+// columns).  With CW = 8 or 4 the columns appear 16 / CW times, as blocks, each block with the
+// q of one kind and zero in the place of the others', so that all kinds lie in one result (8
+// columns of 128 dims: one a cell) and each lane scales what its block holds: the softmax,
+// whose work is by the result, is done once for 4 keys of a lane in place of 16.
+//   lane c = lane % 16:   128 dims  CW 4: column c % 4, cell c / 4 % 2, group c / 8
+//                                   CW 8: column c % 8, group c / 8; a result a cell
+//                          64 dims  CW 8: column c % 8, cell c / 8
+// The weights P go back the same way: a block's columns of O take only the block's cell (its
+// places of operand B, the other cell's are 0) with the weights of the block's group; what a
+// block's group leaves in the other group's dims is not used, and the cells' are added at
+// the end.
+// 64 rows of up to 1023 positions of 32 heads of 128 on 8 in 4 bits: see attn_line.
+template <int D, int BITS, int CW>
 struct Columns {
     using C = Cell<D, BITS>;
-    static constexpr int DT = D / 16;
+    static constexpr int DT = D / 16, GROUPS = C::GROUPS;
+    static_assert(CW == 16 || CW == 8 || (CW == 4 && GROUPS == 2), "columns a lane row can hold");
+    static constexpr bool BY_CELL = CW * GROUPS <= 8;           // a block has one cell
+    static constexpr bool BY_GROUP = CW < 16 && GROUPS == 2;    // a block has one group
+    static constexpr int NG = BY_GROUP ? 1 : GROUPS;            // groups a lane has
+    static constexpr int NC = BY_CELL ? 1 : 2;                  // cells a lane has
+    static constexpr int NQ = (BY_CELL ? 2 : 1) * 2 * GROUPS;   // operands with q
     static constexpr float EXCESS = BITS == 4 ? 128.f : 0.f, MID = BITS == 4 ? 8.f : 128.f;
     // the exponents' reference follows the maximum only when that is more than LAG (log2) above it
     static constexpr float LAG = 8.f;
-    bf16x8_t q[2 * C::GROUPS];
-    float qsum[C::GROUPS];
-    float m, ref, lsum, corr[C::GROUPS];
-    f4 o[DT], psum[C::GROUPS];
+    // Scales and biases of a lane's 4 keys a cell: in its own registers, or (16 columns, where
+    // these would be 32) one word of each cell a lane, for its lane row: item l / 4, position 4 g + l % 4
+    static constexpr bool ROWS = CW == 16;
+    struct Own { uint4 k[NC][NG], v[NC][NG]; };
+    struct Row { uint32_t w[2]; };
+    using Meta = std::conditional_t<ROWS, Row, Own>;
+    struct Affine { float scale, bias; };
+    static __device__ __forceinline__ Affine affine(const Own &x, int j, int y, bool value, int i) {
+        const uint32_t w = dma::wc(value ? x.v[j][y] : x.k[j][y], i);
+        return {__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)};
+    }
+    static __device__ __forceinline__ Affine affine(const Row &x, int j, int y, bool value, int i) {
+        const int n = 4 * ((value ? GROUPS : 0) + y) + i;
+        return {row_lane(__uint_as_float(x.w[j] << 16), n), row_lane(__uint_as_float(x.w[j] & 0xFFFF0000u), n)};
+    }
 
+    bf16x8_t q[NQ];
+    float qsum[NG];
+    float m, ref, lsum, corr[NG];            // m: the maximum, of scores without the scale
+    f4 o[DT], psum[NG];
+    float sl, lag;                           // the scale, in log2 units; LAG without it
+
+    static __device__ __forceinline__ int cell_of(int c) { return BY_CELL ? (GROUPS == 2 ? (c >> 2) & 1 : c >> 3) : 0; }
+    static __device__ __forceinline__ int group_of(int c) { return BY_GROUP ? c >> 3 : 0; }
     static __device__ __forceinline__ bf16x8_t ones() { return as_bf16x8(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u); }
+    static __device__ __forceinline__ f4 mfma(bf16x8_t a, bf16x8_t b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    // 64 lanes' v, of lanes with the same column: the other block's (by cells)
+    static __device__ __forceinline__ float other_cell(float v) { return GROUPS == 2 ? xor4_mov(v) : dpp_mov<DPP_ROR8>(v); }
+
+    static __device__ __forceinline__ void load_meta(Own &x, const uint8_t *c0, const uint8_t *c1, int lane) {
+        const int g = lane >> 4, c = lane & 15;
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+            const uint8_t *cell = (BY_CELL ? cell_of(c) : j) ? c1 : c0;
+#pragma unroll
+            for (int y = 0; y < NG; ++y) {
+                const int grp = BY_GROUP ? group_of(c) : y;
+                x.k[j][y] = *reinterpret_cast<const uint4 *>(cell + C::meta(4 * g, grp));
+                x.v[j][y] = *reinterpret_cast<const uint4 *>(cell + C::meta(4 * g, GROUPS + grp));
+            }
+        }
+    }
+    static __device__ __forceinline__ void load_meta(Row &x, const uint8_t *c0, const uint8_t *c1, int lane) {
+        const int at = C::meta(4 * (lane >> 4) + (lane & 3), (lane >> 2) & (C::ITEMS - 1));
+        x.w[0] = *reinterpret_cast<const uint32_t *>(c0 + at);
+        x.w[1] = *reinterpret_cast<const uint32_t *>(c1 + at);
+    }
 
     // qp: this lane's column's q row (null: none)
-    __device__ __forceinline__ void open(const uint16_t *qp, int g) {
+    __device__ __forceinline__ void open(const uint16_t *qp, int lane, float scale_log2) {
+        const int g = lane >> 4, c = lane & 15;
+        sl = scale_log2;
+        lag = LAG / scale_log2;
+        f4 sum[NG];
 #pragma unroll
-        for (int s = 0; s < 2 * C::GROUPS; ++s) {
-            uint4 x = make_uint4(0u, 0u, 0u, 0u);
-            if (qp) x = *reinterpret_cast<const uint4 *>(qp + 64 * (s >> 1) + 16 * g + 8 * (s & 1));
-            q[s] = as_bf16x8(x);
-        }
+        for (int y = 0; y < NG; ++y) sum[y] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < C::GROUPS; ++j) {
-            f4 s = {0.f, 0.f, 0.f, 0.f};
-            s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones(), q[2 * j], s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones(), q[2 * j + 1], s, 0, 0, 0);
-            qsum[j] = s[0];
-            corr[j] = 0.f;
-            psum[j] = f4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < NQ / (2 * GROUPS); ++j)
+#pragma unroll
+            for (int s = 0; s < 2 * GROUPS; ++s) {
+                uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                const bool mine = (!BY_CELL || cell_of(c) == j) && (!BY_GROUP || group_of(c) == s >> 1);
+                if (qp && mine) x = *reinterpret_cast<const uint4 *>(qp + 64 * (s >> 1) + 16 * g + 8 * (s & 1));
+                q[2 * GROUPS * j + s] = as_bf16x8(x);
+                const int y = BY_GROUP ? 0 : s >> 1;
+                sum[y] = mfma(ones(), q[2 * GROUPS * j + s], sum[y]);
+            }
+#pragma unroll
+        for (int y = 0; y < NG; ++y) {
+            qsum[y] = sum[y][0];
+            corr[y] = 0.f;
+            psum[y] = f4{0.f, 0.f, 0.f, 0.f};
         }
         m = -INFINITY;
         ref = lsum = 0.f;
@@ -114,123 +193,116 @@ struct Columns {
     // The cells' positions t0 .. t0 + 15 and t1 .. t1 + 15; the column sees those up to limit
     // (EDGE; else all).
     template <bool EDGE>
-    __device__ __forceinline__ void take(const CellRegs<D, BITS> (&c)[2], int t0, int t1, int limit, float scale_log2, int lane) {
+    __device__ __forceinline__ void take(const CellRegs<D, BITS> (&c)[2], const Meta &x, int t0, int t1, int limit, int lane) {
         const int g = lane >> 4;
-        // this lane's item of meta: keys' scale and bias in log2 units, the excess taken off;
-        // values' with the middle code
-        float ma[2], mb[2];
+        f4 acc[NC][NG];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float s = __uint_as_float(c[j].meta << 16), b = __uint_as_float(c[j].meta & 0xFFFF0000u);
-            const bool key = (lane & C::GROUPS) == 0;
-            const float f = key ? scale_log2 : 1.f;
-            ma[j] = s * f;
-            mb[j] = fmaf(key ? -EXCESS : MID, s, b) * f;
-        }
-        float p[2][4];
-        f4 acc[2][C::GROUPS];
+        for (int j = 0; j < NC; ++j)
+#pragma unroll
+            for (int y = 0; y < NG; ++y) {
+                const float e = -EXCESS * qsum[y];
+                acc[j][y] = f4{e, e, e, e};
+            }
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int y = 0; y < C::GROUPS; ++y) {
-                f4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    bf16x8_t a;
-                    if (BITS == 4) {
-                        const uint32_t w = c[j].k[2 * y + h];
-                        a = as_bf16x8(nib_pair(w, 0), nib_pair(w, 4), nib_pair(w, 8), nib_pair(w, 12));
-                    } else {
-                        const uint32_t w0 = c[j].k[4 * y + 2 * h], w1 = c[j].k[4 * y + 2 * h + 1];
-                        a = as_bf16x8(byte_pair_lo(w0), byte_pair_hi(w0), byte_pair_lo(w1), byte_pair_hi(w1));
-                    }
-                    s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[2 * y + h], s, 0, 0, 0);
+            for (int s = 0; s < 2 * GROUPS; ++s) {
+                bf16x8_t a;
+                if (BITS == 4) {
+                    const uint32_t w = c[j].k[s];
+                    a = nibbles(w, w >> 4, w >> 8, w >> 12);
+                } else {
+                    const uint32_t w0 = c[j].k[2 * s], w1 = c[j].k[2 * s + 1];
+                    a = as_bf16x8(byte_pair_lo(w0), byte_pair_hi(w0), byte_pair_lo(w1), byte_pair_hi(w1));
                 }
-                acc[j][y] = s;
+                f4 &r = acc[BY_CELL ? 0 : j][BY_GROUP ? 0 : s >> 1];
+                r = mfma(a, q[(BY_CELL ? 2 * GROUPS * j : 0) + s], r);
             }
-        constexpr int I = C::ITEMS;
-        auto score = [&](int j, auto i_tag) {
-            constexpr int i = decltype(i_tag)::value;
-            float s = row_lane<I * i>(ma[j]) * acc[j][0][i];
-            s = fmaf(row_lane<I * i>(mb[j]), qsum[0], s);
-            if constexpr (C::GROUPS == 2) {
-                s = fmaf(row_lane<I * i + 1>(ma[j]), acc[j][1][i], s);
-                s = fmaf(row_lane<I * i + 1>(mb[j]), qsum[1], s);
-            }
-            if (EDGE && (j ? t1 : t0) + 4 * g + i > limit) s = -INFINITY;
-            p[j][i] = s;
-        };
-        using I0 = std::integral_constant<int, 0>;
-        using I1 = std::integral_constant<int, 1>;
-        using I2 = std::integral_constant<int, 2>;
-        using I3 = std::integral_constant<int, 3>;
+        float p[NC][4];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) { score(j, I0{}); score(j, I1{}); score(j, I2{}); score(j, I3{}); }
+        for (int j = 0; j < NC; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float s = 0.f;
+#pragma unroll
+                for (int y = 0; y < NG; ++y) {
+                    const Affine k = affine(x, j, y, false, i);
+                    s = fmaf(k.scale, acc[j][y][i], fmaf(k.bias, qsum[y], s));
+                }
+                if (BY_GROUP) s += dpp_mov<DPP_ROR8>(s);
+                if (EDGE && ((BY_CELL ? cell_of(lane & 15) : j) ? t1 : t0) + 4 * g + i > limit) s = -INFINITY;
+                p[j][i] = s;
+            }
         float bm = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) bm = fmaxf(bm, fmaxf(fmaxf(p[j][0], p[j][1]), fmaxf(p[j][2], p[j][3])));
-        if (__ballot(bm > m + LAG)) {
+        for (int j = 0; j < NC; ++j) bm = fmaxf(bm, fmaxf(fmaxf(p[j][0], p[j][1]), fmaxf(p[j][2], p[j][3])));
+        if (__ballot(bm > m + lag)) {
             bm = fmaxf(bm, __shfl_xor(bm, 16));
             bm = fmaxf(bm, __shfl_xor(bm, 32));
-            const float mn = fmaxf(m, bm);
-            ref = mn == -INFINITY ? 0.f : mn;
-            const float alpha = __builtin_amdgcn_exp2f(m - ref);
+            if (BY_CELL) bm = fmaxf(bm, other_cell(bm));
+            const float mn = fmaxf(m, bm), to = mn == -INFINITY ? 0.f : mn * sl;
+            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - to);
             m = mn;
+            ref = to;
             lsum *= alpha;
 #pragma unroll
-            for (int y = 0; y < C::GROUPS; ++y) {
+            for (int y = 0; y < NG; ++y) {
                 corr[y] *= alpha;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) psum[y][x] *= alpha;
+                for (int z = 0; z < 4; ++z) psum[y][z] *= alpha;
             }
 #pragma unroll
             for (int y = 0; y < DT; ++y)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) o[y][x] *= alpha;
+                for (int z = 0; z < 4; ++z) o[y][z] *= alpha;
         }
+        // P of the lane's cells and groups; a position that the column does not see weighs 0
+        // whatever its scale is
+        uint32_t pw[2][NG][2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < NC; ++j) {
+            float pv[NG][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                p[j][i] = __builtin_amdgcn_exp2f(p[j][i] - ref);
-                lsum += p[j][i];
-            }
-        // P of the groups; a position that the column does not see weighs 0 whatever its scale is
-        bf16x8_t pb[C::GROUPS];
-        float pv[2][C::GROUPS][4];
-        auto weigh = [&](int j, auto i_tag) {
-            constexpr int i = decltype(i_tag)::value;
-            const bool sees = !EDGE || (j ? t1 : t0) + 4 * g + i <= limit;
-            const float a0 = row_lane<I * i + C::GROUPS>(ma[j]), b0 = row_lane<I * i + C::GROUPS>(mb[j]);
-            pv[j][0][i] = sees ? p[j][i] * a0 : 0.f;
-            corr[0] = sees ? fmaf(p[j][i], b0, corr[0]) : corr[0];
-            if constexpr (C::GROUPS == 2) {
-                const float a1 = row_lane<I * i + 3>(ma[j]), b1 = row_lane<I * i + 3>(mb[j]);
-                pv[j][1][i] = sees ? p[j][i] * a1 : 0.f;
-                corr[1] = sees ? fmaf(p[j][i], b1, corr[1]) : corr[1];
-            }
-        };
+                const bool sees = !EDGE || ((BY_CELL ? cell_of(lane & 15) : j) ? t1 : t0) + 4 * g + i <= limit;
+                const float e = __builtin_amdgcn_exp2f(fmaf(p[j][i], sl, -ref));
+                lsum += e;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) { weigh(j, I0{}); weigh(j, I1{}); weigh(j, I2{}); weigh(j, I3{}); }
-        constexpr int X = BITS == 4 ? 2 : 1, Y = BITS == 4 ? 1 : 2;      // order of a value's word
+                for (int y = 0; y < NG; ++y) {
+                    const Affine v = affine(x, j, y, true, i);
+                    pv[y][i] = sees ? e * v.scale : 0.f;
+                    corr[y] = sees ? fmaf(e, fmaf(MID, v.scale, v.bias), corr[y]) : corr[y];
+                }
+            }
+            constexpr int X = BITS == 4 ? 2 : 1, Y = BITS == 4 ? 1 : 2;      // order of a value's word
 #pragma unroll
-        for (int y = 0; y < C::GROUPS; ++y) {
-            pb[y] = as_bf16x8(cvt_pk_bf16(pv[0][y][0], pv[0][y][X]), cvt_pk_bf16(pv[0][y][Y], pv[0][y][3]),
-                              cvt_pk_bf16(pv[1][y][0], pv[1][y][X]), cvt_pk_bf16(pv[1][y][Y], pv[1][y][3]));
-            psum[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones(), pb[y], psum[y], 0, 0, 0);
+            for (int y = 0; y < NG; ++y) {
+                pw[j][y][0] = cvt_pk_bf16(pv[y][0], pv[y][X]);
+                pw[j][y][1] = cvt_pk_bf16(pv[y][Y], pv[y][3]);
+            }
         }
+        bf16x8_t pb[NG];
+        if (BY_CELL) {
+            const uint32_t m1 = cell_of(lane & 15) ? 0xFFFFFFFFu : 0u;
+            pb[0] = as_bf16x8(pw[0][0][0] & ~m1, pw[0][0][1] & ~m1, pw[0][0][0] & m1, pw[0][0][1] & m1);
+        } else {
+#pragma unroll
+            for (int y = 0; y < NG; ++y) pb[y] = as_bf16x8(pw[0][y][0], pw[0][y][1], pw[1][y][0], pw[1][y][1]);
+        }
+#pragma unroll
+        for (int y = 0; y < NG; ++y) psum[y] = mfma(ones(), pb[y], psum[y]);
 #pragma unroll
         for (int y = 0; y < DT; ++y) {
             bf16x8_t a;
             if (BITS == 4) {
                 const uint32_t w0 = c[0].v[y >> 1], w1 = c[1].v[y >> 1];
                 const int s = 4 * (y & 1);
-                a = as_bf16x8(nib_pair(w0, s), nib_pair(w0, 8 + s), nib_pair(w1, s), nib_pair(w1, 8 + s));
+                a = nibbles(w0 >> s, w0 >> (8 + s), w1 >> s, w1 >> (8 + s));
             } else {
                 const uint32_t w0 = c[0].v[y], w1 = c[1].v[y];
                 a = as_bf16x8(byte_pair_lo(w0), byte_pair_hi(w0), byte_pair_lo(w1), byte_pair_hi(w1));
             }
-            o[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pb[y / 4], o[y], 0, 0, 0);
+            o[y] = mfma(a, pb[NG == 1 ? 0 : y / 4], o[y]);
         }
     }
 
@@ -241,7 +313,7 @@ struct Columns {
     static constexpr int SETTLE = 512;
     __device__ __forceinline__ void settle() {
 #pragma unroll
-        for (int j = 0; j < C::GROUPS; ++j) {
+        for (int j = 0; j < NG; ++j) {
             float c = corr[j];
             c += __shfl_xor(c, 16);
             c += __shfl_xor(c, 32);
@@ -249,17 +321,27 @@ struct Columns {
             corr[j] = 0.f;
             psum[j] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int y = 4 * j; y < 4 * j + 4; ++y)
+            for (int y = NG == 1 ? 0 : 4 * j; y < (NG == 1 ? DT : 4 * j + 4); ++y)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) o[y][x] += c;
+                for (int z = 0; z < 4; ++z) o[y][z] += c;
         }
     }
-    // o and the sum of the column's weights
+    // the column's sum of weights; o then is the column's sum of p v, in its dims tiles [first, first + n)
     __device__ __forceinline__ float close() {
         settle();
-        const float l = lsum + __shfl_xor(lsum, 16);
-        return l + __shfl_xor(l, 32);
+        float l = lsum + __shfl_xor(lsum, 16);
+        l += __shfl_xor(l, 32);
+        if (BY_CELL) {
+            l += other_cell(l);
+#pragma unroll
+            for (int y = 0; y < DT; ++y)
+#pragma unroll
+                for (int z = 0; z < 4; ++z) o[y][z] += other_cell(o[y][z]);
+        }
+        return l;
     }
+    // whether this lane writes tile y of the column's dims
+    static __device__ __forceinline__ bool writes(int y, int c) { return (BY_CELL ? cell_of(c) == 0 : true) && (!BY_GROUP || group_of(c) == y / 4); }
 };
 
 // ---------------------------------------------------------------- few columns
@@ -273,16 +355,19 @@ struct Columns {
 // nothing but their run, so there is no barrier; the next 32 keys' codes are on their way while
 // these are computed.
 constexpr int LINE_SHIFT = 7, LINE_KB = 1 << LINE_SHIFT;
+template <int D>
+constexpr int LINE_WAVES = D == 128 ? 2 : 3;             // a SIMD, where lines run alone
 
-template <int D, int BITS>
+template <int D, int BITS, int CW>
 __device__ __forceinline__ void attn_line(const QuantArgs &a, int wg, int w, uint8_t *smem) {
     using C = Cell<D, BITS>;
-    const int threads = blockDim.x, tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    using Cols = Columns<D, BITS, CW>;
+    const int threads = blockDim.x, tid = threadIdx.x, lane = tid & 63, c = lane & (CW - 1), g = lane >> 4;
     // of every sequence: its first row, its keys, its first block and unit in the line
     int32_t *first_row = reinterpret_cast<int32_t *>(smem), *keys = first_row + a.R, *off = keys + a.R, *unit = off + a.R;
     int32_t *wsum = unit + a.R;
-    const int rows = live_rows(a);
-    const int P = a.join ? prefix_keys(a) : 0, pb = own_keyblocks(P, LINE_SHIFT);
+    const int rows = __builtin_amdgcn_readfirstlane(live_rows(a));
+    const int P = __builtin_amdgcn_readfirstlane(a.join ? prefix_keys(a) : 0), pb = own_keyblocks(P, LINE_SHIFT);
 
     int t_before = 0, u_before = 0;
     for (int r0 = 0; r0 < a.R; r0 += threads) {
@@ -317,7 +402,7 @@ __device__ __forceinline__ void attn_line(const QuantArgs &a, int wg, int w, uin
         for (int r = lane + 64 * w; r < a.R; r += SA_THREADS) { a.own_off[r] = off[r]; a.own_unit[r] = unit[r]; }
         if (lane + w == 0) a.own_off[a.R] = t_before;
     }
-    const int total = t_before, run = own_run(total, a.own_wgs);
+    const int total = __builtin_amdgcn_readfirstlane(t_before), run = own_run(total, a.own_wgs);
     int t = (int)min((long)wg * run, (long)total);
     const int t_end = min(t + run, total);
     if (t >= t_end) return;
@@ -325,10 +410,9 @@ __device__ __forceinline__ void attn_line(const QuantArgs &a, int wg, int w, uin
     int r = 0;
     for (int n = a.R; n > 1;) {
         const int half = n >> 1;
-        if (off[r + half] <= t) { r += half; n -= half; }
+        if (__builtin_amdgcn_readfirstlane(off[r + half]) <= t) { r += half; n -= half; }
         else n = half;
     }
-    r = __builtin_amdgcn_readfirstlane(r);
     int u_next = __builtin_amdgcn_readfirstlane(unit[r]);      // unit number of the next unit opened
     int in_seq = t - __builtin_amdgcn_readfirstlane(off[r]);   // block t within sequence r
 
@@ -409,15 +493,21 @@ __device__ __forceinline__ void attn_line(const QuantArgs &a, int wg, int w, uin
         x.b1 = s.table[min((s.kb + 16) >> a.shift, s.width - 1)];
         return x;
     };
-    auto load = [&](const Step &s, const Ids &x, CellRegs<D, BITS> (&regs)[2]) {
+    struct Keys {                // what a step reads
+        CellRegs<D, BITS> c[2];
+        typename Cols::Meta meta;
+    };
+    auto load = [&](const Step &s, const Ids &x, Keys &k) {
         if (s.kb >= s.end) return;           // nothing that is seen
         // (nor is a second cell read that no column sees: the first one again, its keys hidden)
         const int t1 = s.kb + 16 < s.end ? s.kb + 16 : s.kb;
         const int b0 = __builtin_amdgcn_readfirstlane(x.b0), b1 = __builtin_amdgcn_readfirstlane(t1 == s.kb ? x.b0 : x.b1);
-        regs[0].load(cell_at<C::BYTES>(a, s.hk, b0, s.kb), lane);
-        regs[1].load(cell_at<C::BYTES>(a, s.hk, b1, t1), lane);
+        const uint8_t *c0 = cell_at<C::BYTES>(a, s.hk, b0, s.kb), *c1 = cell_at<C::BYTES>(a, s.hk, b1, t1);
+        k.c[0].load(c0, lane);
+        k.c[1].load(c1, lane);
+        Cols::load_meta(k.meta, c0, c1, lane);
     };
-    Columns<D, BITS> col;
+    Cols col;
     auto column = [&](const Step &s) {       // this lane's column's q row
         const int i = (s.col0 + c) / a.G, h = s.hk * a.G + s.col0 + c - i * a.G;
         return i < s.n ? a.q + (size_t)(s.first + i) * a.q_stride + (size_t)h * D : nullptr;
@@ -426,14 +516,15 @@ __device__ __forceinline__ void attn_line(const QuantArgs &a, int wg, int w, uin
         const float ltot = col.close();
         if ((s.col0 + c) / a.G >= s.n || s.part >= a.own_parts || c >= a.part_cols) return;
         const size_t at = (size_t)s.part * a.part_cols + c;
-        if (g == 0) a.own_ml[at] = make_float2(ltot == ltot ? col.m : INFINITY, ltot);
+        if (lane < CW) a.own_ml[at] = make_float2(ltot == ltot ? col.m * a.scale_log2 : INFINITY, ltot);
         float *po = a.own_o + at * D + 4 * g;
 #pragma unroll
-        for (int y = 0; y < D / 16; ++y) *reinterpret_cast<f4 *>(po + 16 * y) = col.o[y];
+        for (int y = 0; y < D / 16; ++y)
+            if (Cols::writes(y, lane & 15)) *reinterpret_cast<f4 *>(po + 16 * y) = col.o[y];
     };
 
     Step s, n;                   // this step, and the next
-    CellRegs<D, BITS> cur[2], nxt[2];
+    Keys cur, nxt;
     open(s);
     load(s, ids_of(s), nxt);
     n = s;
@@ -441,8 +532,7 @@ __device__ __forceinline__ void attn_line(const QuantArgs &a, int wg, int w, uin
     Ids ids = ids_of(n);
     int since = 0, limit = -1;
     for (;;) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) cur[j] = nxt[j];
+        cur = nxt;
         const Step f = n;
         const bool go = more;
         if (go) {
@@ -451,17 +541,17 @@ __device__ __forceinline__ void attn_line(const QuantArgs &a, int wg, int w, uin
             ids = ids_of(n);
         }
         if (s.fresh) {
-            col.open(column(s), g);
+            col.open(column(s), lane, a.scale_log2);
             since = 0;
             const int i = (s.col0 + c) / a.G;
             limit = i >= s.n ? -1 : s.rel + i;
         }
         if (s.col0 < s.n * a.G) {            // (a wave of a wide unit may have no column)
             if (s.kb < s.end) {
-                if (since == Columns<D, BITS>::SETTLE / 32) { col.settle(); since = 0; }
+                if (since == Cols::SETTLE / 32) { col.settle(); since = 0; }
                 ++since;
-                if (s.kb + 32 <= s.all) col.template take<false>(cur, s.kb, s.kb + 16, 0, a.scale_log2, lane);
-                else col.template take<true>(cur, s.kb, s.kb + 16, s.blk < pb ? P - 1 : limit, a.scale_log2, lane);
+                if (s.kb + 32 <= s.all) col.template take<false>(cur.c, cur.meta, s.kb, s.kb + 16, 0, lane);
+                else col.template take<true>(cur.c, cur.meta, s.kb, s.kb + 16, s.blk < pb ? P - 1 : limit, lane);
             }
             if (s.last) end(s);
         }
@@ -474,46 +564,46 @@ __device__ __forceinline__ void attn_line(const QuantArgs &a, int wg, int w, uin
 //
 // How attn_tile's key blocks come into its ring: K [64 keys x D] and Vt [D x 64 keys] in bf16, as
 // the bf16 cache's kernel copies them.  The waves load a key block's codes two blocks ahead and
-// write their values one block ahead; of 4 cells half of the waves have the keys, half the values.
-template <int D, int BITS, int WAVES>
+// write their values one block ahead.  Of
+// a block's 4 cells wave w has half of the words of cell w / 2, keys' and values' alike (8 waves
+// and one path for all of them, so that nothing branches).
+template <int D, int BITS>
 struct Values {
     using Args = QuantArgs;
     using Gm = SaGeo<D>;
     using C = Cell<D, BITS>;
-    static constexpr int COLS = 32 * WAVES;
-    static constexpr int CELLS = 8 / WAVES;          // cells' halves a wave has
-    static constexpr int WORDS = C::LANE / 4;
+    static constexpr int COLS = 256;
+    static constexpr int HALF = C::LANE / 8;         // words of a lane's half
     struct Flow {
-        uint32_t x[CELLS][WORDS];
-        uint32_t meta[CELLS];
+        uint32_t k[HALF], v[HALF];
+        uint32_t km, vm;         // scales and biases: of the lane's position's key; of position 4 g + l % 4's value
     };
     const QuantArgs &a;
     uint8_t *smem;
-    int lane, w;
-    __device__ __forceinline__ Values(const QuantArgs &a_, uint8_t *smem_, int lane_, int w_) : a(a_), smem(smem_), lane(lane_), w(w_) {}
+    int lane, half, cell;
+    __device__ __forceinline__ Values(const QuantArgs &a_, uint8_t *smem_, int lane_, int w)
+        : a(a_), smem(smem_), lane(lane_), half(w & 1), cell(w >> 1) {}
 
-    __device__ __forceinline__ bool values_of(int i) const { return (w * CELLS + i) >= 4; }
-    __device__ __forceinline__ int cell_of(int i) const { return (w * CELLS + i) & 3; }
-    __device__ __forceinline__ void load(Flow &f, int hk, const int32_t *table, int width, int blk) const {
-        constexpr int PER = 4 * C::ITEMS;
-#pragma unroll
-        for (int i = 0; i < CELLS; ++i) {
-            const int t = blk * SA_KB + 16 * cell_of(i);
-            const int b = __builtin_amdgcn_readfirstlane(table[min(t >> a.shift, width - 1)]);
-            const uint8_t *cell = cell_at<C::BYTES>(a, hk, b, t);
-            const uint8_t *p = cell + (values_of(i) ? C::CODES : 0) + lane * C::PLANE;
-#pragma unroll
-            for (int pl = 0; pl < C::PLANES; ++pl) {
-                if (C::PLANE == 16) {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(p + 1024 * pl);
-                    f.x[i][4 * pl] = v.x; f.x[i][4 * pl + 1] = v.y; f.x[i][4 * pl + 2] = v.z; f.x[i][4 * pl + 3] = v.w;
-                } else {
-                    const uint2 v = *reinterpret_cast<const uint2 *>(p);
-                    f.x[i][0] = v.x; f.x[i][1] = v.y;
-                }
-            }
-            f.meta[i] = *reinterpret_cast<const uint32_t *>(cell + 2 * C::CODES + ((lane >> 4) * PER + (lane & (PER - 1))) * 4);
+    static __device__ __forceinline__ void words(uint32_t (&x)[HALF], const uint8_t *p) {
+        if constexpr (HALF == 4) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(p);
+            x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+        } else if constexpr (HALF == 2) {
+            const uint2 v = *reinterpret_cast<const uint2 *>(p);
+            x[0] = v.x; x[1] = v.y;
+        } else {
+            x[0] = *reinterpret_cast<const uint32_t *>(p);
         }
+    }
+    __device__ __forceinline__ void load(Flow &f, int hk, const int32_t *table, int width, int blk) const {
+        const int t = blk * SA_KB + 16 * cell, grp = C::GROUPS == 2 ? half : 0;
+        const int b = __builtin_amdgcn_readfirstlane(table[min(t >> a.shift, width - 1)]);
+        const uint8_t *p = cell_at<C::BYTES>(a, hk, b, t);
+        const int at = C::PLANES == 2 ? 1024 * half + lane * 16 : lane * C::LANE + 4 * HALF * half;
+        words(f.k, p + at);
+        words(f.v, p + C::CODES + at);
+        f.km = *reinterpret_cast<const uint32_t *>(p + C::meta(lane & 15, grp));
+        f.vm = *reinterpret_cast<const uint32_t *>(p + C::meta(4 * (lane >> 4) + (lane & 3), C::GROUPS + grp));
     }
     // code e (0 .. 7) of a word of 4-bit codes, byte e (0 .. 3) of one of 8-bit codes
     static __device__ __forceinline__ float code(uint32_t w, int e) {
@@ -521,52 +611,36 @@ struct Values {
     }
     __device__ __forceinline__ void store(const Flow &f, int st) const {
         const int g = lane >> 4, r = lane & 15;
+        uint8_t *K = smem + st * Gm::STAGE, *V = K + Gm::KTILE;
+        // keys: 8 dims a chunk, D / 64 of them
+        const float ks = __uint_as_float(f.km << 16), kb = __uint_as_float(f.km & 0xFFFF0000u);
 #pragma unroll
-        for (int i = 0; i < CELLS; ++i) {
-            uint8_t *K = smem + st * Gm::STAGE, *V = K + Gm::KTILE;
-            const int ci = cell_of(i);
-            if (!values_of(i)) {
-                const int t = 16 * ci + r;
-                // position r's scale and bias: lane row r / 4 of the meta words has them
+        for (int h = 0; h < C::GROUPS; ++h) {
+            uint32_t o[4];
 #pragma unroll
-                for (int j = 0; j < C::GROUPS; ++j) {
-                    const uint32_t mw = (uint32_t)__shfl((int)f.meta[i], 16 * (r >> 2) + C::ITEMS * (r & 3) + j);
-                    const float s = __uint_as_float(mw << 16), b = __uint_as_float(mw & 0xFFFF0000u);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t o[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if (BITS == 4) {
-                                const uint32_t wd = f.x[i][2 * j + h];
-                                o[e] = cvt_pk_bf16(fmaf(s, code(wd, e), b), fmaf(s, code(wd, 4 + e), b));
-                            } else {
-                                const uint32_t wd = f.x[i][4 * j + 2 * h + (e >> 1)];
-                                o[e] = cvt_pk_bf16(fmaf(s, code(wd, 2 * (e & 1)), b), fmaf(s, code(wd, 2 * (e & 1) + 1), b));
-                            }
-                        }
-                        *reinterpret_cast<uint4 *>(K + sa_kswz<D>(t, 8 * j + 2 * g + h)) = make_uint4(o[0], o[1], o[2], o[3]);
-                    }
+            for (int e = 0; e < 4; ++e) {
+                if (BITS == 4) o[e] = cvt_pk_bf16(fmaf(ks, code(f.k[h], e), kb), fmaf(ks, code(f.k[h], 4 + e), kb));
+                else {
+                    const uint32_t wd = f.k[2 * h + (e >> 1)];
+                    o[e] = cvt_pk_bf16(fmaf(ks, code(wd, 2 * (e & 1)), kb), fmaf(ks, code(wd, 2 * (e & 1) + 1), kb));
                 }
-            } else {
-                const float ms = __uint_as_float(f.meta[i] << 16), mb = __uint_as_float(f.meta[i] & 0xFFFF0000u);
-                auto group = [&](auto j_tag) {
-                    constexpr int j = decltype(j_tag)::value, I = C::ITEMS, B = C::GROUPS + j;
-                    const float s[4] = {row_lane<B>(ms), row_lane<I + B>(ms), row_lane<2 * I + B>(ms), row_lane<3 * I + B>(ms)};
-                    const float b[4] = {row_lane<B>(mb), row_lane<I + B>(mb), row_lane<2 * I + B>(mb), row_lane<3 * I + B>(mb)};
-#pragma unroll
-                    for (int y = 4 * j; y < 4 * j + 4; ++y) {
-                        float v[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            v[e] = fmaf(s[e], BITS == 4 ? code(f.x[i][y >> 1], 2 * e + (y & 1)) : code(f.x[i][y], e), b[e]);
-                        *reinterpret_cast<uint2 *>(V + sa_vswz(16 * y + r, 2 * ci + (g >> 1)) + 8 * (g & 1)) =
-                            make_uint2(cvt_pk_bf16(v[0], v[1]), cvt_pk_bf16(v[2], v[3]));
-                    }
-                };
-                group(std::integral_constant<int, 0>{});
-                if constexpr (C::GROUPS == 2) group(std::integral_constant<int, 1>{});
             }
+            const int chunk = C::GROUPS == 2 ? 8 * half + 2 * g + h : 2 * g + half;
+            *reinterpret_cast<uint4 *>(K + sa_kswz<D>(16 * cell + r, chunk)) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        // values: 4 positions of 2 D / 64 dims
+        const float ms = __uint_as_float(f.vm << 16), mb = __uint_as_float(f.vm & 0xFFFF0000u);
+        float s[4], b[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { s[e] = row_lane(ms, e); b[e] = row_lane(mb, e); }
+#pragma unroll
+        for (int y = 0; y < 2 * C::GROUPS; ++y) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                v[e] = fmaf(s[e], BITS == 4 ? code(f.v[y >> 1], 2 * e + (y & 1)) : code(f.v[y], e), b[e]);
+            *reinterpret_cast<uint2 *>(V + sa_vswz(16 * (2 * C::GROUPS * half + y) + r, 2 * cell + (g >> 1)) + 8 * (g & 1)) =
+                make_uint2(cvt_pk_bf16(v[0], v[1]), cvt_pk_bf16(v[2], v[3]));
         }
     }
     __device__ __forceinline__ void open(Flow &f, int hk, const int32_t *table, int width, int b0) const {
@@ -581,46 +655,48 @@ struct Values {
     __device__ __forceinline__ void landed() const {}
 };
 
-// ---------------------------------------------------------------- both
+// ---------------------------------------------------------------- kernels
 
-template <int D, int BITS, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2))) attn_quantized_kernel(QuantArgs a) {
+// Column tiles and lines: workgroups of 8 waves, which take every register of a CU, of a tile of
+// 256 columns or of two of the line's.
+constexpr int QUANT_WAVES = 8;
+template <int D, int BITS, int CW>
+__global__ void __launch_bounds__(64 * QUANT_WAVES) __attribute__((amdgpu_waves_per_eu(2))) attn_quantized_kernel(QuantArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
     if ((int)blockIdx.x < a.tile_wgs) {
-        attn_tile<D, Values<D, BITS, WAVES>>(a, (int)blockIdx.x, smem);
+        attn_tile<D, Values<D, BITS>>(a, (int)blockIdx.x, smem);
         return;
     }
-    // a workgroup of the line is 4 waves
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    attn_line<D, BITS>(a, ((int)blockIdx.x - a.tile_wgs) * (WAVES / 4) + w / 4, w & 3, smem);
+    attn_line<D, BITS, CW>(a, ((int)blockIdx.x - a.tile_wgs) * (QUANT_WAVES / 4) + w / 4, w & 3, smem);
+}
+
+// Lines alone.
+template <int D, int BITS, int CW>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(LINE_WAVES<D>))) attn_line_kernel(QuantArgs a) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    attn_line<D, BITS, CW>(a, (int)blockIdx.x, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), smem);
 }
 
 // ---------------------------------------------------------------- host side
 
-constexpr int QUANT_WAVES_FEW = 4, QUANT_WAVES_MANY = 8;
-
-// Into how many workgroups a column tile's key blocks are cut.
-int quant_splits(long wgs, long blocks, double part_bytes, bool last_is_whole, long cus) {
+// Into how many workgroups a column tile's key blocks are cut, of `most` that there is room for.
+int quant_splits(long wgs, long blocks, double part_bytes, bool last_is_whole, long most) {
     int best = 1;
     double least = 1e30;
     for (int n = 1; n <= 64 && (n == 1 || n <= blocks); ++n) {
-        const long w = wgs * n;
-        const double block = w <= cus ? 1.6 : 2.2 * ((w + 2 * cus - 1) / (2 * cus));
-        const double walk = (double)((blocks + n - 1) / n) * block;
+        const long rounds = (wgs * n + most - 1) / most;
+        const double walk = (double)((blocks + n - 1) / n) * 2.0 * rounds;
         const double parts = n == 1 && last_is_whole ? 0 : n * (part_bytes / (last_is_whole ? 2.5e6 : 1.3e6) + 0.06);
         if (walk + parts < least) { least = walk + parts; best = n; }
     }
     return best;
 }
 
-struct QuantPlan : SaPlan {
-    int waves = QUANT_WAVES_FEW;
-};
-
 // own_cap, prefix_cap: positions the tables have room for; max_new: at least the rows of
 // the sequence with the most
-QuantPlan plan_quant(long N, long R, long H, long Hkv, long D, long own_cap, long prefix_cap, long max_new) {
-    QuantPlan p;
+SaPlan plan_quant(long N, long R, long H, long Hkv, long D, long own_cap, long prefix_cap, long max_new) {
+    SaPlan p;
     const long G = H / Hkv, cols = N * G, cus = device_info().num_cus;
     if (max_new > N) max_new = N;
     p.own_shift = LINE_SHIFT;
@@ -628,18 +704,21 @@ QuantPlan plan_quant(long N, long R, long H, long Hkv, long D, long own_cap, lon
     p.any_big = max_new > p.small_rows;
     p.join = !p.any_big && prefix_cap > 0 && R == 1;
     p.use_tile = p.any_big || (prefix_cap > 0 && !p.join);
-    p.waves = p.any_big ? QUANT_WAVES_MANY : QUANT_WAVES_FEW;
-    p.tiles = (cols + 32 * p.waves - 1) / (32 * p.waves);
+    p.tiles = (cols + 32 * QUANT_WAVES - 1) / (32 * QUANT_WAVES);
     const long wgs = p.tiles * Hkv;
     const long blocks = (prefix_cap + (p.any_big ? own_cap : 0) + SA_KB - 1) / SA_KB;
-    p.nsplit = p.use_tile ? quant_splits(wgs, blocks, (double)N * H * (8 * D + 16), p.any_big, cus) : 1;
+    // of the CUs, where tiles have the prefix alone, half at least for them, and a tenth for the lines
+    const double tile_work = (double)p.tiles * (prefix_cap / SA_KB + 1) * 2.0, line_work = (double)R * own_cap * 0.5 / 64 * 0.5;
+    const double share = tile_work / (tile_work + line_work);
+    const long most = p.any_big ? cus : (long)(cus * (share < 0.5 ? 0.5 : share > 0.9 ? 0.9 : share));
+    p.nsplit = p.use_tile ? quant_splits(wgs, blocks, (double)N * H * (8 * D + 16), p.any_big, most) : 1;
     const long rows_max = max_new < p.small_rows ? max_new : p.small_rows;
     p.rows_max = (int)rows_max;
     long coltiles = R * ((rows_max * G + 63) / 64);
     if (coltiles > R + cols / 64) coltiles = R + cols / 64;
     const long keyblocks = coltiles * (own_keyblocks((int)own_cap, LINE_SHIFT) + (p.join ? own_keyblocks((int)prefix_cap, LINE_SHIFT) : 0));
-    long ow = p.use_tile && !p.any_big ? 2 * cus - wgs * p.nsplit : 2 * cus;
-    if (ow < cus) ow = cus;
+    long ow = p.use_tile && !p.any_big ? 2 * (cus - wgs * p.nsplit) : 2 * cus;
+    if (ow < cus / 4) ow = cus / 4;
     if (ow > Hkv * keyblocks) ow = Hkv * keyblocks;
     p.own_wgs = (int)(ow < 1 ? 1 : ow);
     p.own_parts = 4 * (Hkv * coltiles + p.own_wgs);
@@ -648,21 +727,25 @@ QuantPlan plan_quant(long N, long R, long H, long Hkv, long D, long own_cap, lon
     return p;
 }
 
-template <int D, int BITS, int WAVES>
-int run_quant(const QuantArgs &a, const QuantPlan &p, hipStream_t stream) {
+template <int D, int BITS, int CW>
+int run_quant(const QuantArgs &a, const SaPlan &p, hipStream_t stream) {
     const int line_lds = 4 * a.R * 4 + 64;
-    const int lds = a.tile_wgs && SaGeo<D>::LDS > line_lds ? SaGeo<D>::LDS : line_lds;
-    auto kern = attn_quantized_kernel<D, BITS, WAVES>;
-    const int per = WAVES / 4;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(a.tile_wgs + (a.own_wgs + per - 1) / per)), dim3(64 * WAVES), lds, stream, a);
+    if (a.tile_wgs == 0) {
+        hipLaunchKernelGGL((attn_line_kernel<D, BITS, CW>), dim3((unsigned)a.own_wgs), dim3(256), line_lds, stream, a);
+    } else {
+        const int lds = SaGeo<D>::LDS > line_lds ? SaGeo<D>::LDS : line_lds, per = QUANT_WAVES / 4;
+        hipLaunchKernelGGL((attn_quantized_kernel<D, BITS, CW>), dim3((unsigned)(a.tile_wgs + (a.own_wgs + per - 1) / per)),
+                           dim3(64 * QUANT_WAVES), lds, stream, a);
+    }
     SC_HIP_CHECK(hipGetLastError());
     return merge_parts<D>(a, p, stream);
 }
 
 template <int D, int BITS>
-int run_quant(const QuantArgs &a, const QuantPlan &p, hipStream_t stream) {
-    return p.waves == QUANT_WAVES_MANY ? run_quant<D, BITS, QUANT_WAVES_MANY>(a, p, stream)
-                                       : run_quant<D, BITS, QUANT_WAVES_FEW>(a, p, stream);
+int run_quant(const QuantArgs &a, const SaPlan &p, hipStream_t stream) {
+    if (D == 128 && p.part_cols <= 4) return run_quant<D, BITS, D == 128 ? 4 : 8>(a, p, stream);
+    if (p.part_cols <= 8) return run_quant<D, BITS, 8>(a, p, stream);
+    return run_quant<D, BITS, 16>(a, p, stream);
 }
 
 bool bad_shape(long N, long R, long H, long Hkv, long D, long own_cap, long prefix_cap, long max_new, int bits) {
@@ -704,7 +787,7 @@ int launch_attention_quantized(const uint16_t *q, long q_stride, const uint8_t *
         return set_error(SC_EINVAL, "attention_quantized: bad row strides");
     if (((uintptr_t)q | (uintptr_t)pool) % 16 || (uintptr_t)out % 8)
         return set_error(SC_EINVAL, "attention_quantized: misaligned pointers");
-    const QuantPlan p = plan_quant(N, R, H, Hkv, D, width * bs, prefix_width * bs, max_new);
+    const SaPlan p = plan_quant(N, R, H, Hkv, D, width * bs, prefix_width * bs, max_new);
     if (!workspace || workspace_bytes < p.bytes || (uintptr_t)workspace % 16)
         return set_error(SC_EINVAL, "attention_quantized: a 16-byte aligned workspace of %ld bytes required", p.bytes);
     // 2^32 threads a launch

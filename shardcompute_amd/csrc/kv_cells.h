@@ -5,7 +5,7 @@
 // head, keys and values, one run of bytes that a wave reads whole lines of:
 //   keys' codes    lane (g, r) of 64 = 16 g + r: position r, dims 16 g .. 16 g + 15 of each group
 //   values' codes  lane (g, l): positions 4 g .. 4 g + 3, dims l, 16 + l, 32 + l, ..
-//   meta           [16 positions][keys' groups, values' groups]: scale | bias << 16
+//   meta           [keys' groups, values' groups][16 positions]: scale | bias << 16
 // A lane's codes are what it feeds as operand A of v_mfma_f32_16x16x32_bf16: keys as rows
 // of S^T = K Q^T, whose result then lies as operand B of O^T += V^T P^T wants it, the 4 positions
 // 4 g .. 4 g + 3 of a cell in lane row g.  A lane's bytes are one 16-byte load (8 with 4 bits
@@ -42,7 +42,7 @@ struct Cell {
         return CODES + (BITS == 4 ? lane * LANE + 4 * (tile >> 1) : 1024 * (tile >> 2) + lane * 16 + 4 * (tile & 3)) + (t & 3);
     }
     // byte of a meta word: item grp of the keys, GROUPS + grp of the values
-    static __host__ __device__ constexpr int meta(int t, int item) { return 2 * CODES + (t * ITEMS + item) * 4; }
+    static __host__ __device__ constexpr int meta(int t, int item) { return 2 * CODES + (item * 16 + t) * 4; }
 };
 
 // bytes of a cell, 0 for a head_dim or a number of bits that there is none for
