@@ -25,6 +25,8 @@
 #include "attn_shared_core.h"
 #include "kv_cells.h"
 
+#include <algorithm>
+
 namespace sc {
 
 namespace {
@@ -132,6 +134,7 @@ struct Columns {
     float m, ref, lsum, corr[NG];            // m: the maximum, of scores without the scale
     f4 o[DT], psum[NG];
     float sl, lag;                           // the scale, in log2 units; LAG without it
+    int since;                               // steps since o was settled
 
     static __device__ __forceinline__ int cell_of(int c) { return BY_CELL ? (GROUPS == 2 ? (c >> 2) & 1 : c >> 3) : 0; }
     static __device__ __forceinline__ int group_of(int c) { return BY_GROUP ? c >> 3 : 0; }
@@ -159,9 +162,17 @@ struct Columns {
         x.w[1] = *reinterpret_cast<const uint32_t *>(c1 + at);
     }
 
-    // qp: this lane's column's q row (null: none)
-    __device__ __forceinline__ void open(const uint16_t *qp, int lane, float scale_log2) {
-        const int g = lane >> 4, c = lane & 15;
+    // this lane's share of its column's q row (null: none)
+    struct Row4 { uint4 x[2 * GROUPS]; };
+    static __device__ __forceinline__ void load_q(Row4 &r, const uint16_t *qp, int lane) {
+#pragma unroll
+        for (int s = 0; s < 2 * GROUPS; ++s) {
+            r.x[s] = make_uint4(0u, 0u, 0u, 0u);
+            if (qp) r.x[s] = *reinterpret_cast<const uint4 *>(qp + 64 * (s >> 1) + 16 * (lane >> 4) + 8 * (s & 1));
+        }
+    }
+    __device__ __forceinline__ void open(const Row4 &r, int lane, float scale_log2) {
+        const int c = lane & 15;
         sl = scale_log2;
         lag = LAG / scale_log2;
         f4 sum[NG];
@@ -171,10 +182,8 @@ struct Columns {
         for (int j = 0; j < NQ / (2 * GROUPS); ++j)
 #pragma unroll
             for (int s = 0; s < 2 * GROUPS; ++s) {
-                uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                const bool mine = (!BY_CELL || cell_of(c) == j) && (!BY_GROUP || group_of(c) == s >> 1);
-                if (qp && mine) x = *reinterpret_cast<const uint4 *>(qp + 64 * (s >> 1) + 16 * g + 8 * (s & 1));
-                q[2 * GROUPS * j + s] = as_bf16x8(x);
+                const uint32_t mine = (!BY_CELL || cell_of(c) == j) && (!BY_GROUP || group_of(c) == s >> 1) ? 0xFFFFFFFFu : 0u;
+                q[2 * GROUPS * j + s] = as_bf16x8(r.x[s].x & mine, r.x[s].y & mine, r.x[s].z & mine, r.x[s].w & mine);
                 const int y = BY_GROUP ? 0 : s >> 1;
                 sum[y] = mfma(ones(), q[2 * GROUPS * j + s], sum[y]);
             }
@@ -186,12 +195,37 @@ struct Columns {
         }
         m = -INFINITY;
         ref = lsum = 0.f;
+        since = 0;
 #pragma unroll
         for (int y = 0; y < DT; ++y) o[y] = f4{0.f, 0.f, 0.f, 0.f};
     }
 
-    // The cells' positions t0 .. t0 + 15 and t1 .. t1 + 15; the column sees those up to limit
-    // (EDGE; else all).
+    // Of the cells' positions t0 .. t0 + 15 and t1 .. t1 + 15 the column sees those up to limit.
+    // A lane whose meta words are its own hides a position by giving it none: values 0, and
+    // -inf (pen) added to a score of 0, whatever the cell holds there.
+    float pen[NC][4];
+    __device__ __forceinline__ void hide(Own &x, int t0, int t1, int limit, int lane) {
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+            const int t = ((BY_CELL ? cell_of(lane & 15) : j) ? t1 : t0) + 4 * (lane >> 4);
+#pragma unroll
+            for (int y = 0; y < NG; ++y) {
+                uint4 &k = x.k[j][y], &v = x.v[j][y];
+                k.x = t > limit ? 0u : k.x; k.y = t + 1 > limit ? 0u : k.y; k.z = t + 2 > limit ? 0u : k.z; k.w = t + 3 > limit ? 0u : k.w;
+                v.x = t > limit ? 0u : v.x; v.y = t + 1 > limit ? 0u : v.y; v.z = t + 2 > limit ? 0u : v.z; v.w = t + 3 > limit ? 0u : v.w;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pen[j][i] = t + i > limit ? -INFINITY : 0.f;
+        }
+    }
+    __device__ __forceinline__ void show() {
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pen[j][i] = 0.f;
+    }
+    // The next 32 keys.  EDGE (with 16 columns): the column sees those up to limit; else all but
+    // the hidden ones.
     template <bool EDGE>
     __device__ __forceinline__ void take(const CellRegs<D, BITS> (&c)[2], const Meta &x, int t0, int t1, int limit, int lane) {
         const int g = lane >> 4;
@@ -223,20 +257,20 @@ struct Columns {
         for (int j = 0; j < NC; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float s = 0.f;
+                float s = ROWS ? 0.f : pen[j][i];
 #pragma unroll
                 for (int y = 0; y < NG; ++y) {
                     const Affine k = affine(x, j, y, false, i);
                     s = fmaf(k.scale, acc[j][y][i], fmaf(k.bias, qsum[y], s));
                 }
-                if (BY_GROUP) s += dpp_mov<DPP_ROR8>(s);
+                if (BY_GROUP) s += dpp_mov<DPP_ROR8>(s);         // (both halves' -inf, or none)
                 if (EDGE && ((BY_CELL ? cell_of(lane & 15) : j) ? t1 : t0) + 4 * g + i > limit) s = -INFINITY;
                 p[j][i] = s;
             }
         float bm = -INFINITY;
 #pragma unroll
         for (int j = 0; j < NC; ++j) bm = fmaxf(bm, fmaxf(fmaxf(p[j][0], p[j][1]), fmaxf(p[j][2], p[j][3])));
-        if (__ballot(bm > m + lag)) {
+        if (since == SETTLE / 32 || __ballot(bm > m + lag)) {
             bm = fmaxf(bm, __shfl_xor(bm, 16));
             bm = fmaxf(bm, __shfl_xor(bm, 32));
             if (BY_CELL) bm = fmaxf(bm, other_cell(bm));
@@ -245,17 +279,9 @@ struct Columns {
             m = mn;
             ref = to;
             lsum *= alpha;
-#pragma unroll
-            for (int y = 0; y < NG; ++y) {
-                corr[y] *= alpha;
-#pragma unroll
-                for (int z = 0; z < 4; ++z) psum[y][z] *= alpha;
-            }
-#pragma unroll
-            for (int y = 0; y < DT; ++y)
-#pragma unroll
-                for (int z = 0; z < 4; ++z) o[y][z] *= alpha;
+            settle(alpha);
         }
+        ++since;
         // P of the lane's cells and groups; a position that the column does not see weighs 0
         // whatever its scale is
         uint32_t pw[2][NG][2];
@@ -307,28 +333,29 @@ struct Columns {
     }
 
     // The excess of the codes and the biases' part go into o, which from then on is the sum of
-    // p v.  Done every SETTLE keys: until then o holds up to EXCESS + MID times a scale more than
-    // the sum itself, whose fp32 roundings would add up over a long walk (512 keys: 16 sums of 32,
-    // at most 16 * 136 * 2^-24 = 2^-13 of a scale).
+    // p v, and is scaled.  Done every SETTLE keys at least: until then o holds up to EXCESS + MID
+    // times a scale more than the sum itself, whose fp32 roundings would add up over a long walk
+    // (512 keys: 16 sums of 32, at most 16 * 136 * 2^-24 = 2^-13 of a scale).
     static constexpr int SETTLE = 512;
-    __device__ __forceinline__ void settle() {
+    __device__ __forceinline__ void settle(float alpha) {
+        since = 0;
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
             float c = corr[j];
             c += __shfl_xor(c, 16);
             c += __shfl_xor(c, 32);
-            c = fmaf(-(EXCESS + MID), psum[j][0], c);
+            c = fmaf(-(EXCESS + MID), psum[j][0], c) * alpha;
             corr[j] = 0.f;
             psum[j] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int y = NG == 1 ? 0 : 4 * j; y < (NG == 1 ? DT : 4 * j + 4); ++y)
 #pragma unroll
-                for (int z = 0; z < 4; ++z) o[y][z] += c;
+                for (int z = 0; z < 4; ++z) o[y][z] = fmaf(o[y][z], alpha, c);
         }
     }
     // the column's sum of weights; o then is the column's sum of p v, in its dims tiles [first, first + n)
     __device__ __forceinline__ float close() {
-        settle();
+        settle(1.f);
         float l = lsum + __shfl_xor(lsum, 16);
         l += __shfl_xor(l, 32);
         if (BY_CELL) {
@@ -355,31 +382,38 @@ struct Columns {
 // nothing but their run, so there is no barrier; the next 32 keys' codes are on their way while
 // these are computed.
 constexpr int LINE_SHIFT = 7, LINE_KB = 1 << LINE_SHIFT;
-template <int D>
-constexpr int LINE_WAVES = D == 128 ? 2 : 3;             // a SIMD, where lines run alone
+// workgroups a CU, and waves a SIMD, where lines run alone
+constexpr int line_waves(int D, int bits) { return D == 64 ? 3 : 2; }
 
-template <int D, int BITS, int CW>
-__device__ __forceinline__ void attn_line(const QuantArgs &a, int wg, int w, uint8_t *smem) {
-    using C = Cell<D, BITS>;
-    using Cols = Columns<D, BITS, CW>;
-    const int threads = blockDim.x, tid = threadIdx.x, lane = tid & 63, c = lane & (CW - 1), g = lane >> 4;
-    // of every sequence: its first row, its keys, its first block and unit in the line
-    int32_t *first_row = reinterpret_cast<int32_t *>(smem), *keys = first_row + a.R, *off = keys + a.R, *unit = off + a.R;
-    int32_t *wsum = unit + a.R;
-    const int rows = __builtin_amdgcn_readfirstlane(live_rows(a));
-    const int P = __builtin_amdgcn_readfirstlane(a.join ? prefix_keys(a) : 0), pb = own_keyblocks(P, LINE_SHIFT);
+struct Line {
+    int32_t *first_row, *keys, *off, *unit;      // of every sequence, in LDS: first row, keys, first block and unit in the line
+    int rows, P, pb;                             // rows of the batch, joined keys of the prefix and their blocks
+    int total;                                   // blocks
+};
+constexpr int line_lds(int R) { return 4 * R * 4 + 64; }
 
+__device__ __forceinline__ Line line_of(const QuantArgs &a, uint8_t *smem) {
+    Line l;
+    l.first_row = reinterpret_cast<int32_t *>(smem);
+    l.keys = l.first_row + a.R;
+    l.off = l.keys + a.R;
+    l.unit = l.off + a.R;
+    int32_t *wsum = l.unit + a.R;
+    l.rows = __builtin_amdgcn_readfirstlane(live_rows(a));
+    l.P = __builtin_amdgcn_readfirstlane(a.join ? prefix_keys(a) : 0);
+    l.pb = own_keyblocks(l.P, LINE_SHIFT);
+    const int threads = blockDim.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     int t_before = 0, u_before = 0;
     for (int r0 = 0; r0 < a.R; r0 += threads) {
-        const int r = r0 + tid, wv = tid >> 6;
+        const int r = r0 + tid;
         int t = 0, u = 0;
         if (r < a.R) {
-            const Seq s = seq_of(a, r, rows);
-            const int kt = pb + own_keyblocks(s.len, LINE_SHIFT);
+            const Seq s = seq_of(a, r, l.rows);
+            const int kt = l.pb + own_keyblocks(s.len, LINE_SHIFT);
             u = kt && s.n <= a.small_rows ? a.Hkv * own_coltiles(s.n, a.G) : 0;
             t = u * kt;
-            first_row[r] = s.first;
-            keys[r] = s.len;
+            l.first_row[r] = s.first;
+            l.keys[r] = s.len;
         }
         int ts = t, us = u;
 #pragma unroll
@@ -395,14 +429,25 @@ __device__ __forceinline__ void attn_line(const QuantArgs &a, int wg, int w, uin
             t_before += wsum[i];
             u_before += wsum[8 + i];
         }
-        if (r < a.R) { off[r] = tb + ts - t; unit[r] = ub + us - u; }
+        if (r < a.R) { l.off[r] = tb + ts - t; l.unit[r] = ub + us - u; }
         __syncthreads();
     }
+    l.total = __builtin_amdgcn_readfirstlane(t_before);
+    return l;
+}
+
+template <int D, int BITS, int CW>
+__device__ __forceinline__ void attn_line(const QuantArgs &a, const Line &l, int wg, int w) {
+    using C = Cell<D, BITS>;
+    using Cols = Columns<D, BITS, CW>;
+    const int lane = threadIdx.x & 63, c = lane & (CW - 1), g = lane >> 4;
+    const int rows = l.rows, P = l.P, pb = l.pb, total = l.total;
+    int32_t *const first_row = l.first_row, *const keys = l.keys, *const off = l.off, *const unit = l.unit;
     if (wg == 0) {
         for (int r = lane + 64 * w; r < a.R; r += SA_THREADS) { a.own_off[r] = off[r]; a.own_unit[r] = unit[r]; }
-        if (lane + w == 0) a.own_off[a.R] = t_before;
+        if (lane + w == 0) a.own_off[a.R] = total;
     }
-    const int total = __builtin_amdgcn_readfirstlane(t_before), run = own_run(total, a.own_wgs);
+    const int run = own_run(total, a.own_wgs);
     int t = (int)min((long)wg * run, (long)total);
     const int t_end = min(t + run, total);
     if (t >= t_end) return;
@@ -416,30 +461,28 @@ __device__ __forceinline__ void attn_line(const QuantArgs &a, int wg, int w, uin
     int u_next = __builtin_amdgcn_readfirstlane(unit[r]);      // unit number of the next unit opened
     int in_seq = t - __builtin_amdgcn_readfirstlane(off[r]);   // block t within sequence r
 
-    struct Step {                // 32 keys of a wave's share of one unit
-        const int32_t *table;
-        int width;
+    struct Unit {                // the workgroup's run of one unit
+        const int32_t *table;    // the sequence's
         int hk, part, first, n;
         int col0;                // this wave's first column
         bool wide;               // a wave takes 16 columns and every key, not all columns and 32 keys of a block
-        int blk, stop, sub;      // the unit's block, and the one its blocks end at; wide: which 32 keys of it
-        int kb, end;             // the first of the 32 keys, and the keys some column sees, of the table
-        int all;                 // keys that every column sees
-        int rel;                 // the unit's row i sees keys up to rel + i (the prefix's: all)
-        int seen_own, all_own;
+        int stop;                // the block its blocks end at
+        int seen, all;           // own keys that some, that every column sees
+        int rel;                 // its row i sees own keys up to rel + i
+    };
+    struct Step {                // 32 keys of it
+        int kb;                  // the first of them in their table
+        bool pre;                // the prefix's
         bool fresh, last;        // the unit's first, last step here
     };
     bool first_unit = true;
-    auto place = [&](Step &s) {  // kb, table and bounds of the step
-        const bool pre = s.blk < pb;
-        s.kb = (pre ? s.blk : s.blk - pb) * LINE_KB + 32 * (s.wide ? s.sub : w);
-        s.table = pre ? a.prefix_table : a.tables + (size_t)r * a.width;
-        s.width = pre ? a.prefix_width : a.width;
-        s.end = pre ? P : s.seen_own;
-        s.all = pre ? P : s.all_own;
-        s.last = s.blk + 1 >= s.stop && (!s.wide || s.sub == 3);
+    int blk = 0, sub = 0;        // the step's block in its unit; of a wide unit, which 32 keys of it
+    auto place = [&](const Unit &u, Step &s) {
+        s.pre = blk < pb;
+        s.kb = (s.pre ? blk : blk - pb) * LINE_KB + 32 * (u.wide ? sub : w);
+        s.last = blk + 1 >= u.stop && (!u.wide || sub == 3);
     };
-    auto open = [&](Step &s) {   // the unit of block t; t moves to its end in the run
+    auto open = [&](Unit &u, Step &s) {      // the unit of block t; t moves to its end in the run
         if (t >= t_end) return false;
         int first, len, n, kt, ct;
         for (;; ++r, in_seq = 0) {
@@ -451,71 +494,77 @@ __device__ __forceinline__ void attn_line(const QuantArgs &a, int wg, int w, uin
             ct = own_coltiles(n, a.G);
             if (in_seq < a.Hkv * ct * kt || r == a.R - 1) break;
         }
-        const int u = in_seq / kt, b0 = in_seq - u * kt, b1 = min(kt, b0 + t_end - t);
+        const int x = in_seq / kt, b0 = in_seq - x * kt, b1 = min(kt, b0 + t_end - t);
         t += b1 - b0;
         in_seq += b1 - b0;
-        if (first_unit) u_next += u;
+        if (first_unit) u_next += x;
         first_unit = false;
-        s.fresh = true;
-        s.first = first;
-        s.n = n;
-        s.hk = u / ct;
-        s.wide = n * a.G > 16;
-        const int c0 = (u - s.hk * ct) * 64;
-        s.col0 = s.wide ? c0 + 16 * w : 0;
-        s.part = 4 * (u_next + wg) + w;
+        u.table = a.tables + (size_t)r * a.width;
+        u.first = first;
+        u.n = n;
+        u.hk = x / ct;
+        u.wide = n * a.G > 16;
+        const int c0 = (x - u.hk * ct) * 64;
+        u.col0 = u.wide ? c0 + 16 * w : 0;
+        u.part = 4 * (u_next + wg) + w;
         ++u_next;
-        s.blk = b0;
-        s.stop = b1;
-        s.sub = 0;
-        s.rel = len - n;
+        u.stop = b1;
+        u.rel = len - n;
         const int last = min((c0 + 63) / a.G, n - 1);          // the unit's last row
-        s.seen_own = clampi(s.rel + last + 1, 0, len);
-        s.all_own = clampi(s.rel + c0 / a.G + 1, 0, len);
-        place(s);
+        u.seen = clampi(u.rel + last + 1, 0, len);
+        u.all = clampi(u.rel + c0 / a.G + 1, 0, len);
+        blk = b0;
+        sub = 0;
+        s.fresh = true;
+        place(u, s);
         return true;
     };
-    auto advance = [&](Step &s) {
-        if (s.wide && s.sub < 3) ++s.sub;
-        else {
-            s.sub = 0;
-            if (++s.blk >= s.stop) return open(s);
-        }
+    auto advance = [&](Unit &u, Step &s) {
         s.fresh = false;
-        place(s);
+        if (u.wide && sub < 3) ++sub;
+        else {
+            sub = 0;
+            if (++blk >= u.stop) return open(u, s);
+        }
+        place(u, s);
         return true;
     };
     // block numbers of a step's two cells
     struct Ids { int b0, b1; };
-    auto ids_of = [&](const Step &s) {
+    auto ids_of = [&](const Unit &u, const Step &s) {
+        const int32_t *table = s.pre ? a.prefix_table : u.table;
+        const int last = (s.pre ? a.prefix_width : a.width) - 1;
         Ids x;
-        x.b0 = s.table[min(s.kb >> a.shift, s.width - 1)];
-        x.b1 = s.table[min((s.kb + 16) >> a.shift, s.width - 1)];
+        x.b0 = table[min(s.kb >> a.shift, last)];
+        x.b1 = table[min((s.kb + 16) >> a.shift, last)];
         return x;
     };
+    auto end_of = [&](const Unit &u, const Step &s) { return s.pre ? P : u.seen; };      // keys that are seen
     struct Keys {                // what a step reads
         CellRegs<D, BITS> c[2];
         typename Cols::Meta meta;
     };
-    auto load = [&](const Step &s, const Ids &x, Keys &k) {
-        if (s.kb >= s.end) return;           // nothing that is seen
+    auto load = [&](const Unit &u, const Step &s, const Ids &x, Keys &k) {
+        const int end = end_of(u, s);
+        if (s.kb >= end) return;             // nothing that is seen
         // (nor is a second cell read that no column sees: the first one again, its keys hidden)
-        const int t1 = s.kb + 16 < s.end ? s.kb + 16 : s.kb;
+        const int t1 = s.kb + 16 < end ? s.kb + 16 : s.kb;
         const int b0 = __builtin_amdgcn_readfirstlane(x.b0), b1 = __builtin_amdgcn_readfirstlane(t1 == s.kb ? x.b0 : x.b1);
-        const uint8_t *c0 = cell_at<C::BYTES>(a, s.hk, b0, s.kb), *c1 = cell_at<C::BYTES>(a, s.hk, b1, t1);
+        const uint8_t *c0 = cell_at<C::BYTES>(a, u.hk, b0, s.kb), *c1 = cell_at<C::BYTES>(a, u.hk, b1, t1);
         k.c[0].load(c0, lane);
         k.c[1].load(c1, lane);
         Cols::load_meta(k.meta, c0, c1, lane);
     };
     Cols col;
-    auto column = [&](const Step &s) {       // this lane's column's q row
-        const int i = (s.col0 + c) / a.G, h = s.hk * a.G + s.col0 + c - i * a.G;
-        return i < s.n ? a.q + (size_t)(s.first + i) * a.q_stride + (size_t)h * D : nullptr;
+    typename Cols::Row4 qn;      // q of the unit whose keys are on their way
+    auto load_q = [&](const Unit &u) {
+        const int i = (u.col0 + c) / a.G, h = u.hk * a.G + u.col0 + c - i * a.G;
+        Cols::load_q(qn, i < u.n ? a.q + (size_t)(u.first + i) * a.q_stride + (size_t)h * D : nullptr, lane);
     };
-    auto end = [&](const Step &s) {          // the part: the unit's columns that are there
+    auto end = [&](const Unit &u) {          // the part: the unit's columns that are there
         const float ltot = col.close();
-        if ((s.col0 + c) / a.G >= s.n || s.part >= a.own_parts || c >= a.part_cols) return;
-        const size_t at = (size_t)s.part * a.part_cols + c;
+        if ((u.col0 + c) / a.G >= u.n || u.part >= a.own_parts || c >= a.part_cols) return;
+        const size_t at = (size_t)u.part * a.part_cols + c;
         if (lane < CW) a.own_ml[at] = make_float2(ltot == ltot ? col.m * a.scale_log2 : INFINITY, ltot);
         float *po = a.own_o + at * D + 4 * g;
 #pragma unroll
@@ -523,40 +572,54 @@ __device__ __forceinline__ void attn_line(const QuantArgs &a, int wg, int w, uin
             if (Cols::writes(y, lane & 15)) *reinterpret_cast<f4 *>(po + 16 * y) = col.o[y];
     };
 
-    Step s, n;                   // this step, and the next
-    Keys cur, nxt;
-    open(s);
-    load(s, ids_of(s), nxt);
-    n = s;
-    bool more = advance(n);
-    Ids ids = ids_of(n);
-    int since = 0, limit = -1;
-    for (;;) {
-        cur = nxt;
-        const Step f = n;
+    Unit u, uf, un;              // of this step, the one whose keys are on their way, the one after it
+    Step s, f, n;
+    Keys k[2];
+    open(un, n);
+    uf = un;
+    f = n;
+    load(uf, f, ids_of(uf, f), k[0]);
+    load_q(uf);
+    bool more = advance(un, n);
+    Ids ids = ids_of(un, n);
+    int limit = -1;
+    auto step = [&](Keys &cur, Keys &nxt) {              // false: the last one
+        if (f.fresh) {
+            u = uf;
+            col.open(qn, lane, a.scale_log2);
+            const int i = (u.col0 + c) / a.G;
+            limit = i >= u.n ? -1 : u.rel + i;
+        }
+        s = f;
         const bool go = more;
         if (go) {
-            load(f, ids, nxt);
-            more = advance(n);
-            ids = ids_of(n);
+            if (n.fresh) uf = un;
+            f = n;
+            load(uf, f, ids, nxt);
+            if (f.fresh) load_q(uf);
+            more = advance(un, n);
+            ids = ids_of(un, n);
         }
-        if (s.fresh) {
-            col.open(column(s), lane, a.scale_log2);
-            since = 0;
-            const int i = (s.col0 + c) / a.G;
-            limit = i >= s.n ? -1 : s.rel + i;
-        }
-        if (s.col0 < s.n * a.G) {            // (a wave of a wide unit may have no column)
-            if (s.kb < s.end) {
-                if (since == Cols::SETTLE / 32) { col.settle(); since = 0; }
-                ++since;
-                if (s.kb + 32 <= s.all) col.template take<false>(cur.c, cur.meta, s.kb, s.kb + 16, 0, lane);
-                else col.template take<true>(cur.c, cur.meta, s.kb, s.kb + 16, s.blk < pb ? P - 1 : limit, lane);
+        const bool edge = s.kb + 32 > (s.pre ? P : u.all);
+        const int lim = s.pre ? P - 1 : limit;
+        if constexpr (Cols::ROWS) {
+            // (a wave of a wide unit may have no column)
+            if (u.col0 < u.n * a.G && s.kb < end_of(u, s)) {
+                if (!edge) col.template take<false>(cur.c, cur.meta, s.kb, s.kb + 16, lim, lane);
+                else col.template take<true>(cur.c, cur.meta, s.kb, s.kb + 16, lim, lane);
             }
-            if (s.last) end(s);
+        } else {
+            if (edge) col.hide(cur.meta, s.kb, s.kb + 16, lim, lane);
+            else col.show();
+            col.template take<false>(cur.c, cur.meta, s.kb, s.kb + 16, lim, lane);
         }
-        if (!go) break;
-        s = f;
+        if (s.last && u.col0 < u.n * a.G) end(u);
+        return go;
+    };
+    if constexpr (Cols::ROWS) {
+        do { k[1] = k[0]; } while (step(k[1], k[0]));
+    } else {
+        while (step(k[0], k[1]) && step(k[1], k[0])) {}
     }
 }
 
@@ -577,6 +640,7 @@ struct Values {
     struct Flow {
         uint32_t k[HALF], v[HALF];
         uint32_t km, vm;         // scales and biases: of the lane's position's key; of position 4 g + l % 4's value
+        int block;               // the next load's: its number in the pool, on its way
     };
     const QuantArgs &a;
     uint8_t *smem;
@@ -595,10 +659,14 @@ struct Values {
             x[0] = *reinterpret_cast<const uint32_t *>(p);
         }
     }
+    __device__ __forceinline__ int block_of(const int32_t *table, int width, int blk) const {
+        return table[min((blk * SA_KB + 16 * cell) >> a.shift, width - 1)];
+    }
+    // the codes of key block blk, and the number of the one after it
     __device__ __forceinline__ void load(Flow &f, int hk, const int32_t *table, int width, int blk) const {
         const int t = blk * SA_KB + 16 * cell, grp = C::GROUPS == 2 ? half : 0;
-        const int b = __builtin_amdgcn_readfirstlane(table[min(t >> a.shift, width - 1)]);
-        const uint8_t *p = cell_at<C::BYTES>(a, hk, b, t);
+        const uint8_t *p = cell_at<C::BYTES>(a, hk, __builtin_amdgcn_readfirstlane(f.block), t);
+        f.block = block_of(table, width, blk + 1);
         const int at = C::PLANES == 2 ? 1024 * half + lane * 16 : lane * C::LANE + 4 * HALF * half;
         words(f.k, p + at);
         words(f.v, p + C::CODES + at);
@@ -644,6 +712,7 @@ struct Values {
         }
     }
     __device__ __forceinline__ void open(Flow &f, int hk, const int32_t *table, int width, int b0) const {
+        f.block = block_of(table, width, b0);
         load(f, hk, table, width, b0);
         store(f, 0);
         load(f, hk, table, width, b0 + 1);
@@ -657,25 +726,67 @@ struct Values {
 
 // ---------------------------------------------------------------- kernels
 
+// Times in us that say how the CUs are shared out between tiles and lines: on a CU of its own a
+// tile's block (64 keys, 256 columns) and a line's (128 keys of a unit), and the bytes a us of
+// parts, which the kernel's end has to bring from the caches to memory and the merge reads.
+// Stamped in the kernel at 64 decoded rows behind 8192 positions, 32 heads of 128 on 8.
+constexpr float tile_block_us(int D) { return D == 128 ? 2.1f : 1.5f; }
+constexpr float line_block_us(int D) { return D == 128 ? 0.95f : 0.6f; }
+constexpr float PART_BYTES_US = 1.3e6f;
+
+// Into how many workgroups each column tile's keys are cut: of 1 .. most the number with which the
+// tiles' workgroups and the lines' on the CUs left are done first.  A lane a number.
+__device__ __forceinline__ int best_cut(int wgs, int blocks, int most, int grid, float tile_us, float line_us, float part_us) {
+    const int lane = threadIdx.x & 63, n = lane + 1;
+    float us = INFINITY;
+    if (n <= most && (wgs * n < grid || line_us == 0.f)) {
+        const float tile = (float)((blocks + n - 1) / n) * tile_us;
+        const float line = line_us == 0.f ? 0.f : line_us / (float)(grid - wgs * n);
+        us = fmaxf(tile, line) + (float)n * part_us;
+    }
+    float least = us;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) least = fminf(least, __shfl_xor(least, x));
+    return max(__ffsll((unsigned long long)__ballot(us == least)), 1);
+}
+
 // Column tiles and lines: workgroups of 8 waves, which take every register of a CU, of a tile of
 // 256 columns or of two of the line's.
 constexpr int QUANT_WAVES = 8;
 template <int D, int BITS, int CW>
 __global__ void __launch_bounds__(64 * QUANT_WAVES) __attribute__((amdgpu_waves_per_eu(2))) attn_quantized_kernel(QuantArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
-    if ((int)blockIdx.x < a.tile_wgs) {
-        attn_tile<D, Values<D, BITS>>(a, (int)blockIdx.x, smem);
+    const int id = (int)blockIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Line l;
+    if (a.cut) {
+        // tiles have the prefix alone, and everything else is in the line: cut by what there is
+        l = line_of(a, smem);
+        const int wgs = a.tiles * a.Hkv, blocks = (prefix_keys(a) + SA_KB - 1) / SA_KB;
+        const float line_us = (float)l.total * line_block_us(D);
+        const float part_us = (float)a.part_rows * a.H * (8 * D + 16) / PART_BYTES_US;
+        a.nsplit = __builtin_amdgcn_readfirstlane(best_cut(wgs, blocks, a.nsplit, (int)gridDim.x, tile_block_us(D), line_us, part_us));
+        a.tile_wgs = wgs * a.nsplit;
+        a.own_wgs = 2 * max((int)gridDim.x - a.tile_wgs, 1);
+        if (id == 0 && threadIdx.x == 0) { a.cut[0] = a.nsplit; a.cut[1] = a.own_wgs; }
+        if (id == 0) {       // (else the line's first workgroup's to write; there may be none)
+            for (int r = threadIdx.x; r < a.R; r += 64 * QUANT_WAVES) { a.own_off[r] = l.off[r]; a.own_unit[r] = l.unit[r]; }
+            if (threadIdx.x == 0) a.own_off[a.R] = l.total;
+        }
+        if (id < a.tile_wgs) __syncthreads();                  // the ring takes the line's LDS
+    }
+    if (id < a.tile_wgs) {
+        attn_tile<D, Values<D, BITS>>(a, id, smem);
         return;
     }
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    attn_line<D, BITS, CW>(a, ((int)blockIdx.x - a.tile_wgs) * (QUANT_WAVES / 4) + w / 4, w & 3, smem);
+    if (!a.cut) l = line_of(a, smem);
+    attn_line<D, BITS, CW>(a, l, (id - a.tile_wgs) * (QUANT_WAVES / 4) + w / 4, w & 3);
 }
 
 // Lines alone.
 template <int D, int BITS, int CW>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(LINE_WAVES<D>))) attn_line_kernel(QuantArgs a) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(line_waves(D, BITS)))) attn_line_kernel(QuantArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
-    attn_line<D, BITS, CW>(a, (int)blockIdx.x, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), smem);
+    attn_line<D, BITS, CW>(a, line_of(a, smem), (int)blockIdx.x, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
 }
 
 // ---------------------------------------------------------------- host side
@@ -695,7 +806,7 @@ int quant_splits(long wgs, long blocks, double part_bytes, bool last_is_whole, l
 
 // own_cap, prefix_cap: positions the tables have room for; max_new: at least the rows of
 // the sequence with the most
-SaPlan plan_quant(long N, long R, long H, long Hkv, long D, long own_cap, long prefix_cap, long max_new) {
+SaPlan plan_quant(long N, long R, long H, long Hkv, long D, int bits, long own_cap, long prefix_cap, long max_new) {
     SaPlan p;
     const long G = H / Hkv, cols = N * G, cus = device_info().num_cus;
     if (max_new > N) max_new = N;
@@ -707,19 +818,17 @@ SaPlan plan_quant(long N, long R, long H, long Hkv, long D, long own_cap, long p
     p.tiles = (cols + 32 * QUANT_WAVES - 1) / (32 * QUANT_WAVES);
     const long wgs = p.tiles * Hkv;
     const long blocks = (prefix_cap + (p.any_big ? own_cap : 0) + SA_KB - 1) / SA_KB;
-    // of the CUs, where tiles have the prefix alone, half at least for them, and a tenth for the lines
-    const double tile_work = (double)p.tiles * (prefix_cap / SA_KB + 1) * 2.0, line_work = (double)R * own_cap * 0.5 / 64 * 0.5;
-    const double share = tile_work / (tile_work + line_work);
-    const long most = p.any_big ? cus : (long)(cus * (share < 0.5 ? 0.5 : share > 0.9 ? 0.9 : share));
-    p.nsplit = p.use_tile ? quant_splits(wgs, blocks, (double)N * H * (8 * D + 16), p.any_big, most) : 1;
+    // where tiles have the prefix alone the kernel cuts them, into nsplit at most
+    p.cut = p.use_tile && !p.any_big && wgs < cus;
+    if (p.cut) p.nsplit = (int)std::min({64L, blocks, (cus - 1) / wgs});
+    else if (p.any_big) p.nsplit = quant_splits(wgs, blocks, (double)N * H * (8 * D + 16), p.any_big, cus);
     const long rows_max = max_new < p.small_rows ? max_new : p.small_rows;
     p.rows_max = (int)rows_max;
     long coltiles = R * ((rows_max * G + 63) / 64);
     if (coltiles > R + cols / 64) coltiles = R + cols / 64;
     const long keyblocks = coltiles * (own_keyblocks((int)own_cap, LINE_SHIFT) + (p.join ? own_keyblocks((int)prefix_cap, LINE_SHIFT) : 0));
-    long ow = p.use_tile && !p.any_big ? 2 * (cus - wgs * p.nsplit) : 2 * cus;
-    if (ow < cus / 4) ow = cus / 4;
-    if (ow > Hkv * keyblocks) ow = Hkv * keyblocks;
+    long ow = p.use_tile ? 2 * cus : line_waves((int)D, bits) * cus;
+    if (!p.cut && ow > Hkv * keyblocks) ow = Hkv * keyblocks;
     p.own_wgs = (int)(ow < 1 ? 1 : ow);
     p.own_parts = 4 * (Hkv * coltiles + p.own_wgs);
     p.part_cols = (int)(rows_max * G < 16 ? (rows_max * G > 1 ? rows_max * G : 1) : 16);
@@ -729,13 +838,13 @@ SaPlan plan_quant(long N, long R, long H, long Hkv, long D, long own_cap, long p
 
 template <int D, int BITS, int CW>
 int run_quant(const QuantArgs &a, const SaPlan &p, hipStream_t stream) {
-    const int line_lds = 4 * a.R * 4 + 64;
+    const int line = line_lds(a.R);
     if (a.tile_wgs == 0) {
-        hipLaunchKernelGGL((attn_line_kernel<D, BITS, CW>), dim3((unsigned)a.own_wgs), dim3(256), line_lds, stream, a);
+        hipLaunchKernelGGL((attn_line_kernel<D, BITS, CW>), dim3((unsigned)a.own_wgs), dim3(256), line, stream, a);
     } else {
-        const int lds = SaGeo<D>::LDS > line_lds ? SaGeo<D>::LDS : line_lds, per = QUANT_WAVES / 4;
-        hipLaunchKernelGGL((attn_quantized_kernel<D, BITS, CW>), dim3((unsigned)(a.tile_wgs + (a.own_wgs + per - 1) / per)),
-                           dim3(64 * QUANT_WAVES), lds, stream, a);
+        const int lds = SaGeo<D>::LDS > line ? SaGeo<D>::LDS : line, per = QUANT_WAVES / 4;
+        const int grid = a.cut ? device_info().num_cus : a.tile_wgs + (a.own_wgs + per - 1) / per;
+        hipLaunchKernelGGL((attn_quantized_kernel<D, BITS, CW>), dim3((unsigned)grid), dim3(64 * QUANT_WAVES), lds, stream, a);
     }
     SC_HIP_CHECK(hipGetLastError());
     return merge_parts<D>(a, p, stream);
@@ -761,7 +870,7 @@ bool bad_shape(long N, long R, long H, long Hkv, long D, long own_cap, long pref
 long attention_quantized_workspace_bytes(long N, long R, long H, long Hkv, long D, long own_cap, long prefix_cap,
                                          long max_new, int bits) {
     if (bad_shape(N, R, H, Hkv, D, own_cap, prefix_cap, max_new, bits) || N == 0) return 0;
-    return plan_quant(N, R, H, Hkv, D, own_cap, prefix_cap, max_new).bytes;
+    return plan_quant(N, R, H, Hkv, D, bits, own_cap, prefix_cap, max_new).bytes;
 }
 
 int launch_attention_quantized(const uint16_t *q, long q_stride, const uint8_t *pool, long n_blocks, long bs, int bits,
@@ -787,7 +896,7 @@ int launch_attention_quantized(const uint16_t *q, long q_stride, const uint8_t *
         return set_error(SC_EINVAL, "attention_quantized: bad row strides");
     if (((uintptr_t)q | (uintptr_t)pool) % 16 || (uintptr_t)out % 8)
         return set_error(SC_EINVAL, "attention_quantized: misaligned pointers");
-    const SaPlan p = plan_quant(N, R, H, Hkv, D, width * bs, prefix_width * bs, max_new);
+    const SaPlan p = plan_quant(N, R, H, Hkv, D, bits, width * bs, prefix_width * bs, max_new);
     if (!workspace || workspace_bytes < p.bytes || (uintptr_t)workspace % 16)
         return set_error(SC_EINVAL, "attention_quantized: a 16-byte aligned workspace of %ld bytes required", p.bytes);
     // 2^32 threads a launch

@@ -47,6 +47,7 @@ struct SaArgs {
     int own_parts, part_cols;
     int own_shift, join;     // log2 of the keys of an own block; join: the prefix's come before a sequence's own
     int32_t *own_off, *own_unit;         // [R + 1]: a sequence's first block (and all of them), its first unit
+    int32_t *cut;            // null, or nsplit and own_wgs as the kernel has chosen them
 };
 
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return min(max(v, lo), hi); }
@@ -452,9 +453,11 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
         if (s.n > a.small_rows && a.nsplit == 1) return;       // written by attn_tile
     }
     const int hk = h / a.G, gq = h - hk * a.G;
+    const int own_wgs = a.cut ? a.cut[1] : a.own_wgs;
+    if (a.cut) tile_parts = a.cut[0];
     const int joined = a.join ? own_keyblocks(prefix_keys(a), a.own_shift) : 0;
     const OwnParts own = own_parts_of(row, s.first, s.n, s.len, hk, gq, a.G, a.small_rows, a.own_off[r], a.own_unit[r],
-                                      a.own_off[a.R], a.own_wgs, a.own_parts, a.part_cols, a.own_shift, joined);
+                                      a.own_off[a.R], own_wgs, a.own_parts, a.part_cols, a.own_shift, joined);
     const int parts = tile_parts + own.n;
     float M = -INFINITY, L = 0.f, acc[PER] = {};
     for (int i0 = 0; i0 * WPR + turn < parts; i0 += 64) {
@@ -535,7 +538,7 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
 
 struct SaPlan {
     int small_rows = 0, rows_max = 0, any_big = 0, nsplit = 1, own_wgs = 0, use_tile = 0, part_cols = 0;
-    int own_shift = 6, join = 0;
+    int own_shift = 6, join = 0, cut = 0;
     long tiles = 0, own_parts = 0, part_rows = 0;
     int by_seq = 0, per_seq = 0;     // the merge, and attn_tile's parts, by sequence: rows of each
     long tile_o = 0, tile_ml = 0, own_o = 0, own_ml = 0, own_idx = 0, bytes = 0;      // workspace offsets
@@ -557,7 +560,7 @@ void lay_out(SaPlan &p, long N, long R, long H, long D) {
     p.tile_ml = at; at += up(tparts * 8);
     p.own_o = at; at += up(p.own_parts * p.part_cols * D * 4);
     p.own_ml = at; at += up(p.own_parts * p.part_cols * 8);
-    p.own_idx = at; at += up((R + 1) * 2 * 4);
+    p.own_idx = at; at += up((R + 1) * 2 * 4 + 8);
     p.bytes = at;
 }
 
@@ -589,6 +592,7 @@ void fill_args(SaArgs &a, const SaPlan &p, void *workspace) {
     a.own_shift = p.own_shift; a.join = p.join;
     a.own_off = reinterpret_cast<int32_t *>(ws + p.own_idx);
     a.own_unit = a.own_off + a.R + 1;
+    a.cut = p.cut ? a.own_unit + a.R + 1 : nullptr;
 }
 
 }  // namespace
