@@ -12,6 +12,11 @@ document, the prompt of several samples) are held once:
 * ``lengths`` int32 ``[sequences]``, ``prefix_len`` ``[1]``: positions held
 * ``free_blocks`` / ``n_free``: a stack of the blocks nobody holds
 
+With ``bits`` 4 or 8 keys and values are held as codes instead, in groups of 64 dims with a
+bf16 scale and bias each (4.5 or 8.5 bits a value): ``pool`` uint8 ``[layers, blocks, kv_heads,
+block_size / 16, bytes]`` in the place of ``k`` and ``vt``.  They are quantized as they are
+appended, new ones included in what a step attends.
+
 All of it is device memory and ``block_tables`` keeps it on the device, so a decode step
 captured in a HIP graph replays as the sequences grow.  ``host_lengths`` and ``host_free``
 are the host's mirror, from which a step that cannot fit is refused before its launch.
@@ -19,7 +24,7 @@ are the host's mirror, from which a step that cannot fit is refused before its l
 A model step is described by a :class:`BlockBatch` (``begin`` / ``begin_prefix``); indexed by
 the layer it gives the :class:`BlockLayerKV` that ``ParallelAttention.attend_qkv`` takes.
 """
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 
@@ -35,8 +40,12 @@ class BlockLayerKV:
 
     def __init__(self, batch: "BlockBatch", layer: int):
         self.batch = batch
-        self.k = batch.cache.k[layer]
-        self.vt = batch.cache.vt[layer]
+        self.bits = batch.cache.bits
+        if self.bits is None:
+            self.k = batch.cache.k[layer]
+            self.vt = batch.cache.vt[layer]
+        else:
+            self.pool = batch.cache.pool[layer]
 
 
 class BlockBatch:
@@ -69,27 +78,36 @@ class BlockBatch:
     def workspace_bytes(self, H: int, Hkv: int, D: int) -> int:
         bs = self.cache.block_size
         pre = 0 if self.prefix_table is None else self.prefix_table.numel() * bs
-        return _lib.attention_shared_workspace_bytes(self.rows, self.tables.shape[0], H, Hkv, D,
-                                                     self.tables.shape[1] * bs, pre, self.max_new)
+        sizes = (self.rows, self.tables.shape[0], H, Hkv, D, self.tables.shape[1] * bs, pre, self.max_new)
+        if self.cache.bits is not None:
+            return _lib.attention_quantized_workspace_bytes(*sizes, bits=self.cache.bits)
+        return _lib.attention_shared_workspace_bytes(*sizes)
 
 
 class BlockKVCache:
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_blocks: int, max_sequences: int,
-                 max_length: int, block_size: int = 64, max_prefix: int = 0, device: Optional[torch.device] = None):
+                 max_length: int, block_size: int = 64, max_prefix: int = 0, device: Optional[torch.device] = None,
+                 bits: Optional[int] = None):
         if block_size not in _lib.BLOCK_SIZES:
             raise ValueError(f"block_size must be one of {_lib.BLOCK_SIZES}, got {block_size}")
         if min(num_layers, num_kv_heads, head_dim, num_blocks, max_sequences, max_length) < 1 or max_prefix < 0:
             raise ValueError("a block cache needs at least one layer, head, block, sequence and position")
         if max_sequences > _lib.SHARED_MAX_SEQUENCES:
             raise ValueError(f"at most {_lib.SHARED_MAX_SEQUENCES} sequences, got {max_sequences}")
+        if bits is not None and bits not in _lib.CACHE_BITS:
+            raise ValueError(f"a block cache holds bf16 (bits None) or {_lib.CACHE_BITS} bits, got {bits}")
         if device is None:
             device = torch.device("cuda", torch.cuda.current_device())
-        self.num_layers, self.num_kv_heads, self.head_dim = num_layers, num_kv_heads, head_dim
+        self.num_layers, self.num_kv_heads, self.head_dim, self.bits = num_layers, num_kv_heads, head_dim, bits
         self.num_blocks, self.max_sequences, self.block_size = num_blocks, max_sequences, block_size
         self.max_length, self.max_prefix, self.device = max_length, max_prefix, device
         bf = torch.bfloat16
-        self.k = torch.zeros((num_layers, num_blocks, num_kv_heads, block_size, head_dim), dtype=bf, device=device)
-        self.vt = torch.zeros((num_layers, num_blocks, num_kv_heads, head_dim, block_size), dtype=bf, device=device)
+        if bits is None:
+            self.k = torch.zeros((num_layers, num_blocks, num_kv_heads, block_size, head_dim), dtype=bf, device=device)
+            self.vt = torch.zeros((num_layers, num_blocks, num_kv_heads, head_dim, block_size), dtype=bf, device=device)
+        else:
+            shape = _lib.quantized_pool_shape(num_blocks, num_kv_heads, block_size, head_dim, bits)
+            self.pool = torch.zeros((num_layers, *shape), dtype=torch.uint8, device=device)
 
         def i32(*shape):
             return torch.zeros(shape, dtype=torch.int32, device=device)
@@ -119,7 +137,7 @@ class BlockKVCache:
 
     @property
     def nbytes(self) -> int:
-        return 2 * self.k.numel() * self.k.element_size()
+        return self.pool.numel() if self.bits is not None else 2 * self.k.numel() * self.k.element_size()
 
     def _plan(self, new: Sequence[int], release: Optional[Sequence[bool]]):
         """(lengths, free blocks) after a step, or an error if it does not fit."""
@@ -183,6 +201,26 @@ class BlockKVCache:
         self.host_free -= need
         self.steps += 1
         return BlockBatch(self, step, tables, positions, positions, False)
+
+    def as_tuple(self, layer: int, sequence: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """``(k, v)`` of one sequence in the reference layout ``[1, kv_heads, length, head_dim]``
+        bf16, the shared prefix's positions first."""
+        if not 0 <= sequence < self.max_sequences:
+            raise IndexError(f"sequence {sequence} of {self.max_sequences}")
+        bs = self.block_size
+
+        def slots_of(table, n):
+            p = torch.arange(n, dtype=torch.int32, device=self.device)
+            return table[(p // bs).long()] * bs + p % bs
+        slots = slots_of(self.tables[sequence], self.host_lengths[sequence])
+        if self.host_prefix:
+            slots = torch.cat([slots_of(self.prefix_table, self.host_prefix), slots])
+        if self.bits is not None:
+            k, v = _lib.read_quantized(self.pool[layer], self.num_kv_heads, self.head_dim, slots, bits=self.bits)
+        else:
+            b, off = (slots // bs).long(), (slots % bs).long()
+            k, v = self.k[layer][b, :, off], self.vt[layer][b, :, :, off]
+        return k.transpose(0, 1)[None].contiguous(), v.transpose(0, 1)[None].contiguous()
 
     def check_status(self):
         """Raise if a step was refused on the device (one captured in a graph and replayed

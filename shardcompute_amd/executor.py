@@ -376,11 +376,13 @@ class ParallelExecutor:
 
     async def generate_batch(self, prompts: Sequence[Sequence[int]], prefix: Optional[Sequence[int]] = None,
                              max_new_tokens: int = 100, temperature: float = 0.0, top_p: float = 0.9,
-                             stop_tokens: Optional[List[int]] = None, block_size: int = 64) -> List[List[int]]:
+                             stop_tokens: Optional[List[int]] = None, block_size: int = 64,
+                             kv_bits: Optional[int] = None) -> List[List[int]]:
         """Tokens for several prompts of any lengths behind one shared ``prefix`` (the same
         prompt several times gives several samples of it at ``temperature`` > 0).
 
-        The prefix is computed and held once, in a :class:`BlockKVCache`; the prompts' own
+        The prefix is computed and held once, in a :class:`BlockKVCache` (``kv_bits`` 4 or 8: keys
+        and values held in so many bits, None: in bf16); the prompts' own
         tokens are taken in as one ragged step, then all sequences decode together
         (``temperature`` 0: the greedy step as a replayed HIP graph).  Returns each prompt's
         new tokens, up to its first stop token, which is included.  Sequences that have
@@ -395,7 +397,7 @@ class ParallelExecutor:
         m, R, prefix = self.model, len(prompts), [int(t) for t in prefix] if prefix is not None else []
         own = [-(-(len(p) + max_new_tokens) // block_size) for p in prompts]
         cache = m.new_block_cache(R, max(own) * block_size, sum(own) + -(-len(prefix) // block_size), block_size,
-                                  len(prefix))
+                                  len(prefix), bits=kv_bits)
         if prefix:
             await m.forward_blocks(prefix, cache.begin_prefix(len(prefix)))
         logits = await m.forward_blocks([t for p in prompts for t in p], cache.begin([len(p) for p in prompts]))

@@ -181,7 +181,8 @@ class ParallelAttention:
         ``[B, local heads, S, cached + S keys]`` (``attention.py:449-450``).
 
         With a :class:`~shardcompute_amd.block_cache.BlockLayerKV` the rows are those of its
-        step: a ragged batch behind a shared prefix, q rotated in place."""
+        step: a ragged batch behind a shared prefix, q rotated in place, keys and values quantized
+        where the cache holds codes."""
         H, Hk, D = self.local_num_heads, self.local_num_kv_heads, self.head_dim
         if isinstance(kv, BlockLayerKV):
             if mask is not None or pos_offset:
@@ -190,6 +191,12 @@ class ParallelAttention:
             if qkv.shape[0] != b.rows:
                 raise ValueError(f"the step has {b.rows} rows, got {qkv.shape[0]}")
             cos_t, sin_t = self.rope.tables(b.cache.rotary_positions, qkv.device)
+            if kv.bits is not None:
+                q = _lib.rope_append_quantized(qkv, H, Hk, D, cos_t, sin_t, kv.pool, st.slots, st.positions,
+                                               bits=kv.bits, out=qkv[:, :H * D])
+                return _lib.attention_quantized(q, H, Hk, D, kv.pool, st.row_starts, st.lengths, b.tables, self.scale,
+                                                bits=kv.bits, prefix_table=b.prefix_table, prefix_len=b.prefix_len,
+                                                max_new=b.max_new, out=out, workspace=workspace)
             q = _lib.rope_append_blocks(qkv, H, Hk, D, cos_t, sin_t, kv.k, kv.vt, st.slots, st.positions,
                                         out=qkv[:, :H * D])
             return _lib.attention_shared(q, H, Hk, D, kv.k, kv.vt, st.row_starts, st.lengths, b.tables, self.scale,

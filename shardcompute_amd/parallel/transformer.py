@@ -279,15 +279,15 @@ class ParallelTransformer:
         return KVCache(self.num_layers, batch, att.local_num_kv_heads, att.head_dim, capacity, device=self.device)
 
     def new_block_cache(self, max_sequences: int, max_length: int, num_blocks: Optional[int] = None,
-                        block_size: int = 64, max_prefix: int = 0) -> BlockKVCache:
+                        block_size: int = 64, max_prefix: int = 0, bits: Optional[int] = None) -> BlockKVCache:
         """A cache in blocks for ``max_sequences`` sequences of up to ``max_length`` own positions
         (rounded up to whole blocks) behind a shared prefix of up to ``max_prefix`` (default:
-        blocks for all of them)."""
+        blocks for all of them).  ``bits``: 4 or 8, keys and values as codes of so many bits."""
         att = self.layers[0].attention
         if num_blocks is None:
             num_blocks = max_sequences * -(-max_length // block_size) + -(-max_prefix // block_size)
         return BlockKVCache(self.num_layers, att.local_num_kv_heads, att.head_dim, num_blocks, max_sequences,
-                            max_length, block_size=block_size, max_prefix=max_prefix, device=self.device)
+                            max_length, block_size=block_size, max_prefix=max_prefix, device=self.device, bits=bits)
 
     def _embed_sync(self, input_ids, out=None):
         if isinstance(self.embed_tokens, VocabParallelEmbedding):

@@ -101,3 +101,18 @@ def test_wrappers_need_gpu_tensors():
                  lambda: _lib.attention_quantized(x, 1, 1, 64, pool, z, z, z, 1.0)):
         with pytest.raises(RuntimeError, match="GPU"):
             call()
+
+
+def test_cache_of_codes_on_the_host():
+    from shardcompute_amd.block_cache import BlockKVCache
+    cpu = torch.device("cpu")
+    for bits in (4, 8):
+        c = BlockKVCache(2, 3, 64, num_blocks=5, max_sequences=3, max_length=40, block_size=32, max_prefix=20, device=cpu,
+                         bits=bits)
+        assert c.pool.shape == (2, *_lib.quantized_pool_shape(5, 3, 32, 64, bits)) and c.pool.dtype is torch.uint8
+        assert c.nbytes == 2 * 5 * 3 * 2 * 16 * (2 * 64 * bits // 8 + 8) and not c.pool.any()
+        assert c._plan([17, 0, 16], None) == ([17, 0, 16], 3)
+    with pytest.raises(ValueError, match="bits"):
+        BlockKVCache(1, 1, 64, 4, 1, 64, device=cpu, bits=3)
+    with pytest.raises(ValueError, match="head_dim"):
+        BlockKVCache(1, 1, 80, 4, 1, 64, device=cpu, bits=4)
