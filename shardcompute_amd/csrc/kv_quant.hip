@@ -29,6 +29,8 @@ struct QuantAppendArgs {
     const int32_t *slots, *positions;
     int N, H, Hkv, shift, table_len;
     long n_slots;
+    int kv_wgs, kv_rows;     // workgroups that have keys and values, rows of one
+    int heads_per_wave;      // of q, the others'
 };
 
 struct Affine { float scale, bias; };
@@ -59,128 +61,227 @@ __device__ __forceinline__ uint4 pack8(const float *x) {
     return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
 }
 
-// A wave takes the heads of one row, D / 16 lanes a head: a lane has the dims i0 .. i0 + 7 and
-// D / 2 above them, so that a pair that is rotated together is in one lane.
+// D / 16 lanes of a row's head: a lane has the dims i0 .. i0 + 7 and D / 2 above them, so that a
+// pair that is rotated together is in one lane.
+template <int D>
+struct Lane {
+    uint4 a1, a2;
+    float c[8], sn[8];
+    __device__ __forceinline__ void values(const uint16_t *p) {
+        a1 = *reinterpret_cast<const uint4 *>(p);
+        a2 = *reinterpret_cast<const uint4 *>(p + D / 2);
+    }
+    __device__ __forceinline__ void angles(const QuantAppendArgs &a, int pos, int i0) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const float4 cv = *reinterpret_cast<const float4 *>(a.cos_t + (size_t)pos * (D / 2) + i0 + 4 * q);
+            const float4 sv = *reinterpret_cast<const float4 *>(a.sin_t + (size_t)pos * (D / 2) + i0 + 4 * q);
+            c[4 * q] = cv.x; c[4 * q + 1] = cv.y; c[4 * q + 2] = cv.z; c[4 * q + 3] = cv.w;
+            sn[4 * q] = sv.x; sn[4 * q + 1] = sv.y; sn[4 * q + 2] = sv.z; sn[4 * q + 3] = sv.w;
+        }
+    }
+    __device__ __forceinline__ void rotate(uint4 &o1, uint4 &o2) const {
+        float x[2][8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float x1 = bfe(a1, e), x2 = bfe(a2, e);
+            x[0][e] = add_rn(mul_rn(x1, c[e]), mul_rn(-x2, sn[e]));
+            x[1][e] = add_rn(mul_rn(x2, c[e]), mul_rn(x1, sn[e]));
+        }
+        o1 = pack8(x[0]);
+        o2 = pack8(x[1]);
+    }
+};
+
+// maxima over the D / 16 lanes of a head (every lane has it)
+template <int D>
+__device__ __forceinline__ float head_max(float v) {
+    v = fmaxf(v, dpp_mov<DPP_XOR1>(v));
+    v = fmaxf(v, dpp_mov<DPP_XOR2>(v));
+    return D == 128 ? fmaxf(v, dpp_mov<DPP_HALF_MIRROR>(v)) : v;
+}
+
+// Workgroups with keys and values have kv_rows rows of one kv head, the others q heads of a row a
+// wave.  Codes go to LDS first, as the rows lie in a cell, and leave from there: a key in
+// pieces of 16 bytes (8 of 4 bits and 64 dims), 4 values of consecutive slots that begin at a
+// multiple of 4 in pieces of 16 too (a lane of the cell: PLANE), other values byte by byte.
+//
+// Bound by memory for prompts, by the chain slot, row, scale, codes, store for single rows.
+constexpr int QA_ROWS = 64, QA_FEW_ROWS = 16;
+constexpr long QA_FEW = 512;
+
 template <int D, int BITS>
 __global__ void __launch_bounds__(256) rope_append_quantized_kernel(QuantAppendArgs a) {
     using C = Cell<D, BITS>;
-    constexpr int LPH = D / 16, HPW = 64 / LPH, HALF = D / 2;
-    const int heads = a.H + 2 * a.Hkv, parts = (heads + HPW - 1) / HPW;
-    const long wid = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63, hl = lane % LPH;
-    const int tok = (int)(wid / parts), h = (int)(wid - (long)tok * parts) * HPW + lane / LPH;
-    if (tok >= a.N || h >= heads) return;
-    const int slot = a.slots[tok], pos = a.positions[tok];
-    if (slot < 0 || slot >= a.n_slots || pos < 0 || pos >= a.table_len) return;
-    const int i0 = 8 * hl;
-    const uint16_t *row = a.qkv + (size_t)tok * a.qkv_stride + (size_t)h * D + i0;
-    const uint4 a1 = *reinterpret_cast<const uint4 *>(row), a2 = *reinterpret_cast<const uint4 *>(row + HALF);
-    float x[2][8];
-    if (h < a.H + a.Hkv) {
-        const float *ct = a.cos_t + (size_t)pos * HALF + i0, *st = a.sin_t + (size_t)pos * HALF + i0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float x1 = bfe(a1, e), x2 = bfe(a2, e), c = ct[e], s = st[e];
-            x[0][e] = add_rn(mul_rn(x1, c), mul_rn(-x2, s));
-            x[1][e] = add_rn(mul_rn(x2, c), mul_rn(x1, s));
-        }
-        const uint4 o1 = pack8(x[0]), o2 = pack8(x[1]);
-        if (h < a.H) {
+    constexpr int LPH = D / 16, HALF = D / 2;
+    constexpr int KROW = D * BITS / 8, KPAD = KROW + 16, VPAD = QA_ROWS + 8;
+    __shared__ __align__(16) uint8_t kcode[QA_ROWS * KPAD];      // [row][plane, g][PLANE]
+    __shared__ __align__(16) uint8_t vcode[D * VPAD];            // [dim][row]
+    __shared__ int slot_of[QA_ROWS + 4];
+    const int tid = threadIdx.x, lane = tid & 63;
+    if ((int)blockIdx.x >= a.kv_wgs) {
+        constexpr int HPW = 64 / LPH;
+        const int parts = (a.H + a.heads_per_wave - 1) / a.heads_per_wave;
+        const long wid = (long)((int)blockIdx.x - a.kv_wgs) * 4 + (tid >> 6);
+        const int tok = (int)(wid / parts), part = (int)(wid - (long)tok * parts);
+        if (tok >= a.N) return;
+        const int i0 = 8 * (lane % LPH), h0 = part * a.heads_per_wave + lane / LPH;
+        const int slot = a.slots[tok], pos = a.positions[tok];
+        const uint16_t *row = a.qkv + (size_t)tok * a.qkv_stride + i0;
+        Lane<D> x;
+        x.values(row + (size_t)min(h0, a.H - 1) * D);            // on its way while the slot and the angles are read
+        if (slot < 0 || slot >= a.n_slots || pos < 0 || pos >= a.table_len) return;
+        x.angles(a, pos, i0);
+        const int h1 = min(a.H, (part + 1) * a.heads_per_wave);
+#pragma unroll 4
+        for (int h = h0; h < h1; h += HPW) {
+            if (h != h0) x.values(row + (size_t)h * D);
+            uint4 o1, o2;
+            x.rotate(o1, o2);
             uint16_t *dst = a.q + (size_t)tok * a.q_stride + (size_t)h * D + i0;
             *reinterpret_cast<uint4 *>(dst) = o1;
             *reinterpret_cast<uint4 *>(dst + HALF) = o2;
-            return;
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) { x[0][e] = bfe(o1, e); x[1][e] = bfe(o2, e); }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) { x[0][e] = bfe(a1, e); x[1][e] = bfe(a2, e); }
+        return;
     }
-    const bool value = h >= a.H + a.Hkv;
-    const int hk = value ? h - a.H - a.Hkv : h - a.H;
-    // the groups' bounds: 128 dims, a group in each half; 64, both halves one group
-    float lo[2], hi[2], zero[2];                // zero: 0, or no number if a value is not finite
-#pragma unroll
-    for (int y = 0; y < 2; ++y) {
-        lo[y] = hi[y] = x[y][0];
-        zero[y] = x[y][0] * 0.f;
-#pragma unroll
-        for (int e = 1; e < 8; ++e) {
-            lo[y] = fminf(lo[y], x[y][e]);
-            hi[y] = fmaxf(hi[y], x[y][e]);
-            zero[y] = fmaf(x[y][e], 0.f, zero[y]);
+    const int hk = (int)blockIdx.x % a.Hkv, t0 = (int)blockIdx.x / a.Hkv * a.kv_rows, rows = min(a.kv_rows, a.N - t0);
+    const int shift = a.shift, cells = 1 << (shift - 4);
+    auto cell_of = [&](int slot) {
+        return a.pool + (((size_t)(slot >> shift) * a.Hkv + hk) * cells + ((slot & ((1 << shift) - 1)) >> 4)) * C::BYTES;
+    };
+    // Threads 0 .. 127 have keys, the others values.
+    constexpr int STEP = 128 / LPH;                              // rows at a time
+    const bool value = tid >= 128;
+    const int hl = lane % LPH, i0 = 8 * hl;
+    for (int r0 = 0; r0 < a.kv_rows; r0 += STEP) {
+        const int r = r0 + (tid & 127) / LPH, tok = t0 + r;
+        int slot = -1, pos = 0;
+        Lane<D> x;
+        if (r < rows) {
+            slot = a.slots[tok];
+            pos = a.positions[tok];
+            x.values(a.qkv + (size_t)tok * a.qkv_stride + (size_t)(a.H + (value ? a.Hkv : 0) + hk) * D + i0);
         }
-    }
-    if (C::GROUPS == 1) {
-        lo[0] = fminf(lo[0], lo[1]);
-        hi[0] = fmaxf(hi[0], hi[1]);
-        zero[0] += zero[1];
-    }
-    Affine af[2];
-#pragma unroll
-    for (int y = 0; y < C::GROUPS; ++y) {
-#pragma unroll
-        for (int m = 1; m < LPH; m <<= 1) {
-            lo[y] = fminf(lo[y], __shfl_xor(lo[y], m));
-            hi[y] = fmaxf(hi[y], __shfl_xor(hi[y], m));
-            zero[y] += __shfl_xor(zero[y], m);
+        if (slot >= a.n_slots || pos < 0 || pos >= a.table_len) slot = -1;
+        if (value && hl == 0 && r < QA_ROWS) slot_of[r] = slot;
+        if (slot < 0) continue;                                  // (all of a head's lanes)
+        if (!value) {
+            x.angles(a, pos, i0);
+            x.rotate(x.a1, x.a2);
         }
-        af[y] = affine_of<BITS>(lo[y], hi[y]);
-        // minima and maxima pass a NaN over: the group's scale keeps it
-        if (zero[y] != 0.f) af[y].scale = af[y].bias = __builtin_nanf("");
-    }
-    if (C::GROUPS == 1) af[1] = af[0];
-    const int t = slot & 15;
-    uint8_t *cell = a.pool + (((size_t)(slot >> a.shift) * a.Hkv + hk) * (1u << (a.shift - 4)) + ((slot & ((1 << a.shift) - 1)) >> 4)) * C::BYTES;
-    if (hl < C::GROUPS)
-        *reinterpret_cast<uint32_t *>(cell + C::meta(t, (value ? C::GROUPS : 0) + hl)) =
-            f2bf(af[hl].scale) | f2bf(af[hl].bias) << 16;
-    uint32_t code[2][8];
-#pragma unroll
-    for (int y = 0; y < 2; ++y)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) code[y][e] = code_of<BITS>(x[y][e], af[y]);
-    if (!value) {
+        float v[2][8], lo[2], hi[2], zero[2];                    // zero: 0, or no number if a value is not finite
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-            uint8_t *dst = cell + C::key_chunk(t, hl + y * LPH);
-            if (BITS == 4) {
-                uint32_t w = 0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) w |= code[y][e] << (4 * ((e >> 1) + 4 * (e & 1)));
-                *reinterpret_cast<uint32_t *>(dst) = w;
-            } else {
-                uint32_t w[2] = {0u, 0u};
+            for (int e = 0; e < 8; ++e) v[y][e] = bfe(y ? x.a2 : x.a1, e);
+            lo[y] = hi[y] = v[y][0];
+            zero[y] = v[y][0] * 0.f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) w[e >> 2] |= code[y][e] << (8 * (e & 3));
-                *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+            for (int e = 1; e < 8; ++e) {
+                lo[y] = fminf(lo[y], v[y][e]);
+                hi[y] = fmaxf(hi[y], v[y][e]);
+                zero[y] = fmaf(v[y][e], 0.f, zero[y]);
             }
         }
-        return;
+        // 128 dims: a group in each half; 64: both halves one group
+        if (C::GROUPS == 1) {
+            lo[0] = fminf(lo[0], lo[1]);
+            hi[0] = fmaxf(hi[0], hi[1]);
+            zero[0] += zero[1];
+        }
+        Affine af[2];
+#pragma unroll
+        for (int y = 0; y < C::GROUPS; ++y) {
+            lo[y] = -head_max<D>(-lo[y]);
+            hi[y] = head_max<D>(hi[y]);
+            af[y] = affine_of<BITS>(lo[y], hi[y]);
+            // minima and maxima pass a NaN over: the group's scale keeps it
+            if (head_max<D>(zero[y] == 0.f ? 0.f : 1.f) != 0.f) af[y].scale = af[y].bias = __builtin_nanf("");
+        }
+        if (C::GROUPS == 1) af[1] = af[0];
+        if (hl < C::GROUPS)
+            *reinterpret_cast<uint32_t *>(cell_of(slot) + C::meta(slot & 15, (value ? C::GROUPS : 0) + hl)) =
+                f2bf(af[hl].scale) | f2bf(af[hl].bias) << 16;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            uint32_t code[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) code[e] = code_of<BITS>(v[y][e], af[y]);
+            const int o = hl + y * LPH;                          // of the row's chunks of 8 dims
+            if (value) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) vcode[(8 * o + e) * VPAD + r] = (uint8_t)code[e];
+            } else {
+                const int grp = o >> 3, g = (o >> 1) & 3;
+                if (BITS == 4) {
+                    uint32_t w = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w |= code[e] << (4 * ((e >> 1) + 4 * (e & 1)));
+                    *reinterpret_cast<uint32_t *>(kcode + r * KPAD + g * C::PLANE + 8 * grp + 4 * (o & 1)) = w;
+                } else {
+                    uint32_t w[2] = {0u, 0u};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[e >> 2] |= code[e] << (8 * (e & 3));
+                    *reinterpret_cast<uint2 *>(kcode + r * KPAD + (4 * grp + g) * 16 + 8 * (o & 1)) = make_uint2(w[0], w[1]);
+                }
+            }
+        }
     }
-    if (BITS == 8) {
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) cell[C::value_byte(t, i0 + y * HALF + e)] = (uint8_t)code[y][e];
-        return;
+    __syncthreads();
+    // keys: a piece is PLANE bytes of a row
+    constexpr int PIECES = 4 * C::PLANES;
+    for (int i = tid; i < rows * PIECES; i += 256) {
+        const int r = i / PIECES, pc = i % PIECES, slot = slot_of[r];
+        if (slot < 0) continue;
+        uint8_t *dst = cell_of(slot) + 1024 * (pc >> 2) + (16 * (pc & 3) + (slot & 15)) * C::PLANE;
+        const uint8_t *src = kcode + r * KPAD + pc * C::PLANE;
+        if (C::PLANE == 16) *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(src);
+        else *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(src);
     }
-    // 4 bits: dims d and d + 16 share a byte, lane ^ 2 has the other; of a pair of lanes one
-    // writes the lower half's bytes and one the upper half's
-    const int y = (hl >> 1) & 1, d0 = (i0 & ~16) + y * HALF;
+    // values: rows r .. r + 3 are a quad if their slots are 4 q .. 4 q + 3
+    auto leads = [&](int r) {
+        const int s = slot_of[r];
+        return r + 3 < rows && s >= 0 && (s & 3) == 0 && slot_of[r + 1] == s + 1 && slot_of[r + 2] == s + 2 && slot_of[r + 3] == s + 3;
+    };
+    constexpr int WORDS = C::PLANE / 4, PER_ROW = 16 * C::PLANES;
+    for (int i = tid; i < rows * PER_ROW; i += 256) {
+        const int r = i / PER_ROW, l = i % 16, pl = i / 16 % C::PLANES;
+        if (!leads(r)) continue;
+        const int slot = slot_of[r];
+        // 4 codes of dim d, rows r .. r + 3: bytes r .. r + 3 of two aligned words
+        auto four = [&](int d) {
+            const uint32_t *p = reinterpret_cast<const uint32_t *>(vcode + d * VPAD + (r & ~3));
+            return __builtin_amdgcn_alignbyte(p[1], p[0], r & 3);
+        };
+        uint32_t w[WORDS];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const uint32_t give = y ? code[0][e] : code[1][e], keep = y ? code[1][e] : code[0][e];
-        const uint32_t got = (uint32_t)__shfl_xor((int)give, 2);
-        cell[C::value_byte(t, d0 + e)] = (uint8_t)(y ? got | keep << 4 : keep | got << 4);
+        for (int m = 0; m < WORDS; ++m)
+            w[m] = BITS == 4 ? four(32 * m + l) | four(32 * m + 16 + l) << 4 : four(16 * (4 * pl + m) + l);
+        uint8_t *dst = cell_of(slot) + C::CODES + 1024 * pl + (16 * ((slot & 15) >> 2) + l) * C::PLANE;
+        if constexpr (WORDS == 4) *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        else *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+    }
+    constexpr int BYTES = D * BITS / 8;
+    for (int i = tid; i < rows * BYTES; i += 256) {
+        const int r = i / BYTES, b = i % BYTES, slot = slot_of[r];
+        if (slot < 0) continue;
+        const int first = r - (slot & 3);
+        if (first >= 0 && leads(first) && slot_of[first] == slot - (slot & 3)) continue;
+        // byte b: of 4 bits, dims 32 m + l and 16 above it
+        const int l = b & 15, m = b >> 4, d = BITS == 4 ? 32 * m + l : 16 * m + l;
+        const uint32_t lo = vcode[d * VPAD + r], up = BITS == 4 ? vcode[(d + 16) * VPAD + r] : 0u;
+        cell_of(slot)[C::value_byte(slot & 15, d)] = (uint8_t)(lo | up << 4);
     }
 }
 
 // ---------------------------------------------------------------- reading back
 //
 // k, v [n, Hkv, D] bf16 of the positions at slots[n]: bf16(scale code + bias), the sum rounded
-// once (as dequantize); 0 for a slot outside the pool.  A thread 8 dims of a key and of a value.
+// once (as dequantize); 0 for a slot outside the pool.  D / 8 lanes of a row of one kv head: a lane
+// has 8 dims of the key, and of the value the dims l, 16 + l, .. of its place in the cell (two
+// places with 64 dims), which go through LDS into the row's order.
+//
+// Bound by memory: 40000 positions of 8 kv heads of 128 in 4 bits, see launch_read_quantized.
 struct QuantReadArgs {
     const uint8_t *pool;
     const int32_t *slots;
@@ -192,40 +293,61 @@ struct QuantReadArgs {
 template <int D, int BITS>
 __global__ void __launch_bounds__(256) read_quantized_kernel(QuantReadArgs a) {
     using C = Cell<D, BITS>;
-    constexpr int OCT = D / 8;
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    const long row = i / (a.Hkv * OCT);
+    constexpr int OCT = D / 8, ROWS = 256 / OCT, PAD = D + 8;
+    __shared__ __align__(16) uint16_t tile[ROWS * PAD];
+    const int hk = (int)(blockIdx.x % (unsigned)a.Hkv), r = threadIdx.x / OCT, o = threadIdx.x % OCT;
+    const long row = (long)(blockIdx.x / (unsigned)a.Hkv) * ROWS + r;
+    const int slot = row < a.n ? a.slots[row] : -1;
+    uint4 key = make_uint4(0u, 0u, 0u, 0u), val = key;
+    const bool there = slot >= 0 && slot < a.n_slots;
+    if (there) {
+        const int t = slot & 15;
+        const uint8_t *cell = a.pool + (((size_t)(slot >> a.shift) * a.Hkv + hk) * (1u << (a.shift - 4)) + ((slot & ((1 << a.shift) - 1)) >> 4)) * C::BYTES;
+        // the place's codes: byte t & 3 of each word is this position's
+        constexpr int PLACES = 16 / OCT, WORDS = C::LANE / 4;
+        uint32_t w[PLACES][WORDS], kw[2], m[C::ITEMS];
+#pragma unroll
+        for (int q = 0; q < PLACES; ++q) {
+            const int l = o + q * OCT;
+#pragma unroll
+            for (int pl = 0; pl < C::PLANES; ++pl) {
+                const uint8_t *p = cell + C::CODES + 1024 * pl + (16 * (t >> 2) + l) * C::PLANE;
+                if constexpr (C::PLANE == 16) {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(p);
+                    w[q][4 * pl] = x.x; w[q][4 * pl + 1] = x.y; w[q][4 * pl + 2] = x.z; w[q][4 * pl + 3] = x.w;
+                } else {
+                    const uint2 x = *reinterpret_cast<const uint2 *>(p);
+                    w[q][0] = x.x; w[q][1] = x.y;
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < BITS / 4; ++e) kw[e] = *reinterpret_cast<const uint32_t *>(cell + C::key_chunk(t, o) + 4 * e);
+#pragma unroll
+        for (int i = 0; i < C::ITEMS; ++i) m[i] = *reinterpret_cast<const uint32_t *>(cell + C::meta(t, i));
+        float x[8];
+        const uint32_t mk = C::GROUPS == 2 && o >= 8 ? m[1] : m[0];
+        const float ks = bf2f(mk & 0xFFFFu), kb = bf2f(mk >> 16);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            x[e] = fmaf(ks, BITS == 4 ? (float)((kw[0] >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u) : ubyte_f32(kw[e >> 2], e & 3), kb);
+        key = pack8(x);
+#pragma unroll
+        for (int q = 0; q < PLACES; ++q)
+#pragma unroll
+            for (int y = 0; y < D / 16; ++y) {
+                const uint32_t mv = m[C::GROUPS + y / 4];
+                uint32_t c = (w[q][BITS == 4 ? y >> 1 : y] >> (8 * (t & 3))) & 0xFFu;
+                if (BITS == 4) c = (y & 1) ? c >> 4 : c & 15u;
+                tile[r * PAD + 16 * y + o + q * OCT] = (uint16_t)f2bf(fmaf(bf2f(mv & 0xFFFFu), (float)c, bf2f(mv >> 16)));
+            }
+    }
+    __syncthreads();
     if (row >= a.n) return;
-    const int rest = (int)(i - row * (a.Hkv * OCT)), hk = rest / OCT, o = rest % OCT;
-    const int slot = a.slots[row];
-    uint16_t *k = a.k + (row * a.Hkv + hk) * D + 8 * o, *v = a.v + (row * a.Hkv + hk) * D + 8 * o;
-    if (slot < 0 || slot >= a.n_slots) {
-        *reinterpret_cast<uint4 *>(k) = *reinterpret_cast<uint4 *>(v) = make_uint4(0u, 0u, 0u, 0u);
-        return;
-    }
-    const int t = slot & 15, grp = o >> 3;
-    const uint8_t *cell = a.pool + (((size_t)(slot >> a.shift) * a.Hkv + hk) * (1u << (a.shift - 4)) + ((slot & ((1 << a.shift) - 1)) >> 4)) * C::BYTES;
-    const uint32_t mk = *reinterpret_cast<const uint32_t *>(cell + C::meta(t, grp));
-    const uint32_t mv = *reinterpret_cast<const uint32_t *>(cell + C::meta(t, C::GROUPS + grp));
-    const float ks = bf2f(mk & 0xFFFFu), kb = bf2f(mk >> 16), vs = bf2f(mv & 0xFFFFu), vb = bf2f(mv >> 16);
-    float x[8];
-    if (BITS == 4) {
-        const uint32_t w = *reinterpret_cast<const uint32_t *>(cell + C::key_chunk(t, o));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = fmaf(ks, (float)((w >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u), kb);
-    } else {
-        const uint2 w = *reinterpret_cast<const uint2 *>(cell + C::key_chunk(t, o));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = fmaf(ks, ubyte_f32(e < 4 ? w.x : w.y, e & 3), kb);
-    }
-    *reinterpret_cast<uint4 *>(k) = pack8(x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        uint32_t c = cell[C::value_byte(t, 8 * o + e)];
-        if (BITS == 4) c = (c >> (4 * ((o >> 1) & 1))) & 15u;
-        x[e] = fmaf(vs, (float)c, vb);
-    }
-    *reinterpret_cast<uint4 *>(v) = pack8(x);
+    if (there) val = *reinterpret_cast<const uint4 *>(tile + r * PAD + 8 * o);
+    const long at = (row * a.Hkv + hk) * D + 8 * o;
+    *reinterpret_cast<uint4 *>(a.k + at) = key;
+    *reinterpret_cast<uint4 *>(a.v + at) = val;
 }
 
 }  // namespace
@@ -254,8 +376,17 @@ int launch_rope_append_quantized(const uint16_t *qkv, long qkv_stride, uint16_t 
     a.cos_t = cos_t; a.sin_t = sin_t; a.slots = slots; a.positions = positions;
     a.N = (int)N; a.H = (int)H; a.Hkv = (int)Hkv; a.shift = shift; a.table_len = (int)table_len;
     a.n_slots = n_blocks * bs;
-    const long hpw = 64 / (D / 16), blocks = (N * ((H + 2 * Hkv + hpw - 1) / hpw) + 3) / 4;
+    // single rows in groups of few, so that the GPU has work (64 rows of 32 + 8 heads of 128)
+    a.kv_rows = N <= QA_FEW ? QA_FEW_ROWS : QA_ROWS;
+    const long kv_wgs = (N + a.kv_rows - 1) / a.kv_rows * Hkv;
+    // a token's q heads over several waves while tokens alone leave CUs idle
+    const long hpw = 64 / (D / 16), cus = device_info().num_cus;
+    long per = N >= 4 * cus ? H : N >= cus ? 2 * hpw : hpw;
+    if (per > H) per = H;
+    a.heads_per_wave = (int)per;
+    const long blocks = kv_wgs + (N * ((H + per - 1) / per) + 3) / 4;
     if (blocks >= (1L << 24)) return set_error(SC_EINVAL, "rope_append_quantized: too many rows");     // 2^32 threads
+    a.kv_wgs = (int)kv_wgs;
     auto kern = D == 128 ? (bits == 4 ? rope_append_quantized_kernel<128, 4> : rope_append_quantized_kernel<128, 8>)
                          : (bits == 4 ? rope_append_quantized_kernel<64, 4> : rope_append_quantized_kernel<64, 8>);
     hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, stream, a);
@@ -277,7 +408,7 @@ int launch_read_quantized(const uint8_t *pool, long n_blocks, long bs, int bits,
         return set_error(SC_EINVAL, "read_quantized: pointers must be 16-byte aligned");
     QuantReadArgs a;
     a.pool = pool; a.slots = slots; a.k = k; a.v = v; a.n = n; a.n_slots = n_blocks * bs; a.Hkv = (int)Hkv; a.shift = shift;
-    const long blocks = (n * Hkv * (D / 8) + 255) / 256;
+    const long rows = 256 / (D / 8), blocks = (n + rows - 1) / rows * Hkv;
     if (blocks >= (1L << 24)) return set_error(SC_EINVAL, "read_quantized: too many rows");            // 2^32 threads
     auto kern = D == 128 ? (bits == 4 ? read_quantized_kernel<128, 4> : read_quantized_kernel<128, 8>)
                          : (bits == 4 ? read_quantized_kernel<64, 4> : read_quantized_kernel<64, 8>);
