@@ -107,7 +107,7 @@ __device__ __forceinline__ float head_max(float v) {
 // multiple of 4 in pieces of 16 too (a lane of the cell: PLANE), other values byte by byte.
 //
 // Bound by memory for prompts, by the chain slot, row, scale, codes, store for single rows.
-constexpr int QA_ROWS = 64, QA_FEW_ROWS = 16;
+constexpr int QA_ROWS = 32, QA_FEW_ROWS = 16;
 constexpr long QA_FEW = 512;
 
 template <int D, int BITS>
@@ -153,17 +153,26 @@ __global__ void __launch_bounds__(256) rope_append_quantized_kernel(QuantAppendA
     constexpr int STEP = 128 / LPH;                              // rows at a time
     const bool value = tid >= 128;
     const int hl = lane % LPH, i0 = 8 * hl;
-    for (int r0 = 0; r0 < a.kv_rows; r0 += STEP) {
-        const int r = r0 + (tid & 127) / LPH, tok = t0 + r;
-        int slot = -1, pos = 0;
-        Lane<D> x;
+    constexpr int TIMES = QA_ROWS / STEP;
+    Lane<D> xs[TIMES];
+    int slots[TIMES], poss[TIMES] = {};
+#pragma unroll
+    for (int u = 0; u < TIMES; ++u) {                            // all loads before the first use
+        const int r = u * STEP + (tid & 127) / LPH, tok = t0 + r;
+        slots[u] = -1;
         if (r < rows) {
-            slot = a.slots[tok];
-            pos = a.positions[tok];
-            x.values(a.qkv + (size_t)tok * a.qkv_stride + (size_t)(a.H + (value ? a.Hkv : 0) + hk) * D + i0);
+            slots[u] = a.slots[tok];
+            poss[u] = a.positions[tok];
+            xs[u].values(a.qkv + (size_t)tok * a.qkv_stride + (size_t)(a.H + (value ? a.Hkv : 0) + hk) * D + i0);
         }
+    }
+#pragma unroll
+    for (int u = 0; u < TIMES; ++u) {
+        const int r = u * STEP + (tid & 127) / LPH, pos = poss[u];
+        int slot = slots[u];
+        Lane<D> &x = xs[u];
         if (slot >= a.n_slots || pos < 0 || pos >= a.table_len) slot = -1;
-        if (value && hl == 0 && r < QA_ROWS) slot_of[r] = slot;
+        if (value && hl == 0) slot_of[r] = slot;
         if (slot < 0) continue;                                  // (all of a head's lanes)
         if (!value) {
             x.angles(a, pos, i0);
@@ -201,7 +210,7 @@ __global__ void __launch_bounds__(256) rope_append_quantized_kernel(QuantAppendA
         if (C::GROUPS == 1) af[1] = af[0];
         if (hl < C::GROUPS)
             *reinterpret_cast<uint32_t *>(cell_of(slot) + C::meta(slot & 15, (value ? C::GROUPS : 0) + hl)) =
-                f2bf(af[hl].scale) | f2bf(af[hl].bias) << 16;
+                f2bf(hl ? af[1].scale : af[0].scale) | f2bf(hl ? af[1].bias : af[0].bias) << 16;
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
             uint32_t code[8];
