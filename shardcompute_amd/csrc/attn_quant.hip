@@ -388,8 +388,21 @@ constexpr int line_waves(int D, int bits) { return D == 64 ? 3 : 2; }
 struct Line {
     int32_t *first_row, *keys, *off, *unit;      // of every sequence, in LDS: first row, keys, first block and unit in the line
     int rows, P, pb;                             // rows of the batch, joined keys of the prefix and their blocks
-    int total;                                   // blocks
+    int total, units;                            // places (blocks first, after places_of also the units' rests), units
+    int rest;                                    // places after a unit's blocks that hold no keys
+    __device__ __forceinline__ int start(int r) const { return off[r] + rest * unit[r]; }
 };
+
+// A unit's opening and end cost as much as a block's keys or nearly (64 rows on 32 heads of 128:
+// workgroups with the short sequences' units took 39 us where the others took 26), so a unit is
+// given a place more than it has blocks, unless that makes runs longer than it can save.
+__device__ __forceinline__ bool with_rest(int total, int units, int wgs) {
+    return 5 * own_run(total + units, wgs) < 8 * own_run(total, wgs);
+}
+__device__ __forceinline__ void places_of(const QuantArgs &a, Line &l) {
+    l.rest = a.own_rest && with_rest(l.total, l.units, a.own_wgs) ? 1 : 0;
+    l.total += l.rest * l.units;
+}
 constexpr int line_lds(int R) { return 4 * R * 4 + 64; }
 
 __device__ __forceinline__ Line line_of(const QuantArgs &a, uint8_t *smem) {
@@ -433,7 +446,15 @@ __device__ __forceinline__ Line line_of(const QuantArgs &a, uint8_t *smem) {
         __syncthreads();
     }
     l.total = __builtin_amdgcn_readfirstlane(t_before);
+    l.units = __builtin_amdgcn_readfirstlane(u_before);
+    l.rest = 0;
     return l;
+}
+
+// for the merge
+__device__ __forceinline__ void write_line(const QuantArgs &a, const Line &l, int i, int n) {
+    for (int r = i; r < a.R; r += n) { a.own_off[r] = l.start(r); a.own_unit[r] = l.unit[r]; }
+    if (i == 0) { a.own_off[a.R] = l.total; a.own_unit[a.R] = l.rest; }
 }
 
 template <int D, int BITS, int CW>
@@ -442,11 +463,8 @@ __device__ __forceinline__ void attn_line(const QuantArgs &a, const Line &l, int
     using Cols = Columns<D, BITS, CW>;
     const int lane = threadIdx.x & 63, c = lane & (CW - 1), g = lane >> 4;
     const int rows = l.rows, P = l.P, pb = l.pb, total = l.total;
-    int32_t *const first_row = l.first_row, *const keys = l.keys, *const off = l.off, *const unit = l.unit;
-    if (wg == 0) {
-        for (int r = lane + 64 * w; r < a.R; r += SA_THREADS) { a.own_off[r] = off[r]; a.own_unit[r] = unit[r]; }
-        if (lane + w == 0) a.own_off[a.R] = total;
-    }
+    int32_t *const first_row = l.first_row, *const keys = l.keys, *const unit = l.unit;
+    if (wg == 0) write_line(a, l, lane + 64 * w, SA_THREADS);
     const int run = own_run(total, a.own_wgs);
     int t = (int)min((long)wg * run, (long)total);
     const int t_end = min(t + run, total);
@@ -455,11 +473,10 @@ __device__ __forceinline__ void attn_line(const QuantArgs &a, const Line &l, int
     int r = 0;
     for (int n = a.R; n > 1;) {
         const int half = n >> 1;
-        if (__builtin_amdgcn_readfirstlane(off[r + half]) <= t) { r += half; n -= half; }
+        if (__builtin_amdgcn_readfirstlane(l.start(r + half)) <= t) { r += half; n -= half; }
         else n = half;
     }
-    int u_next = __builtin_amdgcn_readfirstlane(unit[r]);      // unit number of the next unit opened
-    int in_seq = t - __builtin_amdgcn_readfirstlane(off[r]);   // block t within sequence r
+    int in_seq = t - __builtin_amdgcn_readfirstlane(l.start(r));   // place t within sequence r
 
     struct Unit {                // the workgroup's run of one unit
         const int32_t *table;    // the sequence's
@@ -475,7 +492,6 @@ __device__ __forceinline__ void attn_line(const QuantArgs &a, const Line &l, int
         bool pre;                // the prefix's
         bool fresh, last;        // the unit's first, last step here
     };
-    bool first_unit = true;
     int blk = 0, sub = 0;        // the step's block in its unit; of a wide unit, which 32 keys of it
     auto place = [&](const Unit &u, Step &s) {
         s.pre = blk < pb;
@@ -483,22 +499,30 @@ __device__ __forceinline__ void attn_line(const QuantArgs &a, const Line &l, int
         s.last = blk + 1 >= u.stop && (!u.wide || sub == 3);
     };
     auto open = [&](Unit &u, Step &s) {      // the unit of block t; t moves to its end in the run
-        if (t >= t_end) return false;
-        int first, len, n, kt, ct;
-        for (;; ++r, in_seq = 0) {
+        int first, len, n, kt, ct, x, b0;
+        for (;;) {
+            if (t >= t_end) return false;
             first = __builtin_amdgcn_readfirstlane(first_row[r]);
             len = __builtin_amdgcn_readfirstlane(keys[r]);
             n = (r + 1 < a.R ? __builtin_amdgcn_readfirstlane(first_row[r + 1]) : rows) - first;
             if (n > a.small_rows) n = 0;
             kt = pb + own_keyblocks(len, LINE_SHIFT);
             ct = own_coltiles(n, a.G);
-            if (in_seq < a.Hkv * ct * kt || r == a.R - 1) break;
+            const int places = kt + l.rest;
+            if (kt == 0 || in_seq >= a.Hkv * ct * places) {
+                if (++r == a.R) return false;
+                in_seq = 0;
+                continue;
+            }
+            x = in_seq / places;
+            b0 = in_seq - x * places;
+            if (b0 < kt) break;
+            t += places - b0;
+            in_seq += places - b0;
         }
-        const int x = in_seq / kt, b0 = in_seq - x * kt, b1 = min(kt, b0 + t_end - t);
+        const int b1 = min(kt, b0 + t_end - t);
         t += b1 - b0;
         in_seq += b1 - b0;
-        if (first_unit) u_next += x;
-        first_unit = false;
         u.table = a.tables + (size_t)r * a.width;
         u.first = first;
         u.n = n;
@@ -506,8 +530,7 @@ __device__ __forceinline__ void attn_line(const QuantArgs &a, const Line &l, int
         u.wide = n * a.G > 16;
         const int c0 = (x - u.hk * ct) * 64;
         u.col0 = u.wide ? c0 + 16 * w : 0;
-        u.part = 4 * (u_next + wg) + w;
-        ++u_next;
+        u.part = 4 * (__builtin_amdgcn_readfirstlane(unit[r]) + x + wg) + w;
         u.stop = b1;
         u.rel = len - n;
         const int last = min((c0 + 63) / a.G, n - 1);          // the unit's last row
@@ -575,7 +598,7 @@ __device__ __forceinline__ void attn_line(const QuantArgs &a, const Line &l, int
     Unit u, uf, un;              // of this step, the one whose keys are on their way, the one after it
     Step s, f, n;
     Keys k[2];
-    open(un, n);
+    if (!open(un, n)) return;
     uf = un;
     f = n;
     load(uf, f, ids_of(uf, f), k[0]);
@@ -583,7 +606,13 @@ __device__ __forceinline__ void attn_line(const QuantArgs &a, const Line &l, int
     bool more = advance(un, n);
     Ids ids = ids_of(un, n);
     int limit = -1;
+    // Two waves on a SIMD: each goes first every other step (the older one always: it ended at 25 us
+    // of 40, and the other went on alone; 64 decoded rows take 1 us less so)
+    bool first = wg & 1;
     auto step = [&](Keys &cur, Keys &nxt) {              // false: the last one
+        if (first) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
+        first = !first;
         if (f.fresh) {
             u = uf;
             col.open(qn, lane, a.scale_log2);
@@ -731,17 +760,20 @@ struct Values {
 // parts, which the kernel's end has to bring from the caches to memory and the merge reads.
 // Stamped in the kernel at 64 decoded rows behind 8192 positions, 32 heads of 128 on 8.
 constexpr float tile_block_us(int D) { return D == 128 ? 2.1f : 1.5f; }
-constexpr float line_block_us(int D) { return D == 128 ? 0.95f : 0.6f; }
+constexpr float line_block_us(int D) { return D == 128 ? 2.3f : 1.4f; }
+constexpr float TILE_OPEN_US = 5.f;
 constexpr float PART_BYTES_US = 1.3e6f;
 
 // Into how many workgroups each column tile's keys are cut: of 1 .. most the number with which the
 // tiles' workgroups and the lines' on the CUs left are done first.  A lane a number.
-__device__ __forceinline__ int best_cut(int wgs, int blocks, int most, int grid, float tile_us, float line_us, float part_us) {
+__device__ __forceinline__ int best_cut(int wgs, int blocks, int most, int grid, const Line &l, float tile_us, float line_us, float part_us) {
     const int lane = threadIdx.x & 63, n = lane + 1;
     float us = INFINITY;
-    if (n <= most && (wgs * n < grid || line_us == 0.f)) {
-        const float tile = (float)((blocks + n - 1) / n) * tile_us;
-        const float line = line_us == 0.f ? 0.f : line_us / (float)(grid - wgs * n);
+    if (n <= most && (wgs * n < grid || l.total == 0)) {
+        const float tile = (float)((blocks + n - 1) / n) * tile_us + TILE_OPEN_US;
+        const int own = 2 * max(grid - wgs * n, 1);
+        const float run = with_rest(l.total, l.units, own) ? (float)own_run(l.total + l.units, own) : 1.6f * (float)own_run(l.total, own);
+        const float line = l.total == 0 ? 0.f : run * line_us;
         us = fmaxf(tile, line) + (float)n * part_us;
     }
     float least = us;
@@ -762,23 +794,20 @@ __global__ void __launch_bounds__(64 * QUANT_WAVES) __attribute__((amdgpu_waves_
         // tiles have the prefix alone, and everything else is in the line: cut by what there is
         l = line_of(a, smem);
         const int wgs = a.tiles * a.Hkv, blocks = (prefix_keys(a) + SA_KB - 1) / SA_KB;
-        const float line_us = (float)l.total * line_block_us(D);
         const float part_us = (float)a.part_rows * a.H * (8 * D + 16) / PART_BYTES_US;
-        a.nsplit = __builtin_amdgcn_readfirstlane(best_cut(wgs, blocks, a.nsplit, (int)gridDim.x, tile_block_us(D), line_us, part_us));
+        a.nsplit = __builtin_amdgcn_readfirstlane(best_cut(wgs, blocks, a.nsplit, (int)gridDim.x, l, tile_block_us(D), line_block_us(D), part_us));
         a.tile_wgs = wgs * a.nsplit;
         a.own_wgs = 2 * max((int)gridDim.x - a.tile_wgs, 1);
         if (id == 0 && threadIdx.x == 0) { a.cut[0] = a.nsplit; a.cut[1] = a.own_wgs; }
-        if (id == 0) {       // (else the line's first workgroup's to write; there may be none)
-            for (int r = threadIdx.x; r < a.R; r += 64 * QUANT_WAVES) { a.own_off[r] = l.off[r]; a.own_unit[r] = l.unit[r]; }
-            if (threadIdx.x == 0) a.own_off[a.R] = l.total;
-        }
+        places_of(a, l);
+        if (id == 0) write_line(a, l, threadIdx.x, 64 * QUANT_WAVES);      // (the line may have no workgroup)
         if (id < a.tile_wgs) __syncthreads();                  // the ring takes the line's LDS
     }
     if (id < a.tile_wgs) {
         attn_tile<D, Values<D, BITS>>(a, id, smem);
         return;
     }
-    if (!a.cut) l = line_of(a, smem);
+    if (!a.cut) { l = line_of(a, smem); places_of(a, l); }
     attn_line<D, BITS, CW>(a, l, (id - a.tile_wgs) * (QUANT_WAVES / 4) + w / 4, w & 3);
 }
 
@@ -786,7 +815,9 @@ __global__ void __launch_bounds__(64 * QUANT_WAVES) __attribute__((amdgpu_waves_
 template <int D, int BITS, int CW>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(line_waves(D, BITS)))) attn_line_kernel(QuantArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
-    attn_line<D, BITS, CW>(a, line_of(a, smem), (int)blockIdx.x, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+    Line l = line_of(a, smem);
+    places_of(a, l);
+    attn_line<D, BITS, CW>(a, l, (int)blockIdx.x, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
 }
 
 // ---------------------------------------------------------------- host side
@@ -813,6 +844,7 @@ SaPlan plan_quant(long N, long R, long H, long Hkv, long D, int bits, long own_c
     p.own_shift = LINE_SHIFT;
     p.small_rows = (int)(64 / G > 1 ? 64 / G : 1);
     p.any_big = max_new > p.small_rows;
+    p.own_rest = R > 1;
     p.join = !p.any_big && prefix_cap > 0 && R == 1;
     p.use_tile = p.any_big || (prefix_cap > 0 && !p.join);
     p.tiles = (cols + 32 * QUANT_WAVES - 1) / (32 * QUANT_WAVES);
@@ -826,7 +858,7 @@ SaPlan plan_quant(long N, long R, long H, long Hkv, long D, int bits, long own_c
     p.rows_max = (int)rows_max;
     long coltiles = R * ((rows_max * G + 63) / 64);
     if (coltiles > R + cols / 64) coltiles = R + cols / 64;
-    const long keyblocks = coltiles * (own_keyblocks((int)own_cap, LINE_SHIFT) + (p.join ? own_keyblocks((int)prefix_cap, LINE_SHIFT) : 0));
+    const long keyblocks = coltiles * (own_keyblocks((int)own_cap, LINE_SHIFT) + (p.join ? own_keyblocks((int)prefix_cap, LINE_SHIFT) : 0) + p.own_rest);
     long ow = p.use_tile ? 2 * cus : line_waves((int)D, bits) * cus;
     if (!p.cut && ow > Hkv * keyblocks) ow = Hkv * keyblocks;
     p.own_wgs = (int)(ow < 1 ? 1 : ow);
@@ -862,7 +894,7 @@ bool bad_shape(long N, long R, long H, long Hkv, long D, long own_cap, long pref
            kv_cell_bytes(D, bits) == 0 || own_cap <= 0 || own_cap >= (1L << 30) || prefix_cap < 0 ||
            prefix_cap >= (1L << 30) || max_new < 0 ||
            // attn_line numbers its key blocks in 32 bits
-           R * Hkv * ((H / Hkv + 63) / 64) * ((own_cap + prefix_cap) / LINE_KB + 2) >= (1L << 31);
+           R * Hkv * ((H / Hkv + 63) / 64) * ((own_cap + prefix_cap) / LINE_KB + 3) >= (1L << 31);
 }
 
 }  // namespace

@@ -46,6 +46,7 @@ struct SaArgs {
     float2 *own_ml;
     int own_parts, part_cols;
     int own_shift, join;     // log2 of the keys of an own block; join: the prefix's come before a sequence's own
+    int own_rest;            // own_unit[R] is the number of places after each unit's blocks that hold no keys, else there are none
     int32_t *own_off, *own_unit;         // [R + 1]: a sequence's first block (and all of them), its first unit
     int32_t *cut;            // null, or nsplit and own_wgs as the kernel has chosen them
 };
@@ -457,7 +458,8 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
     if (a.cut) tile_parts = a.cut[0];
     const int joined = a.join ? own_keyblocks(prefix_keys(a), a.own_shift) : 0;
     const OwnParts own = own_parts_of(row, s.first, s.n, s.len, hk, gq, a.G, a.small_rows, a.own_off[r], a.own_unit[r],
-                                      a.own_off[a.R], own_wgs, a.own_parts, a.part_cols, a.own_shift, joined);
+                                      a.own_off[a.R], own_wgs, a.own_parts, a.part_cols, a.own_shift, joined,
+                                      a.own_rest ? a.own_unit[a.R] : 0);
     const int parts = tile_parts + own.n;
     float M = -INFINITY, L = 0.f, acc[PER] = {};
     for (int i0 = 0; i0 * WPR + turn < parts; i0 += 64) {
@@ -538,7 +540,7 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
 
 struct SaPlan {
     int small_rows = 0, rows_max = 0, any_big = 0, nsplit = 1, own_wgs = 0, use_tile = 0, part_cols = 0;
-    int own_shift = 6, join = 0, cut = 0;
+    int own_shift = 6, own_rest = 0, join = 0, cut = 0;
     long tiles = 0, own_parts = 0, part_rows = 0;
     int by_seq = 0, per_seq = 0;     // the merge, and attn_tile's parts, by sequence: rows of each
     long tile_o = 0, tile_ml = 0, own_o = 0, own_ml = 0, own_idx = 0, bytes = 0;      // workspace offsets
@@ -589,7 +591,7 @@ void fill_args(SaArgs &a, const SaPlan &p, void *workspace) {
     a.own_o = reinterpret_cast<float *>(ws + p.own_o);
     a.own_ml = reinterpret_cast<float2 *>(ws + p.own_ml);
     a.own_parts = (int)p.own_parts; a.part_cols = p.part_cols;
-    a.own_shift = p.own_shift; a.join = p.join;
+    a.own_shift = p.own_shift; a.own_rest = p.own_rest; a.join = p.join;
     a.own_off = reinterpret_cast<int32_t *>(ws + p.own_idx);
     a.own_unit = a.own_off + a.R + 1;
     a.cut = p.cut ? a.own_unit + a.R + 1 : nullptr;

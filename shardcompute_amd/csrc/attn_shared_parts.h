@@ -32,17 +32,18 @@ struct OwnParts {
 // blocks of the row's unit, the four waves' or (a wide unit) that of the wave whose column
 // it is.  total: blocks of all sequences.  A row outside the sequence (row starts that begin
 // above 0 or do not ascend) has none, nor has one whose parts would not all be there.
-// shift: log2 of a block's keys; before: blocks that come before the sequence's own.
+// shift: log2 of a block's keys; before: blocks that come before the sequence's own; rest:
+// places in the line, after each unit's blocks, that hold no keys.
 __host__ __device__ __forceinline__ OwnParts own_parts_of(int row, int first, int n, int len, int hk, int gq, int G,
                                                           int small_rows, int off, int unit, int total, int own_wgs,
                                                           int own_parts, int part_cols, int shift = 6,
-                                                          int before = 0) {
+                                                          int before = 0, int rest = 0) {
     OwnParts p = {0, 0, 1, 0};
     const int kt = before + (len > 0 ? own_keyblocks(len, shift) : 0);
     if (row < first || row >= first + n || n > small_rows || kt <= 0) return p;
     const int run = own_run(total, own_wgs), ct = own_coltiles(n, G);
     const int col = (row - first) * G + gq, u = hk * ct + (col >> 6);
-    const int t0 = off + u * kt, w0 = t0 / run, wgs = (t0 + kt - 1) / run - w0 + 1;
+    const int t0 = off + u * (kt + rest), w0 = t0 / run, wgs = (t0 + kt - 1) / run - w0 + 1;
     const bool wide = n * G > 16;
     p.first = 4 * (unit + u + w0) + (wide ? (col >> 4) & 3 : 0);
     p.step = wide ? 4 : 1;

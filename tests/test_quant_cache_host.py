@@ -116,3 +116,85 @@ def test_cache_of_codes_on_the_host():
         BlockKVCache(1, 1, 64, 4, 1, 64, device=cpu, bits=3)
     with pytest.raises(ValueError, match="head_dim"):
         BlockKVCache(1, 1, 80, 4, 1, 64, device=cpu, bits=4)
+
+
+PARTS_SOURCE = r"""
+#include "attn_shared_parts.h"
+extern "C" void parts_of(const int *a, int *out) {
+    const sc::OwnParts p = sc::own_parts_of(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], a[11],
+                                            a[12], a[13], a[14], a[15], a[16]);
+    out[0] = p.first; out[1] = p.n; out[2] = p.step; out[3] = p.col;
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def parts_of(tmp_path_factory):
+    import ctypes
+    import os
+    import shutil
+    import subprocess
+
+    from shardcompute_amd import build
+
+    if not (shutil.which("hipcc") or os.path.exists("/opt/rocm/bin/hipcc")):
+        pytest.skip("no hipcc")
+    d = tmp_path_factory.mktemp("parts")
+    src, lib = d / "parts.hip", d / "parts.so"
+    src.write_text(PARTS_SOURCE)
+    subprocess.run([build.hipcc(), "--cuda-host-only", "-O1", "-std=c++17", "-shared", "-fPIC", "-I", build.CSRC, str(src),
+                    "-o", str(lib)], check=True, capture_output=True)
+    fn = ctypes.CDLL(str(lib)).parts_of
+    I17, I4 = ctypes.c_int * 17, ctypes.c_int * 4
+
+    def call(*a):
+        out = I4()
+        fn(I17(*a), out)
+        return tuple(out)
+    return call
+
+
+@pytest.mark.parametrize("rest", [0, 1, 2])
+@pytest.mark.parametrize("seed", range(6))
+def test_parts_of_units_with_rests(parts_of, rest, seed):
+    """The parts that the merge reads are those of the runs that hold blocks of the row's unit:
+    units' blocks and the empty places after them laid in a line, cut into equal runs."""
+    import random
+
+    rng = random.Random(seed)
+    shift, small, hkv = 7, 16, rng.choice([1, 2, 8])
+    G = rng.choice([1, 4, 8])
+    R, wgs = rng.randint(1, 12), rng.choice([1, 3, 17, 64, 512])
+    ns = [rng.choice([0, 1, 1, 1, 3, 16, 40]) for _ in range(R)]
+    lens = [n + rng.choice([0, 0, 1, 100, 127, 128, 129, 3000]) for n in ns]
+    line, off, unit, units, where = [], [], [], 0, {}
+    for r, (n, ln) in enumerate(zip(ns, lens)):
+        off.append(len(line))
+        unit.append(units)
+        kt = -(-ln // 128)
+        if n == 0 or n > small or kt == 0:
+            continue
+        ct = -(-n * G // 64)
+        for u in range(hkv * ct):
+            where[(r, u)] = units
+            line += [units] * kt + [None] * rest
+            units += 1
+    total = len(line)
+    run = -(-total // wgs) if total else 1
+    first = 0
+    for r, (n, ln) in enumerate(zip(ns, lens)):
+        for i in range(n):
+            for hk in range(hkv):
+                for g in range(G):
+                    p_first, p_n, step, col = parts_of(first + i, first, n, ln, hk, g, G, small, off[r], unit[r], total, wgs,
+                                                       1 << 28, 16, shift, 0, rest)
+                    if n > small:
+                        assert p_n == 0
+                        continue
+                    c = i * G + g
+                    number = where[(r, hk * -(-n * G // 64) + c // 64)]
+                    holders = sorted({t // run for t, x in enumerate(line) if x == number})
+                    waves = [c // 16 % 4] if n * G > 16 else [0, 1, 2, 3]
+                    want = [4 * (number + w) + v for w in holders for v in waves]
+                    assert [p_first + step * j for j in range(p_n)] == want and col == c % 16
+        first += n
