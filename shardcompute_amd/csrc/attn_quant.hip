@@ -26,6 +26,7 @@
 #include "kv_cells.h"
 
 #include <algorithm>
+#include <atomic>
 
 namespace sc {
 
@@ -665,10 +666,12 @@ struct Values {
     using Gm = SaGeo<D>;
     using C = Cell<D, BITS>;
     static constexpr int COLS = 256;
-    static constexpr int HALF = C::LANE / 8;         // words of a lane's half
+    static constexpr bool HALF = true;
+    static constexpr int WORDS = C::LANE / 8;        // words of a lane's half
     struct Flow {
-        uint32_t k[HALF], v[HALF];
+        uint32_t k[WORDS], v[WORDS];
         uint32_t km, vm;         // scales and biases: of the lane's position's key; of position 4 g + l % 4's value
+        int there;               // positions of the cell that are there, from the first
         int block;               // the next load's: its number in the pool, on its way
     };
     const QuantArgs &a;
@@ -677,11 +680,11 @@ struct Values {
     __device__ __forceinline__ Values(const QuantArgs &a_, uint8_t *smem_, int lane_, int w)
         : a(a_), smem(smem_), lane(lane_), half(w & 1), cell(w >> 1) {}
 
-    static __device__ __forceinline__ void words(uint32_t (&x)[HALF], const uint8_t *p) {
-        if constexpr (HALF == 4) {
+    static __device__ __forceinline__ void words(uint32_t (&x)[WORDS], const uint8_t *p) {
+        if constexpr (WORDS == 4) {
             const uint4 v = *reinterpret_cast<const uint4 *>(p);
             x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-        } else if constexpr (HALF == 2) {
+        } else if constexpr (WORDS == 2) {
             const uint2 v = *reinterpret_cast<const uint2 *>(p);
             x[0] = v.x; x[1] = v.y;
         } else {
@@ -691,23 +694,91 @@ struct Values {
     __device__ __forceinline__ int block_of(const int32_t *table, int width, int blk) const {
         return table[min((blk * SA_KB + 16 * cell) >> a.shift, width - 1)];
     }
-    // the codes of key block blk, and the number of the one after it
-    __device__ __forceinline__ void load(Flow &f, int hk, const int32_t *table, int width, int blk) const {
+    // the codes of key block blk, of keys below end, and the number of the one after it
+    __device__ __forceinline__ void load(Flow &f, int hk, const int32_t *table, int width, int end, int blk) const {
         const int t = blk * SA_KB + 16 * cell, grp = C::GROUPS == 2 ? half : 0;
         const uint8_t *p = cell_at<C::BYTES>(a, hk, __builtin_amdgcn_readfirstlane(f.block), t);
         f.block = block_of(table, width, blk + 1);
-        const int at = C::PLANES == 2 ? 1024 * half + lane * 16 : lane * C::LANE + 4 * HALF * half;
+        const int at = C::PLANES == 2 ? 1024 * half + lane * 16 : lane * C::LANE + 4 * WORDS * half;
         words(f.k, p + at);
         words(f.v, p + C::CODES + at);
         f.km = *reinterpret_cast<const uint32_t *>(p + C::meta(lane & 15, grp));
         f.vm = *reinterpret_cast<const uint32_t *>(p + C::meta(4 * (lane >> 4) + (lane & 3), C::GROUPS + grp));
+        f.there = end - t;
     }
     // code e (0 .. 7) of a word of 4-bit codes, byte e (0 .. 3) of one of 8-bit codes
     static __device__ __forceinline__ float code(uint32_t w, int e) {
         return BITS == 4 ? (float)((w >> (4 * e)) & 15u) : ubyte_f32(w, e);
     }
-    __device__ __forceinline__ void store(const Flow &f, int st) const {
+    // fp16 holds these positions' values times 2^HALF_UP as exactly as it can: none reaches
+    // its largest, and the scale is whole, or what is dropped of it small beside the values
+    static __device__ __forceinline__ bool in_range(uint32_t meta) {
+        constexpr float TOP = BITS == 4 ? 15.f : 255.f;
+        const float s = __uint_as_float(meta << 16), b = __uint_as_float(meta & 0xFFFF0000u), e = fmaf(s, TOP, b);
+        const float most = fmaxf(fabsf(b), fabsf(e));
+        return fabsf(b) < pow2(15 - HALF_UP) && fabsf(e) < pow2(15 - HALF_UP) &&
+               (fabsf(s) >= pow2(-14 - HALF_UP) || most >= pow2(-11) || most == 0.f);
+    }
+    // Whether a stage's values were in range: a byte a wave, written with them.
+    using Looks = uint2;
+    __device__ __forceinline__ uint8_t *looks(int st) const { return smem + Gm::LDS + 8 * st; }
+    __device__ __forceinline__ Looks looks_of(int st) const { return *reinterpret_cast<const uint2 *>(looks(st)); }
+    static __device__ __forceinline__ bool fits(Looks x) { return __builtin_amdgcn_readfirstlane((int)(x.x | x.y)) == 0; }
+    // the values of a position that is not there become 0, whatever its cell holds
+    __device__ __forceinline__ void drop(Flow &f) const {
+        f.km = (lane & 15) < f.there ? f.km : 0u;
+        f.vm = 4 * (lane >> 4) + (lane & 3) < f.there ? f.vm : 0u;
+    }
+    // a pair of codes, whole numbers of 1024 + code in fp16, as values
+    static __device__ __forceinline__ uint32_t pair(uint32_t codes, uint32_t s, uint32_t b) {
+        const half2_t c = __builtin_bit_cast(half2_t, codes) - half2_t{(_Float16)1024.f, (_Float16)1024.f};
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c, __builtin_bit_cast(half2_t, s), __builtin_bit_cast(half2_t, b)));
+    }
+    static __device__ __forceinline__ uint32_t up(uint32_t meta) {       // scale and bias
+        return cvt_pk_f16(__uint_as_float(meta << 16) * pow2(HALF_UP), __uint_as_float(meta & 0xFFFF0000u) * pow2(HALF_UP));
+    }
+    __device__ __forceinline__ void store_half(Flow &f, int st) const {
+        drop(f);
+        // (by every lane, without a branch)
+        looks(st)[2 * cell + half] = __ballot(!in_range(f.km) || !in_range(f.vm)) != 0ull;
         const int g = lane >> 4, r = lane & 15;
+        uint8_t *K = smem + st * Gm::STAGE, *V = K + Gm::KTILE;
+        uint32_t mask = 0x000F000Fu, one = 0x64006400u;
+        asm("" : "+s"(mask));
+        asm("" : "+v"(one));
+        const uint32_t km = up(f.km);
+        const uint32_t ks = __builtin_amdgcn_perm(km, km, 0x01000100u), kb = __builtin_amdgcn_perm(km, km, 0x03020302u);
+#pragma unroll
+        for (int h = 0; h < C::GROUPS; ++h) {
+            uint32_t o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (BITS == 4) o[e] = pair(dma::and_or(f.k[h] >> (4 * e), mask, one), ks, kb);
+                else o[e] = pair(__builtin_amdgcn_perm(one, f.k[2 * h + (e >> 1)], e & 1 ? 0x07030702u : 0x05010500u), ks, kb);
+            }
+            const int chunk = C::GROUPS == 2 ? 8 * half + 2 * g + h : 2 * g + half;
+            *reinterpret_cast<uint4 *>(K + sa_kswz<D>(16 * cell + r, chunk)) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        const float vm = __uint_as_float(up(f.vm));
+        uint32_t m[4], s[2], b[2];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m[e] = __float_as_uint(row_lane(vm, e));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            s[e] = __builtin_amdgcn_perm(m[2 * e + 1], m[2 * e], 0x05040100u);
+            b[e] = __builtin_amdgcn_perm(m[2 * e + 1], m[2 * e], 0x07060302u);
+        }
+#pragma unroll
+        for (int y = 0; y < 2 * C::GROUPS; ++y) {
+            const uint32_t w = BITS == 4 ? (f.v[y >> 1] >> (4 * (y & 1))) & 0x0F0F0F0Fu : f.v[y];
+            *reinterpret_cast<uint2 *>(V + sa_vswz(16 * (2 * C::GROUPS * half + y) + r, 2 * cell + (g >> 1)) + 8 * (g & 1)) =
+                make_uint2(pair(__builtin_amdgcn_perm(one, w, 0x05010500u), s[0], b[0]),
+                           pair(__builtin_amdgcn_perm(one, w, 0x07030702u), s[1], b[1]));
+        }
+    }
+    __device__ __forceinline__ void store(const Flow &f, int st) const {
+        int g = lane >> 4, r = lane & 15;
+        asm volatile("" : "+v"(g), "+v"(r));             // opaque, as the bf16 blocks' addresses in attn_tile
         uint8_t *K = smem + st * Gm::STAGE, *V = K + Gm::KTILE;
         // keys: 8 dims a chunk, D / 64 of them
         const float ks = __uint_as_float(f.km << 16), kb = __uint_as_float(f.km & 0xFFFF0000u);
@@ -740,15 +811,22 @@ struct Values {
                 make_uint2(cvt_pk_bf16(v[0], v[1]), cvt_pk_bf16(v[2], v[3]));
         }
     }
-    __device__ __forceinline__ void open(Flow &f, int hk, const int32_t *table, int width, int b0) const {
+    __device__ __forceinline__ void open(Flow &f, int hk, const int32_t *table, int width, int end, int b0) const {
         f.block = block_of(table, width, b0);
-        load(f, hk, table, width, b0);
-        store(f, 0);
-        load(f, hk, table, width, b0 + 1);
+        load(f, hk, table, width, end, b0);
+        store_half(f, 0);
+        load(f, hk, table, width, end, b0 + 1);
     }
-    __device__ __forceinline__ void next(Flow &f, int hk, const int32_t *table, int width, int blk, int st) const {
-        store(f, st ^ 1);
-        load(f, hk, table, width, blk + 2);
+    __device__ __forceinline__ void next(Flow &f, int hk, const int32_t *table, int width, int end, int blk, int st) const {
+        store_half(f, st ^ 1);
+        load(f, hk, table, width, end, blk + 2);
+    }
+    __device__ __forceinline__ void again(int hk, const int32_t *table, int width, int end, int blk, int st) const {
+        Flow f;
+        f.block = block_of(table, width, blk);
+        load(f, hk, table, width, end, blk);
+        drop(f);
+        store(f, st);
     }
     __device__ __forceinline__ void landed() const {}
 };
@@ -874,8 +952,20 @@ int run_quant(const QuantArgs &a, const SaPlan &p, hipStream_t stream) {
     if (a.tile_wgs == 0) {
         hipLaunchKernelGGL((attn_line_kernel<D, BITS, CW>), dim3((unsigned)a.own_wgs), dim3(256), line, stream, a);
     } else {
-        const int lds = SaGeo<D>::LDS > line ? SaGeo<D>::LDS : line, per = QUANT_WAVES / 4;
+        const int tile = SaGeo<D>::LDS + 16, lds = tile > line ? tile : line, per = QUANT_WAVES / 4;
         const int grid = a.cut ? device_info().num_cus : a.tile_wgs + (a.own_wgs + per - 1) / per;
+        if (lds > 65536) {
+            // more than 64 KB of LDS has to be allowed, once a device
+            static std::atomic<uint64_t> allowed;
+            int dev = 0;
+            SC_HIP_CHECK(hipGetDevice(&dev));
+            const uint64_t bit = 1ull << (dev & 63);
+            if (!(allowed.load() & bit)) {
+                SC_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_quantized_kernel<D, BITS, CW>),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, std::max(tile, line_lds(SA_MAX_SEQ))));
+                allowed.fetch_or(bit);
+            }
+        }
         hipLaunchKernelGGL((attn_quantized_kernel<D, BITS, CW>), dim3((unsigned)grid), dim3(64 * QUANT_WAVES), lds, stream, a);
     }
     SC_HIP_CHECK(hipGetLastError());

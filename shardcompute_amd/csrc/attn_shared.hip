@@ -55,6 +55,7 @@ struct Stager {
     using Gm = SaGeo<D>;
     using Args = SharedArgs;
     static constexpr int COLS = SA_COLS;
+    static constexpr bool HALF = false;
     // cache blocks of a key block: ONE, its block's number; else those of the wave's 16
     // keys of K and of the lane's two chunks of Vt
     struct Ids { int k, v0, v1; };

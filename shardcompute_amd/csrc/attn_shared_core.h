@@ -137,8 +137,46 @@ __device__ __forceinline__ uint4 finite8(uint4 v) {
 }
 __device__ __forceinline__ uint4 and4(uint4 v, uint4 m) { return make_uint4(v.x & m.x, v.y & m.y, v.z & m.z, v.w & m.w); }
 
-// S: how the key blocks come into the ring (Args, COLS, Flow; open: the first, next: the one
-// after blk, landed: what was begun is there).
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef float float2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t cvt_pk_f16(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(float2_t{a, b}, half2_t));
+}
+__device__ __forceinline__ uint32_t word_of(bf16x8_t v, int e) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(u4, v)[e];
+}
+__device__ __forceinline__ half8_t as_half8(bf16x8_t v) { return __builtin_bit_cast(half8_t, v); }
+__device__ __forceinline__ f32x16_t mfma32x32x16_f16(bf16x8_t a, bf16x8_t b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(as_half8(a), as_half8(b), c, 0, 0, 0);
+}
+
+// Where a stager has HALF, the values are rounded to 11 bits in place of 8: a key block comes as
+// fp16, times 2^HALF_UP, where its range holds all of it (fits), 0 in the place of keys that are
+// not there, else as bf16.  q then is kept as fp16: a column whose largest |q| is outside
+// [2^-8, 2^15) is scaled by a power of two, so that what fp16 drops of q is 2^-17 of that at
+// most.  P is 2^HALF_P times the probability, which may exceed 1 by 2^LAZY: at most 2^15, and
+// a weight below 2^-32 of the largest is dropped.
+constexpr int HALF_UP = 5, HALF_P = 7;
+constexpr float pow2(int n) { return n >= 0 ? (float)(1 << n) : 1.f / (float)(1 << -n); }
+
+// q as the bf16 blocks' scores take it, which are scaled by 2^-HALF_UP as the others
+__device__ __forceinline__ bf16x8_t q_bf16(bf16x8_t v) {
+    uint32_t y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        uint32_t w = word_of(v, e);
+        asm volatile("" : "+v"(w));                      // opaque: not kept beside q over the loop
+        const half2_t x = __builtin_bit_cast(half2_t, w);
+        y[e] = cvt_pk_bf16((float)x[0] * pow2(HALF_UP), (float)x[1] * pow2(HALF_UP));
+    }
+    return as_bf16x8(y[0], y[1], y[2], y[3]);
+}
+
+// S: how the key blocks come into the ring (Args, COLS, HALF, Flow; open: the first, next: the one
+// after blk, landed: what was begun is there.  HALF: looks_of and fits say whether the one in a
+// stage fits, if not, again brings it as bf16).
 template <int D, class S>
 __device__ __forceinline__ void attn_tile(const typename S::Args &a, int id, uint8_t *smem) {
     using Gm = SaGeo<D>;
@@ -188,12 +226,39 @@ __device__ __forceinline__ void attn_tile(const typename S::Args &a, int id, uin
         if (col_ok) v = *reinterpret_cast<const uint4 *>(a.q + (size_t)row * a.q_stride + (size_t)h * D + 16 * ks + 8 * lh);
         qv[ks] = as_bf16x8(v);
     }
+    float sc = a.scale_log2;
+    if constexpr (S::HALF) {
+        uint32_t top = 0;                                // the largest |q|
+#pragma unroll
+        for (int ks = 0; ks < Gm::KSTEPS; ++ks)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t x = word_of(qv[ks], e);
+                top = max(top, max(x << 16 & 0x7FFFFFFFu, x & 0x7FFF0000u));
+            }
+        top = max(top, (uint32_t)__shfl_xor((int)top, 32)) >> 23;
+        // (its exponent, biased; a q that is no number keeps it)
+        const bool keep = (top >= 127 - 8 && top < 127 + 15) || top == 255;
+        const uint32_t up = keep ? 127u : 254u - clampi((int)top, 16, 238);
+        const float by = __uint_as_float(up << 23);
+#pragma unroll
+        for (int ks = 0; ks < Gm::KSTEPS; ++ks) {
+            uint32_t y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t x = word_of(qv[ks], e);
+                y[e] = cvt_pk_f16(__uint_as_float(x << 16) * by, __uint_as_float(x & 0xFFFF0000u) * by);
+            }
+            qv[ks] = as_bf16x8(y[0], y[1], y[2], y[3]);
+        }
+        sc = fmaxf(sc * __uint_as_float((254u - up) << 23) * pow2(-HALF_UP), 1e-37f);
+    }
     f32x16_t o[Gm::DB];
 #pragma unroll
     for (int db = 0; db < Gm::DB; ++db) o[db] = f32x16_t{};
     float m = -INFINITY, lsum = 0.f;
-    const float sc = a.scale_log2;
     const int arow = sa_swap23(li);
+    const uint32_t kat0 = sa_kswz<D>(arow, lh), vat0 = sa_vswz(li, lh);
     const S stager(a, smem, lane, w);
 
     // key blocks [b0, b1) of one table with `end` keys; the column sees keys <= limit
@@ -213,12 +278,26 @@ __device__ __forceinline__ void attn_tile(const typename S::Args &a, int id, uin
         // operand read is a loop-invariant lane offset plus an immediate
         auto block = [&](int blk, auto mask_tag, auto stage) {
             constexpr bool MASK = decltype(mask_tag)::value;
+            constexpr bool F16 = S::HALF && !MASK;
             const int st = stage;
             const int kb = blk * SA_KB;
-            const uint8_t *K = smem + st * Gm::STAGE;
+            const uint8_t *K = smem + (S::HALF ? 0 : st * Gm::STAGE);        // (of HALF in kplace and vplace)
             const uint8_t *V = K + Gm::KTILE;
-            if (blk + 1 < b1) stager.next(flow, hk, table, width, blk, st);
-            if (!MASK || kb <= hi) {                     // else: nothing of it is seen by the wave
+            // operands' places: of HALF, whose registers are scarcer, from two offsets by one more
+            // instruction each (opaque, else all are kept over the loop)
+            uint32_t kat = kat0 + st * Gm::STAGE, vat = vat0 + st * Gm::STAGE;
+            if constexpr (S::HALF) asm volatile("" : "+v"(kat), "+v"(vat));
+            auto kplace = [&](int kh, int ks) {
+                if constexpr (S::HALF) return (kat ^ (uint32_t)(ks << 5)) + 32 * kh * Gm::KROW;
+                else return sa_kswz<D>(32 * kh + arow, 2 * ks + lh);
+            };
+            auto vplace = [&](int db, int s4) {
+                if constexpr (S::HALF) return (vat ^ (uint32_t)(s4 << 5)) + 32 * 128 * db;
+                else return sa_vswz(32 * db + li, 2 * s4 + lh);
+            };
+            if constexpr (!S::HALF)
+                if (blk + 1 < b1) stager.next(flow, hk, table, width, blk, st);
+            if ((!MASK && !F16) || kb <= hi) {           // else: nothing of it is seen by the wave
                 f32x16_t sacc[2] = {f32x16_t{}, f32x16_t{}};
                 // operand reads SA_AHEAD ahead of their MFMAs (the scheduler, left alone,
                 // issues each read just before its MFMA)
@@ -227,8 +306,9 @@ __device__ __forceinline__ void attn_tile(const typename S::Args &a, int id, uin
                 for (int ks = 0; ks < Gm::KSTEPS; ++ks)
 #pragma unroll
                     for (int kh = 0; kh < 2; ++kh) {
-                        const bf16x8_t ka = as_bf16x8(*reinterpret_cast<const uint4 *>(K + sa_kswz<D>(32 * kh + arow, 2 * ks + lh)));
-                        sacc[kh] = mfma32x32x16(ka, qv[ks], sacc[kh]);
+                        const bf16x8_t ka = as_bf16x8(*reinterpret_cast<const uint4 *>(K + kplace(kh, ks)));
+                        if constexpr (F16) sacc[kh] = mfma32x32x16_f16(ka, qv[ks], sacc[kh]);
+                        else sacc[kh] = mfma32x32x16(ka, S::HALF ? q_bf16(qv[ks]) : qv[ks], sacc[kh]);
                     }
                 __builtin_amdgcn_sched_group_barrier(0x100, SA_AHEAD, 0);
 #pragma unroll
@@ -238,7 +318,7 @@ __device__ __forceinline__ void attn_tile(const typename S::Args &a, int id, uin
                 }
                 __builtin_amdgcn_sched_group_barrier(0x008, SA_AHEAD, 0);
                 __builtin_amdgcn_sched_barrier(0);
-                if (MASK) {
+                if (MASK || (F16 && kb + SA_KB - 1 > lo)) {
                     const int rel = limit - kb - 8 * lh;
 #pragma unroll
                     for (int kh = 0; kh < 2; ++kh)
@@ -258,7 +338,7 @@ __device__ __forceinline__ void attn_tile(const typename S::Args &a, int id, uin
                     m = bm;
                 }
                 // (a column that has seen no key yet has m = -inf: probabilities 0, not NaN)
-                const float nms = m == -INFINITY ? 0.f : -m * sc;
+                const float nms = (m == -INFINITY ? 0.f : -m * sc) + (S::HALF ? HALF_P : 0);
                 float ps = 0.f;
 #pragma unroll
                 for (int kh = 0; kh < 2; ++kh)
@@ -288,7 +368,7 @@ __device__ __forceinline__ void attn_tile(const typename S::Args &a, int id, uin
                         const uint4 mk = keep_below(kb + 16 * s4 + 8 * lh, end);
 #pragma unroll
                         for (int db = 0; db < Gm::DB; ++db)
-                            bits |= nonfinite_bits(and4(*reinterpret_cast<const uint4 *>(V + sa_vswz(32 * db + li, 2 * s4 + lh)), mk));
+                            bits |= nonfinite_bits(and4(*reinterpret_cast<const uint4 *>(V + vplace(db, s4)), mk));
                     }
                     bad = any_nonfinite(bits);
                 }
@@ -296,20 +376,23 @@ __device__ __forceinline__ void attn_tile(const typename S::Args &a, int id, uin
 #pragma unroll
                 for (int s4 = 0; s4 < 4; ++s4) {
                     const int kh = s4 >> 1, q0 = 8 * (s4 & 1), c = 2 * s4 + lh;
-                    const bf16x8_t pb = as_bf16x8(cvt_pk_bf16(sacc[kh][q0], sacc[kh][q0 + 1]),
-                                                  cvt_pk_bf16(sacc[kh][q0 + 2], sacc[kh][q0 + 3]),
-                                                  cvt_pk_bf16(sacc[kh][q0 + 4], sacc[kh][q0 + 5]),
-                                                  cvt_pk_bf16(sacc[kh][q0 + 6], sacc[kh][q0 + 7]));
+                    auto pair = [&](int i) {
+                        if constexpr (F16) return cvt_pk_f16(sacc[kh][q0 + i], sacc[kh][q0 + i + 1]);
+                        else if constexpr (S::HALF) return cvt_pk_bf16(sacc[kh][q0 + i] * pow2(HALF_UP), sacc[kh][q0 + i + 1] * pow2(HALF_UP));
+                        else return cvt_pk_bf16(sacc[kh][q0 + i], sacc[kh][q0 + i + 1]);
+                    };
+                    const bf16x8_t pb = as_bf16x8(pair(0), pair(2), pair(4), pair(6));
                     uint4 mk;
                     if (MASK) mk = keep_below(kb + 8 * c, end);
 #pragma unroll
                     for (int db = 0; db < Gm::DB; ++db) {
-                        uint4 v = *reinterpret_cast<const uint4 *>(V + sa_vswz(32 * db + li, c));
+                        uint4 v = *reinterpret_cast<const uint4 *>(V + vplace(db, s4));
                         if (MASK) {
                             v = and4(v, mk);
                             if (bad) v = finite8(v);
                         }
-                        o[db] = mfma32x32x16(as_bf16x8(v), pb, o[db]);
+                        if constexpr (F16) o[db] = mfma32x32x16_f16(as_bf16x8(v), pb, o[db]);
+                        else o[db] = mfma32x32x16(as_bf16x8(v), pb, o[db]);
                     }
                 }
                 if (!MASK) {
@@ -334,7 +417,7 @@ __device__ __forceinline__ void attn_tile(const typename S::Args &a, int id, uin
 #pragma unroll
                             for (int r = 0; r < 16; ++r) {
                                 const int d = 32 * db + 8 * (r >> 2) + 4 * half + (r & 3);
-                                const uint32_t x = *reinterpret_cast<const uint16_t *>(V + sa_vswz(d, j >> 3) + 2 * (j & 7));
+                                const uint32_t x = *reinterpret_cast<const uint16_t *>(V + (S::HALF ? st * Gm::STAGE : 0) + sa_vswz(d, j >> 3) + 2 * (j & 7));
                                 if (sees && (x & 0x7F80u) == 0x7F80u) o[db][r] += bf2f(x);
                             }
                     }
@@ -344,19 +427,39 @@ __device__ __forceinline__ void attn_tile(const typename S::Args &a, int id, uin
             stager.landed();
             __syncthreads();
         };
-        stager.open(flow, hk, table, width, b0);
-        stager.landed();
-        __syncthreads();
-        using S0 = std::integral_constant<int, 0>;
-        using S1 = std::integral_constant<int, 1>;
-        const int bf = min(b1, (lo + 1) / SA_KB);        // key blocks below it need no mask
-        int blk = b0;
-        for (; blk + 1 < bf; blk += 2) {
-            block(blk, std::false_type{}, S0{});
-            block(blk + 1, std::false_type{}, S1{});
+        if constexpr (S::HALF) {
+            stager.open(flow, hk, table, width, end, b0);
+            __syncthreads();
+            for (int blk = b0; blk < b1; ++blk) {
+                bool half = true;
+                for (; blk < b1; ++blk) {
+                    const int st = (blk - b0) & 1;
+                    const typename S::Looks looks = stager.looks_of(st);
+                    if (blk + 1 < b1) stager.next(flow, hk, table, width, end, blk, st);
+                    half = stager.fits(looks);
+                    if (!half) break;
+                    block(blk, std::false_type{}, st);
+                }
+                if (half) break;
+                stager.again(hk, table, width, end, blk, (blk - b0) & 1);
+                __syncthreads();
+                block(blk, std::true_type{}, (blk - b0) & 1);
+            }
+        } else {
+            stager.open(flow, hk, table, width, b0);
+            stager.landed();
+            __syncthreads();
+            using S0 = std::integral_constant<int, 0>;
+            using S1 = std::integral_constant<int, 1>;
+            const int bf = min(b1, (lo + 1) / SA_KB);        // key blocks below it need no mask
+            int blk = b0;
+            for (; blk + 1 < bf; blk += 2) {
+                block(blk, std::false_type{}, S0{});
+                block(blk + 1, std::false_type{}, S1{});
+            }
+            if (blk < bf) block(blk++, std::false_type{}, S0{});
+            for (; blk < b1; ++blk) block(blk, std::true_type{}, (blk - b0) & 1);
         }
-        if (blk < bf) block(blk++, std::false_type{}, S0{});
-        for (; blk < b1; ++blk) block(blk, std::true_type{}, (blk - b0) & 1);
     };
 
     // q's loads end here: a wait at their first use, in the loop, would also wait for the
@@ -383,7 +486,7 @@ __device__ __forceinline__ void attn_tile(const typename S::Args &a, int id, uin
         at += nb;
     }
 
-    const float ltot = lsum + __shfl_xor(lsum, 32);
+    const float ltot = (lsum + __shfl_xor(lsum, 32)) * (S::HALF ? pow2(HALF_UP) : 1.f);      // (of P as o has it)
     if (!col_ok) return;
     if (big && a.nsplit == 1) {
         const float inv = ltot == 0.f ? 0.f : 1.f / ltot;      // (a row without a key: 0)
@@ -407,7 +510,7 @@ __device__ __forceinline__ void attn_tile(const typename S::Args &a, int id, uin
             *reinterpret_cast<float4 *>(po + 32 * db + 8 * r4 + 4 * lh) =
                 make_float4(o[db][4 * r4], o[db][4 * r4 + 1], o[db][4 * r4 + 2], o[db][4 * r4 + 3]);
     if (lh == 0)     // (a sum that is no number: nor is the row)
-        a.tile_ml[part] = make_float2(ltot == ltot ? m * sc : INFINITY, ltot);
+        a.tile_ml[part] = make_float2(ltot == ltot ? m * sc - (S::HALF ? HALF_P + HALF_UP : 0) : INFINITY, ltot);
 }
 
 // ---------------------------------------------------------------- merge
