@@ -421,3 +421,33 @@ def test_a_stored_value_is_the_quantizers(device):
     for bits in BITS:
         v = stored(x, bits)[0]
         assert ((_quantized_rows(x, bits).double() - v).abs() <= 2.0 ** -8 * v.abs() + 2.0 ** -20).all()
+
+
+# factors of the keys, the values, q; every how many positions they are taken (1: everywhere)
+MAGNITUDES = [(1, 3000, 1, 1), (1, 1e-5, 1, 1), (1, 2.0 ** -10, 1, 1), (3000, 1, 1 / 3000, 1), (1e-6, 1, 1e6, 1), (1e20, 1, 1e-20, 1),
+              (1e-9, 1e30, 1e9, 1), (1, 1, 0, 1), (1, 2000, 1, 97), (2.0 ** -6, 1e-4, 1, 3), (0, 0, 1, 50)]
+
+
+@pytest.mark.parametrize("kf,vf,qf,every", MAGNITUDES)
+@pytest.mark.parametrize("new,H,Hkv", [([1, 1, 1], 8, 2), ([1, 200, 130], 8, 2), ([2, 300, 1], 4, 4)])
+@pytest.mark.parametrize("D,bits", [(64, 4), (128, 4), (64, 8), (128, 8)])
+def test_attention_over_the_range_of_bf16(device, kf, vf, qf, every, new, H, Hkv, D, bits):
+    """Keys, values and q far from 1, some positions' or all: the column tiles take blocks whose
+    values fp16 cannot hold as bf16.  The bound, relative to what a row's sums are of, holds for
+    either: fp16 rounds to 2^-12 of a value, and what it drops of smaller ones is below 2^-12 of
+    their group's largest."""
+    print(f"magnitudes {kf} {vf} {qf} every {every} new={new} D={D} bits={bits}", flush=True)
+    c = QuantCache(bits, [40, 300, 9], new, 500, 64, H, Hkv, D, pad=1)
+    there = ~torch.isnan(c.k[:, 0, :, 0])
+    chosen = torch.arange(there.numel(), device="cuda").view(there.shape) % every == 0
+    c.k *= torch.where(chosen, kf, 1.0)[:, None, :, None].to(c.k.dtype)
+    c.vt *= torch.where(chosen, vf, 1.0)[:, None, None, :].to(c.vt.dtype)
+    c.q *= qf
+    at = there.nonzero()
+    write(c.pool, c.k[at[:, 0], :, at[:, 1]], c.vt[at[:, 0], :, :, at[:, 1]], at[:, 0] * c.bs + at[:, 1], bits)
+    exact, bound = c.exact()
+    rows = c.starts[-1]
+    got = c.attend(max_new=c.max_new)[:rows].double().view(rows, H, D)
+    assert torch.isfinite(got).all()
+    err = (got - exact[:rows]).abs()
+    assert (err <= bound[:rows] + 1e-36).all(), float((err / bound[:rows].clamp(min=1e-36)).max())
