@@ -106,9 +106,11 @@ __device__ __forceinline__ float head_max(float v) {
 // pieces of 16 bytes (8 of 4 bits and 64 dims), 4 values of consecutive slots that begin at a
 // multiple of 4 in pieces of 16 too (a lane of the cell: PLANE), other values byte by byte.
 //
-// Bound by memory for prompts, by the chain slot, row, scale, codes, store for single rows.
+// Bound by memory for prompts (22000 rows of 8 + 1 heads of 128 in 8 bits, 113 MB: 28.4 us, 4.0 TB/s),
+// for single rows by the chain slot, row, scale, codes, store (64 rows of 32 + 8 heads in 4 bits:
+// 5.7 us).  A wave with the keys of one row and no LDS, its values stored byte by byte: 48.8 and 9.7 us.
 constexpr int QA_ROWS = 32, QA_FEW_ROWS = 16;
-constexpr long QA_FEW = 512;
+constexpr long QA_FEW = 512;          // rows up to which the groups are the smaller
 
 template <int D, int BITS>
 __global__ void __launch_bounds__(256) rope_append_quantized_kernel(QuantAppendArgs a) {
@@ -290,13 +292,17 @@ __global__ void __launch_bounds__(256) rope_append_quantized_kernel(QuantAppendA
 // has 8 dims of the key, and of the value the dims l, 16 + l, .. of its place in the cell (two
 // places with 64 dims), which go through LDS into the row's order.
 //
-// Bound by memory: 40000 positions of 8 kv heads of 128 in 4 bits, see launch_read_quantized.
+// Bound by memory: 40000 positions of 8 kv heads of 128 in 4 bits 34 us (210 MB: 6.1 TB/s).  More
+// than QR_THROUGH bytes of output go past the caches, which would lose what comes in for what no
+// reader finds there in time: with 164 MB, pools in turn, 34 us in place of 49; 15 MB take 9.5 us
+// either way, and are there for who reads them next.
+constexpr long QR_THROUGH = 64L << 20;
 struct QuantReadArgs {
     const uint8_t *pool;
     const int32_t *slots;
     uint16_t *k, *v;
     long n, n_slots;
-    int Hkv, shift;
+    int Hkv, shift, through;
 };
 
 template <int D, int BITS>
@@ -355,8 +361,14 @@ __global__ void __launch_bounds__(256) read_quantized_kernel(QuantReadArgs a) {
     if (row >= a.n) return;
     if (there) val = *reinterpret_cast<const uint4 *>(tile + r * PAD + 8 * o);
     const long at = (row * a.Hkv + hk) * D + 8 * o;
-    *reinterpret_cast<uint4 *>(a.k + at) = key;
-    *reinterpret_cast<uint4 *>(a.v + at) = val;
+    typedef uint32_t words __attribute__((ext_vector_type(4)));
+    if (a.through) {
+        __builtin_nontemporal_store(__builtin_bit_cast(words, key), reinterpret_cast<words *>(a.k + at));
+        __builtin_nontemporal_store(__builtin_bit_cast(words, val), reinterpret_cast<words *>(a.v + at));
+    } else {
+        *reinterpret_cast<uint4 *>(a.k + at) = key;
+        *reinterpret_cast<uint4 *>(a.v + at) = val;
+    }
 }
 
 }  // namespace
@@ -385,10 +397,12 @@ int launch_rope_append_quantized(const uint16_t *qkv, long qkv_stride, uint16_t 
     a.cos_t = cos_t; a.sin_t = sin_t; a.slots = slots; a.positions = positions;
     a.N = (int)N; a.H = (int)H; a.Hkv = (int)Hkv; a.shift = shift; a.table_len = (int)table_len;
     a.n_slots = n_blocks * bs;
-    // single rows in groups of few, so that the GPU has work (64 rows of 32 + 8 heads of 128)
+    // few rows in smaller groups, so that more of the GPU has work: 64 rows of 32 + 8 heads of 128
+    // 5.7 us, in groups of 32 rows 8.9; 22000 rows of 8 + 1 heads 28.4 us, in groups of 64 31.5
     a.kv_rows = N <= QA_FEW ? QA_FEW_ROWS : QA_ROWS;
     const long kv_wgs = (N + a.kv_rows - 1) / a.kv_rows * Hkv;
-    // a token's q heads over several waves while tokens alone leave CUs idle
+    // A token's q heads over several waves while tokens alone leave CUs idle; from 4 tokens a CU on a
+    // wave each.  (8600 rows of 32 heads of 64: 19.9 us, all in their own waves 20.8.)
     const long hpw = 64 / (D / 16), cus = device_info().num_cus;
     long per = N >= 4 * cus ? H : N >= cus ? 2 * hpw : hpw;
     if (per > H) per = H;
@@ -417,6 +431,7 @@ int launch_read_quantized(const uint8_t *pool, long n_blocks, long bs, int bits,
         return set_error(SC_EINVAL, "read_quantized: pointers must be 16-byte aligned");
     QuantReadArgs a;
     a.pool = pool; a.slots = slots; a.k = k; a.v = v; a.n = n; a.n_slots = n_blocks * bs; a.Hkv = (int)Hkv; a.shift = shift;
+    a.through = n * Hkv * D * 4 > QR_THROUGH;
     const long rows = 256 / (D / 8), blocks = (n + rows - 1) / rows * Hkv;
     if (blocks >= (1L << 24)) return set_error(SC_EINVAL, "read_quantized: too many rows");            // 2^32 threads
     auto kern = D == 128 ? (bits == 4 ? read_quantized_kernel<128, 4> : read_quantized_kernel<128, 8>)
