@@ -20,7 +20,8 @@
 //                      small_rows): the codes straight from memory into the operands' registers;
 //                      the work cut evenly over the workgroups whatever the lengths are
 //   attn_tile          (attn_shared_core.h) the prefix, then the own keys of sequences with many
-//                      rows: the workgroup turns each key block into bf16 values in LDS once
+//                      rows: the workgroup turns each key block into values in LDS once, in fp16
+//                      where its range holds them, else in bf16
 //   attn_merge_kernel  joins the parts of a row by their softmax maxima and sums
 #include "attn_shared_core.h"
 #include "kv_cells.h"
@@ -100,7 +101,8 @@ struct CellRegs {
 // places of operand B, the other cell's are 0) with the weights of the block's group; what a
 // block's group leaves in the other group's dims is not used, and the cells' are added at
 // the end.
-// 64 rows of up to 1023 positions of 32 heads of 128 on 8 in 4 bits: see attn_line.
+// One row of 131072 positions, 32 heads of 128 on 8 in 4 bits (4 columns): CW 4 36.7 us, 8 38.4, 16
+// 46.9; 256 rows of the 70B shard's heads in 8 bits (8 columns) 40.8, with 16 53.2.
 template <int D, int BITS, int CW>
 struct Columns {
     using C = Cell<D, BITS>;
@@ -382,9 +384,18 @@ struct Columns {
 // part, number 4 (unit + workgroup) + wave, as in attn_shared.hip.  The waves of a workgroup share
 // nothing but their run, so there is no barrier; the next 32 keys' codes are on their way while
 // these are computed.
+//
+// Bound by memory where the sequences are long: 131072 positions of one, 32 heads of 128 on 8 in
+// 4 bits, 151 MB, 30.3 us, of which 26 from the first key on (5.8 TB/s); by the VALU of the
+// codes, the affine sums and the softmax, about 300 instructions a wave and step of 32 keys, where
+// codes come from a cache.
 constexpr int LINE_SHIFT = 7, LINE_KB = 1 << LINE_SHIFT;
-// workgroups a CU, and waves a SIMD, where lines run alone
-constexpr int line_waves(int D, int bits) { return D == 64 ? 3 : 2; }
+// Workgroups a CU, and waves a SIMD, where lines run alone: 64 dims leave room for three, of 4 bits
+// and 64 sequences of 4000 positions 29.5 us in place of 30.8, 256 of up to 900 31.0 of 32.6.  Few
+// units would be cut into more parts than their merge gains by: one sequence of 65536 positions
+// 22.8 us with two, 26.9 with three.  128 dims with three spill: 131072 positions 38 us, with two 31.
+constexpr int line_waves(int D) { return D == 64 ? 3 : 2; }
+constexpr int FEW_UNITS = 32;
 
 struct Line {
     int32_t *first_row, *keys, *off, *unit;      // of every sequence, in LDS: first row, keys, first block and unit in the line
@@ -655,11 +666,18 @@ __device__ __forceinline__ void attn_line(const QuantArgs &a, const Line &l, int
 
 // ---------------------------------------------------------------- many columns
 //
-// How attn_tile's key blocks come into its ring: K [64 keys x D] and Vt [D x 64 keys] in bf16, as
+// How attn_tile's key blocks come into its ring: K [64 keys x D] and Vt [D x 64 keys], placed as
 // the bf16 cache's kernel copies them.  The waves load a key block's codes two blocks ahead and
-// write their values one block ahead.  Of
-// a block's 4 cells wave w has half of the words of cell w / 2, keys' and values' alike (8 waves
-// and one path for all of them, so that nothing branches).
+// write their values one block ahead.  Of a block's 4 cells wave w has half of the words of cell
+// w / 2, keys' and values' alike (8 waves and one path for all of them, so that nothing branches).
+//
+// The values are fp16, scale code + bias rounded once to 11 bits (pairs of 1024 + code, less 1024,
+// one fused multiply-add): outputs are off by their own rounding, 0.0017 (relative, rms), where
+// values rounded to bf16's 8 bits make it 0.0033.  A block that fp16 cannot hold (in_range) is
+// read again and written in bf16 by its readers, who find it marked.
+// A block of 256 columns is bound by the power of its products and the VALU of its softmax and
+// values: 615 GFLOP of 16 prompts behind 4096 positions 737 us (835 TFLOP/s), with bf16 values 711:
+// the same instructions on 11 in place of 8 bits lower the clock.
 template <int D, int BITS>
 struct Values {
     using Args = QuantArgs;
@@ -833,10 +851,13 @@ struct Values {
 
 // ---------------------------------------------------------------- kernels
 
-// Times in us that say how the CUs are shared out between tiles and lines: on a CU of its own a
-// tile's block (64 keys, 256 columns) and a line's (128 keys of a unit), and the bytes a us of
-// parts, which the kernel's end has to bring from the caches to memory and the merge reads.
-// Stamped in the kernel at 64 decoded rows behind 8192 positions, 32 heads of 128 on 8.
+// Times in us that say how the CUs are shared out between tiles and lines, on a CU of its own: a
+// tile's block (64 keys, 256 columns), what a tile takes beside its blocks, a place of a line's run
+// (128 keys of a unit, two runs on a CU), and the bytes a us of parts, which the kernel's end has
+// to bring from the caches to memory and the merge reads.  Stamped in the kernel at 64 decoded rows
+// behind 8192 positions, 32 heads of 128 on 8: tiles end at 28 to 33 us, lines at 21 to 31.  Places
+// taken for 1.8 us or parts for half as much change that case by less than 1 %; 24 rows of 5 on 32
+// heads of 64 take 31.9 us in place of 29.2 with the parts at half.
 constexpr float tile_block_us(int D) { return D == 128 ? 2.1f : 1.5f; }
 constexpr float line_block_us(int D) { return D == 128 ? 2.3f : 1.4f; }
 constexpr float TILE_OPEN_US = 5.f;
@@ -891,7 +912,7 @@ __global__ void __launch_bounds__(64 * QUANT_WAVES) __attribute__((amdgpu_waves_
 
 // Lines alone.
 template <int D, int BITS, int CW>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(line_waves(D, BITS)))) attn_line_kernel(QuantArgs a) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(line_waves(D)))) attn_line_kernel(QuantArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
     Line l = line_of(a, smem);
     places_of(a, l);
@@ -900,7 +921,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(line_w
 
 // ---------------------------------------------------------------- host side
 
-// Into how many workgroups a column tile's key blocks are cut, of `most` that there is room for.
+// Into how many workgroups a column tile's key blocks are cut where sequences of many rows are
+// among them, of `most` that there is room for: the walk at 2 us a block against the parts.  (A
+// prompt of 2048 rows in 33 column tiles on 8 kv heads stays whole: two cuts of each would write
+// and read 140 MB of parts, 50 us, for half of a walk of 67.)
 int quant_splits(long wgs, long blocks, double part_bytes, bool last_is_whole, long most) {
     int best = 1;
     double least = 1e30;
@@ -915,14 +939,16 @@ int quant_splits(long wgs, long blocks, double part_bytes, bool last_is_whole, l
 
 // own_cap, prefix_cap: positions the tables have room for; max_new: at least the rows of
 // the sequence with the most
-SaPlan plan_quant(long N, long R, long H, long Hkv, long D, int bits, long own_cap, long prefix_cap, long max_new) {
+SaPlan plan_quant(long N, long R, long H, long Hkv, long D, long own_cap, long prefix_cap, long max_new) {
     SaPlan p;
     const long G = H / Hkv, cols = N * G, cus = device_info().num_cus;
     if (max_new > N) max_new = N;
     p.own_shift = LINE_SHIFT;
     p.small_rows = (int)(64 / G > 1 ? 64 / G : 1);
     p.any_big = max_new > p.small_rows;
-    p.own_rest = R > 1;
+    p.own_rest = R > 1;                      // (a sequence's own units are alike)
+    // one sequence: the prefix is keys of its own line (65536 positions, 32 heads of 128 on 8: 28 us, as
+    // column tiles 79; 500 positions 15 either way)
     p.join = !p.any_big && prefix_cap > 0 && R == 1;
     p.use_tile = p.any_big || (prefix_cap > 0 && !p.join);
     p.tiles = (cols + 32 * QUANT_WAVES - 1) / (32 * QUANT_WAVES);
@@ -937,7 +963,7 @@ SaPlan plan_quant(long N, long R, long H, long Hkv, long D, int bits, long own_c
     long coltiles = R * ((rows_max * G + 63) / 64);
     if (coltiles > R + cols / 64) coltiles = R + cols / 64;
     const long keyblocks = coltiles * (own_keyblocks((int)own_cap, LINE_SHIFT) + (p.join ? own_keyblocks((int)prefix_cap, LINE_SHIFT) : 0) + p.own_rest);
-    long ow = p.use_tile ? 2 * cus : line_waves((int)D, bits) * cus;
+    long ow = (p.use_tile || R * Hkv < FEW_UNITS ? 2 : line_waves((int)D)) * cus;
     if (!p.cut && ow > Hkv * keyblocks) ow = Hkv * keyblocks;
     p.own_wgs = (int)(ow < 1 ? 1 : ow);
     p.own_parts = 4 * (Hkv * coltiles + p.own_wgs);
@@ -992,7 +1018,7 @@ bool bad_shape(long N, long R, long H, long Hkv, long D, long own_cap, long pref
 long attention_quantized_workspace_bytes(long N, long R, long H, long Hkv, long D, long own_cap, long prefix_cap,
                                          long max_new, int bits) {
     if (bad_shape(N, R, H, Hkv, D, own_cap, prefix_cap, max_new, bits) || N == 0) return 0;
-    return plan_quant(N, R, H, Hkv, D, bits, own_cap, prefix_cap, max_new).bytes;
+    return plan_quant(N, R, H, Hkv, D, own_cap, prefix_cap, max_new).bytes;
 }
 
 int launch_attention_quantized(const uint16_t *q, long q_stride, const uint8_t *pool, long n_blocks, long bs, int bits,
@@ -1018,7 +1044,7 @@ int launch_attention_quantized(const uint16_t *q, long q_stride, const uint8_t *
         return set_error(SC_EINVAL, "attention_quantized: bad row strides");
     if (((uintptr_t)q | (uintptr_t)pool) % 16 || (uintptr_t)out % 8)
         return set_error(SC_EINVAL, "attention_quantized: misaligned pointers");
-    const SaPlan p = plan_quant(N, R, H, Hkv, D, bits, width * bs, prefix_width * bs, max_new);
+    const SaPlan p = plan_quant(N, R, H, Hkv, D, width * bs, prefix_width * bs, max_new);
     if (!workspace || workspace_bytes < p.bytes || (uintptr_t)workspace % 16)
         return set_error(SC_EINVAL, "attention_quantized: a 16-byte aligned workspace of %ld bytes required", p.bytes);
     // 2^32 threads a launch

@@ -239,7 +239,7 @@ __device__ __forceinline__ void attn_tile(const typename S::Args &a, int id, uin
         top = max(top, (uint32_t)__shfl_xor((int)top, 32)) >> 23;
         // (its exponent, biased; a q that is no number keeps it)
         const bool keep = (top >= 127 - 8 && top < 127 + 15) || top == 255;
-        const uint32_t up = keep ? 127u : 254u - clampi((int)top, 16, 238);
+        const uint32_t up = keep ? 127u : 254u - clampi((int)top, 16, 240);
         const float by = __uint_as_float(up << 23);
 #pragma unroll
         for (int ks = 0; ks < Gm::KSTEPS; ++ks) {
