@@ -397,6 +397,17 @@ constexpr int LINE_SHIFT = 7, LINE_KB = 1 << LINE_SHIFT;
 constexpr int line_waves(int D) { return D == 64 ? 3 : 2; }
 constexpr int FEW_UNITS = 32;
 
+// sum of the lanes' values up to this one's: within rows of 16, then over the rows
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);          // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);          // lane 15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);          // lane 31 into rows 2 and 3
+    return v;
+}
+
 struct Line {
     int32_t *first_row, *keys, *off, *unit;      // of every sequence, in LDS: first row, keys, first block and unit in the line
     int rows, P, pb;                             // rows of the batch, joined keys of the prefix and their blocks
@@ -440,16 +451,11 @@ __device__ __forceinline__ Line line_of(const QuantArgs &a, uint8_t *smem) {
             l.first_row[r] = s.first;
             l.keys[r] = s.len;
         }
-        int ts = t, us = u;
-#pragma unroll
-        for (int x = 1; x < 64; x <<= 1) {
-            const int t2 = __shfl_up(ts, x), u2 = __shfl_up(us, x);
-            if (lane >= x) { ts += t2; us += u2; }
-        }
+        const int ts = wave_scan(t), us = wave_scan(u);
         if (lane == 63) { wsum[wv] = ts; wsum[8 + wv] = us; }
         __syncthreads();
         int tb = t_before, ub = u_before;
-        for (int i = 0; i < threads >> 6; ++i) {
+        for (int i = 0; i < (min(threads, a.R - r0) + 63) >> 6; ++i) {       // the waves that have a sequence
             if (i < wv) { tb += wsum[i]; ub += wsum[8 + i]; }
             t_before += wsum[i];
             u_before += wsum[8 + i];

@@ -451,3 +451,29 @@ def test_attention_over_the_range_of_bf16(device, kf, vf, qf, every, new, H, Hkv
     assert torch.isfinite(got).all()
     err = (got - exact[:rows]).abs()
     assert (err <= bound[:rows] + 1e-36).all(), float((err / bound[:rows].clamp(min=1e-36)).max())
+
+
+@pytest.mark.parametrize("slots", ["from 5", "every seventh missing", "any order"])
+@pytest.mark.parametrize("D,bits", [(64, 4), (128, 4), (64, 8), (128, 8)])
+def test_append_of_many_rows_leaves_what_few_at_a_time_do(device, D, bits, slots):
+    """Runs of slots that begin and break anywhere, rows that are left out among them: the same
+    bytes as row by row, and no others touched."""
+    H, Hkv, n, nb, bs = 4, 2, 600, 12, 64
+    g = torch.Generator(device="cuda")
+    g.manual_seed(D + bits)
+    at = {"from 5": torch.arange(5, 5 + n), "every seventh missing": torch.arange(nb * bs)[torch.arange(nb * bs) % 7 != 3][:n],
+          "any order": torch.randperm(nb * bs, generator=torch.Generator().manual_seed(1))[:n]}[slots].to("cuda", torch.int32)
+    at[17::40] = -1
+    qkv = torch.randn((n, (H + 2 * Hkv) * D), generator=g, device="cuda").bfloat16()
+    angles = torch.rand((50, D // 2), generator=g, device="cuda") * 6
+    cos, sin = angles.cos().contiguous(), angles.sin().contiguous()
+    pos = torch.arange(n, device="cuda", dtype=torch.int32) % 50
+    shape = _lib.quantized_pool_shape(nb, Hkv, bs, D, bits)
+    one, few = (torch.full(shape, 0xA5, dtype=torch.uint8, device="cuda") for _ in range(2))
+    q = _lib.rope_append_quantized(qkv, H, Hkv, D, cos, sin, one, at, pos, bits=bits, out=torch.zeros((n, H * D), device="cuda").bfloat16())
+    for i in range(0, n, 1 if slots == "any order" else 3):
+        rows = slice(i, i + (1 if slots == "any order" else 3))
+        part = _lib.rope_append_quantized(qkv[rows], H, Hkv, D, cos, sin, few, at[rows], pos[rows], bits=bits,
+                                          out=torch.zeros((qkv[rows].shape[0], H * D), device="cuda").bfloat16())
+        assert torch.equal(part, q[rows])
+    assert torch.equal(one, few)
