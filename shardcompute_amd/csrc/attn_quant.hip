@@ -356,7 +356,7 @@ struct Columns {
                 for (int z = 0; z < 4; ++z) o[y][z] = fmaf(o[y][z], alpha, c);
         }
     }
-    // the column's sum of weights; o then is the column's sum of p v, in its dims tiles [first, first + n)
+    // the column's sum of weights; o then is the column's sum of p v, in the tiles that the lane writes
     __device__ __forceinline__ float close() {
         settle(1.f);
         float l = lsum + __shfl_xor(lsum, 16);
@@ -874,7 +874,7 @@ constexpr float PART_BYTES_US = 1.3e6f;
 __device__ __forceinline__ int best_cut(int wgs, int blocks, int most, int grid, const Line &l, float tile_us, float line_us, float part_us) {
     const int lane = threadIdx.x & 63, n = lane + 1;
     float us = INFINITY;
-    if (n <= most && (wgs * n < grid || l.total == 0)) {
+    if (n <= most) {                                       // (so that a CU is left)
         const float tile = (float)((blocks + n - 1) / n) * tile_us + TILE_OPEN_US;
         const int own = 2 * max(grid - wgs * n, 1);
         const float run = with_rest(l.total, l.units, own) ? (float)own_run(l.total + l.units, own) : 1.6f * (float)own_run(l.total, own);
@@ -928,16 +928,17 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(line_w
 // ---------------------------------------------------------------- host side
 
 // Into how many workgroups a column tile's key blocks are cut where sequences of many rows are
-// among them, of `most` that there is room for: the walk at 2 us a block against the parts.  (A
+// among them, of `most` that run at a time: the walk at 2 us a block against the parts, which are
+// written and read at 2.5 TB/s (a tile that is not cut writes its rows' outputs itself).  (A
 // prompt of 2048 rows in 33 column tiles on 8 kv heads stays whole: two cuts of each would write
 // and read 140 MB of parts, 50 us, for half of a walk of 67.)
-int quant_splits(long wgs, long blocks, double part_bytes, bool last_is_whole, long most) {
+int quant_splits(long wgs, long blocks, double part_bytes, long most) {
     int best = 1;
     double least = 1e30;
     for (int n = 1; n <= 64 && (n == 1 || n <= blocks); ++n) {
         const long rounds = (wgs * n + most - 1) / most;
         const double walk = (double)((blocks + n - 1) / n) * 2.0 * rounds;
-        const double parts = n == 1 && last_is_whole ? 0 : n * (part_bytes / (last_is_whole ? 2.5e6 : 1.3e6) + 0.06);
+        const double parts = n == 1 ? 0 : n * (part_bytes / 2.5e6 + 0.06);
         if (walk + parts < least) { least = walk + parts; best = n; }
     }
     return best;
@@ -963,7 +964,7 @@ SaPlan plan_quant(long N, long R, long H, long Hkv, long D, long own_cap, long p
     // where tiles have the prefix alone the kernel cuts them, into nsplit at most
     p.cut = p.use_tile && !p.any_big && wgs < cus;
     if (p.cut) p.nsplit = (int)std::min({64L, blocks, (cus - 1) / wgs});
-    else if (p.any_big) p.nsplit = quant_splits(wgs, blocks, (double)N * H * (8 * D + 16), p.any_big, cus);
+    else if (p.any_big) p.nsplit = quant_splits(wgs, blocks, (double)N * H * (8 * D + 16), cus);
     const long rows_max = max_new < p.small_rows ? max_new : p.small_rows;
     p.rows_max = (int)rows_max;
     long coltiles = R * ((rows_max * G + 63) / 64);

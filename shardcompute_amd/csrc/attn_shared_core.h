@@ -20,7 +20,7 @@ using f4 = dma::f4;
 
 constexpr int SA_KB = 64, SA_THREADS = 256;
 constexpr int SA_AHEAD = 4;                              // operand reads in flight ahead of the MFMAs
-constexpr int SA_MAX_SEQ = 2048;         // attn_own keeps two numbers of each in LDS
+constexpr int SA_MAX_SEQ = 2048;         // attn_own keeps two numbers of each in LDS, attn_line (attn_quant.hip) four
 constexpr int SA_CU_LDS = 160 * 1024;    // of a CU
 
 // What the kernels over a cache of either kind share; a kernel's own arguments are derived from

@@ -198,3 +198,31 @@ def test_parts_of_units_with_rests(parts_of, rest, seed):
                     want = [4 * (number + w) + v for w in holders for v in waves]
                     assert [p_first + step * j for j in range(p_n)] == want and col == c % 16
         first += n
+
+
+def _up(v):
+    return -(-v // 256) * 256
+
+
+@pytest.mark.parametrize("rows,R,H,Hkv,D,own,prefix", [
+    (24, 1, 32, 8, 128, 64, 0), (24, 1, 32, 8, 128, 4096, 0), (64, 1, 32, 8, 128, 131072, 0), (100, 3, 32, 4, 64, 700, 5000),
+    (2049, 1, 32, 8, 128, 2112, 0), (2049, 1, 32, 8, 128, 131072, 0), (2079, 32, 32, 8, 128, 2112, 0), (9000, 16, 8, 1, 128, 1024, 4096),
+])
+def test_workspace_of_prompts_is_that_of_their_cut(rows, R, H, Hkv, D, own, prefix):
+    """Column tiles of 256 (row, head) columns on 256 CUs, their keys cut into as many workgroups as
+    make the walk (2 us a block of 64 keys, rounds of 256 workgroups) and the parts (2.5 TB/s and
+    0.06 us each; none if uncut) least."""
+    cus, G = 256, H // Hkv
+    wgs, blocks = -(-rows * G // 256) * Hkv, -(-(own + prefix) // 64)
+
+    def us(n):
+        return -(-blocks // n) * 2.0 * -(-wgs * n // cus) + (n > 1) * n * (rows * H * (8 * D + 16) / 2.5e6 + 0.06)
+    cut = min(range(1, min(64, blocks) + 1), key=us)
+    small = max(64 // G, 1)                  # rows of a sequence whose own keys are the line's
+    few = R * small < rows and cut == 1
+    tile = cut * (R * small if few else rows) * H
+    coltiles = min(R * -(-small * G // 64), R + rows * G // 64)
+    keyblocks = coltiles * (-(-own // 128) + (R > 1))
+    line = 4 * (Hkv * coltiles + max(min(2 * cus, Hkv * keyblocks), 1)) * min(small * G, 16)
+    want = sum(_up(n * b) for n in (tile, line) for b in (4 * D, 8)) + _up((R + 1) * 8 + 8)
+    assert _lib.attention_quantized_workspace_bytes(rows, R, H, Hkv, D, own, prefix, rows, bits=4) == want
