@@ -35,6 +35,8 @@ namespace {
 
 struct QuantArgs : SaArgs {
     const uint8_t *pool;
+    int cus;                 // of the device
+    float part_us;           // of prompt_part_us
 };
 
 // the cell of position t (a multiple of 16) of a table, kv head hk
@@ -406,6 +408,17 @@ __device__ __forceinline__ int wave_scan(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);          // lane 15 into rows 1 and 3
     v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);          // lane 31 into rows 2 and 3
     return v;
+}
+
+// the largest of the lanes' values, none below 0
+__device__ __forceinline__ int wave_top(int v) {
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));
+    return __builtin_amdgcn_readlane(v, 63);
 }
 
 struct Line {
@@ -887,6 +900,41 @@ __device__ __forceinline__ int best_cut(int wgs, int blocks, int most, int grid,
     return max(__ffsll((unsigned long long)__ballot(us == least)), 1);
 }
 
+// Where sequences of many rows are among them, column tiles of `wgs` workgroups, each with `blocks`
+// key blocks that are cut into n: the walk at 2 us a block, `cus` workgroups at a time, and the
+// parts, which are written and read at 2.5 TB/s (a tile that is not cut writes its rows' outputs
+// itself).  (A prompt of 2048 rows in 33 column tiles on 8 kv heads stays whole: two cuts of each
+// would write and read 140 MB of parts, 50 us, for half of a walk of 67.)  More blocks have their
+// least time at the same n or a larger one, so that a cut planned for the tables' room is enough
+// for whatever they hold.
+template <class I>
+__host__ __device__ __forceinline__ float cut_us(I wgs, I blocks, I n, I cus, float part_us) {
+    const float walk = (float)blocks / (float)n * 2.f * (float)((wgs * n + cus - 1) / cus);
+    return walk + (n == 1 ? 0.f : (float)n * part_us);
+}
+float prompt_part_us(long part_rows, long H, long D) { return (float)(part_rows * H * (8 * D + 16)) / 2.5e6f + 0.06f; }
+
+// The cut by the keys that are held, those of the prefix and of the longest sequence with many rows,
+// whatever the tables have room for: the n of the least time, less what leaves the longest walk as
+// it is.  32 heads of 128 on 8 in 4 bits, tables with room for 131072 positions: a prompt of 2049 rows
+// 82 us (75 where the tables end with it; cut for the room 258, in 12 pieces of which most hold no
+// key), of 64 rows 15.2 (14.5; 22.2).  The lengths are read before the tile begins, 1 to 1.5 us where
+// the cut for the room is as good: 24 rows behind 30000 held positions 39.4 us (38.6).
+__device__ __forceinline__ int held_cut(const QuantArgs &a) {
+    const int lane = threadIdx.x & 63, n = lane + 1, rows = live_rows(a), P = prefix_keys(a);
+    int longest = 0;
+    for (int r = lane; r < a.R; r += 64) {
+        const Seq s = seq_of(a, r, rows);
+        if (s.n > a.small_rows) longest = max(longest, s.len);
+    }
+    const int blocks = (P + wave_top(longest) + SA_KB - 1) / SA_KB;
+    const float us = n == 1 || n <= min(a.nsplit, blocks) ? cut_us(a.tiles * a.Hkv, blocks, n, a.cus, a.part_us) : INFINITY;
+    // (times are not negative: their bits are in their order)
+    const int less = 0x7F800000 - __float_as_int(us);
+    const int best = __ffsll((unsigned long long)__ballot(less == wave_top(less))), walk = max((blocks + best - 1) / best, 1);
+    return max((blocks + walk - 1) / walk, 1);
+}
+
 // Column tiles and lines: workgroups of 8 waves, which take every register of a CU, of a tile of
 // 256 columns or of two of the line's.
 constexpr int QUANT_WAVES = 8;
@@ -895,7 +943,9 @@ __global__ void __launch_bounds__(64 * QUANT_WAVES) __attribute__((amdgpu_waves_
     extern __shared__ __align__(16) uint8_t smem[];
     const int id = (int)blockIdx.x, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Line l;
-    if (a.cut) {
+    // sequences with many rows are there only with 16 columns (small_rows of them make as many at least)
+    const bool many = CW == 16 && a.any_big;
+    if (a.cut && !many) {
         // tiles have the prefix alone, and everything else is in the line: cut by what there is
         l = line_of(a, smem);
         const int wgs = a.tiles * a.Hkv, blocks = (prefix_keys(a) + SA_KB - 1) / SA_KB;
@@ -909,10 +959,16 @@ __global__ void __launch_bounds__(64 * QUANT_WAVES) __attribute__((amdgpu_waves_
         if (id < a.tile_wgs) __syncthreads();                  // the ring takes the line's LDS
     }
     if (id < a.tile_wgs) {
+        if (a.cut && many) {
+            a.nsplit = held_cut(a);
+            if (id >= a.tiles * a.Hkv * a.nsplit) return;
+        }
         attn_tile<D, Values<D, BITS>>(a, id, smem);
+        // (after the tile, which reads the lengths again)
+        if (a.cut && many && id == 0 && threadIdx.x == 0) { a.cut[0] = a.nsplit; a.cut[1] = a.own_wgs; }
         return;
     }
-    if (!a.cut) { l = line_of(a, smem); places_of(a, l); }
+    if (!a.cut || many) { l = line_of(a, smem); places_of(a, l); }
     attn_line<D, BITS, CW>(a, l, (id - a.tile_wgs) * (QUANT_WAVES / 4) + w / 4, w & 3);
 }
 
@@ -927,19 +983,14 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(line_w
 
 // ---------------------------------------------------------------- host side
 
-// Into how many workgroups a column tile's key blocks are cut where sequences of many rows are
-// among them, of `most` that run at a time: the walk at 2 us a block against the parts, which are
-// written and read at 2.5 TB/s (a tile that is not cut writes its rows' outputs itself).  (A
-// prompt of 2048 rows in 33 column tiles on 8 kv heads stays whole: two cuts of each would write
-// and read 140 MB of parts, 50 us, for half of a walk of 67.)
-int quant_splits(long wgs, long blocks, double part_bytes, long most) {
+// The cut that is planned, for the keys that the tables have room for: what the workspace holds,
+// and the most that held_cut takes.
+int quant_splits(long wgs, long blocks, long cus, float part_us) {
     int best = 1;
-    double least = 1e30;
+    float least = INFINITY;
     for (int n = 1; n <= 64 && (n == 1 || n <= blocks); ++n) {
-        const long rounds = (wgs * n + most - 1) / most;
-        const double walk = (double)((blocks + n - 1) / n) * 2.0 * rounds;
-        const double parts = n == 1 ? 0 : n * (part_bytes / 2.5e6 + 0.06);
-        if (walk + parts < least) { least = walk + parts; best = n; }
+        const float us = cut_us(wgs, blocks, (long)n, cus, part_us);
+        if (us < least) { least = us; best = n; }
     }
     return best;
 }
@@ -961,17 +1012,18 @@ SaPlan plan_quant(long N, long R, long H, long Hkv, long D, long own_cap, long p
     p.tiles = (cols + 32 * QUANT_WAVES - 1) / (32 * QUANT_WAVES);
     const long wgs = p.tiles * Hkv;
     const long blocks = (prefix_cap + (p.any_big ? own_cap : 0) + SA_KB - 1) / SA_KB;
-    // where tiles have the prefix alone the kernel cuts them, into nsplit at most
-    p.cut = p.use_tile && !p.any_big && wgs < cus;
-    if (p.cut) p.nsplit = (int)std::min({64L, blocks, (cus - 1) / wgs});
-    else if (p.any_big) p.nsplit = quant_splits(wgs, blocks, (double)N * H * (8 * D + 16), cus);
+    // the kernel cuts them, into nsplit at most; where tiles have the prefix alone it shares the CUs out
+    const bool shared = p.use_tile && !p.any_big && wgs < cus;
+    if (shared) p.nsplit = (int)std::min({64L, blocks, (cus - 1) / wgs});
+    else if (p.any_big) p.nsplit = quant_splits(wgs, blocks, cus, prompt_part_us(N, H, D));
+    p.cut = shared || p.nsplit > 1;
     const long rows_max = max_new < p.small_rows ? max_new : p.small_rows;
     p.rows_max = (int)rows_max;
     long coltiles = R * ((rows_max * G + 63) / 64);
     if (coltiles > R + cols / 64) coltiles = R + cols / 64;
     const long keyblocks = coltiles * (own_keyblocks((int)own_cap, LINE_SHIFT) + (p.join ? own_keyblocks((int)prefix_cap, LINE_SHIFT) : 0) + p.own_rest);
     long ow = (p.use_tile || R * Hkv < FEW_UNITS ? 2 : line_waves((int)D)) * cus;
-    if (!p.cut && ow > Hkv * keyblocks) ow = Hkv * keyblocks;
+    if (!shared && ow > Hkv * keyblocks) ow = Hkv * keyblocks;
     p.own_wgs = (int)(ow < 1 ? 1 : ow);
     p.own_parts = 4 * (Hkv * coltiles + p.own_wgs);
     p.part_cols = (int)(rows_max * G < 16 ? (rows_max * G > 1 ? rows_max * G : 1) : 16);
@@ -986,7 +1038,7 @@ int run_quant(const QuantArgs &a, const SaPlan &p, hipStream_t stream) {
         hipLaunchKernelGGL((attn_line_kernel<D, BITS, CW>), dim3((unsigned)a.own_wgs), dim3(256), line, stream, a);
     } else {
         const int tile = SaGeo<D>::LDS + 16, lds = tile > line ? tile : line, per = QUANT_WAVES / 4;
-        const int grid = a.cut ? device_info().num_cus : a.tile_wgs + (a.own_wgs + per - 1) / per;
+        const int grid = a.cut && !a.any_big ? a.cus : a.tile_wgs + (a.own_wgs + per - 1) / per;
         if (lds > 65536) {
             // more than 64 KB of LDS has to be allowed, once a device
             static std::atomic<uint64_t> allowed;
@@ -1065,6 +1117,8 @@ int launch_attention_quantized(const uint16_t *q, long q_stride, const uint8_t *
     a.width = (int)width; a.shift = shift; a.n_blocks = (int)n_blocks; a.prefix_width = (int)prefix_width;
     fill_args(a, p, workspace);
     a.pair_half = 0;
+    a.cus = device_info().num_cus;
+    a.part_us = prompt_part_us(p.part_rows, H, D);
     a.scale_log2 = scale * 1.4426950408889634f;
     if (D == 128) return bits == 4 ? run_quant<128, 4>(a, p, stream) : run_quant<128, 8>(a, p, stream);
     return bits == 4 ? run_quant<64, 4>(a, p, stream) : run_quant<64, 8>(a, p, stream);

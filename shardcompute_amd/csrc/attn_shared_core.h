@@ -537,6 +537,7 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
     const long wid = WPR == 4 ? (long)blockIdx.x : (long)blockIdx.x * 4 + w;
     const int turn = WPR == 4 ? w : 0;
     const int rows = live_rows(a);
+    if (a.cut) tile_parts = a.cut[0];
     int row = (int)(wid / a.H), r;
     const int h = (int)(wid - (long)row * a.H);
     Seq s;
@@ -554,11 +555,10 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(SaArgs a, int tile_part
         r = find_seq(a, row);
         s = seq_of(a, r, rows);
         if (row < s.first || row >= s.first + s.n) return;     // no sequence's row
-        if (s.n > a.small_rows && a.nsplit == 1) return;       // written by attn_tile
+        if (s.n > a.small_rows && tile_parts <= 1) return;     // written by attn_tile
     }
     const int hk = h / a.G, gq = h - hk * a.G;
     const int own_wgs = a.cut ? a.cut[1] : a.own_wgs;
-    if (a.cut) tile_parts = a.cut[0];
     const int joined = a.join ? own_keyblocks(prefix_keys(a), a.own_shift) : 0;
     const OwnParts own = own_parts_of(row, s.first, s.n, s.len, hk, gq, a.G, a.small_rows, a.own_off[r], a.own_unit[r],
                                       a.own_off[a.R], own_wgs, a.own_parts, a.part_cols, a.own_shift, joined,

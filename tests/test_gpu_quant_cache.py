@@ -477,3 +477,29 @@ def test_append_of_many_rows_leaves_what_few_at_a_time_do(device, D, bits, slots
                                           out=torch.zeros((qkv[rows].shape[0], H * D), device="cuda").bfloat16())
         assert torch.equal(part, q[rows])
     assert torch.equal(one, few)
+
+
+@pytest.mark.parametrize("held,new,prefix,bs,H,Hkv,D", [
+    ([0], [24], 0, 64, 32, 8, 128), ([0], [64], 0, 16, 32, 8, 64), ([100, 0], [100, 1], 0, 64, 8, 2, 128),
+    ([3, 0, 70, 500, 9], [40, 30, 1, 1, 0], 200, 32, 8, 1, 64), ([0, 10], [300, 90], 1000, 64, 8, 8, 128),
+    ([0], [2049], 0, 64, 32, 8, 64),
+])
+@pytest.mark.parametrize("bits", BITS)
+def test_attention_is_by_the_positions_held_not_by_the_tables_room(device, held, new, prefix, bs, H, Hkv, D, bits):
+    """Many rows behind tables with room for 131072 positions: the bits of tables that end with the
+    sequences, and no more of the workspace written than those need at all."""
+    print(f"room {bits} bits {held} + {new} prefix={prefix} bs={bs} H={H} Hkv={Hkv} D={D}", flush=True)
+    tight = QuantCache(bits, held, new, prefix, bs, H, Hkv, D, pad=2)
+    want = tight.attend(out=torch.full_like(tight.q, 5.0))
+    if tight.N < 1000:
+        assert_attention(want, *tight.exact(), tight.starts[-1])
+    most = tight.workspace_bytes(tight.N)
+    wide = QuantCache(bits, held, new, prefix, bs, H, Hkv, D, pad=2, width=131072 // bs)
+    assert torch.equal(wide.pool, tight.pool)
+    if prefix:
+        wide.prefix_table = torch.cat([wide.prefix_table, wide.prefix_table.new_full((100,), -3)])
+    need = wide.workspace_bytes(wide.N)
+    ws = torch.full((need,), 77, dtype=torch.uint8, device="cuda")
+    got = wide.attend(out=torch.full_like(wide.q, 5.0), workspace=ws)
+    assert torch.equal(got, want)
+    assert int((ws != 77).sum()) <= most

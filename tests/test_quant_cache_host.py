@@ -216,7 +216,7 @@ def test_workspace_of_prompts_is_that_of_their_cut(rows, R, H, Hkv, D, own, pref
     wgs, blocks = -(-rows * G // 256) * Hkv, -(-(own + prefix) // 64)
 
     def us(n):
-        return -(-blocks // n) * 2.0 * -(-wgs * n // cus) + (n > 1) * n * (rows * H * (8 * D + 16) / 2.5e6 + 0.06)
+        return blocks / n * 2.0 * -(-wgs * n // cus) + (n > 1) * n * (rows * H * (8 * D + 16) / 2.5e6 + 0.06)
     cut = min(range(1, min(64, blocks) + 1), key=us)
     small = max(64 // G, 1)                  # rows of a sequence whose own keys are the line's
     few = R * small < rows and cut == 1
