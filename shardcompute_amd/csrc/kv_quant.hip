@@ -292,17 +292,16 @@ __global__ void __launch_bounds__(256) rope_append_quantized_kernel(QuantAppendA
 // has 8 dims of the key, and of the value the dims l, 16 + l, .. of its place in the cell (two
 // places with 64 dims), which go through LDS into the row's order.
 //
-// Bound by memory: 40000 positions of 8 kv heads of 128 in 4 bits 34 us (210 MB: 6.1 TB/s).  More
-// than QR_THROUGH bytes of output go past the caches, which would lose what comes in for what no
-// reader finds there in time: with 164 MB, pools in turn, 34 us in place of 49; 15 MB take 9.5 us
-// either way, and are there for who reads them next.
-constexpr long QR_THROUGH = 64L << 20;
+// Bound by memory: 40000 positions of 8 kv heads of 128 in 4 bits (164 MB of outputs, a pool of 46):
+// 35 us into outputs that the caches hold with two pools in turn, 48 with four, 53 into outputs that
+// were not written lately.  With stores past the caches it takes 34 to 36 in each case, but with
+// whoever uses the outputs next (one pass over them) 103 us in place of 95: ordinary stores.
 struct QuantReadArgs {
     const uint8_t *pool;
     const int32_t *slots;
     uint16_t *k, *v;
     long n, n_slots;
-    int Hkv, shift, through;
+    int Hkv, shift;
 };
 
 template <int D, int BITS>
@@ -361,14 +360,8 @@ __global__ void __launch_bounds__(256) read_quantized_kernel(QuantReadArgs a) {
     if (row >= a.n) return;
     if (there) val = *reinterpret_cast<const uint4 *>(tile + r * PAD + 8 * o);
     const long at = (row * a.Hkv + hk) * D + 8 * o;
-    typedef uint32_t words __attribute__((ext_vector_type(4)));
-    if (a.through) {
-        __builtin_nontemporal_store(__builtin_bit_cast(words, key), reinterpret_cast<words *>(a.k + at));
-        __builtin_nontemporal_store(__builtin_bit_cast(words, val), reinterpret_cast<words *>(a.v + at));
-    } else {
-        *reinterpret_cast<uint4 *>(a.k + at) = key;
-        *reinterpret_cast<uint4 *>(a.v + at) = val;
-    }
+    *reinterpret_cast<uint4 *>(a.k + at) = key;
+    *reinterpret_cast<uint4 *>(a.v + at) = val;
 }
 
 }  // namespace
@@ -431,7 +424,6 @@ int launch_read_quantized(const uint8_t *pool, long n_blocks, long bs, int bits,
         return set_error(SC_EINVAL, "read_quantized: pointers must be 16-byte aligned");
     QuantReadArgs a;
     a.pool = pool; a.slots = slots; a.k = k; a.v = v; a.n = n; a.n_slots = n_blocks * bs; a.Hkv = (int)Hkv; a.shift = shift;
-    a.through = n * Hkv * D * 4 > QR_THROUGH;
     const long rows = 256 / (D / 8), blocks = (n + rows - 1) / rows * Hkv;
     if (blocks >= (1L << 24)) return set_error(SC_EINVAL, "read_quantized: too many rows");            // 2^32 threads
     auto kern = D == 128 ? (bits == 4 ? read_quantized_kernel<128, 4> : read_quantized_kernel<128, 8>)
