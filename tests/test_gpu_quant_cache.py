@@ -503,3 +503,37 @@ def test_attention_is_by_the_positions_held_not_by_the_tables_room(device, held,
     got = wide.attend(out=torch.full_like(wide.q, 5.0), workspace=ws)
     assert torch.equal(got, want)
     assert int((ws != 77).sum()) <= most
+
+
+# A rounding to bf16 of numbers spread over their range is 0.00166 of them (rms: half a step is 2^-8 at
+# most, evenly spread within it, over numbers evenly spread within a factor of two).
+ONE_ROUNDING = 0.00166
+
+
+def _norm_off(got, exact, rows):
+    got, exact = got[:rows].double().view(rows, *exact.shape[1:]), exact[:rows]
+    return float((got - exact).norm() / exact.norm())
+
+
+@pytest.mark.parametrize("held,new,prefix,H,Hkv", [([40, 300], [200, 130], 500, 8, 2), ([1000], [64], 0, 32, 8),
+                                                   ([9, 0, 500], [70, 300, 90], 2100, 8, 1)])
+@pytest.mark.parametrize("D,bits", [(64, 4), (128, 4), (64, 8), (128, 8)])
+def test_column_tiles_keep_eleven_bits(device, held, new, prefix, H, Hkv, D, bits):
+    """Many rows, keys, values and q of about 1: the output's own rounding and fp16's, an eighth of it,
+    of keys, weights and values (with the scores' spread of 1: 0.0017 together).  One more rounding to
+    8 bits makes it 0.0023 (bf16 values and weights 0.0033)."""
+    c = QuantCache(bits, held, new, prefix, 64, H, Hkv, D)
+    off = _norm_off(c.attend(max_new=c.max_new), c.exact()[0], c.starts[-1])
+    assert off <= 1.2 * ONE_ROUNDING, off
+
+
+@pytest.mark.parametrize("held,new,prefix,H,Hkv", [([300, 900, 77], [1, 1, 2], 0, 8, 2), ([700], [1], 600, 32, 8),
+                                                   ([80, 200, 900], [5, 3, 8], 0, 8, 1), ([400, 90], [16, 9], 0, 4, 2)])
+@pytest.mark.parametrize("D,bits", [(64, 4), (128, 4), (64, 8), (128, 8)])
+def test_lines_round_the_weights_alone(device, held, new, prefix, H, Hkv, D, bits):
+    """Few rows: the output's rounding and that of the weights, which meet values taken about the
+    middle code (their squares 1.11 times the values': half a step of 0.3 and the range's middle, 0.3
+    beside 0): 0.0024 together, one more of either 0.0029."""
+    c = QuantCache(bits, held, new, prefix, 64, H, Hkv, D)
+    off = _norm_off(c.attend(max_new=c.max_new), c.exact()[0], c.starts[-1])
+    assert off <= 1.6 * ONE_ROUNDING, off
