@@ -428,8 +428,9 @@ int sc_read_quantized_bf16(const uint8_t *pool, int64_t n_blocks, int64_t block_
  * sc_attention_shared_bf16 over a quantized pool: the same rows, tables, prefix, clamping and
  * limits, keys and values being scale * code + bias (magnitudes below 2^100 and 2^80).  Slots
  * that no row attends may hold anything.  Of few new rows a sequence's own values meet weights
- * rounded to bf16; of many, and of the prefix, values and weights are rounded to fp16 (2^-12)
- * where 64 keys of a kv head lie in its range, else to bf16.
+ * rounded to bf16 (2^-8 at most); of many, and of the prefix, keys, values and weights are rounded
+ * to fp16 (2^-11) where 64 keys of a kv head lie in its range (in 8 bits a key or value may be
+ * off by 2^-11 of its group's largest beside that), else to bf16.
  */
 int64_t sc_attention_quantized_workspace_bytes(int64_t N, int64_t R, int64_t H, int64_t Hkv, int64_t D, int64_t own_cap,
                                                int64_t prefix_cap, int64_t max_new, int bits);

@@ -747,8 +747,10 @@ struct Values {
     static __device__ __forceinline__ float code(uint32_t w, int e) {
         return BITS == 4 ? (float)((w >> (4 * e)) & 15u) : ubyte_f32(w, e);
     }
-    // fp16 holds these positions' values times 2^HALF_UP as exactly as it can: none reaches
-    // its largest, and the scale is whole, or what is dropped of it small beside the values
+    // fp16 holds these positions' values times 2^HALF_UP: none reaches its largest, and the scale
+    // is whole, or what is dropped of it, 2^(-25 - HALF_UP) at most, is TOP times that in a value: below
+    // 2^-22 in 8 bits (2^-26 in 4), 2^-11 (2^-15) of the group's largest.  (Rounded to bf16 in its place, such
+    // keys move scores by 2^-8 of themselves: 0.0027 off in place of 0.0017 with scales of 2^-22.1.)
     static __device__ __forceinline__ bool in_range(uint32_t meta) {
         constexpr float TOP = BITS == 4 ? 15.f : 255.f;
         const float s = __uint_as_float(meta << 16), b = __uint_as_float(meta & 0xFFFF0000u), e = fmaf(s, TOP, b);

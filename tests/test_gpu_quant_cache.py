@@ -537,3 +537,29 @@ def test_lines_round_the_weights_alone(device, held, new, prefix, H, Hkv, D, bit
     c = QuantCache(bits, held, new, prefix, 64, H, Hkv, D)
     off = _norm_off(c.attend(max_new=c.max_new), c.exact()[0], c.starts[-1])
     assert off <= 1.6 * ONE_ROUNDING, off
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_column_tiles_of_groups_whose_scale_fp16_cannot_hold(device, D):
+    """Keys of 8 bits in groups from 2^-11 to 2^-11 + 15 / 2^18, either sign: scales of 2^-22.1, of which
+    fp16 (at 32 times them) drops up to 2^-30, 255 times as much of a key, below 2^-11 of the group's
+    largest.  Scores of q about 2^12: 0.0006 off by the keys' rounding to 11 bits and by what is
+    dropped; the output's rounding is 0.00166.  Keys rounded to bf16 would move scores by 0.0045."""
+    c = QuantCache(8, [40, 300], [200, 130], 500, 64, 8, 2, D)
+    there = ~torch.isnan(c.k[:, 0, :, 0])
+    g = torch.Generator(device="cuda")
+    g.manual_seed(D)
+    nb, Hkv, bs = c.k.shape[:3]
+    j = torch.randint(0, 16, c.k.shape, generator=g, device="cuda").view(nb, Hkv, bs, D // 64, 64)
+    j[..., 0], j[..., 1] = 0, 15
+    sign = torch.randint(0, 2, j.shape[:-1], generator=g, device="cuda")[..., None] * 2 - 1
+    k = (sign * (2.0 ** -11 + j * 2.0 ** -18)).view(c.k.shape)
+    c.k = torch.where(there[:, None, :, None], k, float("nan")).to(torch.bfloat16)
+    assert torch.equal(c.k[there[:, None].expand(nb, Hkv, bs)].double(), k[there[:, None].expand(nb, Hkv, bs)].double())
+    c.q *= 4096
+    at = there.nonzero()
+    write(c.pool, c.k[at[:, 0], :, at[:, 1]], c.vt[at[:, 0], :, :, at[:, 1]], at[:, 0] * bs + at[:, 1], 8)
+    scales = stored(c.k[at[:, 0], :, at[:, 1]], 8)[1].abs()
+    assert 2.0 ** -23 < scales.min() and scales.max() < 2.0 ** -22
+    off = _norm_off(c.attend(max_new=c.max_new), c.exact()[0], c.starts[-1])
+    assert off <= 1.2 * ONE_ROUNDING, off
