@@ -563,3 +563,36 @@ def test_column_tiles_of_groups_whose_scale_fp16_cannot_hold(device, D):
     assert 2.0 ** -23 < scales.min() and scales.max() < 2.0 ** -22
     off = _norm_off(c.attend(max_new=c.max_new), c.exact()[0], c.starts[-1])
     assert off <= 1.2 * ONE_ROUNDING, off
+
+
+@pytest.mark.parametrize("H,Hkv,D,bits", [(32, 8, 128, 4), (8, 1, 64, 8)])
+def test_captured_prompts_of_growing_lengths(device, H, Hkv, D, bits):
+    """Attention of many rows in a graph, tables with room for more than they hold: replayed as the
+    lengths grow from one key block to hundreds, and as rows go from one sequence to another, bit for
+    bit the eager call, two graphs over one workspace in turn."""
+    bs, N = 64, 60
+    c = QuantCache(bits, [20000 - 30, 700, 90], [30, 18, 12], 0, bs, H, Hkv, D, width=40000 // bs)
+    need = c.workspace_bytes(N)
+    ws, out = torch.empty(need, dtype=torch.uint8, device="cuda"), torch.empty_like(c.q)
+    steps = [([0, 30, 48, 60], [30, 18, 12]), ([0, 30, 48, 60], [9000, 700, 12]), ([0, 30, 48, 60], [20000, 718, 102]),
+             ([0, 1, 2, 60], [20000, 718, 64]), ([0, 0, 0, 60], [20000, 718, 102]), ([0, 60, 60, 60], [4000, 0, 5])]
+    want = []
+    for starts, lengths in steps:
+        c.row_starts.copy_(i32(starts))
+        c.lens.copy_(i32(lengths))
+        want.append(c.attend(max_new=N).clone())
+    graphs = []
+    for _ in range(2):
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            c.attend(max_new=N, out=out, workspace=ws)
+        graphs.append(gr)
+    for i in range(2 * len(steps)):
+        starts, lengths = steps[i % len(steps)]
+        c.row_starts.copy_(i32(starts))
+        c.lens.copy_(i32(lengths))
+        out.fill_(5.0)
+        ws.fill_(255)
+        graphs[i % 2 if i < len(steps) else 1 - i % 2].replay()
+        assert torch.equal(out, want[i % len(steps)]), i
