@@ -596,3 +596,20 @@ def test_captured_prompts_of_growing_lengths(device, H, Hkv, D, bits):
         ws.fill_(255)
         graphs[i % 2 if i < len(steps) else 1 - i % 2].replay()
         assert torch.equal(out, want[i % len(steps)]), i
+
+
+@pytest.mark.parametrize("held,new,prefix,bs,H,Hkv,D", [
+    ([100, 3000, 0], [1, 1, 1], 700, 64, 32, 8, 128), ([5000], [1], 0, 16, 8, 1, 64), ([40], [2], 900, 32, 32, 8, 128),
+    ([(37 * i) % 900 for i in range(64)], [1] * 64, 5000, 64, 32, 8, 128), ([10, 600], [5, 8], 0, 64, 8, 1, 64),
+    ([(61 * i) % 400 for i in range(200)], [1, 0, 2, 1] * 50, 90, 16, 32, 4, 64),
+])
+@pytest.mark.parametrize("bits", BITS)
+def test_attention_of_few_rows_in_roomy_tables(device, held, new, prefix, bs, H, Hkv, D, bits):
+    """Few rows a sequence: the same bits from tables that end with the sequences and from ones with
+    room for 40000 positions, the prefix's too."""
+    tight = QuantCache(bits, held, new, prefix, bs, H, Hkv, D, pad=1)
+    want = tight.attend(max_new=tight.max_new, out=torch.full_like(tight.q, 5.0))
+    wide = QuantCache(bits, held, new, prefix, bs, H, Hkv, D, pad=1, width=40000 // bs)
+    if prefix:
+        wide.prefix_table = torch.cat([wide.prefix_table, wide.prefix_table.new_full((500,), -3)])
+    assert torch.equal(wide.attend(max_new=wide.max_new, out=torch.full_like(wide.q, 5.0)), want)
