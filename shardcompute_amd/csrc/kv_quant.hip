@@ -107,8 +107,9 @@ __device__ __forceinline__ float head_max(float v) {
 // multiple of 4 in pieces of 16 too (a lane of the cell: PLANE), other values byte by byte.
 //
 // Prompts: 22000 rows of 8 + 1 heads of 128 in 8 bits, 113 MB, 28.1 us: 4.0 TB/s, 63 % of what a large
-// copy moves; what holds it there has not been found.  Single rows are bound by the chain slot, row, scale, codes, store (64 rows of 32 + 8 heads in 4 bits:
-// 5.7 us).  A wave with the keys of one row and no LDS, its values stored byte by byte: 48.8 and 9.7 us.
+// copy moves; what holds it there has not been found.  Single rows are bound by the chain slot, row,
+// scale, codes, store (64 rows of 32 + 8 heads in 4 bits: 5.7 us).  A wave with the keys of one row
+// and no LDS, its values stored byte by byte: 48.8 and 9.7 us.
 constexpr int QA_ROWS = 32, QA_FEW_ROWS = 16;
 constexpr long QA_FEW = 512;          // rows up to which the groups are the smaller
 

@@ -613,3 +613,17 @@ def test_attention_of_few_rows_in_roomy_tables(device, held, new, prefix, bs, H,
     if prefix:
         wide.prefix_table = torch.cat([wide.prefix_table, wide.prefix_table.new_full((500,), -3)])
     assert torch.equal(wide.attend(max_new=wide.max_new, out=torch.full_like(wide.q, 5.0)), want)
+
+
+@pytest.mark.parametrize("D,bits", [(64, 8), (128, 4)])
+def test_attention_of_prompts_among_the_most_sequences(device, D, bits):
+    """2048 sequences, three of them with many rows, the last among them, in tables with room to spare:
+    every sequence's length counts for the cut, wherever it is."""
+    R = _lib.SHARED_MAX_SEQUENCES
+    held, new = [(11 * i) % 70 if i % 5 else 0 for i in range(R)], [i % 2 for i in range(R)]
+    held[70], new[70], new[1000], held[-1], new[-1] = 5, 90, 70, 1500, 40
+    c = QuantCache(bits, held, new, 90, 64, 4, 2, D, pad=1, width=200)
+    exact, bound = c.exact()
+    got = c.attend(max_new=c.max_new, out=torch.full_like(c.q, 5.0))
+    assert_attention(got, exact, bound, c.starts[-1])
+    assert (got[c.starts[-1]:] == 5).all()
